@@ -36,17 +36,17 @@ def listed():
         return {"name": name, "op": "int8_forward", "rows": rows, "in": n_in, "out": n_out, "degree": degree, "dtype": dtype}
 
     return [
-        # the update of one layer of the narrow degree-32 stack (configuration 5): 33 matrices of 64 x 64
+        # the update of one layer of the narrow degree-32 stack: 33 matrices of 64 x 64
         muon("muon 64x64 degree 32", 64, 64, 32),
-        # the update of the 784 -> 64 layer of the image classifier (configuration 2): tall matrices
+        # the update of the 784 -> 64 layer of the image classifier: tall matrices
         muon("muon 784x64 degree 4", 784, 64, 4),
-        # the update of the wide layer (configuration 3): nine square matrices, the usual heavy step
+        # the update of the wide layer: nine square matrices, the usual heavy step
         muon("muon 1024x1024 degree 8", 1024, 1024, 8),
         # one matrix of the classifier's 64 -> 10 head: the smallest call, latency alone
         orth("orthogonalize 64x10 f32", 1, 64, 10, "float32"),
         # ragged 16-bit gradients, no size a multiple of a tile
         orth("orthogonalize 3x777x1000 bf16", 3, 777, 1000, "bfloat16"),
-        # a degree of each of the four 2048 x 2048 layers of the deep stack (configuration 4), 16-bit gradients
+        # a degree of each of the four 2048 x 2048 layers of the deep stack, 16-bit gradients
         orth("orthogonalize 4x2048x2048 bf16", 4, 2048, 2048, "bfloat16"),
         # one sample through the wide layer's matrix: bound by reading the 8 MB of weights
         matmul("int8 1x8192 to 1024 f32", 1, 8192, 1024, "float32"),
@@ -56,7 +56,7 @@ def listed():
         matmul("int8 65536x8192 to 1024 bf16", 65536, 8192, 1024, "bfloat16"),
         # one sample through one layer of the deep stack
         forward("int8 layer 1x2048 to 2048 d4", 1, 2048, 2048, 4, "bfloat16"),
-        # a batch (one row more than the configuration's) of the classifier's first layer
+        # a batch (one row more than a usual 256) of the classifier's first layer
         forward("int8 layer 257x784 to 64 d4", 257, 784, 64, 4, "float16"),
         # one layer of the deep stack on its full batch
         forward("int8 layer 32768x2048 to 2048", 32768, 2048, 2048, 4, "bfloat16"),
