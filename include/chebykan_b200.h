@@ -312,6 +312,77 @@ int chebykan_adam_step_graph(float* param, const float* grad, float* exp_avg,
                              float grad_scale, void* stream);
 
 /*
+ * Muon update and the orthogonalisation inside it.  The reference trains with torch.optim optimizers
+ * (README.md:59-66); these stand beside chebykan_sgd_step / chebykan_adam_step as torch.optim.Muon stands
+ * beside torch.optim.SGD / Adam.
+ *
+ * chebykan_orthogonalize: out = NS(G) for `batch` matrices G[m][n], by `steps` Newton-Schulz steps
+ *     X_0 = G / max(|G|_F, eps);   A = X X^T;   X <- (a I + b A + c A^2) X
+ * run on the shorter side (a matrix with m > n is worked on as its transpose).  The usual coefficients
+ * (3.4445, -4.7750, 2.0315) push every singular value that is not tiny into about [0.7, 1.2] in five steps.
+ *   - g: element (i, r, c) at g[i*stride_batch + r*stride_row + c*stride_col] (element strides, >= 0), of
+ *     `dtype`; out: [batch][m][n] contiguous, of `dtype`; it may not overlap g;
+ *   - mode CHEBYKAN_MODE_FP32X3: operands held as two fp16 numbers each (22 significant bits), three products
+ *     per multiplication, fp32 results; CHEBYKAN_MODE_TF32: operands rounded to fp16 (tf32's 11 significant
+ *     bits), one product.  fp32 accumulation in both.  Other modes: CHEBYKAN_EUNSUPPORTED;
+ *   - a matrix with a NaN or an infinity comes back as NaN, a zero matrix as zero;
+ *   - 1 <= steps <= 32, eps > 0, m, n <= 65536, batch <= 65535; coefficients under which a singular value can
+ *     leave [0, 7] within the steps are refused (CHEBYKAN_EINVAL).
+ *
+ * chebykan_muon_step: one update of coefficients [in][out][deg+1].  With g = grad_scale * grad:
+ *     buf <- buf + (1 - momentum) (g - buf);   u = nesterov ? g + momentum (buf - g) : buf
+ *     param[:,:,d] <- (1 - lr*weight_decay) param[:,:,d] - lr*update_scale * NS(u[:,:,d])   for every degree d
+ * (torch.optim.Muon's update with each degree's in x out slice as a matrix; deg = 0 updates one plain matrix).
+ * param, grad and buf are contiguous fp32 and may not overlap.  No host state: safe to capture and replay.
+ */
+#define CHEBYKAN_DTYPE_FP32 0
+#define CHEBYKAN_DTYPE_BF16 1
+#define CHEBYKAN_DTYPE_FP16 2
+
+int64_t chebykan_orthogonalize_workspace_bytes(int64_t batch, int64_t m, int64_t n, int mode);
+int chebykan_orthogonalize(const void* g, int64_t stride_batch, int64_t stride_row, int64_t stride_col,
+                           int dtype, void* out, void* workspace, int64_t workspace_bytes, int64_t batch,
+                           int64_t m, int64_t n, int64_t steps, float a, float b, float c, float eps,
+                           int mode, int32_t* status, void* stream);
+int64_t chebykan_muon_workspace_bytes(int64_t in, int64_t out, int64_t deg, int mode);
+int chebykan_muon_step(float* param, const float* grad, float* buf, void* workspace,
+                       int64_t workspace_bytes, int64_t in, int64_t out, int64_t deg, float lr,
+                       float weight_decay, float momentum, int nesterov, float update_scale,
+                       int64_t steps, float a, float b, float c, float eps, float grad_scale,
+                       int mode, int32_t* status, void* stream);
+
+/*
+ * 8-bit forward of a Chebyshev layer (inference), below the math modes of chebykan_fwd.  The reference has
+ * no quantised path; the layer it serves is kan/layers/chebykan.py:53-67.
+ *
+ * chebykan_int8_pack_coeffs: coefficients [in][out][deg+1] (deg >= 1) to
+ *     wq[out][deg][in_pad] with in_pad = in rounded up to 16 (padding zero), degrees 1..deg,
+ *     w_scale[o] = max |C[:,o,1:]| / 127 and wq = round(C / w_scale) (ties to even; an all-zero output has
+ *     scale 0 and zeros), bias[o] = sum_i C[i][o][0] (degree 0 is the constant 1).
+ * chebykan_int8_basis: q[B][deg][in_pad] and scale[B] from x[B][in] (`dtype`): with T_d = T_d(tanh x),
+ *     scale[r] = max |T_1..T_deg of the row| / 127,  q = round(T_d / scale).  A row with a NaN has a NaN scale
+ *     and zeros.  The basis is evaluated in fp32: where T_d / scale lies within its rounding error of a
+ *     half, q may be the neighbouring integer.
+ * chebykan_int8_matmul: y[r][o] = (sum_k q[r][k] wq[o][k]) * q_scale[r] * w_scale[o] + bias[o], y contiguous
+ *     [M][N] of `dtype`, bias may be NULL.  Rows of q / wq are ldq / ldw bytes apart.  The integer sum is exact:
+ *     K <= 131071.  Row strides that are not a multiple of 16 cost a padded copy in the workspace.
+ * chebykan_int8_fwd: the two in a row; the quantised rows live in the workspace.
+ */
+int chebykan_int8_pack_coeffs(const float* coeffs, int8_t* wq, float* w_scale, float* bias, int64_t in,
+                              int64_t out, int64_t deg, void* stream);
+int chebykan_int8_basis(const void* x, int dtype, int8_t* q, float* scale, int64_t B, int64_t in,
+                        int64_t deg, void* stream);
+int64_t chebykan_int8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t ldq, int64_t ldw);
+int chebykan_int8_matmul(const int8_t* q, int64_t ldq, const float* q_scale, const int8_t* wq, int64_t ldw,
+                         const float* w_scale, const float* bias, void* y, int dtype, void* workspace,
+                         int64_t workspace_bytes, int64_t M, int64_t N, int64_t K, int32_t* status,
+                         void* stream);
+int64_t chebykan_int8_fwd_workspace_bytes(int64_t B, int64_t in, int64_t out, int64_t deg);
+int chebykan_int8_fwd(const void* x, int x_dtype, const int8_t* wq, const float* w_scale,
+                      const float* bias, void* y, int y_dtype, void* workspace, int64_t workspace_bytes,
+                      int64_t B, int64_t in, int64_t out, int64_t deg, int32_t* status, void* stream);
+
+/*
  * One-launch training step of a single SMALL layer: forward, mean-squared-error loss, backward and the
  * optimizer update as one kernel of one CTA.  Replaces one iteration of the reference's example loop
  * (README.md:57-69: optimizer.zero_grad(); loss = MSELoss()(layer(x), target); loss.backward();

@@ -15,6 +15,7 @@ LIB_PATH = os.path.join(_HERE, "libchebykan_b200.so")
 
 MODE_FP32, MODE_TF32, MODE_BF16, MODE_FP32X3 = 0, 1, 2, 3
 MODES = {"fp32": MODE_FP32, "tf32": MODE_TF32, "bf16": MODE_BF16, "fp32x3": MODE_FP32X3}
+DTYPE_FP32, DTYPE_BF16, DTYPE_FP16 = 0, 1, 2
 OP_FWD, OP_BWD_DCOEFF, OP_BWD_DX = 0, 1, 2
 FAMILY_CHEBYSHEV, FAMILY_JACOBI, FAMILY_HERMITE, FAMILY_HERMITE_PROB = 0, 1, 2, 3
 
@@ -67,6 +68,22 @@ SIGNATURES = {
                                    c_float, c_float, c_int64, c_float, c_void_p]),
     "chebykan_adam_step_graph": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_float, c_float,
                                          c_float, c_float, c_void_p, c_float, c_void_p]),
+    "chebykan_orthogonalize_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int]),
+    "chebykan_orthogonalize": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p, c_int64, c_int64,
+                                       c_int64, c_int64, c_int64, c_float, c_float, c_float, c_float, c_int, c_void_p,
+                                       c_void_p]),
+    "chebykan_muon_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int]),
+    "chebykan_muon_step": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_float,
+                                   c_float, c_float, c_int, c_float, c_int64, c_float, c_float, c_float, c_float, c_float,
+                                   c_int, c_void_p, c_void_p]),
+    "chebykan_int8_pack_coeffs": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p]),
+    "chebykan_int8_basis": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p]),
+    "chebykan_int8_matmul_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int64, c_int64]),
+    "chebykan_int8_matmul": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int,
+                                     c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p]),
+    "chebykan_int8_fwd_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int64]),
+    "chebykan_int8_fwd": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int64,
+                                  c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p]),
     "chebykan_small_train_step_supported": (c_int, [c_int64, c_int64, c_int64, c_int64]),
     "chebykan_small_train_step": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                           c_int64, c_int64, c_int64, c_int64, c_int, c_float, c_float, c_float, c_float,

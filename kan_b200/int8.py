@@ -1,0 +1,63 @@
+"""Inference with a Chebyshev layer's coefficients in 8 bits.
+
+``quantize_int8`` turns a trained model's ``ChebyKANLayer`` modules into
+``Int8ChebyKANLayer``: coefficients of the degrees from 1 in 8-bit integers with
+a scale per output, the basis quantised row by row on the way in, an exact
+integer product, and the degree-0 term as a bias (``chebykan_int8_fwd``).  A
+quarter of the fp32 coefficients' memory; the quantisation error is about one
+percent of the output (the rounding of both factors to 8 bits).  Inference only.
+"""
+from __future__ import annotations
+
+import copy
+
+import torch
+import torch.nn as nn
+
+from . import ops
+
+
+def _is_cheby(m) -> bool:
+    return hasattr(m, "cheby_coeffs") and hasattr(m, "math_mode") and hasattr(m, "_packed")
+
+
+class Int8ChebyKANLayer(nn.Module):
+    """8-bit form of a trained ``ChebyKANLayer`` on the GPU; same flatten rule, output in `out_dtype`."""
+
+    def __init__(self, layer: nn.Module, out_dtype: torch.dtype = torch.float32):
+        super().__init__()
+        if not _is_cheby(layer):
+            raise TypeError("Int8ChebyKANLayer is built from a ChebyKANLayer")
+        if layer.degree < 1:
+            raise ValueError("the 8-bit forward needs a degree of at least 1")
+        if not layer.cheby_coeffs.is_cuda:
+            raise RuntimeError("move the layer to a CUDA device first: kan_b200 has no CPU path")
+        self.input_dim, self.output_dim, self.degree = layer.input_dim, layer.output_dim, layer.degree
+        self.out_dtype = out_dtype
+        wq, w_scale, bias = ops.int8_pack_coeffs(layer.cheby_coeffs.detach().contiguous())
+        self.register_buffer("wq", wq)
+        self.register_buffer("w_scale", w_scale)
+        self.register_buffer("bias", bias)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if torch.is_grad_enabled() and x.requires_grad:
+            raise RuntimeError("the 8-bit layer is for inference: it has no gradient (call it under torch.no_grad())")
+        x = x.view(-1, self.input_dim).contiguous()
+        if x.numel() and x.data_ptr() % 16:
+            x = x.clone()
+        return ops.int8_forward(x, self.wq, self.w_scale, self.bias, self.degree, out_dtype=self.out_dtype)
+
+    def extra_repr(self) -> str:
+        return f"input_dim={self.input_dim}, output_dim={self.output_dim}, degree={self.degree}"
+
+
+def quantize_int8(model: nn.Module) -> nn.Module:
+    """The model with every ``ChebyKANLayer`` in 8 bits.  Other modules (and their parameters) are shared with `model`,
+    which stays as it is."""
+    if _is_cheby(model):
+        return Int8ChebyKANLayer(model)
+    if not any(_is_cheby(m) for m in model.modules()):
+        return model
+    clone = copy.copy(model)
+    clone._modules = {name: None if child is None else quantize_int8(child) for name, child in model._modules.items()}
+    return clone

@@ -449,6 +449,242 @@ def adam_step_graph(param: torch.Tensor, grad: torch.Tensor, exp_avg: torch.Tens
     _lib.check(rc, "chebykan_adam_step_graph")
 
 
+# ---------------------------------------------------------------------------------------------------------------
+# Muon update and Newton-Schulz orthogonalisation
+# ---------------------------------------------------------------------------------------------------------------
+_DTYPES = {torch.float32: _lib.DTYPE_FP32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16}
+NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+def _dtype(dtype, name: str) -> int:
+    if dtype not in _DTYPES:
+        raise RuntimeError(f"{name} must be float32, bfloat16 or float16, got {str(dtype).replace('torch.', '')}")
+    return _DTYPES[dtype]
+
+
+def _require_any(t: torch.Tensor, name: str, dtype=None, device=None, contiguous: bool = True) -> None:
+    """CUDA tensor of one of the floating types (or of exactly `dtype`), on `device`, contiguous and aligned."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor: kan_b200 has no CPU path")
+    if dtype is None:
+        _dtype(t.dtype, name)
+    elif t.dtype != dtype:
+        raise RuntimeError(f"{name} must be {str(dtype).replace('torch.', '')}, got {str(t.dtype).replace('torch.', '')}")
+    if device is not None and t.device != device:
+        raise RuntimeError(f"{name} is on {t.device}, expected {device}")
+    if contiguous:
+        if not t.is_contiguous():
+            raise RuntimeError(f"{name} must be contiguous")
+        if t.data_ptr() % 16 != 0 and t.numel() > 0:
+            raise RuntimeError(f"{name} must be 16-byte aligned")
+
+
+def orthogonalize(g: torch.Tensor, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float = 1e-7, mode=None,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """Newton-Schulz orthogonalisation of a matrix [m, n] or a batch [b, m, n], any strides; the result is contiguous.
+
+    X = g / max(|g|_F, eps), then `steps` times X <- (a I + b A + c A A) X with A = X X^T on the shorter side.
+    `mode` 'fp32x3' multiplies operands of 22 significant bits in three products, 'tf32' operands of 11 bits in one;
+    the default is 'tf32' for bfloat16 tensors, whose 8 bits hide the difference, and 'fp32x3' for the others.
+    A matrix with a NaN or an infinity gives NaN, a zero matrix zeros."""
+    _require_any(g, "g", contiguous=False)
+    if g.dim() not in (2, 3):
+        raise RuntimeError("g must have shape [m, n] or [batch, m, n]")
+    dt = _dtype(g.dtype, "g")
+    if out is None:
+        out = torch.empty(g.shape, dtype=g.dtype, device=g.device)
+    else:
+        _require_any(out, "out", dtype=g.dtype, device=g.device)
+        if out.shape != g.shape:
+            raise RuntimeError(f"out must have shape {list(g.shape)}")
+    m = _mode(mode if mode is not None else ("tf32" if dt == _lib.DTYPE_BF16 else "fp32x3"))
+    batch, rows, cols = (1, *g.shape) if g.dim() == 2 else g.shape
+    sb, sr, sc = (0, *g.stride()) if g.dim() == 2 else g.stride()
+    lib = _lib.load()
+    ws_bytes = lib.chebykan_orthogonalize_workspace_bytes(batch, rows, cols, m)
+    _lib.check(ws_bytes, "chebykan_orthogonalize_workspace_bytes")
+    ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=g.device)
+    a, b, c = coefficients
+    with _Range("chebykan.orthogonalize"), torch.cuda.device(g.device):
+        rc = lib.chebykan_orthogonalize(g.data_ptr(), sb, sr, sc, dt, out.data_ptr(), ws.data_ptr(), ws_bytes, batch, rows,
+                                        cols, steps, a, b, c, eps, m, status_tensor(g.device).data_ptr(), _stream(g))
+    _lib.check(rc, "chebykan_orthogonalize")
+    return out
+
+
+def muon_scale(shape, adjust: str = "original") -> float:
+    """Factor on the learning rate for a parameter [in, out, degree+1] (each degree maps `in` inputs to `out` outputs) or
+    a plain matrix [rows, columns]: 'original' sqrt(max(1, rows / columns)), 'match_rms_adamw' 0.2 sqrt(max(rows,
+    columns)), with outputs as rows in the first form."""
+    rows, cols = (shape[1], shape[0]) if len(shape) == 3 else (shape[0], shape[1])
+    if adjust == "original":
+        return max(1.0, rows / cols) ** 0.5
+    if adjust == "match_rms_adamw":
+        return 0.2 * max(rows, cols) ** 0.5
+    raise ValueError(f"adjust must be 'original' or 'match_rms_adamw', got {adjust!r}")
+
+
+def muon_step(param: torch.Tensor, grad: torch.Tensor, momentum_buffer: torch.Tensor, lr: float, weight_decay: float = 0.1,
+              momentum: float = 0.95, nesterov: bool = True, coefficients=NS_COEFFICIENTS, eps: float = 1e-7, steps: int = 5,
+              adjust: str = "original", grad_scale: float = 1.0, mode="fp32x3") -> None:
+    """One Muon update in place of coefficients [in, out, degree+1] (every degree's in x out slice is a matrix of its own)
+    or of a matrix [m, n]; `momentum_buffer` has the parameter's shape and starts at zero.  Safe to capture in a CUDA
+    graph.  `mode`: the operands' precision inside the orthogonalisation, as for ``orthogonalize``."""
+    _require(param, "param")
+    if param.dim() not in (2, 3):
+        raise RuntimeError("param must have shape [in, out, degree+1] or [m, n]: use SGD or Adam for vectors")
+    for t, n in ((grad, "grad"), (momentum_buffer, "momentum_buffer")):
+        _require(t, n)
+        if t.shape != param.shape:
+            raise RuntimeError(f"{n} and param shapes differ")
+        if t.device != param.device:
+            raise RuntimeError(f"{n} and param are on different devices")
+    n_in, n_out = param.shape[:2]
+    degree = param.shape[2] - 1 if param.dim() == 3 else 0
+    m = _mode(mode)
+    lib = _lib.load()
+    ws_bytes = lib.chebykan_muon_workspace_bytes(n_in, n_out, degree, m)
+    _lib.check(ws_bytes, "chebykan_muon_workspace_bytes")
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=param.device)
+    a, b, c = coefficients
+    with _Range("chebykan.muon"), torch.cuda.device(param.device):
+        rc = lib.chebykan_muon_step(param.data_ptr(), grad.data_ptr(), momentum_buffer.data_ptr(), ws.data_ptr(), ws_bytes,
+                                    n_in, n_out, degree, lr, weight_decay, momentum, int(bool(nesterov)),
+                                    muon_scale(param.shape, adjust), steps, a, b, c, eps, grad_scale, m,
+                                    status_tensor(param.device).data_ptr(), _stream(param))
+    _lib.check(rc, "chebykan_muon_step")
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# 8-bit forward (inference)
+# ---------------------------------------------------------------------------------------------------------------
+def int8_width(in_dim: int, degree: int) -> int:
+    """Values in a row of 8-bit basis values or coefficients: degrees 1..degree of the inputs, padded to 16."""
+    return degree * (-(-in_dim // 16) * 16)
+
+
+def int8_pack_coeffs(coeffs: torch.Tensor):
+    """coeffs[in, out, degree+1] -> (wq, w_scale, bias): 8-bit coefficients wq[out, degree * in_pad] of the degrees from 1
+    (degree-major, inputs padded with zeros to a multiple of 16), a scale per output, and degree 0 summed over the
+    inputs."""
+    _require(coeffs, "coeffs")
+    if coeffs.dim() != 3:
+        raise RuntimeError("coeffs must have shape [in, out, degree+1]")
+    n_in, n_out, dp1 = coeffs.shape
+    if dp1 < 2:
+        raise RuntimeError("the 8-bit forward needs a degree of at least 1")
+    wq = torch.empty(n_out, int8_width(n_in, dp1 - 1), dtype=torch.int8, device=coeffs.device)
+    w_scale = torch.empty(n_out, dtype=torch.float32, device=coeffs.device)
+    bias = torch.empty(n_out, dtype=torch.float32, device=coeffs.device)
+    with _Range("chebykan.int8_pack"), torch.cuda.device(coeffs.device):
+        rc = _lib.load().chebykan_int8_pack_coeffs(coeffs.data_ptr(), wq.data_ptr(), w_scale.data_ptr(), bias.data_ptr(),
+                                                   n_in, n_out, dp1 - 1, _stream(coeffs))
+    _lib.check(rc, "chebykan_int8_pack_coeffs")
+    return wq, w_scale, bias
+
+
+def int8_basis(x: torch.Tensor, degree: int):
+    """x[B, in] (fp32, bf16 or fp16) -> (q, scale): T_1..T_degree of tanh(x) as 8-bit rows [B, degree * in_pad] in the
+    layout of ``int8_pack_coeffs``, with a scale per row (its largest magnitude over 127)."""
+    _require_any(x, "x")
+    if x.dim() != 2:
+        raise RuntimeError("x must have shape [B, in]")
+    B, n_in = x.shape
+    q = torch.empty(B, int8_width(n_in, max(degree, 0)), dtype=torch.int8, device=x.device)
+    scale = torch.empty(B, dtype=torch.float32, device=x.device)
+    with _Range("chebykan.int8_basis"), torch.cuda.device(x.device):
+        rc = _lib.load().chebykan_int8_basis(x.data_ptr(), _dtype(x.dtype, "x"), q.data_ptr(), scale.data_ptr(), B, n_in,
+                                             degree, _stream(x))
+    _lib.check(rc, "chebykan_int8_basis")
+    return q, scale
+
+
+def _require_int8(t: torch.Tensor, name: str, device=None) -> None:
+    """int8 matrix on the GPU with adjacent columns; rows may be any distance apart."""
+    _require_any(t, name, dtype=torch.int8, device=device, contiguous=False)
+    if t.dim() != 2:
+        raise RuntimeError(f"{name} must be a matrix")
+    if t.numel() and ((t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1])):
+        raise RuntimeError(f"the rows of {name} must be contiguous and may not overlap")
+    if t.numel() and t.data_ptr() % 16 != 0:
+        raise RuntimeError(f"{name} must be 16-byte aligned")
+
+
+def int8_matmul(q: torch.Tensor, q_scale: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor,
+                bias: torch.Tensor | None = None, out_dtype=torch.float32, out: torch.Tensor | None = None) -> torch.Tensor:
+    """y[M, N] = (q[M, K] wq[N, K]^T) * q_scale[M] * w_scale[N] + bias[N] for int8 matrices; the integer sums are exact
+    (K up to 131071).  Row strides that are multiples of 16 bytes are read in place, others through a padded copy."""
+    _require_int8(q, "q")
+    _require_int8(wq, "wq", q.device)
+    M, K = q.shape
+    N = wq.shape[0]
+    if wq.shape[1] != K:
+        raise RuntimeError(f"q has {K} columns, wq {wq.shape[1]}")
+    for t, n, size in ((q_scale, "q_scale", M), (w_scale, "w_scale", N), (bias, "bias", N)):
+        if t is None and n == "bias":
+            continue
+        _require_any(t, n, dtype=torch.float32, device=q.device)
+        if t.numel() != size:
+            raise RuntimeError(f"{n} must have {size} elements")
+    if out is None:
+        out = torch.empty(M, N, dtype=out_dtype, device=q.device)
+    else:
+        _require_any(out, "out", device=q.device)
+        if out.shape != (M, N):
+            raise RuntimeError(f"out must have shape [{M}, {N}]")
+    dt = _dtype(out.dtype, "out")
+    ldq = q.stride(0) if M > 1 else max(K, 1)
+    ldw = wq.stride(0) if N > 1 else max(K, 1)
+    lib = _lib.load()
+    ws_bytes = lib.chebykan_int8_matmul_workspace_bytes(M, N, K, ldq, ldw)
+    _lib.check(ws_bytes, "chebykan_int8_matmul_workspace_bytes")
+    ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=q.device)
+    with _Range("chebykan.int8_matmul"), torch.cuda.device(q.device):
+        rc = lib.chebykan_int8_matmul(q.data_ptr(), ldq, q_scale.data_ptr(), wq.data_ptr(), ldw, w_scale.data_ptr(),
+                                      bias.data_ptr() if bias is not None else None, out.data_ptr(), dt, ws.data_ptr(),
+                                      ws_bytes, M, N, K, status_tensor(q.device).data_ptr(), _stream(q))
+    _lib.check(rc, "chebykan_int8_matmul")
+    return out
+
+
+def int8_forward(x: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor, bias: torch.Tensor | None, degree: int,
+                 out_dtype=torch.float32, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Forward of a Chebyshev layer from coefficients packed by ``int8_pack_coeffs``: y[B, out] of `out_dtype` from x[B, in]
+    (fp32, bf16 or fp16).  ``int8_basis`` followed by ``int8_matmul`` in one call."""
+    _require_any(x, "x")
+    if x.dim() != 2:
+        raise RuntimeError("x must have shape [B, in]")
+    B, n_in = x.shape
+    _require_any(wq, "wq", dtype=torch.int8, device=x.device)
+    if wq.dim() != 2 or wq.shape[1] != int8_width(n_in, degree):
+        raise RuntimeError(f"wq must have shape [out, {int8_width(n_in, degree)}] for {n_in} inputs and degree {degree}")
+    N = wq.shape[0]
+    for t, n in ((w_scale, "w_scale"), (bias, "bias")):
+        if t is None and n == "bias":
+            continue
+        _require_any(t, n, dtype=torch.float32, device=x.device)
+        if t.numel() != N:
+            raise RuntimeError(f"{n} must have {N} elements")
+    if out is None:
+        out = torch.empty(B, N, dtype=out_dtype, device=x.device)
+    else:
+        _require_any(out, "out", device=x.device)
+        if out.shape != (B, N):
+            raise RuntimeError(f"out must have shape [{B}, {N}]")
+    lib = _lib.load()
+    ws_bytes = lib.chebykan_int8_fwd_workspace_bytes(B, n_in, N, degree)
+    _lib.check(ws_bytes, "chebykan_int8_fwd_workspace_bytes")
+    ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=x.device)
+    with _Range("chebykan.int8_forward"), torch.cuda.device(x.device):
+        rc = lib.chebykan_int8_fwd(x.data_ptr(), _dtype(x.dtype, "x"), wq.data_ptr(), w_scale.data_ptr(),
+                                   bias.data_ptr() if bias is not None else None, out.data_ptr(), _dtype(out.dtype, "out"),
+                                   ws.data_ptr(), ws_bytes, B, n_in, N, degree, status_tensor(x.device).data_ptr(), _stream(x))
+    _lib.check(rc, "chebykan_int8_fwd")
+    return out
+
+
 def forward_host(x_host: torch.Tensor, coeffs_host: torch.Tensor, mode, scratch: torch.Tensor | None = None,
                  out: torch.Tensor | None = None):
     """Forward with HOST tensors through chebykan_fwd_host; returns (y_host, scratch).

@@ -1,4 +1,4 @@
-"""SGD and Adam whose updates run in the library's CUDA kernels.
+"""SGD, Adam and Muon whose updates run in the library's CUDA kernels.
 
 Stand in for ``torch.optim.SGD(params, lr)`` and ``torch.optim.Adam(params,
 lr)`` as the reference's training loop uses them (README.md:59-66): no
@@ -6,6 +6,10 @@ momentum / weight decay for SGD; Adam with betas (0.9, 0.999), eps 1e-8, bias
 correction, no weight decay, no amsgrad.  Works on any contiguous fp32 CUDA
 parameter (ChebyKAN coefficients, LayerNorm weights, ...).  ``grad_scale``
 multiplies every gradient first (1/world_size after a sum all-reduce).
+
+``Muon`` stands in for ``torch.optim.Muon`` in the same way (same arguments and
+defaults) and also takes coefficient tensors [in, out, degree+1], whose degree
+slices are orthogonalised as matrices of their own.
 """
 from __future__ import annotations
 
@@ -101,5 +105,51 @@ class Adam(_Base):
                 st["step"] += 1
                 ops.adam_step(p.data, p.grad.contiguous(), st["exp_avg"], st["exp_avg_sq"], st["step"], self.lr,
                               self.betas[0], self.betas[1], self.eps, self.grad_scale)
+            _bump(p)
+        self._after_step()
+
+
+class Muon(_Base):
+    """Momentum, then Newton-Schulz orthogonalisation of the update, then a decayed step (``ops.muon_step``).
+
+    For matrices [m, n] and coefficient tensors [in, out, degree+1]; give vectors (LayerNorm weights, biases) to SGD or
+    Adam.  ``math_mode`` is the precision inside the orthogonalisation: 'fp32x3' (fp32 results) or 'tf32' (operands of
+    11 significant bits, a third of the products).  Keeps no host-side state: steps can be captured in a CUDA graph."""
+
+    def __init__(self, params, lr: float = 1e-3, weight_decay: float = 0.1, momentum: float = 0.95, nesterov: bool = True,
+                 ns_coefficients=ops.NS_COEFFICIENTS, eps: float = 1e-7, ns_steps: int = 5, adjust_lr_fn: str | None = None,
+                 *, math_mode: str = "fp32x3"):
+        params = list(params)
+        for p in params:
+            if p.dim() not in (2, 3):
+                raise ValueError("Muon takes matrices and coefficient tensors [in, out, degree+1]; give parameters of "
+                                 f"shape {list(p.shape)} to SGD or Adam")
+            if p.numel() == 0:
+                raise ValueError("Muon got an empty parameter")
+        if math_mode not in ("fp32x3", "tf32"):
+            raise ValueError("math_mode must be 'fp32x3' or 'tf32'")
+        if not 0.0 <= momentum < 1.0:
+            raise ValueError("momentum must be in [0, 1)")
+        super().__init__(params, lr)
+        self.weight_decay = float(weight_decay)
+        self.momentum = float(momentum)
+        self.nesterov = bool(nesterov)
+        self.ns_coefficients = tuple(float(v) for v in ns_coefficients)
+        self.eps = float(eps)
+        self.ns_steps = int(ns_steps)
+        self.adjust_lr_fn = adjust_lr_fn or "original"
+        self.math_mode = math_mode
+        for p in params:
+            ops.muon_scale(p.shape, self.adjust_lr_fn)       # refuses an unknown rule here, not in the first step
+        self.state = {p: {"momentum_buffer": torch.zeros_like(p)} for p in params}
+
+    @torch.no_grad()
+    def step(self) -> None:
+        for p in self.params:
+            if p.grad is None:
+                continue
+            ops.muon_step(p.data, p.grad.contiguous(), self.state[p]["momentum_buffer"], self.lr, self.weight_decay,
+                          self.momentum, self.nesterov, self.ns_coefficients, self.eps, self.ns_steps, self.adjust_lr_fn,
+                          self.grad_scale, self.math_mode)
             _bump(p)
         self._after_step()
