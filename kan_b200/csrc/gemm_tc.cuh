@@ -1,0 +1,407 @@
+// D[M][N] = L[M][K] R on tcgen05, for 16-bit floating and 8-bit integer operands: the pipeline shared by the products of
+// the Newton-Schulz steps and of the 8-bit forward.  What happens to the accumulator is the epilogue's, a template argument.
+//
+//   warp 0     TMA: one stage = 128 bytes of K of the tile's L rows (128 per CTA) and of R, 128-byte swizzle, no multicast.
+//              R is either [N][K] (K-major) or [K][N] (boxes of 64 K rows x 64 columns, read through an MN-major descriptor)
+//   warp 1     MMA: one elected lane issues tcgen05.mma and the commits that free stages and publish accumulators
+//   warps 2-5  epilogue: tcgen05.ld, then the epilogue's emit() on 32 columns of a row at a time
+//
+// CG = 2: a pair of CTAs works on 256 rows with cta_group::2, each staging its own 128 rows of L and half of R's columns,
+// which halves R's traffic out of L2 and the shared-memory reads per MMA.  The even CTA's thread issues the MMAs.
+// PP = 3: both operands come as two fp16 planes (head and tail) and three products are summed: head x head in one
+// accumulator, head x tail and tail x head in another, each over KCHUNK K blocks only.  The tensor pipe's fp32 sums
+// truncate, by about 2^-26 of the accumulator per MMA: short sums of their own, added up in registers by the epilogue
+// warps with round-to-nearest, keep the result at fp32 quality.
+// Two accumulator buffers alternate, so an epilogue (or a chunk's addition) overlaps the next MMAs.
+// Every wait is bounded (see tc_common.cuh).
+#pragma once
+#include "tc_common.cuh"
+
+namespace chebykan {
+namespace gemm {
+using namespace tc;
+
+enum Kind { F16 = 0, I8 = 1 };
+
+template <Kind KIND_, int PP_, int CG_, int BN_, bool RMN_>
+struct Config {
+    static constexpr Kind KIND = KIND_;
+    static constexpr int PP = PP_, CG = CG_, BN = BN_;
+    static constexpr bool RMN = RMN_;
+    static constexpr int PLANES = PP == 3 ? 2 : 1;
+    static constexpr int BM = 128 * CG;                        // rows of a tile
+    static constexpr int KE = KIND == I8 ? 128 : 64;           // K elements per stage (128 bytes)
+    static constexpr int L_PANEL = 128 * 128, R_PANEL = BN / CG * 128;
+    static constexpr int STAGE = PLANES * (L_PANEL + R_PANEL);
+    static constexpr int STAGES = (200 * 1024) / STAGE > 8 ? 8 : (200 * 1024) / STAGE;
+    static constexpr int KCHUNK = PP == 3 ? 4 : (1 << 30);
+    static constexpr int ACC_COLS = PP == 3 ? 2 * BN : BN;     // columns of one accumulator buffer
+    static constexpr int TMEM_COLS = 2 * ACC_COLS;
+    static constexpr int BARS = 2 * STAGES + 5;
+    static constexpr int BAR_OFFSET = STAGES * STAGE;
+    static constexpr int SMEM = BAR_OFFSET + BARS * 8 + 16 + 1024;
+    static constexpr uint32_t IDESC = KIND == I8
+        ? (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24)
+        : (1u << 4) | ((RMN ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+    static_assert(TMEM_COLS <= 512 && (TMEM_COLS & (TMEM_COLS - 1)) == 0, "accumulators must fit tensor memory");
+    static_assert(KIND == F16 || (PP == 1 && !RMN), "integer products have one plane and K-major operands");
+};
+constexpr int THREADS = 192;
+enum { ST_LOAD = 21, ST_MMA = 22, ST_MMA_ACC = 23, ST_EPILOGUE = 24 };
+
+struct Tiles {
+    int M, N;
+    int nkb;              // K blocks of a tile
+    int ntm, ntn;         // tile rows and columns
+    int per_batch;        // tiles of one matrix
+    int sym;              // only tiles that reach the diagonal or lie above it
+    int64_t total;
+};
+
+// position of tile t: matrix b, first row, first column
+template <int BM, int BN>
+__device__ __forceinline__ void decode(const Tiles& g, int64_t t, int& b, int& m0, int& n0) {
+    b = (int)(t / g.per_batch);
+    int r = (int)(t - (int64_t)b * g.per_batch);
+    if (!g.sym) {
+        m0 = r / g.ntn * BM;
+        n0 = r % g.ntn * BN;
+        return;
+    }
+    int tm = 0;
+    for (;; ++tm) {
+        const int first = tm * BM / BN, count = g.ntn - first;
+        if (r < count) { m0 = tm * BM; n0 = (first + r) * BN; return; }
+        r -= count;
+    }
+}
+inline int sym_tiles(int ntm, int ntn, int bm, int bn) {
+    int n = 0;
+    for (int tm = 0; tm < ntm; ++tm) n += ntn - tm * bm / bn;
+    return n;
+}
+
+template <Kind KIND, int CG>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    if constexpr (KIND == F16) {
+        if constexpr (CG == 2) umma2<CHEBYKAN_MODE_BF16>(d, a, b, idesc, accumulate);
+        else umma<CHEBYKAN_MODE_BF16>(d, a, b, idesc, accumulate);
+    } else if constexpr (CG == 2) {
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                     "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+    } else {
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                     "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+    }
+}
+__device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void load_3d_pair(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar) : "memory");
+}
+// operand of [K][N] boxes: 64 columns per 128-byte row, rows are K; 8-row groups 1024 bytes apart, the next 64 columns
+// one box (64 rows, 8192 bytes) further
+__device__ __forceinline__ uint64_t mn_desc(uint32_t addr) {
+    return (make_smem_desc(addr) & ~((uint64_t)0x3fff << 16)) | ((uint64_t)(8192 >> 4) << 16);
+}
+
+template <class C, class Epi>
+__global__ void __launch_bounds__(THREADS, 1)
+gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ CUtensorMap map_r, const Tiles g,
+            const typename Epi::Args args, int32_t* status) {
+    constexpr int CG = C::CG, BN = C::BN, S = C::STAGES, PLANES = C::PLANES;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+    const uint32_t bars = base + C::BAR_OFFSET;
+    auto full = [&](int s) { return bars + 8u * s; };
+    auto empty = [&](int s) { return bars + 8u * (S + s); };
+    auto acc_full = [&](int a) { return bars + 8u * (2 * S + a); };
+    auto acc_empty = [&](int a) { return bars + 8u * (2 * S + 2 + a); };
+    const uint32_t drain = bars + 8u * (2 * S + 4);
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + C::BAR_OFFSET + C::BARS * 8);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + C::BAR_OFFSET + C::BARS * 8 + 4);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = CG == 2 ? cluster_ctarank() : 0u;
+    const int64_t unit = blockIdx.x / CG, units = gridDim.x / CG;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
+        for (int a = 0; a < 2; ++a) { mbar_init(acc_full(a), 1); mbar_init(acc_empty(a), 128 * CG); }
+        mbar_init(drain, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        if (CG == 2) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
+                         ::"r"(smem_u32((const void*)tmem_slot)), "r"((uint32_t)C::TMEM_COLS) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                         ::"r"(smem_u32((const void*)tmem_slot)), "r"((uint32_t)C::TMEM_COLS) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (CG == 2) cluster_sync_all();      // the peer's barriers exist before anything arrives on them
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int s = 0; uint32_t ph = 0;
+            bool alive = true;
+            for (int64_t t = unit; t < g.total && alive; t += units) {
+                int b, m0, n0;
+                decode<C::BM, BN>(g, t, b, m0, n0);
+                const int row = m0 + (int)rank * 128, col = n0 + (int)rank * (BN / CG);
+                for (int kb = 0; kb < g.nkb; ++kb) {
+                    if (!mbar_wait(empty(s), ph ^ 1u, abort_flag, status, ST_LOAD)) { alive = false; break; }
+                    const uint32_t dst = base + s * C::STAGE;
+                    uint32_t bar = full(s);
+                    if (rank == 0) mbar_arrive_expect_tx(bar, (uint32_t)(C::STAGE * CG));
+                    if (CG == 2) bar = mapa_cluster(bar, 0);
+                    auto load = [&](uint32_t to, const CUtensorMap* map, int c0, int c1, int z) {
+                        if (CG == 2) load_3d_pair(to, map, c0, c1, z, bar);
+                        else load_3d(to, map, c0, c1, z, bar);
+                    };
+#pragma unroll
+                    for (int p = 0; p < PLANES; ++p) {
+                        const int z = b * PLANES + p;
+                        load(dst + p * C::L_PANEL, &map_l, kb * C::KE, row, z);
+                        const uint32_t rd = dst + PLANES * C::L_PANEL + p * C::R_PANEL;
+                        if (C::RMN) {
+#pragma unroll
+                            for (int q = 0; q < BN / CG / 64; ++q) load(rd + q * 8192, &map_r, col + q * 64, kb * C::KE, z);
+                        } else {
+                            load(rd, &map_r, kb * C::KE, col, z);
+                        }
+                    }
+                    if (++s == S) { s = 0; ph ^= 1u; }
+                }
+            }
+            if (!alive) {
+                // let the copies already issued land before the CTA gives up its shared memory
+                const uint64_t t0 = globaltimer_ns();
+                while (globaltimer_ns() - t0 < 200000ull) { }
+            }
+        }
+    } else if (warp == 1) {
+        if (rank == 0) {
+            const bool elected = elect_one_sync();
+            int s = 0; uint32_t ph = 0;
+            int acc = 0; uint32_t acc_ph = 0;
+            bool alive = true;
+            const uint64_t l_desc = make_smem_desc(base);
+            const uint64_t r_desc = C::RMN ? mn_desc(base + PLANES * C::L_PANEL) : make_smem_desc(base + PLANES * C::L_PANEL);
+            const uint32_t l_hi = (uint32_t)(l_desc >> 32), r_hi = (uint32_t)(r_desc >> 32);
+            constexpr uint32_t L_TAIL = C::L_PANEL >> 4, R_TAIL = C::R_PANEL >> 4;
+            constexpr uint32_t R_STEP = C::RMN ? 2048 >> 4 : 32 >> 4;      // 16 rows of K, or 32 bytes of a row
+            for (int64_t t = unit; t < g.total && alive; t += units)
+                for (int kb0 = 0; kb0 < g.nkb && alive; kb0 += C::KCHUNK) {
+                    const int kb1 = g.nkb - kb0 < C::KCHUNK ? g.nkb : kb0 + C::KCHUNK;
+                    if (!__all_sync(0xffffffffu, mbar_wait(acc_empty(acc), acc_ph ^ 1u, abort_flag, status, ST_MMA_ACC))) { alive = false; break; }
+                    tc_fence_after();
+                    const uint32_t d = tmem + (uint32_t)(acc * C::ACC_COLS);
+                    for (int kb = kb0; kb < kb1; ++kb) {
+                        if (!__all_sync(0xffffffffu, mbar_wait(full(s), ph, abort_flag, status, ST_MMA))) { alive = false; break; }
+                        tc_fence_after();
+                        const uint32_t off = (uint32_t)((s * C::STAGE) >> 4);
+                        const uint32_t l_lo = (uint32_t)l_desc + off, r_lo = (uint32_t)r_desc + off;
+                        const uint32_t later = (uint32_t)(kb != kb0);
+                        if (elected) {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const uint32_t la = l_lo + 2u * k, ra = r_lo + R_STEP * k;
+                                mma<C::KIND, CG>(d, desc_from_words(la, l_hi), desc_from_words(ra, r_hi), C::IDESC, k ? 1u : later);
+                                if constexpr (C::PP == 3) {
+                                    mma<C::KIND, CG>(d + BN, desc_from_words(la, l_hi), desc_from_words(ra + R_TAIL, r_hi), C::IDESC, k ? 1u : later);
+                                    mma<C::KIND, CG>(d + BN, desc_from_words(la + L_TAIL, l_hi), desc_from_words(ra, r_hi), C::IDESC, 1u);
+                                }
+                            }
+                            if (CG == 2) umma2_commit_both(empty(s)); else umma_commit(empty(s));
+                        }
+                        __syncwarp();
+                        if (++s == S) { s = 0; ph ^= 1u; }
+                    }
+                    if (alive && elected) { if (CG == 2) umma2_commit_both(acc_full(acc)); else umma_commit(acc_full(acc)); }
+                    __syncwarp();
+                    acc ^= 1;
+                    if (acc == 0) acc_ph ^= 1u;
+                }
+            if (!alive && elected) {
+                // wait (bounded) until the MMAs already issued have retired
+                if (CG == 2) umma2_commit(drain); else umma_commit(drain);
+                const uint64_t t0 = globaltimer_ns();
+                while (!mbar_try_wait(drain, 0) && globaltimer_ns() - t0 < 10000000ull) { }
+            }
+            __syncwarp();
+        }
+    } else {
+        const int q = warp & 3;               // quarter of the tensor memory's lanes that this warp may read
+        int acc = 0; uint32_t acc_ph = 0;
+        bool alive = true;
+        auto release = [&](int a) {
+            tc_fence_before();
+            if (CG == 2 && rank != 0) mbar_arrive_cluster(mapa_cluster(acc_empty(a), 0));
+            else mbar_arrive(acc_empty(a));
+        };
+        for (int64_t t = unit; t < g.total && alive; t += units) {
+            int b, m0, n0;
+            decode<C::BM, BN>(g, t, b, m0, n0);
+            const int row = m0 + (int)rank * 128 + q * 32 + lane;
+            // symmetric results: the warp's 32 x 32 block also goes to its transposed place where no tile computes that
+            auto mirrored = [&](int col0) {
+                return g.sym && (row / BN + 1) * BN <= col0 / C::BM * C::BM;
+            };
+            int ncols = g.N - n0;
+            if (ncols > BN) ncols = BN;
+            const int nch = (ncols + 31) >> 5;
+            if constexpr (C::PP == 3) {
+                float v[BN];
+                for (int kb0 = 0; kb0 < g.nkb; kb0 += C::KCHUNK) {
+                    const bool ok = mbar_wait(acc_full(acc), acc_ph, abort_flag, status, ST_EPILOGUE);
+                    if (!__all_sync(0xffffffffu, ok)) { alive = false; break; }
+                    tc_fence_after();
+                    const uint32_t ta = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * C::ACC_COLS);
+#pragma unroll
+                    for (int c = 0; c < BN / 32; ++c)
+                        if (c < nch) {
+                            uint32_t r0[32], r1[32];
+                            tmem_ld32(ta + c * 32, r0);
+                            tmem_ld32(ta + BN + c * 32, r1);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) {
+                                const float part = __uint_as_float(r0[e]) + __uint_as_float(r1[e]);
+                                v[c * 32 + e] = kb0 == 0 ? part : v[c * 32 + e] + part;
+                            }
+                        }
+                    release(acc);
+                    acc ^= 1;
+                    if (acc == 0) acc_ph ^= 1u;
+                }
+                if (!alive) break;
+#pragma unroll
+                for (int c = 0; c < BN / 32; ++c)
+                    if (c < nch) {
+                        uint32_t r[32];
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(v[c * 32 + e]);
+                        Epi::emit(args, g, b, row, n0 + c * 32, r, mirrored(n0 + c * 32));
+                    }
+            } else {
+                const bool ok = mbar_wait(acc_full(acc), acc_ph, abort_flag, status, ST_EPILOGUE);
+                if (!__all_sync(0xffffffffu, ok)) { alive = false; break; }
+                tc_fence_after();
+                const uint32_t ta = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * C::ACC_COLS);
+                // two register buffers: the load of the next 32 columns is in flight while these are written
+                uint32_t ra[32], rb[32];
+                tmem_ld32(ta, ra);
+#pragma unroll 1
+                for (int c = 0; c < nch; c += 2) {
+                    tmem_ld_wait();
+                    if (c + 1 < nch) tmem_ld32(ta + (c + 1) * 32, rb); else release(acc);
+                    Epi::emit(args, g, b, row, n0 + c * 32, ra, mirrored(n0 + c * 32));
+                    if (c + 1 < nch) {
+                        tmem_ld_wait();
+                        if (c + 2 < nch) tmem_ld32(ta + (c + 2) * 32, ra); else release(acc);
+                        Epi::emit(args, g, b, row, n0 + (c + 1) * 32, rb, mirrored(n0 + (c + 1) * 32));
+                    }
+                }
+                acc ^= 1;
+                if (acc == 0) acc_ph ^= 1u;
+            }
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    // neither CTA of a pair leaves (or frees tensor memory) while the other may still arrive on its barriers
+    if (CG == 2) cluster_sync_all();
+    if (warp == 1) {
+        tc_fence_after();
+        if (CG == 2)
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)C::TMEM_COLS) : "memory");
+        else
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)C::TMEM_COLS) : "memory");
+    }
+}
+
+// map of `slabs` row-major matrices [rows][cols], rows pitch_bytes and matrices slab_bytes apart, read in boxes of
+// box_cols x box_rows with 128-byte swizzle; what lies outside a matrix reads as zero
+inline int make_map(CUtensorMap* map, Kind kind, const void* base, int64_t cols, int64_t rows, int64_t slabs, int64_t pitch_bytes,
+                    int64_t slab_bytes, int box_cols, int box_rows) {
+    EncodeTiledFn encode = get_encode_fn();
+    if (!encode) return CHEBYKAN_ECUDA;
+    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)slabs};
+    const cuuint64_t strides[2] = {(cuuint64_t)pitch_bytes, (cuuint64_t)slab_bytes};
+    const cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1};
+    const cuuint32_t one[3] = {1, 1, 1};
+    const CUresult r = encode(map, kind == I8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                              const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) { set_last_cuda_error((int)r); return CHEBYKAN_ECUDA; }
+    return CHEBYKAN_OK;
+}
+
+template <class C>
+Tiles tiles_of(int M, int N, int K, int batch, bool sym) {
+    Tiles g;
+    g.M = M; g.N = N;
+    g.nkb = (int)ceil_div(K, C::KE);
+    g.ntm = (int)ceil_div(M, C::BM);
+    g.ntn = (int)ceil_div(N, C::BN);
+    g.sym = sym;
+    g.per_batch = sym ? sym_tiles(g.ntm, g.ntn, C::BM, C::BN) : g.ntm * g.ntn;
+    g.total = (int64_t)g.per_batch * batch;
+    return g;
+}
+
+// persistent launch, one CTA (or pair) per SM (or two)
+template <class C, class Epi>
+int launch(const CUtensorMap& map_l, const CUtensorMap& map_r, const Tiles& g, const typename Epi::Args& args, int32_t* status,
+           cudaStream_t s) {
+    static int max_units[64] = {0};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) return CHEBYKAN_EINVAL;
+    auto kernel = gemm_kernel<C, Epi>;
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = C::SMEM; cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = C::CG; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr; cfg.numAttrs = 1;
+    if (max_units[dev] == 0) {
+        int rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+        if (rc) return rc;
+        int sms = 148, n = 0;
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+        n = sms / C::CG;
+        if (C::CG == 2) {
+            cfg.gridDim = dim3((unsigned)(sms & ~1));
+            int clusters = 0;
+            if ((rc = check_cuda(cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg)))) return rc;
+            if (clusters < 1) return CHEBYKAN_ECUDA;
+            if (clusters < n) n = clusters;
+        }
+        max_units[dev] = n;
+    }
+    const int64_t units = g.total < max_units[dev] ? g.total : max_units[dev];
+    cfg.gridDim = dim3((unsigned)(units * C::CG));
+    return check_cuda(cudaLaunchKernelEx(&cfg, kernel, map_l, map_r, g, args, status));
+}
+
+}  // namespace gemm
+}  // namespace chebykan

@@ -1,109 +1,140 @@
-// The three products of a Newton-Schulz step (see newton_schulz.cuh for the operands' layout).
+// The three products of a Newton-Schulz step on tcgen05 (gemm_tc.cuh; see newton_schulz.cuh for the operands' layout):
+//   A = X X^T            both operands are X's rows; symmetric
+//   P = a I + b A + c A A      both operands are A's rows (A is symmetric); symmetric
+//   X' = P X             P's rows against X as it lies, [K][N]: no transposed copy of X exists
+// The symmetric two compute the tiles on and above the diagonal and write each block to both places.
+#include "gemm_tc.cuh"
 #include "newton_schulz.cuh"
 
 namespace chebykan {
 namespace ns {
 namespace {
+using gemm::Tiles;
 
 enum { GRAM = 0, POLY = 1, APPLY = 2 };
-constexpr int T = 64, KT = 16;
 
-struct Args {
-    const __half* left;       // [M][K] planes
-    const __half* right;      // GRAM, POLY: [N][K] planes; APPLY: [K][N] planes
-    __half* out;              // planes [M][N], or null
-    float* out32;             // fp32 [M][N] (APPLY's last step)
+struct EpiArgs {
+    const __half* a;          // POLY: A's planes
+    __half* out;              // planes, or null (APPLY's last step)
+    float* out32;             // [batch][M][N]
     const float *alpha, *alpha_next;
-    int M, N, K, pitch_l, pitch_r, pitch_o, planes;
-    int64_t slab_l, slab_r, slab_o;
+    int pitch;                // of out (and of a)
+    int64_t slab;
     float ca, cb, cc;
 };
 
-__device__ __forceinline__ float value(const __half* p, int64_t slab, int planes) {
-    float v = __half2float(p[0]);
-    if (planes == 2) v += __half2float(p[slab]);
-    return v;
+__device__ __forceinline__ uint32_t pack2(__half x, __half y) {
+    return (uint32_t)__half_as_ushort(x) | ((uint32_t)__half_as_ushort(y) << 16);
 }
 
-// 64 x 64 outputs per block, 4 x 4 per thread, fp32 on the CUDA cores
-template <int KIND>
-__global__ void __launch_bounds__(256) product_kernel(const Args p) {
-    __shared__ float sl[KT][T + 1], sr[KT][T + 1];
-    const int b = blockIdx.z, m0 = blockIdx.y * T, n0 = blockIdx.x * T;
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const __half* left = p.left + (int64_t)b * p.planes * p.slab_l;
-    const __half* right = p.right + (int64_t)b * p.planes * p.slab_r;
-    float acc[4][4] = {};
-    for (int k0 = 0; k0 < p.K; k0 += KT) {
-        for (int e = threadIdx.x; e < T * KT; e += 256) {
-            const int k = e % KT, r = e / KT;
-            const bool okk = k0 + k < p.K;
-            sl[k][r] = (okk && m0 + r < p.M) ? value(left + (int64_t)(m0 + r) * p.pitch_l + k0 + k, p.slab_l, p.planes) : 0.f;
-            if (KIND != APPLY)
-                sr[k][r] = (okk && n0 + r < p.N) ? value(right + (int64_t)(n0 + r) * p.pitch_r + k0 + k, p.slab_r, p.planes) : 0.f;
-        }
-        if (KIND == APPLY)
-            for (int e = threadIdx.x; e < T * KT; e += 256) {
-                const int r = e % T, k = e / T;
-                sr[k][r] = (k0 + k < p.K && n0 + r < p.N)
-                               ? value(right + (int64_t)(k0 + k) * p.pitch_r + n0 + r, p.slab_r, p.planes) : 0.f;
+template <int KIND, int PLANES>
+struct Epilogue {
+    using Args = EpiArgs;
+    // 32 consecutive columns of one row
+    static __device__ __forceinline__ void emit(const Args& p, const Tiles& g, int b, int row, int col0, uint32_t (&r)[32], bool mirror) {
+        const int64_t slab0 = (int64_t)b * PLANES * p.slab;
+        float factor;
+        if (KIND == GRAM) { const float al = p.alpha[b]; factor = al * al * exp2f((float)A_EXP); }
+        else if (KIND == POLY) factor = p.cc * exp2f(-2.f * A_EXP + P_EXP);
+        else factor = exp2f(-(float)P_EXP) * p.alpha[b] / (p.out ? p.alpha_next[b] : 1.f);
+        if (row >= g.M) return;
+        if (KIND == APPLY && p.out == nullptr) {
+            float* dst = p.out32 + ((int64_t)b * g.M + row) * g.N + col0;
+            if ((g.N & 3) == 0) {
+#pragma unroll
+                for (int e = 0; e < 32; e += 4)
+                    if (col0 + e < g.N)
+                        *reinterpret_cast<float4*>(dst + e) = make_float4(__uint_as_float(r[e]) * factor, __uint_as_float(r[e + 1]) * factor,
+                                                                          __uint_as_float(r[e + 2]) * factor, __uint_as_float(r[e + 3]) * factor);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                    if (col0 + e < g.N) dst[e] = __uint_as_float(r[e]) * factor;
             }
-        __syncthreads();
+            return;
+        }
+        const int64_t at = slab0 + (int64_t)row * p.pitch + col0;
+        // eight columns (16 bytes of a plane) at a time; a row's last group may run into its padding, which nothing reads
 #pragma unroll
-        for (int k = 0; k < KT; ++k)
+        for (int c = 0; c < 32; c += 8) {
+            if (col0 + c >= g.N) break;
+            __half hi[8], lo[8];
+            uint4 ah, al;
+            if (KIND == POLY) {
+                ah = *reinterpret_cast<const uint4*>(p.a + at + c);
+                if (PLANES == 2) al = *reinterpret_cast<const uint4*>(p.a + at + c + p.slab);
+            }
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int e = 0; e < 8; ++e) {
+                float v = __uint_as_float(r[c + e]) * factor;
+                if (KIND == POLY) {
+                    float a = __half2float(reinterpret_cast<const __half*>(&ah)[e]);
+                    if (PLANES == 2) a += __half2float(reinterpret_cast<const __half*>(&al)[e]);
+                    v = fmaf(p.cb * exp2f((float)(P_EXP - A_EXP)), a, v);
+                    if (col0 + c + e == row) v += p.ca * exp2f((float)P_EXP);
+                }
+                split_half(v, hi[e], lo[e]);
+            }
+            *reinterpret_cast<uint4*>(p.out + at + c) = make_uint4(pack2(hi[0], hi[1]), pack2(hi[2], hi[3]), pack2(hi[4], hi[5]), pack2(hi[6], hi[7]));
+            if (PLANES == 2)
+                *reinterpret_cast<uint4*>(p.out + at + c + p.slab) = make_uint4(pack2(lo[0], lo[1]), pack2(lo[2], lo[3]), pack2(lo[4], lo[5]), pack2(lo[6], lo[7]));
+            if (KIND != APPLY && mirror) {
+                // the warp's lanes hold consecutive rows: 64 bytes of one row of the transposed block
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sl[k][ty * 4 + i], sr[k][tx * 4 + j], acc[i][j]);
-        __syncthreads();
+                for (int e = 0; e < 8; ++e)
+                    if (col0 + c + e < g.N) {
+                        const int64_t to = slab0 + (int64_t)(col0 + c + e) * p.pitch + row;
+                        p.out[to] = hi[e];
+                        if (PLANES == 2) p.out[to + p.slab] = lo[e];
+                    }
+            }
+        }
     }
-    const float al = p.alpha ? p.alpha[b] : 1.f;
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const int m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-            if (m >= p.M || n >= p.N) continue;
-            const int64_t at = (int64_t)b * p.planes * p.slab_o + (int64_t)m * p.pitch_o + n;
-            float v;
-            if (KIND == GRAM) v = acc[i][j] * al * al * exp2f((float)A_EXP);
-            else if (KIND == POLY) {
-                const float av = value(p.left + (int64_t)b * p.planes * p.slab_l + (int64_t)m * p.pitch_l + n, p.slab_l, p.planes) * exp2f(-(float)A_EXP);
-                v = fmaf(p.cc, acc[i][j] * exp2f(-2.f * A_EXP), p.cb * av);
-                if (m == n) v += p.ca;
-                v *= exp2f((float)P_EXP);
-            } else v = acc[i][j] * exp2f(-(float)P_EXP) * al;
-            if (KIND == APPLY && p.out == nullptr) {
-                p.out32[((int64_t)b * p.M + m) * p.N + n] = v;
-                continue;
-            }
-            if (KIND == APPLY) v /= p.alpha_next[b];
-            __half hi, lo;
-            split_half(v, hi, lo);
-            p.out[at] = hi;
-            if (p.planes == 2) p.out[at + p.slab_o] = lo;
-        }
+};
+
+template <int KIND, int PP, int CG>
+int run(const __half* left, const __half* right, int M, int N, int K, int pitch_l, int pitch_r, int64_t slab_l, int64_t slab_r, int batch,
+        const EpiArgs& args, int32_t* status, cudaStream_t s) {
+    using C = gemm::Config<gemm::F16, PP, CG, PP == 3 ? 128 : 256, KIND == APPLY>;
+    CUtensorMap ml, mr;
+    int rc = gemm::make_map(&ml, gemm::F16, left, K, M, (int64_t)batch * C::PLANES, 2 * pitch_l, 2 * slab_l, C::KE, 128);
+    if (rc) return rc;
+    if (KIND == APPLY) rc = gemm::make_map(&mr, gemm::F16, right, N, K, (int64_t)batch * C::PLANES, 2 * pitch_r, 2 * slab_r, 64, 64);
+    else rc = gemm::make_map(&mr, gemm::F16, right, K, N, (int64_t)batch * C::PLANES, 2 * pitch_r, 2 * slab_r, C::KE, C::BN / C::CG);
+    if (rc) return rc;
+    return gemm::launch<C, Epilogue<KIND, C::PLANES>>(ml, mr, gemm::tiles_of<C>(M, N, K, batch, KIND != APPLY), args, status, s);
 }
 
+// CTA pairs (tiles of 256 rows) where there are enough of them to occupy every SM; single CTAs otherwise
+template <int KIND, int PP>
+int choose(const __half* left, const __half* right, int M, int N, int K, int pitch_l, int pitch_r, int64_t slab_l, int64_t slab_r, int batch,
+           const EpiArgs& args, int32_t* status, cudaStream_t s) {
+    using Pair = gemm::Config<gemm::F16, PP, 2, PP == 3 ? 128 : 256, KIND == APPLY>;
+    if (gemm::tiles_of<Pair>(M, N, K, batch, KIND != APPLY).total >= 74)
+        return run<KIND, PP, 2>(left, right, M, N, K, pitch_l, pitch_r, slab_l, slab_r, batch, args, status, s);
+    return run<KIND, PP, 1>(left, right, M, N, K, pitch_l, pitch_r, slab_l, slab_r, batch, args, status, s);
+}
 template <int KIND>
-int launch(const Args& p, int batch, cudaStream_t s) {
-    const dim3 grid((unsigned)ceil_div(p.N, T), (unsigned)ceil_div(p.M, T), (unsigned)batch);
-    product_kernel<KIND><<<grid, 256, 0, s>>>(p);
-    return check_cuda(cudaGetLastError());
+int product(const Shape& sh, const __half* left, const __half* right, int N, int K, int pitch_l, int pitch_r, int64_t slab_l, int64_t slab_r,
+            const EpiArgs& args, int32_t* status, cudaStream_t s) {
+    if (sh.planes == 2)
+        return choose<KIND, 3>(left, right, sh.s, N, K, pitch_l, pitch_r, slab_l, slab_r, sh.batch, args, status, s);
+    return choose<KIND, 1>(left, right, sh.s, N, K, pitch_l, pitch_r, slab_l, slab_r, sh.batch, args, status, s);
 }
 }  // namespace
 
-int launch_gram(const __half* x, __half* a, const float* alpha, const Shape& sh, int32_t*, cudaStream_t s) {
-    Args p{x, x, a, nullptr, alpha, nullptr, sh.s, sh.s, sh.l, sh.ls, sh.ls, sh.ss, sh.planes, sh.x_slab(), sh.x_slab(), sh.a_slab(), 0, 0, 0};
-    return launch<GRAM>(p, sh.batch, s);
+int launch_gram(const __half* x, __half* a, const float* alpha, const Shape& sh, int32_t* status, cudaStream_t s) {
+    const EpiArgs args{nullptr, a, nullptr, alpha, nullptr, sh.ss, sh.a_slab(), 0, 0, 0};
+    return product<GRAM>(sh, x, x, sh.s, sh.l, sh.ls, sh.ls, sh.x_slab(), sh.x_slab(), args, status, s);
 }
-int launch_poly(const __half* a, __half* q, float ca, float cb, float cc, const Shape& sh, int32_t*, cudaStream_t s) {
-    Args p{a, a, q, nullptr, nullptr, nullptr, sh.s, sh.s, sh.s, sh.ss, sh.ss, sh.ss, sh.planes, sh.a_slab(), sh.a_slab(), sh.a_slab(), ca, cb, cc};
-    return launch<POLY>(p, sh.batch, s);
+int launch_poly(const __half* a, __half* q, float ca, float cb, float cc, const Shape& sh, int32_t* status, cudaStream_t s) {
+    const EpiArgs args{a, q, nullptr, nullptr, nullptr, sh.ss, sh.a_slab(), ca, cb, cc};
+    return product<POLY>(sh, a, a, sh.s, sh.s, sh.ss, sh.ss, sh.a_slab(), sh.a_slab(), args, status, s);
 }
-int launch_apply(const __half* q, const __half* x, __half* x_next, float* o, const float* alpha,
-                 const float* alpha_next, const Shape& sh, int32_t*,
-                 cudaStream_t s) {
-    Args p{q, x, x_next, o, alpha, alpha_next, sh.s, sh.l, sh.s, sh.ss, sh.ls, sh.ls, sh.planes, sh.a_slab(), sh.x_slab(), sh.x_slab(), 0, 0, 0};
-    return launch<APPLY>(p, sh.batch, s);
+int launch_apply(const __half* q, const __half* x, __half* x_next, float* o, const float* alpha, const float* alpha_next, const Shape& sh,
+                 int32_t* status, cudaStream_t s) {
+    const EpiArgs args{nullptr, x_next, o, alpha, alpha_next, sh.ls, sh.x_slab(), 0, 0, 0};
+    return product<APPLY>(sh, q, x, sh.l, sh.s, sh.ss, sh.ls, sh.a_slab(), sh.x_slab(), args, status, s);
 }
 
 }  // namespace ns
