@@ -298,7 +298,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ C
                         uint32_t r[32];
 #pragma unroll
                         for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(v[c * 32 + e]);
-                        Epi::emit(args, g, b, row, n0 + c * 32, r, mirrored(n0 + c * 32));
+                        Epi::template emit<32>(args, g, b, row, n0 + c * 32, r, mirrored(n0 + c * 32));
                     }
             } else {
                 const bool ok = mbar_wait(acc_full(acc), acc_ph, abort_flag, status, ST_EPILOGUE);
@@ -312,11 +312,11 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ C
                 for (int c = 0; c < nch; c += 2) {
                     tmem_ld_wait();
                     if (c + 1 < nch) tmem_ld32(ta + (c + 1) * 32, rb); else release(acc);
-                    Epi::emit(args, g, b, row, n0 + c * 32, ra, mirrored(n0 + c * 32));
+                    Epi::template emit<32>(args, g, b, row, n0 + c * 32, ra, mirrored(n0 + c * 32));
                     if (c + 1 < nch) {
                         tmem_ld_wait();
                         if (c + 2 < nch) tmem_ld32(ta + (c + 2) * 32, ra); else release(acc);
-                        Epi::emit(args, g, b, row, n0 + (c + 1) * 32, rb, mirrored(n0 + (c + 1) * 32));
+                        Epi::template emit<32>(args, g, b, row, n0 + (c + 1) * 32, rb, mirrored(n0 + (c + 1) * 32));
                     }
                 }
                 acc ^= 1;
@@ -336,6 +336,247 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ C
         else
             asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)C::TMEM_COLS) : "memory");
     }
+}
+
+// ---- few tiles: the K range of a tile split over the CTAs of a cluster ------------------------------------------------
+// One tile of 128 x BN per cluster of SPLIT CTAs (SPLIT a run-time power of two up to 8).  Every CTA sums its share of the
+// K blocks in tensor memory, leaves the partial tile in its shared memory, and after a cluster barrier adds up 128 / SPLIT
+// rows of all partials through distributed shared memory, in rank order, and writes them: one launch, no scratch, no
+// atomics, the same result every time.
+__device__ __forceinline__ void ld_cluster_v4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <class C>
+struct SplitSmem {
+    static constexpr int PITCH = (C::BN + 4) * 4;                   // bytes of a partial row: 16-byte stores of 8 rows meet no bank twice
+    static constexpr int PARTIAL = 128 * PITCH;
+    static constexpr int RING = C::STAGES * C::STAGE > PARTIAL ? C::STAGES * C::STAGE : PARTIAL;
+    static constexpr int BARS = 2 * C::STAGES + 5;
+    static constexpr int TOTAL = RING + BARS * 8 + 16 + 1024;
+};
+
+template <class C, class Epi>
+__global__ void __launch_bounds__(THREADS, 1)
+split_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ CUtensorMap map_r, const Tiles g,
+             const typename Epi::Args args, int split, int32_t* status) {
+    static_assert(C::CG == 1, "one CTA per accumulator");
+    using L = SplitSmem<C>;
+    constexpr int BN = C::BN, S = C::STAGES, PLANES = C::PLANES;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+    const uint32_t bars = base + L::RING;
+    auto full = [&](int s) { return bars + 8u * s; };
+    auto empty = [&](int s) { return bars + 8u * (S + s); };
+    auto acc_full = [&](int a) { return bars + 8u * (2 * S + a); };
+    auto acc_empty = [&](int a) { return bars + 8u * (2 * S + 2 + a); };
+    const uint32_t drain = bars + 8u * (2 * S + 4);
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + L::RING + L::BARS * 8);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + L::RING + L::BARS * 8 + 4);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)cluster_ctarank();
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
+        for (int a = 0; a < 2; ++a) { mbar_init(acc_full(a), 1); mbar_init(acc_empty(a), 128); }
+        mbar_init(drain, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_u32((const void*)tmem_slot)), "r"((uint32_t)C::TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    int b, m0, n0;
+    decode<C::BM, BN>(g, blockIdx.x / split, b, m0, n0);
+    // this CTA's K blocks (every CTA has at least one: the launch sees to it)
+    const int k_first = (int)((int64_t)g.nkb * rank / split), k_last = (int)((int64_t)g.nkb * (rank + 1) / split);
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int s = 0; uint32_t ph = 0;
+            bool alive = true;
+            for (int kb = k_first; kb < k_last; ++kb) {
+                if (!mbar_wait(empty(s), ph ^ 1u, abort_flag, status, ST_LOAD)) { alive = false; break; }
+                const uint32_t dst = base + s * C::STAGE;
+                mbar_arrive_expect_tx(full(s), (uint32_t)C::STAGE);
+#pragma unroll
+                for (int p = 0; p < PLANES; ++p) {
+                    const int z = b * PLANES + p;
+                    load_3d(dst + p * C::L_PANEL, &map_l, kb * C::KE, m0, z, full(s));
+                    const uint32_t rd = dst + PLANES * C::L_PANEL + p * C::R_PANEL;
+                    if (C::RMN) {
+#pragma unroll
+                        for (int q = 0; q < BN / 64; ++q) load_3d(rd + q * 8192, &map_r, n0 + q * 64, kb * C::KE, z, full(s));
+                    } else {
+                        load_3d(rd, &map_r, kb * C::KE, n0, z, full(s));
+                    }
+                }
+                if (++s == S) { s = 0; ph ^= 1u; }
+            }
+            if (!alive) {
+                const uint64_t t0 = globaltimer_ns();
+                while (globaltimer_ns() - t0 < 200000ull) { }
+            }
+        }
+    } else if (warp == 1) {
+        const bool elected = elect_one_sync();
+        int s = 0; uint32_t ph = 0;
+        int acc = 0; uint32_t acc_ph = 0;
+        bool alive = true;
+        const uint64_t l_desc = make_smem_desc(base);
+        const uint64_t r_desc = C::RMN ? mn_desc(base + PLANES * C::L_PANEL) : make_smem_desc(base + PLANES * C::L_PANEL);
+        const uint32_t l_hi = (uint32_t)(l_desc >> 32), r_hi = (uint32_t)(r_desc >> 32);
+        constexpr uint32_t L_TAIL = C::L_PANEL >> 4, R_TAIL = C::R_PANEL >> 4;
+        constexpr uint32_t R_STEP = C::RMN ? 2048 >> 4 : 32 >> 4;
+        for (int kb0 = k_first; kb0 < k_last && alive; kb0 += C::KCHUNK) {
+            const int kb1 = k_last - kb0 < C::KCHUNK ? k_last : kb0 + C::KCHUNK;
+            if (!__all_sync(0xffffffffu, mbar_wait(acc_empty(acc), acc_ph ^ 1u, abort_flag, status, ST_MMA_ACC))) { alive = false; break; }
+            tc_fence_after();
+            const uint32_t d = tmem + (uint32_t)(acc * C::ACC_COLS);
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!__all_sync(0xffffffffu, mbar_wait(full(s), ph, abort_flag, status, ST_MMA))) { alive = false; break; }
+                tc_fence_after();
+                const uint32_t off = (uint32_t)((s * C::STAGE) >> 4);
+                const uint32_t l_lo = (uint32_t)l_desc + off, r_lo = (uint32_t)r_desc + off;
+                const uint32_t later = (uint32_t)(kb != kb0);
+                if (elected) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t la = l_lo + 2u * k, ra = r_lo + R_STEP * k;
+                        mma<C::KIND, 1>(d, desc_from_words(la, l_hi), desc_from_words(ra, r_hi), C::IDESC, k ? 1u : later);
+                        if constexpr (C::PP == 3) {
+                            mma<C::KIND, 1>(d + BN, desc_from_words(la, l_hi), desc_from_words(ra + R_TAIL, r_hi), C::IDESC, k ? 1u : later);
+                            mma<C::KIND, 1>(d + BN, desc_from_words(la + L_TAIL, l_hi), desc_from_words(ra, r_hi), C::IDESC, 1u);
+                        }
+                    }
+                    umma_commit(empty(s));
+                }
+                __syncwarp();
+                if (++s == S) { s = 0; ph ^= 1u; }
+            }
+            if (alive && elected) umma_commit(acc_full(acc));
+            __syncwarp();
+            acc ^= 1;
+            if (acc == 0) acc_ph ^= 1u;
+        }
+        if (!alive && elected) {
+            umma_commit(drain);
+            const uint64_t t0 = globaltimer_ns();
+            while (!mbar_try_wait(drain, 0) && globaltimer_ns() - t0 < 10000000ull) { }
+        }
+        __syncwarp();
+    } else {
+        const int q = warp & 3;
+        int acc = 0; uint32_t acc_ph = 0;
+        bool alive = true;
+        uint32_t v[BN];
+        for (int kb0 = k_first; kb0 < k_last; kb0 += C::KCHUNK) {
+            const bool ok = mbar_wait(acc_full(acc), acc_ph, abort_flag, status, ST_EPILOGUE);
+            if (!__all_sync(0xffffffffu, ok)) { alive = false; break; }
+            tc_fence_after();
+            const uint32_t ta = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * C::ACC_COLS);
+#pragma unroll
+            for (int c = 0; c < BN / 32; ++c) {
+                uint32_t r0[32], r1[32];
+                tmem_ld32(ta + c * 32, r0);
+                if (C::PP == 3) tmem_ld32(ta + BN + c * 32, r1);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                    if constexpr (C::PP == 3) {
+                        const float part = __uint_as_float(r0[e]) + __uint_as_float(r1[e]);
+                        v[c * 32 + e] = __float_as_uint(kb0 == k_first ? part : __uint_as_float(v[c * 32 + e]) + part);
+                    } else {
+                        v[c * 32 + e] = r0[e];
+                    }
+                }
+            }
+            tc_fence_before();
+            mbar_arrive(acc_empty(acc));
+            acc ^= 1;
+            if (acc == 0) acc_ph ^= 1u;
+        }
+        if (alive) {
+            // the last accumulator is complete, so every MMA has read its stages and the ring is free for the partial tile
+            const uint32_t dst = base + (uint32_t)((q * 32 + lane) * L::PITCH);
+#pragma unroll
+            for (int e = 0; e < BN; e += 4)
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + e * 4), "r"(v[e]), "r"(v[e + 1]), "r"(v[e + 2]), "r"(v[e + 3]) : "memory");
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();                    // every CTA's partial tile is in place
+    {
+        const int rows = 128 / split;
+        for (int w = threadIdx.x; w < rows * (BN / 8); w += THREADS) {
+            const int r_in = w / (BN / 8), col = w % (BN / 8) * 8;
+            const int lrow = rank * rows + r_in;
+            if (m0 + lrow >= g.M || n0 + col >= g.N) continue;
+            uint32_t sum[8];
+            const uint32_t at = base + (uint32_t)(lrow * L::PITCH + col * 4);
+            for (int k = 0; k < split; ++k) {
+                uint32_t r0[4], r1[4];
+                const uint32_t from = mapa_cluster(at, (uint32_t)k);
+                ld_cluster_v4(from, r0);
+                ld_cluster_v4(from + 16, r1);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if constexpr (C::KIND == I8) {
+                        sum[e] = k ? sum[e] + r0[e] : r0[e];
+                        sum[4 + e] = k ? sum[4 + e] + r1[e] : r1[e];
+                    } else {
+                        sum[e] = k ? __float_as_uint(__uint_as_float(sum[e]) + __uint_as_float(r0[e])) : r0[e];
+                        sum[4 + e] = k ? __float_as_uint(__uint_as_float(sum[4 + e]) + __uint_as_float(r1[e])) : r1[e];
+                    }
+                }
+            }
+            const int row = m0 + lrow;
+            Epi::template emit<8>(args, g, b, row, n0 + col, sum, g.sym && (row / BN + 1) * BN <= (n0 + col) / C::BM * C::BM);
+        }
+    }
+    __syncthreads();
+    cluster_sync_all();                    // nobody leaves while its shared memory is still read
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)C::TMEM_COLS) : "memory");
+    }
+}
+
+// how many CTAs share a tile: as many as keep two K blocks each and the SMs no more than full
+inline int split_of(const Tiles& g, int sms = 148) {
+    int split = 1;
+    while (split < 8 && g.total * split * 2 <= sms && g.nkb >= 4 * split) split *= 2;
+    return split;
+}
+
+template <class C, class Epi>
+int launch_split(const CUtensorMap& map_l, const CUtensorMap& map_r, const Tiles& g, const typename Epi::Args& args, int split,
+                 int32_t* status, cudaStream_t s) {
+    static bool ready[64] = {false};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) return CHEBYKAN_EINVAL;
+    auto kernel = split_kernel<C, Epi>;
+    if (!ready[dev]) {
+        const int rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SplitSmem<C>::TOTAL));
+        if (rc) return rc;
+        ready[dev] = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(g.total * split)); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = SplitSmem<C>::TOTAL; cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)split; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr; cfg.numAttrs = 1;
+    return check_cuda(cudaLaunchKernelEx(&cfg, kernel, map_l, map_r, g, args, split, status));
 }
 
 // map of `slabs` row-major matrices [rows][cols], rows pitch_bytes and matrices slab_bytes apart, read in boxes of

@@ -154,13 +154,15 @@ int launch_basis(const void* x, int dtype, int8_t* q, float* scale, int64_t B, i
 }
 
 bool dtype_ok(int dtype) { return dtype >= CHEBYKAN_DTYPE_FP32 && dtype <= CHEBYKAN_DTYPE_FP16; }
-// B rows of in values: the layer limits of the other entry points, an exact integer sum, and a 32-bit grid
+// row numbers are 32-bit inside the kernels, and a tile may reach past the last row
+constexpr int64_t MAX_ROWS = 0x7fffffff - 4096;
+// B rows of in values: the layer limits of the other entry points and an exact integer sum
 bool layer_ok(int64_t B, int64_t in, int64_t out, int64_t deg) {
-    return B >= 0 && B <= 0x7fffffff && in >= 1 && in <= (1 << 20) && out >= 1 && out <= (1 << 20) && deg >= 1 && deg <= 127 &&
+    return B >= 0 && B <= MAX_ROWS && in >= 1 && in <= (1 << 20) && out >= 1 && out <= (1 << 20) && deg >= 1 && deg <= 127 &&
            in_pad(in) * deg <= MAX_K;
 }
 bool product_ok(int64_t M, int64_t N, int64_t K, int64_t ldq, int64_t ldw) {
-    return M >= 0 && M <= 0x7fffffff && N >= 1 && N <= (1 << 20) && K >= 0 && K <= MAX_K && ldq >= K && ldw >= K &&
+    return M >= 0 && M <= MAX_ROWS && N >= 1 && N <= (1 << 20) && K >= 0 && K <= MAX_K && ldq >= K && ldw >= K &&
            ldq <= ((int64_t)1 << 32) && ldw <= ((int64_t)1 << 32);
 }
 int64_t a256(int64_t b) { return round_up(b, 256); }

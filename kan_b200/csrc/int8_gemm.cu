@@ -1,64 +1,191 @@
-// Product of 8-bit integer matrices with a scale per row and per column.
+// Product of 8-bit integer matrices with a scale per row and per column:
+//   y[r][o] = (sum_k q[r][k] wq[o][k]) * q_scale[r] * w_scale[o] + bias[o]
+// The sum is exact in int32 whatever its order, so the kernels below give the same bits.
+//
+//   up to 8 rows     row_kernel: bound by reading wq once; CUDA cores, four products per instruction
+//   few tiles        tcgen05 kind::i8, one tile per cluster, K split over its CTAs (gemm_tc.cuh)
+//   else             tcgen05 kind::i8, persistent pairs on 256 x 256 tiles
+#include "gemm_tc.cuh"
 #include "int8.cuh"
 
 namespace chebykan {
 namespace int8 {
 namespace {
+using gemm::Tiles;
 
-constexpr int T = 64, KT = 64;
+struct EpiArgs {
+    const float *q_scale, *w_scale, *bias;
+    void* y;
+};
 
-// 64 x 64 outputs per block, 4 x 4 per thread, four products per instruction
 template <typename OUT>
-__global__ void __launch_bounds__(256) dot_kernel(const Product p) {
-    __shared__ int sq[KT / 4][T + 1], sw[KT / 4][T + 1];
-    const int64_t m0 = blockIdx.x * (int64_t)T, n0 = blockIdx.y * (int64_t)T;
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    int acc[4][4] = {};
-    for (int64_t k0 = 0; k0 < p.K; k0 += KT) {
-        for (int e = threadIdx.x; e < T * KT / 4; e += 256) {
-            const int k = e % (KT / 4), r = e / (KT / 4);
-            uint32_t a = 0, b = 0;
-            for (int j = 0; j < 4; ++j) {
-                const int64_t kk = k0 + 4 * k + j;
-                if (kk >= p.K) break;
-                if (m0 + r < p.M) a |= (uint32_t)(uint8_t)p.q[(m0 + r) * p.ldq + kk] << (8 * j);
-                if (n0 + r < p.N) b |= (uint32_t)(uint8_t)p.wq[(n0 + r) * p.ldw + kk] << (8 * j);
+struct Epilogue {
+    using Args = EpiArgs;
+    template <int NC>
+    static __device__ __forceinline__ void emit(const Args& p, const Tiles& g, int, int row, int col0, uint32_t (&r)[NC], bool) {
+        if (row >= g.M) return;
+        const float qs = __ldg(p.q_scale + row);
+        OUT* dst = reinterpret_cast<OUT*>(p.y) + (int64_t)row * g.N + col0;
+        constexpr int V = 16 / (int)sizeof(OUT);          // values of a 16-byte store
+        const bool vec = g.N % V == 0;
+#pragma unroll
+        for (int c = 0; c < NC; c += V) {
+            OUT out[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const int col = col0 + c + e;
+                if (col < g.N)
+                    out[e] = to_type<OUT>(fmaf((float)(int)r[c + e] * qs, __ldg(p.w_scale + col), p.bias ? __ldg(p.bias + col) : 0.f));
             }
-            sq[k][r] = (int)a;
-            sw[k][r] = (int)b;
+            if (vec && col0 + c < g.N) {
+                *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(out);
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    if (col0 + c + e < g.N) dst[c + e] = out[e];
+            }
         }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < KT / 4; ++k)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(sq[k][ty * 4 + i], sw[k][tx * 4 + j], acc[i][j]);
-        __syncthreads();
     }
-    OUT* y = reinterpret_cast<OUT*>(p.y);
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const int64_t m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-            if (m < p.M && n < p.N)
-                y[m * p.N + n] = to_type<OUT>(fmaf((float)acc[i][j] * p.q_scale[m], p.w_scale[n], p.bias ? p.bias[n] : 0.f));
-        }
+};
+
+// ---- up to 8 rows ---------------------------------------------------------------------------------------------------
+// A warp per output column: lanes take 16 bytes of the column's weights each, eight loads in flight, against the same
+// bytes of every row (from the caches).  Bytes past K are zero.
+__device__ __forceinline__ int4 load16(const int8_t* p, int64_t k, int64_t K) {
+    if (k + 16 <= K) return __ldg(reinterpret_cast<const int4*>(p + k));
+    int w[4] = {0, 0, 0, 0};
+    for (int e = 0; e < 16 && k + e < K; ++e) w[e >> 2] |= (int)((uint32_t)(uint8_t)p[k + e] << (8 * (e & 3)));
+    return make_int4(w[0], w[1], w[2], w[3]);
+}
+template <typename OUT, int ROWS>
+__global__ void __launch_bounds__(256) row_kernel(const Product p) {
+    const int lane = threadIdx.x & 31;
+    const int64_t o = blockIdx.x * (int64_t)8 + (threadIdx.x >> 5);
+    if (o >= p.N) return;
+    const int8_t* w = p.wq + o * p.ldw;
+    int acc[ROWS] = {};
+    constexpr int U = ROWS <= 2 ? 8 : 4;
+    for (int64_t k0 = lane * 16; k0 < p.K; k0 += U * 512) {
+        int4 wv[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (k0 + u * 512 < p.K) wv[u] = load16(w, k0 + u * 512, p.K);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (k0 + u * 512 < p.K)
+#pragma unroll
+                for (int r = 0; r < ROWS; ++r)
+                    if (r < p.M) {
+                        const int4 v = load16(p.q + r * p.ldq, k0 + u * 512, p.K);
+                        acc[r] = __dp4a(v.x, wv[u].x, __dp4a(v.y, wv[u].y, __dp4a(v.z, wv[u].z, __dp4a(v.w, wv[u].w, acc[r]))));
+                    }
+    }
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+        for (int d = 16; d; d >>= 1) acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], d);
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+        if (lane == r && r < p.M)
+            reinterpret_cast<OUT*>(p.y)[r * p.N + o] =
+                to_type<OUT>(fmaf((float)acc[r] * p.q_scale[r], p.w_scale[o], p.bias ? p.bias[o] : 0.f));
+}
+
+// no columns at all: the sums are zero
+template <typename OUT>
+__global__ void __launch_bounds__(256) empty_kernel(const Product p) {
+    for (int64_t e = blockIdx.x * (int64_t)256 + threadIdx.x; e < p.M * p.N; e += (int64_t)gridDim.x * 256)
+        reinterpret_cast<OUT*>(p.y)[e] = to_type<OUT>(fmaf(0.f * p.q_scale[e / p.N], p.w_scale[e % p.N], p.bias ? p.bias[e % p.N] : 0.f));
+}
+
+// rows of any byte pitch -> rows of a pitch that is a multiple of 16
+__global__ void __launch_bounds__(256) pad_kernel(const int8_t* __restrict__ src, int64_t ld, int8_t* __restrict__ dst, int64_t pitch, int64_t rows, int64_t K) {
+    const int64_t words = pitch / 4;
+    for (int64_t e = blockIdx.x * (int64_t)256 + threadIdx.x; e < rows * words; e += (int64_t)gridDim.x * 256) {
+        const int64_t r = e / words, k = e % words * 4;
+        uint32_t v = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (k + j < K) v |= (uint32_t)(uint8_t)src[r * ld + k + j] << (8 * j);
+        *reinterpret_cast<uint32_t*>(dst + r * pitch + k) = v;
+    }
 }
 
 template <typename OUT>
-int launch_typed(const Product& p, cudaStream_t s) {
-    const dim3 grid((unsigned)ceil_div(p.M, T), (unsigned)ceil_div(p.N, T));
-    dot_kernel<OUT><<<grid, 256, 0, s>>>(p);
+int launch_rows(const Product& p, cudaStream_t s) {
+    const unsigned grid = (unsigned)ceil_div(p.N, 8);
+    if (p.M == 1) row_kernel<OUT, 1><<<grid, 256, 0, s>>>(p);
+    else if (p.M == 2) row_kernel<OUT, 2><<<grid, 256, 0, s>>>(p);
+    else if (p.M <= 4) row_kernel<OUT, 4><<<grid, 256, 0, s>>>(p);
+    else row_kernel<OUT, 8><<<grid, 256, 0, s>>>(p);
     return check_cuda(cudaGetLastError());
 }
+
+template <class C>
+int maps_of(const Product& p, CUtensorMap* mq, CUtensorMap* mw) {
+    const int rc = gemm::make_map(mq, gemm::I8, p.q, p.K, p.M, 1, p.ldq, p.ldq, C::KE, 128);      // one slab: its distance is not used
+    return rc ? rc : gemm::make_map(mw, gemm::I8, p.wq, p.K, p.N, 1, p.ldw, p.ldw, C::KE, C::BN / C::CG);
+}
+
+template <class C, typename OUT>
+int run_split(const Product& p, const Tiles& g, const EpiArgs& args, int32_t* status, cudaStream_t s) {
+    CUtensorMap mq, mw;
+    const int rc = maps_of<C>(p, &mq, &mw);
+    if (rc) return rc;
+    return gemm::launch_split<C, Epilogue<OUT>>(mq, mw, g, args, gemm::split_of(g), status, s);
+}
+template <class C, typename OUT>
+int run_persistent(const Product& p, const EpiArgs& args, int32_t* status, cudaStream_t s) {
+    CUtensorMap mq, mw;
+    const int rc = maps_of<C>(p, &mq, &mw);
+    if (rc) return rc;
+    return gemm::launch<C, Epilogue<OUT>>(mq, mw, gemm::tiles_of<C>((int)p.M, (int)p.N, (int)p.K, 1, false), args, status, s);
+}
+
+template <typename OUT>
+int launch_typed(const Product& p, int32_t* status, cudaStream_t s) {
+    if (p.K == 0) {
+        empty_kernel<OUT><<<(unsigned)(ceil_div(p.M * p.N, 256) < 148 * 8 ? ceil_div(p.M * p.N, 256) : 148 * 8), 256, 0, s>>>(p);
+        return check_cuda(cudaGetLastError());
+    }
+    if (p.M <= 8) return launch_rows<OUT>(p, s);
+    const EpiArgs args{p.q_scale, p.w_scale, p.bias, p.y};
+    using Pair = gemm::Config<gemm::I8, 1, 2, 256, false>;
+    using Narrow = gemm::Config<gemm::I8, 1, 1, 64, false>;
+    using Wide = gemm::Config<gemm::I8, 1, 1, 128, false>;
+    // tiles of 128 x 64 as long as that leaves SMs idle, of 128 x 128 up to one each, pairs on 256 x 256 beyond
+    const int M = (int)p.M, N = (int)p.N, K = (int)p.K;
+    const Tiles narrow = gemm::tiles_of<Narrow>(M, N, K, 1, false), wide = gemm::tiles_of<Wide>(M, N, K, 1, false);
+    if (narrow.total <= 148) return run_split<Narrow, OUT>(p, narrow, args, status, s);
+    if (wide.total <= 148) return run_split<Wide, OUT>(p, wide, args, status, s);
+    return run_persistent<Pair, OUT>(p, args, status, s);
+}
+
+int64_t a256(int64_t b) { return round_up(b, 256); }
 }  // namespace
 
-int64_t matmul_workspace_bytes(int64_t, int64_t, int64_t, int64_t, int64_t) { return 0; }
+int64_t matmul_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t ldq, int64_t ldw) {
+    const int64_t pitch = round_up(K, 16);
+    return (ldq % 16 ? a256(M * pitch) : 0) + (ldw % 16 ? a256(N * pitch) : 0);
+}
 
-int launch_matmul(const Product& p, void*, int32_t*, cudaStream_t s) {
-    if (p.dtype == CHEBYKAN_DTYPE_FP32) return launch_typed<float>(p, s);
-    if (p.dtype == CHEBYKAN_DTYPE_BF16) return launch_typed<__nv_bfloat16>(p, s);
-    return launch_typed<__half>(p, s);
+int launch_matmul(const Product& given, void* ws, int32_t* status, cudaStream_t s) {
+    Product p = given;
+    const int64_t pitch = round_up(p.K, 16);
+    int8_t* at = reinterpret_cast<int8_t*>(ws);
+    auto pad = [&](const int8_t*& m, int64_t& ld, int64_t rows) -> int {
+        if (ld % 16 == 0 || p.K == 0) return CHEBYKAN_OK;
+        const int64_t blocks = ceil_div(rows * pitch / 4, 256);
+        pad_kernel<<<(unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, s>>>(m, ld, at, pitch, rows, p.K);
+        m = at; ld = pitch; at += a256(rows * pitch);
+        return check_cuda(cudaGetLastError());
+    };
+    int rc;
+    if ((rc = pad(p.q, p.ldq, p.M))) return rc;
+    if ((rc = pad(p.wq, p.ldw, p.N))) return rc;
+    if (p.dtype == CHEBYKAN_DTYPE_FP32) return launch_typed<float>(p, status, s);
+    if (p.dtype == CHEBYKAN_DTYPE_BF16) return launch_typed<__nv_bfloat16>(p, status, s);
+    return launch_typed<__half>(p, status, s);
 }
 
 }  // namespace int8

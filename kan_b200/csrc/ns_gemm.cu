@@ -30,8 +30,9 @@ __device__ __forceinline__ uint32_t pack2(__half x, __half y) {
 template <int KIND, int PLANES>
 struct Epilogue {
     using Args = EpiArgs;
-    // 32 consecutive columns of one row
-    static __device__ __forceinline__ void emit(const Args& p, const Tiles& g, int b, int row, int col0, uint32_t (&r)[32], bool mirror) {
+    // NC consecutive columns of one row
+    template <int NC>
+    static __device__ __forceinline__ void emit(const Args& p, const Tiles& g, int b, int row, int col0, uint32_t (&r)[NC], bool mirror) {
         const int64_t slab0 = (int64_t)b * PLANES * p.slab;
         float factor;
         if (KIND == GRAM) { const float al = p.alpha[b]; factor = al * al * exp2f((float)A_EXP); }
@@ -42,13 +43,13 @@ struct Epilogue {
             float* dst = p.out32 + ((int64_t)b * g.M + row) * g.N + col0;
             if ((g.N & 3) == 0) {
 #pragma unroll
-                for (int e = 0; e < 32; e += 4)
+                for (int e = 0; e < NC; e += 4)
                     if (col0 + e < g.N)
                         *reinterpret_cast<float4*>(dst + e) = make_float4(__uint_as_float(r[e]) * factor, __uint_as_float(r[e + 1]) * factor,
                                                                           __uint_as_float(r[e + 2]) * factor, __uint_as_float(r[e + 3]) * factor);
             } else {
 #pragma unroll
-                for (int e = 0; e < 32; ++e)
+                for (int e = 0; e < NC; ++e)
                     if (col0 + e < g.N) dst[e] = __uint_as_float(r[e]) * factor;
             }
             return;
@@ -56,7 +57,7 @@ struct Epilogue {
         const int64_t at = slab0 + (int64_t)row * p.pitch + col0;
         // eight columns (16 bytes of a plane) at a time; a row's last group may run into its padding, which nothing reads
 #pragma unroll
-        for (int c = 0; c < 32; c += 8) {
+        for (int c = 0; c < NC; c += 8) {
             if (col0 + c >= g.N) break;
             __half hi[8], lo[8];
             uint4 ah, al;
