@@ -11,32 +11,6 @@ namespace chebykan {
 namespace ns {
 namespace {
 
-// ---- where a matrix's elements come from ----------------------------------------------------------------------
-// u(i, r, c) of matrix i.  Strided: a tensor of any strides and type.  Momentum: the degree slices of a coefficient
-// gradient [in][out][deg+1] after the momentum update (buf already holds the new value).
-template <typename T>
-struct StridedSource {
-    const T* g;
-    int64_t sb, sr, sc;
-    __device__ __forceinline__ float load(int64_t i, int64_t r, int64_t c) const {
-        return (float)g[i * sb + r * sr + c * sc];
-    }
-};
-struct MomentumSource {
-    const float *grad, *buf;
-    int64_t out;
-    int dp1;
-    float momentum, gs;
-    int nesterov;
-    __device__ __forceinline__ float at(int64_t e) const {
-        const float m = buf[e];
-        if (!nesterov) return m;
-        const float g = grad[e] * gs;
-        return fmaf(momentum, m - g, g);
-    }
-    __device__ __forceinline__ float load(int64_t i, int64_t r, int64_t c) const { return at((r * out + c) * dp1 + i); }
-};
-
 // sum over the block in a fixed order; the total is returned to thread 0
 __device__ __forceinline__ double block_sum(double v, double* smem) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -90,28 +64,6 @@ momentum_kernel(const float* __restrict__ grad, float* __restrict__ buf, int64_t
     }
 }
 
-// power of two that puts the norm into [2^14, 2^15), the factor that is left of 1 / max(norm, eps), and the scale of the
-// later X: growth bounds log2 of what the steps multiply a small X by, and below eps 2^-growth that leaves X under 1,
-// which its scale then makes up for.  A norm that is not finite makes the whole matrix NaN.
-__device__ __forceinline__ void scales_of(const double* partial, float eps, int growth, double* pow2, float* alpha, float* later) {
-    double t = 0.;
-    for (int k = 0; k < NORM_BLOCKS; ++k) t += partial[k];
-    const double norm = sqrt(t);
-    *pow2 = 1.; *alpha = 1.f; *later = exp2f(-(float)X_EXP);
-    if (!(norm <= 1.7e308)) { *alpha = __int_as_float(0x7fc00000); return; }
-    if (norm == 0.) return;
-    int e;
-    frexp(norm, &e);                       // norm = f 2^e, f in [1/2, 1)
-    *pow2 = ldexp(1., 15 - e);
-    *alpha = (float)(1. / (fmax(norm, (double)eps) * *pow2));
-    if (norm < eps) {
-        int r;
-        frexp(norm / eps, &r);             // |X_0| < 2^r
-        const int up = -r - growth;
-        if (up > 0) *later = (float)ldexp(1., -X_EXP - (up < 110 ? up : 110));
-    }
-}
-
 // X_0 planes of one matrix tile: 32 x 32 elements, transposed on the way where the matrix is tall
 template <typename Src>
 __global__ void __launch_bounds__(256)
@@ -122,7 +74,9 @@ pack_kernel(Src src, int64_t m, int64_t n, __half* __restrict__ x, float* __rest
     const int64_t b = blockIdx.z, r0 = blockIdx.y * 32, c0 = blockIdx.x * 32;
     if (threadIdx.x == 0) {
         float al, later;
-        scales_of(partial + b * NORM_BLOCKS, eps, growth, &pow2, &al, &later);
+        double t = 0.;
+        for (int k = 0; k < NORM_BLOCKS; ++k) t += partial[b * NORM_BLOCKS + k];
+        scales_of(sqrt(t), eps, growth, &pow2, &al, &later);
         if (blockIdx.x == 0 && blockIdx.y == 0) { alpha[b] = al; alpha[sh.batch + b] = later; }
     }
     __syncthreads();
@@ -142,11 +96,6 @@ pack_kernel(Src src, int64_t m, int64_t n, __half* __restrict__ x, float* __rest
             if (sh.planes == 2) dst[at + sh.x_slab()] = lo;
         }
 }
-
-template <typename T> __device__ __forceinline__ T from_float(float v);
-template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
-template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
 // out[b][m][n] from o[b][s][l]
 template <typename T>
@@ -188,6 +137,7 @@ Shape shape_of(int64_t batch, int64_t m, int64_t n, int mode) {
 
 Workspace layout_of(const Shape& sh) {
     Workspace w{};
+    if (small_supported(sh)) return w;           // one launch that keeps everything on chip
     const int64_t xb = a256(2 * sh.x_slab() * sh.planes * sh.batch), ab = a256(2 * sh.a_slab() * sh.planes * sh.batch);
     int64_t at = 0;
     w.x0 = at; at += xb;
@@ -293,15 +243,18 @@ int chebykan_orthogonalize(const void* g, int64_t stride_batch, int64_t stride_r
         steps < 1 || steps > 32 || !(eps > 0.f) || !coefficients_ok(steps, a, b, c, &growth))
         return CHEBYKAN_EINVAL;
     if (batch == 0 || m == 0 || n == 0) return CHEBYKAN_OK;
-    if (!g || !out || !workspace || !status) return CHEBYKAN_EINVAL;
+    if (!g || !out || !status) return CHEBYKAN_EINVAL;
     if (!aligned16(out) || !aligned16(workspace)) return CHEBYKAN_EALIGN;
-    if (workspace_bytes < need) return CHEBYKAN_EWORKSPACE;
+    if (workspace_bytes < need || (need > 0 && !workspace)) return CHEBYKAN_EWORKSPACE;
     int rc = check_device();
     if (rc) return rc;
     const Shape sh = shape_of(batch, m, n, mode);
+    cudaStream_t s = (cudaStream_t)stream;
+    if (small_supported(sh))
+        return launch_small_orthogonalize(g, dtype, stride_batch, stride_row, stride_col, out, m, n, sh,
+                                          {(int)steps, a, b, c, eps, growth}, status, s);
     const Workspace w = layout_of(sh);
     char* ws = reinterpret_cast<char*>(workspace);
-    cudaStream_t s = (cudaStream_t)stream;
     if (dtype == CHEBYKAN_DTYPE_FP32)
         return orthogonalize_typed<float>(g, stride_batch, stride_row, stride_col, out, ws, w, sh, m, n, steps, a, b, c, eps, growth, status, s);
     if (dtype == CHEBYKAN_DTYPE_BF16)
@@ -322,18 +275,21 @@ int chebykan_muon_step(float* param, const float* grad, float* buf, void* worksp
     const int64_t need = chebykan_muon_workspace_bytes(in, out, deg, mode);
     if (need < 0) return (int)need;
     int growth = 0;
-    if (!param || !grad || !buf || !workspace || !status || steps < 1 || steps > 32 || !(eps > 0.f) ||
+    if (!param || !grad || !buf || !status || steps < 1 || steps > 32 || !(eps > 0.f) ||
         !(momentum >= 0.f && momentum < 1.f) || !coefficients_ok(steps, a, b, c, &growth))
         return CHEBYKAN_EINVAL;
     if (!aligned16(param) || !aligned16(grad) || !aligned16(buf) || !aligned16(workspace)) return CHEBYKAN_EALIGN;
-    if (workspace_bytes < need) return CHEBYKAN_EWORKSPACE;
+    if (workspace_bytes < need || (need > 0 && !workspace)) return CHEBYKAN_EWORKSPACE;
     int rc = check_device();
     if (rc) return rc;
     const int dp1 = (int)deg + 1;
     const Shape sh = shape_of(dp1, in, out, mode);
+    cudaStream_t s = (cudaStream_t)stream;
+    if (small_supported(sh))
+        return launch_small_muon(param, grad, buf, in, out, dp1, 1.f - lr * weight_decay, lr * update_scale, momentum, nesterov,
+                                 grad_scale, sh, {(int)steps, a, b, c, eps, growth}, status, s);
     const Workspace w = layout_of(sh);
     char* ws = reinterpret_cast<char*>(workspace);
-    cudaStream_t s = (cudaStream_t)stream;
     momentum_kernel<<<NORM_BLOCKS, 256, 0, s>>>(grad, buf, in * out * dp1, dp1, momentum, nesterov, grad_scale,
                                                 reinterpret_cast<double*>(ws + w.partial));
     if ((rc = check_cuda(cudaGetLastError()))) return rc;

@@ -40,6 +40,56 @@ __device__ __forceinline__ void split_half(float v, __half& hi, __half& lo) {
     lo = __float2half_rn(v - __half2float(hi));
 }
 
+// ---- where a matrix's elements come from ----------------------------------------------------------------------
+// u(i, r, c) of matrix i.  Strided: a tensor of any strides and type.  Momentum: the degree slices of a coefficient
+// gradient [in][out][deg+1] after the momentum update (buf already holds the new value).
+template <typename T>
+struct StridedSource {
+    const T* g;
+    int64_t sb, sr, sc;
+    __device__ __forceinline__ float load(int64_t i, int64_t r, int64_t c) const {
+        return (float)g[i * sb + r * sr + c * sc];
+    }
+};
+struct MomentumSource {
+    const float *grad, *buf;
+    int64_t out;
+    int dp1;
+    float momentum, gs;
+    int nesterov;
+    __device__ __forceinline__ float at(int64_t e) const {
+        const float m = buf[e];
+        if (!nesterov) return m;
+        const float g = grad[e] * gs;
+        return fmaf(momentum, m - g, g);
+    }
+    __device__ __forceinline__ float load(int64_t i, int64_t r, int64_t c) const { return at((r * out + c) * dp1 + i); }
+};
+
+// power of two that puts the norm into [2^14, 2^15), the factor that is left of 1 / max(norm, eps), and the scale of the
+// later X: growth bounds log2 of what the steps multiply a small X by, and below eps 2^-growth that leaves X under 1,
+// which its scale then makes up for.  A norm that is not finite makes the whole matrix NaN.
+__device__ __forceinline__ void scales_of(double norm, float eps, int growth, double* pow2, float* alpha, float* later) {
+    *pow2 = 1.; *alpha = 1.f; *later = exp2f(-(float)X_EXP);
+    if (!(norm <= 1.7e308)) { *alpha = __int_as_float(0x7fc00000); return; }
+    if (norm == 0.) return;
+    int e;
+    frexp(norm, &e);                       // norm = f 2^e, f in [1/2, 1)
+    *pow2 = ldexp(1., 15 - e);
+    *alpha = (float)(1. / (fmax(norm, (double)eps) * *pow2));
+    if (norm < eps) {
+        int r;
+        frexp(norm / eps, &r);             // |X_0| < 2^r
+        const int up = -r - growth;
+        if (up > 0) *later = (float)ldexp(1., -X_EXP - (up < 110 ? up : 110));
+    }
+}
+
+template <typename T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
 // A = X X^T with X = alpha[b] * stored
 int launch_gram(const __half* x, __half* a, const float* alpha, const Shape& sh, int32_t* status, cudaStream_t s);
 // P = ca I + cb A + cc A A
@@ -47,6 +97,19 @@ int launch_poly(const __half* a, __half* p, float ca, float cb, float cc, const 
 // X' = P X as planes (x_next, stored over alpha_next[b]), or as fp32 [batch][s][l] (o) where x_next is null
 int launch_apply(const __half* p, const __half* x, __half* x_next, float* o, const float* alpha, const float* alpha_next,
                  const Shape& sh, int32_t* status, cudaStream_t s);
+
+
+// ---- whole calls for small matrices in one launch (ns_small.cu) ----
+struct Steps {
+    int n;
+    float a, b, c, eps;
+    int growth;
+};
+bool small_supported(const Shape& sh);
+int launch_small_orthogonalize(const void* g, int dtype, int64_t sb, int64_t sr, int64_t sc, void* out, int64_t m, int64_t n, const Shape& sh,
+                               const Steps& st, int32_t* status, cudaStream_t s);
+int launch_small_muon(float* param, const float* grad, float* buf, int64_t in, int64_t out, int dp1, float keep, float step, float momentum,
+                      int nesterov, float gs, const Shape& sh, const Steps& st, int32_t* status, cudaStream_t s);
 
 }  // namespace ns
 }  // namespace chebykan

@@ -1,0 +1,456 @@
+// Newton-Schulz orthogonalisation and the whole Muon step of small matrices (shorter side up to 128, longer up to 2048) in
+// one launch.
+//
+// A matrix of this size is a few microseconds of reading and no arithmetic to speak of, but 3 * steps products that wait
+// for one another: as launches of their own each costs a launch, a pipeline's start and its drain (about 9 us; 150 us for
+// five steps on 33 matrices of 64 x 64).  Here a cluster of up to 8 CTAs keeps the matrix in shared memory throughout.  Every
+// CTA holds a slice of up to 256 columns of X, rows padded to 128, as fp16 planes in 64-column panels of 128-byte swizzled
+// rows, which serve as they lie as both operands of A = X X^T (K-major) and as the right operand of P X (MN-major).  A and P
+// share one buffer: a row of P is formed from the same row of A by the thread that then overwrites it.
+//   A  = X X^T   each CTA over its columns; with several CTAs the fp32 partial results are added in rank order through
+//                distributed shared memory, each CTA reducing a band of rows, which the others then fetch
+//   P  = a I + b A + c A A    every CTA for itself
+//   X' = P X     on the CTA's own columns
+// Products are tcgen05.mma (cta_group::1, M = 128) issued by one elected lane; between two of them all eight warps turn the
+// accumulator into the next operand.  Sums run over at most 256 columns, so the tensor pipe's truncation stays below 1e-6
+// (see gemm_tc.cuh).
+#include <math.h>
+#include "newton_schulz.cuh"
+#include "tc_common.cuh"
+
+namespace chebykan {
+namespace ns {
+namespace {
+using namespace tc;
+
+constexpr int THREADS = 256;
+constexpr int PANEL = 128 * 128;                 // 128 rows of 64 fp16 columns
+constexpr int MAX_CLUSTER = 8, MAX_SLICE = 256;
+enum { ST_GRAM = 31, ST_POLY = 32, ST_APPLY = 33 };
+
+struct Geometry {
+    int s, l;
+    int cluster, slice;      // CTAs per matrix, columns per CTA (a multiple of 64)
+    int s16, acc;            // rows rounded up to 16; columns of one accumulator
+    int planes, tall;
+    int x_bytes, a_bytes;    // shared memory: X planes, and the buffer of A / P / partial sums
+};
+
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ double ld_cluster_f64(uint32_t addr) {
+    double v;
+    asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(addr) : "memory");
+    return v;
+}
+// 16 bytes (8 columns from col) of a row of panels
+__device__ __forceinline__ uint32_t chunk_at(int row, int col) {
+    return (uint32_t)((col >> 6) * PANEL + row * 128 + ((((col & 63) >> 3) ^ (row & 7)) << 4));
+}
+__device__ __forceinline__ uint32_t half2_bits(__half x, __half y) {
+    return (uint32_t)__half_as_ushort(x) | ((uint32_t)__half_as_ushort(y) << 16);
+}
+
+// ---- the two uses: where elements come from and where results go ----
+template <typename T>
+struct OrthogonalizeIo {
+    StridedSource<T> src;
+    T* out;
+    int64_t m, n;
+    __device__ __forceinline__ double first(int64_t b, int64_t r, int64_t c) const { return (double)src.load(b, r, c); }
+    __device__ __forceinline__ float again(int64_t b, int64_t r, int64_t c) const { return src.load(b, r, c); }
+    __device__ __forceinline__ void store(int64_t b, int64_t r, int64_t c, float v) const { out[(b * m + r) * n + c] = from_float<T>(v); }
+};
+struct MuonIo {
+    float* param;
+    const float* grad;
+    float* buf;
+    int64_t out;
+    int dp1, nesterov;
+    float momentum, gs, keep, step;
+    __device__ __forceinline__ float update(int64_t e, float m) const {
+        const float g = grad[e] * gs;
+        return nesterov ? fmaf(momentum, m - g, g) : m;
+    }
+    // the first visit moves the momentum; the second, by the same thread, finds it moved
+    __device__ __forceinline__ double first(int64_t b, int64_t r, int64_t c) const {
+        const int64_t e = (r * out + c) * dp1 + b;
+        const float old = buf[e], m = fmaf(1.f - momentum, grad[e] * gs - old, old);
+        buf[e] = m;
+        return (double)update(e, m);
+    }
+    __device__ __forceinline__ float again(int64_t b, int64_t r, int64_t c) const {
+        const int64_t e = (r * out + c) * dp1 + b;
+        return update(e, buf[e]);
+    }
+    __device__ __forceinline__ void store(int64_t b, int64_t r, int64_t c, float v) const {
+        const int64_t e = (r * out + c) * dp1 + b;
+        param[e] = fmaf(-step, v, keep * param[e]);
+    }
+};
+
+template <class Io, int PLANES>
+__global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io io, const Geometry g, const Steps st, int32_t* status) {
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+    uint8_t* tail = gen + g.x_bytes + g.a_bytes;
+    double* red = reinterpret_cast<double*>(tail);                               // [8], and the CTA's sum in [8]
+    float* scales = reinterpret_cast<float*>(tail + 80);                         // alpha of X_0 and of the later X
+    double* pow2 = reinterpret_cast<double*>(tail + 88);
+    const uint32_t bar = base + (uint32_t)(g.x_bytes + g.a_bytes) + 96;
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(tail + 104);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 108);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)cluster_ctarank();
+    const int64_t b = blockIdx.x / g.cluster;
+    const int col0 = rank * g.slice;
+    const int cols = g.l - col0 < g.slice ? g.l - col0 : g.slice;               // at least 1
+    const uint32_t xs = base, as = base + (uint32_t)g.x_bytes;
+    const int x_plane = g.x_bytes / PLANES, a_plane = (g.s16 + 63) / 64 * PANEL;
+    const uint32_t tmem_cols = (uint32_t)(PLANES * g.acc);
+
+    if (threadIdx.x == 0) {
+        mbar_init(bar, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_u32((const void*)tmem_slot)), "r"(tmem_cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+
+    // ---- norm (and momentum), then X_0 ----
+    // elements in the order of the matrix's own columns, so that reads are coalesced whichever side is the shorter
+    const int count = g.s * cols;
+    auto place = [&](int e, int& r, int& c) {
+        if (g.tall) { c = e / g.s; r = e - c * g.s; } else { r = e / cols; c = e - r * cols; }
+    };
+    double sum = 0.;
+    for (int e = threadIdx.x; e < count; e += THREADS) {
+        int r, c;
+        place(e, r, c);
+        const double v = g.tall ? io.first(b, col0 + c, r) : io.first(b, r, col0 + c);
+        sum += v * v;
+    }
+    for (uint32_t at = threadIdx.x * 16; at < (uint32_t)(g.x_bytes + g.a_bytes); at += THREADS * 16)
+        *reinterpret_cast<uint4*>(gen + at) = make_uint4(0, 0, 0, 0);           // rows and columns of padding
+#pragma unroll
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    if (lane == 0) red[warp] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double t = 0.;
+        for (int w = 0; w < THREADS / 32; ++w) t += red[w];
+        red[8] = t;
+    }
+    __syncthreads();
+    if (g.cluster > 1) cluster_sync_all();
+    if (threadIdx.x == 0) {
+        double t = red[8];
+        if (g.cluster > 1) {
+            t = 0.;
+            for (int k = 0; k < g.cluster; ++k) t += ld_cluster_f64(mapa_cluster(base + (uint32_t)(g.x_bytes + g.a_bytes) + 64, (uint32_t)k));
+        }
+        scales_of(sqrt(t), st.eps, st.growth, pow2, &scales[0], &scales[1]);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    {
+        const double p2 = *pow2;
+        for (int e = threadIdx.x; e < count; e += THREADS) {
+            int r, c;
+            place(e, r, c);
+            const float v = (float)((double)(g.tall ? io.again(b, col0 + c, r) : io.again(b, r, col0 + c)) * p2);
+            __half hi, lo;
+            split_half(v, hi, lo);
+            uint8_t* at = gen + chunk_at(r, c) + 2 * (c & 7);
+            *reinterpret_cast<__half*>(at) = hi;
+            if (PLANES == 2) *reinterpret_cast<__half*>(at + x_plane) = lo;
+        }
+    }
+
+    // ---- one product: operands in shared memory, rows of 128; returns with the accumulator readable by every thread ----
+    const bool elected = warp == 0 && elect_one_sync();
+    uint32_t phase = 0;
+    // left: K-major panels from `left`; right: the same, or X as [K][N].  ksteps of 16, n columns
+    auto product = [&](uint32_t left, int left_plane, uint32_t right, int right_plane, bool mn, int ksteps, int n, int code) {
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncthreads();
+        if (warp == 0) {
+            tc_fence_after();
+            if (elected) {
+                const uint32_t idesc = (1u << 4) | ((mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+                for (int k = 0; k < ksteps; ++k) {
+                    const uint32_t kmaj = (uint32_t)((k >> 2) * PANEL + (k & 3) * 32);
+                    uint64_t l[PLANES], r[PLANES];
+#pragma unroll
+                    for (int p = 0; p < PLANES; ++p) {
+                        l[p] = make_smem_desc(left + (uint32_t)(p * left_plane) + kmaj);
+                        if (mn)
+                            r[p] = (make_smem_desc(right + (uint32_t)(p * right_plane) + (uint32_t)(k * 2048)) & ~((uint64_t)0x3fff << 16)) |
+                                   ((uint64_t)(PANEL >> 4) << 16);
+                        else
+                            r[p] = make_smem_desc(right + (uint32_t)(p * right_plane) + kmaj);
+                    }
+                    umma<CHEBYKAN_MODE_BF16>(tmem, l[0], r[0], idesc, k > 0);
+                    if (PLANES == 2) {
+                        umma<CHEBYKAN_MODE_BF16>(tmem + g.acc, l[0], r[PLANES - 1], idesc, k > 0);
+                        umma<CHEBYKAN_MODE_BF16>(tmem + g.acc, l[PLANES - 1], r[0], idesc, 1u);
+                    }
+                }
+                umma_commit(bar);
+            }
+            __syncwarp();
+        }
+        mbar_wait(bar, phase, abort_flag, status, code);
+        phase ^= 1u;
+        __syncwarp();
+        tc_fence_after();
+    };
+    const int q = warp & 3, half = warp >> 2;          // lanes of tensor memory, and which of two interleaved column groups
+    const int row = q * 32 + lane;
+    // visits the accumulator's columns 16 at a time: f(first column, values)
+    auto columns = [&](int n, auto f) {
+        for (int c = half * 16; c < n; c += 32) {
+            __syncwarp();                               // the loads are warp-collective
+            uint32_t v[16], w[16];
+            const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)c;
+            tmem_ld16(at, v);
+            if (PLANES == 2) tmem_ld16(at + g.acc, w);
+            tmem_ld_wait();
+            float x[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[e] = __uint_as_float(v[e]) + (PLANES == 2 ? __uint_as_float(w[e]) : 0.f);
+            f(c, x);
+        }
+    };
+    auto put = [&](uint32_t dst, int plane, int r, int c, const float (&x)[8]) {       // 8 columns of a row, both planes
+        __half hi[8], lo[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) split_half(x[e], hi[e], lo[e]);
+        const uint32_t at = dst + chunk_at(r, c);
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(half2_bits(hi[0], hi[1])), "r"(half2_bits(hi[2], hi[3])),
+                     "r"(half2_bits(hi[4], hi[5])), "r"(half2_bits(hi[6], hi[7])) : "memory");
+        if (PLANES == 2)
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at + (uint32_t)plane), "r"(half2_bits(lo[0], lo[1])),
+                         "r"(half2_bits(lo[2], lo[3])), "r"(half2_bits(lo[4], lo[5])), "r"(half2_bits(lo[6], lo[7])) : "memory");
+    };
+
+    const int npan = (cols + 63) / 64;
+    for (int k = 0; k < st.n; ++k) {
+        const float al = scales[k ? 1 : 0];
+        // A = X X^T
+        product(xs, x_plane, xs, x_plane, false, npan * 4, g.s16, ST_GRAM);
+        const float fa = al * al * exp2f((float)A_EXP);
+        if (g.cluster == 1) {
+            columns(g.s16, [&](int c, const float (&x)[16]) {
+                if (row >= g.s) return;
+#pragma unroll
+                for (int j = 0; j < 16; j += 8) {
+                    float y[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y[e] = x[j + e] * fa;
+                    put(as, a_plane, row, c + j, y);
+                }
+            });
+        } else {
+            // partial sums, rows (s16 + 4) floats apart: 16-byte accesses of 8 rows meet no bank twice
+            const int pitch = (g.s16 + 4) * 4;
+            columns(g.s16, [&](int c, const float (&x)[16]) {
+                if (row >= g.s) return;
+#pragma unroll
+                for (int j = 0; j < 16; j += 4)
+                    *reinterpret_cast<float4*>(gen + g.x_bytes + row * pitch + (c + j) * 4) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+            });
+            tc_fence_before();
+            __syncthreads();
+            cluster_sync_all();
+            // this CTA's band of rows, 8 columns per thread; a band of at most 64 rows x 16 groups is 4 per thread
+            const int band = (g.s + g.cluster - 1) / g.cluster, r0 = rank * band;
+            const int nrow = g.s - r0 < band ? (g.s - r0 > 0 ? g.s - r0 : 0) : band;
+            const int groups = g.s16 / 8, todo = nrow * groups;
+            float y[4][8];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int w = threadIdx.x + u * THREADS;
+                if (w < todo) {
+                    const uint32_t at = as + (uint32_t)((r0 + w / groups) * pitch + w % groups * 32);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y[u][e] = 0.f;
+                    for (int p = 0; p < g.cluster; ++p) {
+                        const uint32_t from = mapa_cluster(at, (uint32_t)p);
+                        const float4 v0 = ld_cluster_f4(from), v1 = ld_cluster_f4(from + 16);
+                        y[u][0] += v0.x; y[u][1] += v0.y; y[u][2] += v0.z; y[u][3] += v0.w;
+                        y[u][4] += v1.x; y[u][5] += v1.y; y[u][6] += v1.z; y[u][7] += v1.w;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y[u][e] *= fa;
+                }
+            }
+            cluster_sync_all();              // all partial sums are read: the buffer becomes A
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int w = threadIdx.x + u * THREADS;
+                if (w < todo) put(as, a_plane, r0 + w / groups, w % groups * 8, y[u]);
+            }
+            cluster_sync_all();
+            // the other bands; nobody overwrites its own before the barrier below is complete
+            for (int w = threadIdx.x; w < g.s * groups; w += THREADS) {
+                const int r = w / groups, owner = r / band;
+                if (owner == rank) continue;
+                const uint32_t at = as + chunk_at(r, w % groups * 8), from = mapa_cluster(at, (uint32_t)owner);
+#pragma unroll
+                for (int p = 0; p < PLANES; ++p) {
+                    const float4 v = ld_cluster_f4(from + (uint32_t)(p * a_plane));
+                    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at + (uint32_t)(p * a_plane)), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+                }
+            }
+            __syncwarp();
+            cluster_arrive();
+        }
+        // P = a I + b A + c A A
+        product(as, a_plane, as, a_plane, false, g.s16 / 16, g.s16, ST_POLY);
+        if (g.cluster > 1) cluster_wait();
+        columns(g.s16, [&](int c, const float (&x)[16]) {
+            if (row >= g.s) return;
+#pragma unroll
+            for (int j = 0; j < 16; j += 8) {
+                const uint32_t at = as + chunk_at(row, c + j);
+                uint32_t h[4], t[4];
+                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(at));
+                if (PLANES == 2)
+                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(t[0]), "=r"(t[1]), "=r"(t[2]), "=r"(t[3]) : "r"(at + (uint32_t)a_plane));
+                float y[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    float a = __half2float(__ushort_as_half((unsigned short)(h[e >> 1] >> (16 * (e & 1)))));
+                    if (PLANES == 2) a += __half2float(__ushort_as_half((unsigned short)(t[e >> 1] >> (16 * (e & 1)))));
+                    y[e] = fmaf(st.b * exp2f((float)(P_EXP - A_EXP)), a, x[j + e] * (st.c * exp2f((float)(P_EXP - 2 * A_EXP))));
+                    if (c + j + e == row) y[e] += st.a * exp2f((float)P_EXP);
+                }
+                put(as, a_plane, row, c + j, y);
+            }
+        });
+        // X' = P X
+        product(as, a_plane, xs, x_plane, true, g.s16 / 16, npan * 64, ST_APPLY);
+        const bool last = k + 1 == st.n;
+        const float fx = exp2f(-(float)P_EXP) * al / (last ? 1.f : scales[1]);
+        columns(npan * 64, [&](int c, const float (&x)[16]) {
+            if (row >= g.s) return;
+            if (last) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (c + e < cols) {
+                        if (g.tall) io.store(b, col0 + c + e, row, x[e] * fx);
+                        else io.store(b, row, col0 + c + e, x[e] * fx);
+                    }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 16; j += 8) {
+                    float y[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y[e] = x[j + e] * fx;
+                    put(xs, x_plane, row, c + j, y);
+                }
+            }
+        });
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (g.cluster > 1) cluster_sync_all();
+    if (warp == 0) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(tmem_cols) : "memory");
+    }
+}
+
+Geometry geometry(const Shape& sh, bool tall) {
+    Geometry g;
+    g.s = sh.s; g.l = sh.l; g.planes = sh.planes; g.tall = tall;
+    // as few CTAs as hold the matrix
+    g.cluster = 1;
+    while (g.cluster * MAX_SLICE < sh.l) g.cluster *= 2;
+    g.slice = (int)round_up(ceil_div(sh.l, g.cluster), 64);
+    while (g.cluster > 1 && (g.cluster - 1) * g.slice >= sh.l) --g.cluster;     // rounding may leave the last ones nothing
+    g.s16 = (int)round_up(sh.s, 16);
+    g.acc = 32;
+    while (g.acc < g.s16 || g.acc < g.slice) g.acc *= 2;
+    g.x_bytes = sh.planes * g.slice / 64 * PANEL;
+    const int operand = sh.planes * (int)ceil_div(g.s16, 64) * PANEL, partial = (int)round_up(128 * (g.s16 + 4) * 4, 1024);
+    g.a_bytes = g.cluster > 1 && partial > operand ? partial : operand;
+    return g;
+}
+
+template <class Io, int PLANES>
+int launch(const Io& io, const Geometry& g, int64_t batch, const Steps& st, int32_t* status, cudaStream_t s) {
+    constexpr int MOST = 2 * (MAX_SLICE / 64) * PANEL + 128 * 132 * 4 + 2048;
+    static bool ready[64] = {false};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) return CHEBYKAN_EINVAL;
+    auto kernel = small_kernel<Io, PLANES>;
+    if (!ready[dev]) {
+        const int rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST));
+        if (rc) return rc;
+        ready[dev] = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(batch * g.cluster)); cfg.blockDim = dim3(THREADS);
+    // A CTA that waits for tensor memory may not hold up a cluster whose other CTAs are waited for: kernels with clusters
+    // take more than half of an SM's shared memory, so that no two of them share one.
+    size_t smem = (size_t)(g.x_bytes + g.a_bytes + 128 + 1024);
+    if (g.cluster > 1 && smem < 116 * 1024) smem = 116 * 1024;
+    cfg.dynamicSmemBytes = smem; cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)g.cluster; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr; cfg.numAttrs = 1;
+    return check_cuda(cudaLaunchKernelEx(&cfg, kernel, io, g, st, status));
+}
+template <class Io>
+int launch_planes(const Io& io, const Geometry& g, int64_t batch, const Steps& st, int32_t* status, cudaStream_t s) {
+    return g.planes == 2 ? launch<Io, 2>(io, g, batch, st, status, s) : launch<Io, 1>(io, g, batch, st, status, s);
+}
+template <typename T>
+int orthogonalize_typed(const void* g, int64_t sb, int64_t sr, int64_t sc, void* out, int64_t m, int64_t n, const Shape& sh, const Steps& st,
+                        int32_t* status, cudaStream_t s) {
+    const OrthogonalizeIo<T> io{{reinterpret_cast<const T*>(g), sb, sr, sc}, reinterpret_cast<T*>(out), m, n};
+    return launch_planes(io, geometry(sh, m > n), sh.batch, st, status, s);
+}
+}  // namespace
+
+bool small_supported(const Shape& sh) { return sh.s <= 128 && sh.l <= MAX_CLUSTER * MAX_SLICE; }
+
+int launch_small_orthogonalize(const void* g, int dtype, int64_t sb, int64_t sr, int64_t sc, void* out, int64_t m, int64_t n, const Shape& sh,
+                               const Steps& st, int32_t* status, cudaStream_t s) {
+    if (dtype == CHEBYKAN_DTYPE_FP32) return orthogonalize_typed<float>(g, sb, sr, sc, out, m, n, sh, st, status, s);
+    if (dtype == CHEBYKAN_DTYPE_BF16) return orthogonalize_typed<__nv_bfloat16>(g, sb, sr, sc, out, m, n, sh, st, status, s);
+    return orthogonalize_typed<__half>(g, sb, sr, sc, out, m, n, sh, st, status, s);
+}
+int launch_small_muon(float* param, const float* grad, float* buf, int64_t in, int64_t out, int dp1, float keep, float step, float momentum,
+                      int nesterov, float gs, const Shape& sh, const Steps& st, int32_t* status, cudaStream_t s) {
+    const MuonIo io{param, grad, buf, out, dp1, nesterov, momentum, gs, keep, step};
+    return launch_planes(io, geometry(sh, in > out), dp1, st, status, s);
+}
+
+}  // namespace ns
+}  // namespace chebykan

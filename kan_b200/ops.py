@@ -481,6 +481,47 @@ def _require_any(t: torch.Tensor, name: str, dtype=None, device=None, contiguous
             raise RuntimeError(f"{name} must be 16-byte aligned")
 
 
+def _vector(t: torch.Tensor, name: str, size: int, device) -> int:
+    """Address of an fp32 vector of `size` elements."""
+    _require_any(t, name, torch.float32, device)
+    if t.numel() != size:
+        raise RuntimeError(f"{name} must have {size} elements")
+    return t.data_ptr()
+
+
+def _result(out: torch.Tensor | None, shape, dtype, device) -> torch.Tensor:
+    """`out` checked, or a new tensor of `dtype`."""
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    _require_any(out, "out", None, device)
+    if out.shape != shape:
+        raise RuntimeError(f"out must have shape {list(shape)}")
+    return out
+
+
+def _scratch(nbytes: int, what: str, device):
+    """(tensor, address) of a workspace; (None, None) for one of no bytes, which small calls then need not allocate."""
+    if nbytes <= 0:
+        _lib.check(nbytes, what)
+        return None, None
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return ws, ws.data_ptr()
+
+
+def _launch(name: str, device, *args) -> None:
+    """Library call `name`(*args, status, stream) on the current stream of `device`.  The smallest of these operators run
+    for a few microseconds, so the device is only switched where it has to be and no context manager is entered."""
+    idx = device.index
+    fn = getattr(_lib.load(), name)
+    if torch._C._cuda_getDevice() == idx and not _NVTX:
+        rc = fn(*args, status_tensor(device).data_ptr(), torch._C._cuda_getCurrentRawStream(idx))
+    else:
+        with _Range(name.replace("chebykan_", "chebykan.")), torch.cuda.device(device):
+            rc = fn(*args, status_tensor(device).data_ptr(), torch._C._cuda_getCurrentRawStream(idx))
+    if rc:
+        _lib.check(rc, name)
+
+
 def orthogonalize(g: torch.Tensor, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float = 1e-7, mode=None,
                   out: torch.Tensor | None = None) -> torch.Tensor:
     """Newton-Schulz orthogonalisation of a matrix [m, n] or a batch [b, m, n], any strides; the result is contiguous.
@@ -493,24 +534,17 @@ def orthogonalize(g: torch.Tensor, steps: int = 5, coefficients=NS_COEFFICIENTS,
     if g.dim() not in (2, 3):
         raise RuntimeError("g must have shape [m, n] or [batch, m, n]")
     dt = _dtype(g.dtype, "g")
-    if out is None:
-        out = torch.empty(g.shape, dtype=g.dtype, device=g.device)
-    else:
-        _require_any(out, "out", dtype=g.dtype, device=g.device)
-        if out.shape != g.shape:
-            raise RuntimeError(f"out must have shape {list(g.shape)}")
+    out = _result(out, g.shape, g.dtype, g.device)
+    if out.dtype != g.dtype:
+        raise RuntimeError("out must have the type of g")
     m = _mode(mode if mode is not None else ("tf32" if dt == _lib.DTYPE_BF16 else "fp32x3"))
     batch, rows, cols = (1, *g.shape) if g.dim() == 2 else g.shape
     sb, sr, sc = (0, *g.stride()) if g.dim() == 2 else g.stride()
-    lib = _lib.load()
-    ws_bytes = lib.chebykan_orthogonalize_workspace_bytes(batch, rows, cols, m)
-    _lib.check(ws_bytes, "chebykan_orthogonalize_workspace_bytes")
-    ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=g.device)
+    ws_bytes = _lib.load().chebykan_orthogonalize_workspace_bytes(batch, rows, cols, m)
+    ws, ws_ptr = _scratch(ws_bytes, "chebykan_orthogonalize_workspace_bytes", g.device)
     a, b, c = coefficients
-    with _Range("chebykan.orthogonalize"), torch.cuda.device(g.device):
-        rc = lib.chebykan_orthogonalize(g.data_ptr(), sb, sr, sc, dt, out.data_ptr(), ws.data_ptr(), ws_bytes, batch, rows,
-                                        cols, steps, a, b, c, eps, m, status_tensor(g.device).data_ptr(), _stream(g))
-    _lib.check(rc, "chebykan_orthogonalize")
+    _launch("chebykan_orthogonalize", g.device, g.data_ptr(), sb, sr, sc, dt, out.data_ptr(), ws_ptr, ws_bytes, batch, rows,
+            cols, steps, a, b, c, eps, m)
     return out
 
 
@@ -544,17 +578,12 @@ def muon_step(param: torch.Tensor, grad: torch.Tensor, momentum_buffer: torch.Te
     n_in, n_out = param.shape[:2]
     degree = param.shape[2] - 1 if param.dim() == 3 else 0
     m = _mode(mode)
-    lib = _lib.load()
-    ws_bytes = lib.chebykan_muon_workspace_bytes(n_in, n_out, degree, m)
-    _lib.check(ws_bytes, "chebykan_muon_workspace_bytes")
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=param.device)
+    ws_bytes = _lib.load().chebykan_muon_workspace_bytes(n_in, n_out, degree, m)
+    ws, ws_ptr = _scratch(ws_bytes, "chebykan_muon_workspace_bytes", param.device)
     a, b, c = coefficients
-    with _Range("chebykan.muon"), torch.cuda.device(param.device):
-        rc = lib.chebykan_muon_step(param.data_ptr(), grad.data_ptr(), momentum_buffer.data_ptr(), ws.data_ptr(), ws_bytes,
-                                    n_in, n_out, degree, lr, weight_decay, momentum, int(bool(nesterov)),
-                                    muon_scale(param.shape, adjust), steps, a, b, c, eps, grad_scale, m,
-                                    status_tensor(param.device).data_ptr(), _stream(param))
-    _lib.check(rc, "chebykan_muon_step")
+    _launch("chebykan_muon_step", param.device, param.data_ptr(), grad.data_ptr(), momentum_buffer.data_ptr(), ws_ptr, ws_bytes,
+            n_in, n_out, degree, lr, weight_decay, momentum, int(bool(nesterov)), muon_scale(param.shape, adjust), steps, a, b, c,
+            eps, grad_scale, m)
 
 
 # ---------------------------------------------------------------------------------------------------------------
@@ -603,13 +632,15 @@ def int8_basis(x: torch.Tensor, degree: int):
 
 def _require_int8(t: torch.Tensor, name: str, device=None) -> None:
     """int8 matrix on the GPU with adjacent columns; rows may be any distance apart."""
-    _require_any(t, name, dtype=torch.int8, device=device, contiguous=False)
+    _require_any(t, name, torch.int8, device, contiguous=False)
     if t.dim() != 2:
         raise RuntimeError(f"{name} must be a matrix")
-    if t.numel() and ((t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1])):
-        raise RuntimeError(f"the rows of {name} must be contiguous and may not overlap")
-    if t.numel() and t.data_ptr() % 16 != 0:
-        raise RuntimeError(f"{name} must be 16-byte aligned")
+    if t.numel():
+        (rows, cols), (sr, sc) = t.shape, t.stride()
+        if (cols > 1 and sc != 1) or (rows > 1 and sr < cols):
+            raise RuntimeError(f"the rows of {name} must be contiguous and may not overlap")
+        if t.data_ptr() % 16 != 0:
+            raise RuntimeError(f"{name} must be 16-byte aligned")
 
 
 def int8_matmul(q: torch.Tensor, q_scale: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor,
@@ -622,30 +653,16 @@ def int8_matmul(q: torch.Tensor, q_scale: torch.Tensor, wq: torch.Tensor, w_scal
     N = wq.shape[0]
     if wq.shape[1] != K:
         raise RuntimeError(f"q has {K} columns, wq {wq.shape[1]}")
-    for t, n, size in ((q_scale, "q_scale", M), (w_scale, "w_scale", N), (bias, "bias", N)):
-        if t is None and n == "bias":
-            continue
-        _require_any(t, n, dtype=torch.float32, device=q.device)
-        if t.numel() != size:
-            raise RuntimeError(f"{n} must have {size} elements")
-    if out is None:
-        out = torch.empty(M, N, dtype=out_dtype, device=q.device)
-    else:
-        _require_any(out, "out", device=q.device)
-        if out.shape != (M, N):
-            raise RuntimeError(f"out must have shape [{M}, {N}]")
-    dt = _dtype(out.dtype, "out")
-    ldq = q.stride(0) if M > 1 else max(K, 1)
-    ldw = wq.stride(0) if N > 1 else max(K, 1)
-    lib = _lib.load()
-    ws_bytes = lib.chebykan_int8_matmul_workspace_bytes(M, N, K, ldq, ldw)
-    _lib.check(ws_bytes, "chebykan_int8_matmul_workspace_bytes")
-    ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=q.device)
-    with _Range("chebykan.int8_matmul"), torch.cuda.device(q.device):
-        rc = lib.chebykan_int8_matmul(q.data_ptr(), ldq, q_scale.data_ptr(), wq.data_ptr(), ldw, w_scale.data_ptr(),
-                                      bias.data_ptr() if bias is not None else None, out.data_ptr(), dt, ws.data_ptr(),
-                                      ws_bytes, M, N, K, status_tensor(q.device).data_ptr(), _stream(q))
-    _lib.check(rc, "chebykan_int8_matmul")
+    device = q.device
+    qs, ws_, bs = (_vector(q_scale, "q_scale", M, device), _vector(w_scale, "w_scale", N, device),
+                   None if bias is None else _vector(bias, "bias", N, device))
+    out = _result(out, (M, N), out_dtype, device)
+    # the pitch of a single row does not matter
+    ldq, ldw = (t.stride(0) if t.shape[0] > 1 else -(-K // 16) * 16 for t in (q, wq))
+    ws_bytes = _lib.load().chebykan_int8_matmul_workspace_bytes(M, N, K, ldq, ldw)
+    ws, ws_ptr = _scratch(ws_bytes, "chebykan_int8_matmul_workspace_bytes", device)
+    _launch("chebykan_int8_matmul", device, q.data_ptr(), ldq, qs, wq.data_ptr(), ldw, ws_, bs, out.data_ptr(),
+            _dtype(out.dtype, "out"), ws_ptr, ws_bytes, M, N, K)
     return out
 
 
@@ -661,27 +678,13 @@ def int8_forward(x: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor, bias:
     if wq.dim() != 2 or wq.shape[1] != int8_width(n_in, degree):
         raise RuntimeError(f"wq must have shape [out, {int8_width(n_in, degree)}] for {n_in} inputs and degree {degree}")
     N = wq.shape[0]
-    for t, n in ((w_scale, "w_scale"), (bias, "bias")):
-        if t is None and n == "bias":
-            continue
-        _require_any(t, n, dtype=torch.float32, device=x.device)
-        if t.numel() != N:
-            raise RuntimeError(f"{n} must have {N} elements")
-    if out is None:
-        out = torch.empty(B, N, dtype=out_dtype, device=x.device)
-    else:
-        _require_any(out, "out", device=x.device)
-        if out.shape != (B, N):
-            raise RuntimeError(f"out must have shape [{B}, {N}]")
-    lib = _lib.load()
-    ws_bytes = lib.chebykan_int8_fwd_workspace_bytes(B, n_in, N, degree)
-    _lib.check(ws_bytes, "chebykan_int8_fwd_workspace_bytes")
-    ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=x.device)
-    with _Range("chebykan.int8_forward"), torch.cuda.device(x.device):
-        rc = lib.chebykan_int8_fwd(x.data_ptr(), _dtype(x.dtype, "x"), wq.data_ptr(), w_scale.data_ptr(),
-                                   bias.data_ptr() if bias is not None else None, out.data_ptr(), _dtype(out.dtype, "out"),
-                                   ws.data_ptr(), ws_bytes, B, n_in, N, degree, status_tensor(x.device).data_ptr(), _stream(x))
-    _lib.check(rc, "chebykan_int8_fwd")
+    device = x.device
+    ws_, bs = _vector(w_scale, "w_scale", N, device), None if bias is None else _vector(bias, "bias", N, device)
+    out = _result(out, (B, N), out_dtype, device)
+    ws_bytes = _lib.load().chebykan_int8_fwd_workspace_bytes(B, n_in, N, degree)
+    ws, ws_ptr = _scratch(ws_bytes, "chebykan_int8_fwd_workspace_bytes", device)
+    _launch("chebykan_int8_fwd", device, x.data_ptr(), _dtype(x.dtype, "x"), wq.data_ptr(), ws_, bs, out.data_ptr(),
+            _dtype(out.dtype, "out"), ws_ptr, ws_bytes, B, n_in, N, degree)
     return out
 
 

@@ -15,12 +15,13 @@ def lib(built_lib):
 
 def test_workspace_queries(lib):
     x3, tf32 = _lib.MODE_FP32X3, _lib.MODE_TF32
-    assert lib.chebykan_orthogonalize_workspace_bytes(1, 64, 64, x3) > lib.chebykan_orthogonalize_workspace_bytes(1, 64, 64, tf32) > 0
+    assert lib.chebykan_orthogonalize_workspace_bytes(1, 640, 640, x3) > lib.chebykan_orthogonalize_workspace_bytes(1, 640, 640, tf32) > 0
+    assert lib.chebykan_orthogonalize_workspace_bytes(3, 2048, 128, x3) == 0        # small matrices stay on chip
     assert lib.chebykan_orthogonalize_workspace_bytes(1, 64, 64, _lib.MODE_BF16) == -3
     assert lib.chebykan_orthogonalize_workspace_bytes(1, 64, 64, 9) == -1
     assert lib.chebykan_orthogonalize_workspace_bytes(1, 65537, 64, x3) == -1
     assert lib.chebykan_orthogonalize_workspace_bytes(65536, 64, 64, x3) == -1
-    assert lib.chebykan_muon_workspace_bytes(64, 64, 32, x3) > 0
+    assert lib.chebykan_muon_workspace_bytes(640, 640, 32, x3) > 0
     assert lib.chebykan_muon_workspace_bytes(64, 64, 128, x3) == -1
     assert lib.chebykan_muon_workspace_bytes(0, 64, 4, x3) == -1
     assert lib.chebykan_int8_matmul_workspace_bytes(5, 6, 131072, 131072, 131072) == -1      # the sum could overflow
@@ -32,7 +33,7 @@ def test_workspace_queries(lib):
 
 
 def orth(lib, **kw):
-    a = dict(g=P, sb=0, sr=64, sc=1, dtype=0, out=P, ws=P, ws_bytes=1 << 40, batch=1, m=64, n=64, steps=5, a=3.4445, b=-4.775,
+    a = dict(g=P, sb=0, sr=64, sc=1, dtype=0, out=P, ws=P, ws_bytes=1 << 40, batch=1, m=640, n=640, steps=5, a=3.4445, b=-4.775,
              c=2.0315, eps=1e-7, mode=_lib.MODE_FP32X3, status=P, stream=None)
     a.update(kw)
     return lib.chebykan_orthogonalize(*a.values())
@@ -40,30 +41,30 @@ def orth(lib, **kw):
 
 def test_orthogonalize_refuses(lib):
     for kw in (dict(sr=-1), dict(dtype=3), dict(steps=0), dict(steps=33), dict(eps=0.0), dict(eps=float("nan")), dict(g=None), dict(out=None),
-               dict(ws=None), dict(status=None), dict(mode=9), dict(batch=-1)):
+               dict(status=None), dict(mode=9), dict(batch=-1)):
         assert orth(lib, **kw) == -1, kw
     # coefficients under which singular values grow without bound, or are no numbers
     assert orth(lib, a=30.0) == -1 and orth(lib, a=float("nan")) == -1 and orth(lib, c=float("inf")) == -1
     assert orth(lib, mode=_lib.MODE_FP32) == -3
     assert orth(lib, out=P + 4) == -2 and orth(lib, ws=P + 8) == -2
-    assert orth(lib, ws_bytes=100) == -6
+    assert orth(lib, ws_bytes=100) == -6 and orth(lib, ws=None) == -6
     assert orth(lib, batch=0) == 0 and orth(lib, m=0, g=None) == 0
 
 
 def muon(lib, **kw):
-    a = dict(param=P, grad=P, buf=P, ws=P, ws_bytes=1 << 40, n_in=64, n_out=64, deg=4, lr=0.1, wd=0.1, mu=0.95, nesterov=1, scale=1.0,
+    a = dict(param=P, grad=P, buf=P, ws=P, ws_bytes=1 << 40, n_in=640, n_out=640, deg=4, lr=0.1, wd=0.1, mu=0.95, nesterov=1, scale=1.0,
              steps=5, a=3.4445, b=-4.775, c=2.0315, eps=1e-7, gs=1.0, mode=_lib.MODE_FP32X3, status=P, stream=None)
     a.update(kw)
     return lib.chebykan_muon_step(*a.values())
 
 
 def test_muon_step_refuses(lib):
-    for kw in (dict(param=None), dict(grad=None), dict(buf=None), dict(ws=None), dict(status=None), dict(deg=-1), dict(deg=128), dict(n_in=0),
+    for kw in (dict(param=None), dict(grad=None), dict(buf=None), dict(status=None), dict(deg=-1), dict(deg=128), dict(n_in=0),
                dict(mu=1.0), dict(mu=-0.1), dict(mu=float("nan")), dict(steps=0), dict(eps=-1.0), dict(b=40.0)):
         assert muon(lib, **kw) == -1, kw
     assert muon(lib, mode=_lib.MODE_BF16) == -3
     assert muon(lib, grad=P + 4) == -2
-    assert muon(lib, ws_bytes=100) == -6
+    assert muon(lib, ws_bytes=100) == -6 and muon(lib, ws=None) == -6
 
 
 def test_int8_refuses(lib):
