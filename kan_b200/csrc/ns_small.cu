@@ -30,7 +30,7 @@ enum { ST_GRAM = 31, ST_POLY = 32, ST_APPLY = 33 };
 
 struct Geometry {
     int s, l;
-    int cluster, slice;      // CTAs per matrix, columns per CTA (a multiple of 64)
+    int cluster, slice;      // CTAs per matrix, columns per CTA (a multiple of 16)
     int s16, acc;            // rows rounded up to 16; columns of one accumulator
     int planes, tall;
     int x_bytes, a_bytes;    // shared memory: X planes, and the buffer of A / P / partial sums
@@ -63,15 +63,22 @@ __device__ __forceinline__ uint32_t half2_bits(__half x, __half y) {
     return (uint32_t)__half_as_ushort(x) | ((uint32_t)__half_as_ushort(y) << 16);
 }
 
-// ---- the two uses: where elements come from and where results go ----
+// ---- the two uses: where elements come from and where results go.  Elements are addressed by their offset; what a batch of
+// them needs from memory is fetched before any of it is used, so that the latencies overlap. ----
 template <typename T>
 struct OrthogonalizeIo {
     StridedSource<T> src;
     T* out;
     int64_t m, n;
-    __device__ __forceinline__ double first(int64_t b, int64_t r, int64_t c) const { return (double)src.load(b, r, c); }
-    __device__ __forceinline__ float again(int64_t b, int64_t r, int64_t c) const { return src.load(b, r, c); }
-    __device__ __forceinline__ void store(int64_t b, int64_t r, int64_t c, float v) const { out[(b * m + r) * n + c] = from_float<T>(v); }
+    struct Raw { T g; };
+    struct Old {};
+    __device__ __forceinline__ int64_t in_at(int64_t b, int64_t r, int64_t c) const { return b * src.sb + r * src.sr + c * src.sc; }
+    __device__ __forceinline__ Raw fetch(int64_t e) const { return {src.g[e]}; }
+    __device__ __forceinline__ double first(int64_t, const Raw& v) const { return (double)(float)v.g; }
+    __device__ __forceinline__ float again(const Raw& v) const { return (float)v.g; }
+    __device__ __forceinline__ int64_t out_at(int64_t b, int64_t r, int64_t c) const { return (b * m + r) * n + c; }
+    __device__ __forceinline__ Old fetch_out(int64_t) const { return {}; }
+    __device__ __forceinline__ void store(int64_t e, const Old&, float v) const { out[e] = from_float<T>(v); }
 };
 struct MuonIo {
     float* param;
@@ -80,25 +87,21 @@ struct MuonIo {
     int64_t out;
     int dp1, nesterov;
     float momentum, gs, keep, step;
-    __device__ __forceinline__ float update(int64_t e, float m) const {
-        const float g = grad[e] * gs;
-        return nesterov ? fmaf(momentum, m - g, g) : m;
-    }
+    struct Raw { float g, m; };
+    struct Old { float p; };
+    __device__ __forceinline__ int64_t in_at(int64_t b, int64_t r, int64_t c) const { return (r * out + c) * dp1 + b; }
+    __device__ __forceinline__ Raw fetch(int64_t e) const { return {grad[e] * gs, buf[e]}; }
+    __device__ __forceinline__ float update(float g, float m) const { return nesterov ? fmaf(momentum, m - g, g) : m; }
     // the first visit moves the momentum; the second, by the same thread, finds it moved
-    __device__ __forceinline__ double first(int64_t b, int64_t r, int64_t c) const {
-        const int64_t e = (r * out + c) * dp1 + b;
-        const float old = buf[e], m = fmaf(1.f - momentum, grad[e] * gs - old, old);
+    __device__ __forceinline__ double first(int64_t e, const Raw& v) const {
+        const float m = fmaf(1.f - momentum, v.g - v.m, v.m);
         buf[e] = m;
-        return (double)update(e, m);
+        return (double)update(v.g, m);
     }
-    __device__ __forceinline__ float again(int64_t b, int64_t r, int64_t c) const {
-        const int64_t e = (r * out + c) * dp1 + b;
-        return update(e, buf[e]);
-    }
-    __device__ __forceinline__ void store(int64_t b, int64_t r, int64_t c, float v) const {
-        const int64_t e = (r * out + c) * dp1 + b;
-        param[e] = fmaf(-step, v, keep * param[e]);
-    }
+    __device__ __forceinline__ float again(const Raw& v) const { return update(v.g, v.m); }
+    __device__ __forceinline__ int64_t out_at(int64_t b, int64_t r, int64_t c) const { return in_at(b, r, c); }
+    __device__ __forceinline__ Old fetch_out(int64_t e) const { return {param[e]}; }
+    __device__ __forceinline__ void store(int64_t e, const Old& old, float v) const { param[e] = fmaf(-step, v, keep * old.p); }
 };
 
 template <class Io, int PLANES>
@@ -140,13 +143,30 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io io, const Ge
     auto place = [&](int e, int& r, int& c) {
         if (g.tall) { c = e / g.s; r = e - c * g.s; } else { r = e / cols; c = e - r * cols; }
     };
+    constexpr int U = 8;
+    // f(place in the slice, offset in memory, what was fetched) for this thread's elements, U fetches in flight
+    auto elements = [&](auto f) {
+        for (int e0 = threadIdx.x; e0 < count; e0 += U * THREADS) {
+            int r[U], c[U];
+            int64_t at[U];
+            typename Io::Raw raw[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (e0 + u * THREADS < count) {
+                    place(e0 + u * THREADS, r[u], c[u]);
+                    at[u] = g.tall ? io.in_at(b, col0 + c[u], r[u]) : io.in_at(b, r[u], col0 + c[u]);
+                    raw[u] = io.fetch(at[u]);
+                }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (e0 + u * THREADS < count) f(r[u], c[u], at[u], raw[u]);
+        }
+    };
     double sum = 0.;
-    for (int e = threadIdx.x; e < count; e += THREADS) {
-        int r, c;
-        place(e, r, c);
-        const double v = g.tall ? io.first(b, col0 + c, r) : io.first(b, r, col0 + c);
+    elements([&](int, int, int64_t at, const typename Io::Raw& raw) {
+        const double v = io.first(at, raw);
         sum += v * v;
-    }
+    });
     for (uint32_t at = threadIdx.x * 16; at < (uint32_t)(g.x_bytes + g.a_bytes); at += THREADS * 16)
         *reinterpret_cast<uint4*>(gen + at) = make_uint4(0, 0, 0, 0);           // rows and columns of padding
 #pragma unroll
@@ -174,16 +194,13 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io io, const Ge
     const uint32_t tmem = *tmem_slot;
     {
         const double p2 = *pow2;
-        for (int e = threadIdx.x; e < count; e += THREADS) {
-            int r, c;
-            place(e, r, c);
-            const float v = (float)((double)(g.tall ? io.again(b, col0 + c, r) : io.again(b, r, col0 + c)) * p2);
+        elements([&](int r, int c, int64_t, const typename Io::Raw& raw) {
             __half hi, lo;
-            split_half(v, hi, lo);
+            split_half((float)((double)io.again(raw) * p2), hi, lo);
             uint8_t* at = gen + chunk_at(r, c) + 2 * (c & 7);
             *reinterpret_cast<__half*>(at) = hi;
             if (PLANES == 2) *reinterpret_cast<__half*>(at + x_plane) = lo;
-        }
+        });
     }
 
     // ---- one product: operands in shared memory, rows of 128; returns with the accumulator readable by every thread ----
@@ -254,11 +271,11 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io io, const Ge
                          "r"(half2_bits(lo[2], lo[3])), "r"(half2_bits(lo[4], lo[5])), "r"(half2_bits(lo[6], lo[7])) : "memory");
     };
 
-    const int npan = (cols + 63) / 64;
+    const int cols16 = (cols + 15) & ~15;
     for (int k = 0; k < st.n; ++k) {
         const float al = scales[k ? 1 : 0];
         // A = X X^T
-        product(xs, x_plane, xs, x_plane, false, npan * 4, g.s16, ST_GRAM);
+        product(xs, x_plane, xs, x_plane, false, cols16 / 16, g.s16, ST_GRAM);
         const float fa = al * al * exp2f((float)A_EXP);
         if (g.cluster == 1) {
             columns(g.s16, [&](int c, const float (&x)[16]) {
@@ -283,9 +300,10 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io io, const Ge
             tc_fence_before();
             __syncthreads();
             cluster_sync_all();
-            // this CTA's band of rows, 8 columns per thread; a band of at most 64 rows x 16 groups is 4 per thread
-            const int band = (g.s + g.cluster - 1) / g.cluster, r0 = rank * band;
-            const int nrow = g.s - r0 < band ? (g.s - r0 > 0 ? g.s - r0 : 0) : band;
+            // this CTA's band of rows, 8 columns per thread; a band of at most 64 rows x 16 groups is 4 per thread.  Rows
+            // from s to s16 become zero: the next product reads them, and the partial sums have been lying there.
+            const int band = (g.s16 + g.cluster - 1) / g.cluster, r0 = rank * band;
+            const int nrow = g.s16 - r0 < band ? (g.s16 - r0 > 0 ? g.s16 - r0 : 0) : band;
             const int groups = g.s16 / 8, todo = nrow * groups;
             float y[4][8];
 #pragma unroll
@@ -295,14 +313,14 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io io, const Ge
                     const uint32_t at = as + (uint32_t)((r0 + w / groups) * pitch + w % groups * 32);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) y[u][e] = 0.f;
-                    for (int p = 0; p < g.cluster; ++p) {
+                    for (int p = 0; p < g.cluster && r0 + w / groups < g.s; ++p) {
                         const uint32_t from = mapa_cluster(at, (uint32_t)p);
                         const float4 v0 = ld_cluster_f4(from), v1 = ld_cluster_f4(from + 16);
                         y[u][0] += v0.x; y[u][1] += v0.y; y[u][2] += v0.z; y[u][3] += v0.w;
                         y[u][4] += v1.x; y[u][5] += v1.y; y[u][6] += v1.z; y[u][7] += v1.w;
                     }
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) y[u][e] *= fa;
+                    for (int e = 0; e < 8; ++e) y[u][e] = r0 + w / groups < g.s ? y[u][e] * fa : 0.f;
                 }
             }
             cluster_sync_all();              // all partial sums are read: the buffer becomes A
@@ -313,7 +331,7 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io io, const Ge
             }
             cluster_sync_all();
             // the other bands; nobody overwrites its own before the barrier below is complete
-            for (int w = threadIdx.x; w < g.s * groups; w += THREADS) {
+            for (int w = threadIdx.x; w < g.s16 * groups; w += THREADS) {
                 const int r = w / groups, owner = r / band;
                 if (owner == rank) continue;
                 const uint32_t at = as + chunk_at(r, w % groups * 8), from = mapa_cluster(at, (uint32_t)owner);
@@ -350,18 +368,21 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io io, const Ge
             }
         });
         // X' = P X
-        product(as, a_plane, xs, x_plane, true, g.s16 / 16, npan * 64, ST_APPLY);
+        product(as, a_plane, xs, x_plane, true, g.s16 / 16, cols16, ST_APPLY);
         const bool last = k + 1 == st.n;
         const float fx = exp2f(-(float)P_EXP) * al / (last ? 1.f : scales[1]);
-        columns(npan * 64, [&](int c, const float (&x)[16]) {
+        columns(cols16, [&](int c, const float (&x)[16]) {
             if (row >= g.s) return;
             if (last) {
+                typename Io::Old old[16];
+                const int64_t at = g.tall ? io.out_at(b, col0 + c, row) : io.out_at(b, row, col0 + c);
+                const int64_t pitch = g.tall ? io.out_at(b, 1, 0) - io.out_at(b, 0, 0) : io.out_at(b, 0, 1) - io.out_at(b, 0, 0);
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
-                    if (c + e < cols) {
-                        if (g.tall) io.store(b, col0 + c + e, row, x[e] * fx);
-                        else io.store(b, row, col0 + c + e, x[e] * fx);
-                    }
+                    if (c + e < cols) old[e] = io.fetch_out(at + e * pitch);
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (c + e < cols) io.store(at + e * pitch, old[e], x[e] * fx);
             } else {
 #pragma unroll
                 for (int j = 0; j < 16; j += 8) {
@@ -386,15 +407,16 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io io, const Ge
 Geometry geometry(const Shape& sh, bool tall) {
     Geometry g;
     g.s = sh.s; g.l = sh.l; g.planes = sh.planes; g.tall = tall;
-    // as few CTAs as hold the matrix
-    g.cluster = 1;
-    while (g.cluster * MAX_SLICE < sh.l) g.cluster *= 2;
-    g.slice = (int)round_up(ceil_div(sh.l, g.cluster), 64);
-    while (g.cluster > 1 && (g.cluster - 1) * g.slice >= sh.l) --g.cluster;     // rounding may leave the last ones nothing
+    // slices of 128 columns while that leaves SMs idle (a thread's share of the reading is what they divide), else as few
+    // CTAs as hold the matrix
+    g.cluster = (int)ceil_div(sh.l, MAX_SLICE / 2);
+    if (g.cluster > MAX_CLUSTER || (int64_t)g.cluster * sh.batch > 148) g.cluster = (int)ceil_div(sh.l, MAX_SLICE);
+    g.slice = (int)round_up(ceil_div(sh.l, g.cluster), 16);
+    g.cluster = (int)ceil_div(sh.l, g.slice);                                    // rounding may leave the last one nothing
     g.s16 = (int)round_up(sh.s, 16);
     g.acc = 32;
     while (g.acc < g.s16 || g.acc < g.slice) g.acc *= 2;
-    g.x_bytes = sh.planes * g.slice / 64 * PANEL;
+    g.x_bytes = sh.planes * (int)ceil_div(g.slice, 64) * PANEL;
     const int operand = sh.planes * (int)ceil_div(g.s16, 64) * PANEL, partial = (int)round_up(128 * (g.s16 + 4) * 4, 1024);
     g.a_bytes = g.cluster > 1 && partial > operand ? partial : operand;
     return g;
