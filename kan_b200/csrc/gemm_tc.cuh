@@ -1,5 +1,6 @@
 // D[M][N] = L[M][K] R on tcgen05, for 16-bit floating and 8-bit integer operands: the pipeline shared by the products of
-// the Newton-Schulz steps and of the 8-bit forward.  What happens to the accumulator is the epilogue's, a template argument.
+// the Newton-Schulz steps and of the 8-bit forward.  What happens to the accumulator is the epilogue's, a template argument: emit() takes NC
+// columns of a row, fetch() asks one step earlier for what emit() will read from memory.
 //
 //   warp 0     TMA: one stage = 128 bytes of K of the tile's L rows (128 per CTA) and of R, 128-byte swizzle, no multicast.
 //              R is either [N][K] (K-major) or [K][N] (boxes of 64 K rows x 64 columns, read through an MN-major descriptor)
@@ -105,6 +106,13 @@ __device__ __forceinline__ void load_3d_pair(uint32_t dst, const CUtensorMap* ma
     asm volatile(
         "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
         ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr) : "memory");
 }
 // operand of [K][N] boxes: 64 columns per 128-byte row, rows are K; 8-row groups 1024 bytes apart, the next 64 columns
 // one box (64 rows, 8192 bytes) further
@@ -267,6 +275,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ C
             int ncols = g.N - n0;
             if (ncols > BN) ncols = BN;
             const int nch = (ncols + 31) >> 5;
+            typename Epi::template Fetched<32> fa, fb;
+            Epi::template fetch<32>(args, g, b, row, n0, fa);      // in flight while the MMAs run
             if constexpr (C::PP == 3) {
                 float v[BN];
                 for (int kb0 = 0; kb0 < g.nkb; kb0 += C::KCHUNK) {
@@ -275,16 +285,16 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ C
                     tc_fence_after();
                     const uint32_t ta = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * C::ACC_COLS);
 #pragma unroll
-                    for (int c = 0; c < BN / 32; ++c)
-                        if (c < nch) {
-                            uint32_t r0[32], r1[32];
-                            tmem_ld32(ta + c * 32, r0);
-                            tmem_ld32(ta + BN + c * 32, r1);
+                    for (int c = 0; c < BN / 16; ++c)
+                        if (c < 2 * nch) {
+                            uint32_t r0[16], r1[16];
+                            tmem_ld16(ta + c * 16, r0);
+                            tmem_ld16(ta + BN + c * 16, r1);
                             tmem_ld_wait();
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) {
+                            for (int e = 0; e < 16; ++e) {
                                 const float part = __uint_as_float(r0[e]) + __uint_as_float(r1[e]);
-                                v[c * 32 + e] = kb0 == 0 ? part : v[c * 32 + e] + part;
+                                v[c * 16 + e] = kb0 == 0 ? part : v[c * 16 + e] + part;
                             }
                         }
                     release(acc);
@@ -298,7 +308,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ C
                         uint32_t r[32];
 #pragma unroll
                         for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(v[c * 32 + e]);
-                        Epi::template emit<32>(args, g, b, row, n0 + c * 32, r, mirrored(n0 + c * 32));
+                        if (c + 1 < BN / 32) Epi::template fetch<32>(args, g, b, row, n0 + (c + 1) * 32, c & 1 ? fa : fb);
+                        Epi::template emit<32>(args, g, b, row, n0 + c * 32, r, mirrored(n0 + c * 32), c & 1 ? fb : fa);
                     }
             } else {
                 const bool ok = mbar_wait(acc_full(acc), acc_ph, abort_flag, status, ST_EPILOGUE);
@@ -311,12 +322,22 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ C
 #pragma unroll 1
                 for (int c = 0; c < nch; c += 2) {
                     tmem_ld_wait();
-                    if (c + 1 < nch) tmem_ld32(ta + (c + 1) * 32, rb); else release(acc);
-                    Epi::template emit<32>(args, g, b, row, n0 + c * 32, ra, mirrored(n0 + c * 32));
+                    if (c + 1 < nch) {
+                        tmem_ld32(ta + (c + 1) * 32, rb);
+                        Epi::template fetch<32>(args, g, b, row, n0 + (c + 1) * 32, fb);
+                    } else {
+                        release(acc);
+                    }
+                    Epi::template emit<32>(args, g, b, row, n0 + c * 32, ra, mirrored(n0 + c * 32), fa);
                     if (c + 1 < nch) {
                         tmem_ld_wait();
-                        if (c + 2 < nch) tmem_ld32(ta + (c + 2) * 32, ra); else release(acc);
-                        Epi::template emit<32>(args, g, b, row, n0 + (c + 1) * 32, rb, mirrored(n0 + (c + 1) * 32));
+                        if (c + 2 < nch) {
+                            tmem_ld32(ta + (c + 2) * 32, ra);
+                            Epi::template fetch<32>(args, g, b, row, n0 + (c + 2) * 32, fa);
+                        } else {
+                            release(acc);
+                        }
+                        Epi::template emit<32>(args, g, b, row, n0 + (c + 1) * 32, rb, mirrored(n0 + (c + 1) * 32), fb);
                     }
                 }
                 acc ^= 1;
@@ -539,7 +560,9 @@ split_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ 
                 }
             }
             const int row = m0 + lrow;
-            Epi::template emit<8>(args, g, b, row, n0 + col, sum, g.sym && (row / BN + 1) * BN <= (n0 + col) / C::BM * C::BM);
+            typename Epi::template Fetched<8> f;
+            Epi::template fetch<8>(args, g, b, row, n0 + col, f);
+            Epi::template emit<8>(args, g, b, row, n0 + col, sum, g.sym && (row / BN + 1) * BN <= (n0 + col) / C::BM * C::BM, f);
         }
     }
     __syncthreads();

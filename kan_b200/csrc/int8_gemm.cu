@@ -21,8 +21,13 @@ struct EpiArgs {
 template <typename OUT>
 struct Epilogue {
     using Args = EpiArgs;
+    struct Nothing {};
+    template <int NC> using Fetched = Nothing;
     template <int NC>
-    static __device__ __forceinline__ void emit(const Args& p, const Tiles& g, int, int row, int col0, uint32_t (&r)[NC], bool) {
+    static __device__ __forceinline__ void fetch(const Args&, const Tiles&, int, int, int, Nothing&) {}
+    template <int NC>
+    static __device__ __forceinline__ void emit(const Args& p, const Tiles& g, int, int row, int col0, uint32_t (&r)[NC], bool,
+                                                const Nothing&) {
         if (row >= g.M) return;
         const float qs = __ldg(p.q_scale + row);
         OUT* dst = reinterpret_cast<OUT*>(p.y) + (int64_t)row * g.N + col0;
@@ -30,7 +35,7 @@ struct Epilogue {
         const bool vec = g.N % V == 0;
 #pragma unroll
         for (int c = 0; c < NC; c += V) {
-            OUT out[V];
+            alignas(16) OUT out[V];
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 const int col = col0 + c + e;

@@ -25,101 +25,214 @@ __device__ __forceinline__ double block_sum(double v, double* smem) {
     return t;
 }
 
-// partial[b][block] = sum of squares (in double: no gradient's square over- or underflows, and the sum over millions of
-// elements keeps its digits)
+// A matrix as rows that lie closest together in memory: element (r, c) at r*pitch + c*step, step <= pitch.
+struct Plane {
+    int64_t rows, cols, pitch, step, batch;       // batch: distance of matrices
+};
+
+__device__ __forceinline__ float load1(const float* p) { return *p; }
+__device__ __forceinline__ float load1(const __half* p) { return __half2float(*p); }
+__device__ __forceinline__ float load1(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+
+// eight neighbours from p: one or two 16-byte loads where p allows (the address is the same modulo 16 for a whole matrix,
+// or the branch is a coin that all threads throw alike), else eight loads; values past `left` are zero
 template <typename T>
-__global__ void __launch_bounds__(256) norm_kernel(StridedSource<T> src, int64_t m, int64_t n, double* partial) {
+__device__ __forceinline__ void load8(const T* p, int64_t step, int64_t left, float (&v)[8]) {
+    if (step == 1 && left >= 8 && (reinterpret_cast<uintptr_t>(p) & 15u) == 0) {
+        alignas(16) T t[8];
+        *reinterpret_cast<uint4*>(t) = *reinterpret_cast<const uint4*>(p);
+        if (sizeof(T) == 4) *reinterpret_cast<uint4*>(t + 8 - 16 / sizeof(T)) = *reinterpret_cast<const uint4*>(p + 8 - 16 / sizeof(T));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = load1(t + e);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = e < left ? load1(p + e * step) : 0.f;
+    }
+}
+
+// partial[b][block] = sum of squares (in double: no gradient's square over- or underflows, and the sum over millions of
+// elements keeps its digits).  Two groups of eight elements per thread in flight.
+template <typename T>
+__global__ void __launch_bounds__(256) norm_kernel(const T* __restrict__ g, const Plane pl, double* __restrict__ partial) {
     __shared__ double smem[8];
+    const T* src = g + blockIdx.y * pl.batch;
+    const int64_t groups = (pl.cols + 7) / 8, total = pl.rows * groups, stride = (int64_t)gridDim.x * 256;
     double v = 0.;
-    for (int64_t e = blockIdx.x * 256 + threadIdx.x; e < m * n; e += (int64_t)gridDim.x * 256) {
-        const double g = src.load(blockIdx.y, e / n, e % n);
-        v += g * g;
+    for (int64_t e = blockIdx.x * 256 + threadIdx.x; e < total; e += 2 * stride) {
+        float x[2][8];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int64_t w = e + u * stride, r = w / groups, c = (w - r * groups) * 8;
+            if (w < total) load8(src + r * pl.pitch + c * pl.step, pl.step, pl.cols - c, x[u]);
+            else
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[u][k] = 0.f;
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v = fma((double)x[u][k], (double)x[u][k], v);
     }
     v = block_sum(v, smem);
     if (threadIdx.x == 0) partial[blockIdx.y * NORM_BLOCKS + blockIdx.x] = v;
 }
 
-// momentum update of the whole tensor and, per degree, the partial sums of squares of the update u.  The active threads
-// are a multiple of deg+1, so a thread stays on one degree as the block strides along the contiguous tensor.
+// Momentum of the whole tensor, and the update u turned from [in*out][deg+1] to a plane per degree, through a tile in shared
+// memory (deg+1 made odd, so that a column of it meets every bank): both sides are contiguous.  With `partial` also the
+// sums of squares of each degree's u.
+// deg+1 up to 40: 256 elements of every degree in a tile, above: 64 (42 KB at most)
+__host__ __device__ constexpr int tile_width(int dp1) { return dp1 <= 40 ? 256 : 64; }
+
 __global__ void __launch_bounds__(256)
-momentum_kernel(const float* __restrict__ grad, float* __restrict__ buf, int64_t n, int dp1, float momentum, int nesterov,
-                float gs, double* __restrict__ partial) {
-    __shared__ double smem[256];
-    const int active = 256 / dp1 * dp1;
-    double v = 0.;
-    if ((int)threadIdx.x < active)
-        for (int64_t e = blockIdx.x * (int64_t)active + threadIdx.x; e < n; e += (int64_t)gridDim.x * active) {
-            const float g = grad[e] * gs;
-            const float m = fmaf(1.f - momentum, g - buf[e], buf[e]);
-            buf[e] = m;
-            const double u = nesterov ? fmaf(momentum, m - g, g) : m;
-            v += u * u;
+momentum_kernel(const float* __restrict__ grad, float* __restrict__ buf, float* __restrict__ u, int64_t pairs, int dp1, float momentum,
+                int nesterov, float gs, double* __restrict__ partial) {
+    extern __shared__ float tile[];
+    __shared__ double sums[128];
+    const int width = tile_width(dp1), odd = dp1 | 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int d = threadIdx.x; d < dp1; d += 256) sums[d] = 0.;
+    const int64_t tiles = (pairs + width - 1) / width;
+    for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
+        const int64_t p0 = t * width;
+        const int count = (int)((pairs - p0 < width ? pairs - p0 : width) * dp1);
+        __syncthreads();                           // the tile is free
+        for (int e0 = threadIdx.x; e0 < count; e0 += 4 * 256) {
+            float g[4], m[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (e0 + k * 256 < count) { g[k] = grad[p0 * dp1 + e0 + k * 256] * gs; m[k] = buf[p0 * dp1 + e0 + k * 256]; }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int e = e0 + k * 256;
+                if (e < count) {
+                    m[k] = fmaf(1.f - momentum, g[k] - m[k], m[k]);
+                    buf[p0 * dp1 + e] = m[k];
+                    tile[e / dp1 * odd + e % dp1] = nesterov ? fmaf(momentum, m[k] - g[k], g[k]) : m[k];
+                }
+            }
         }
-    smem[threadIdx.x] = v;
+        __syncthreads();
+        const int n = count / dp1;
+        for (int d = warp; d < dp1; d += 8) {
+            double v = 0.;
+            for (int w = lane; w < n; w += 32) {
+                const float x = tile[w * odd + d];
+                u[d * pairs + p0 + w] = x;
+                v = fma((double)x, (double)x, v);
+            }
+            if (partial != nullptr) {
+#pragma unroll
+                for (int k = 16; k; k >>= 1) v += __shfl_down_sync(0xffffffffu, v, k);
+                if (lane == 0) sums[d] += v;       // only this warp touches degree d
+            }
+        }
+    }
     __syncthreads();
-    if ((int)threadIdx.x < dp1) {
-        double t = 0.;
-        for (int k = threadIdx.x; k < active; k += dp1) t += smem[k];
-        partial[(int64_t)threadIdx.x * NORM_BLOCKS + blockIdx.x] = t;
+    if (partial != nullptr)
+        for (int d = threadIdx.x; d < dp1; d += 256) partial[(int64_t)d * NORM_BLOCKS + blockIdx.x] = sums[d];
+}
+
+// param = keep * param - step * O, O one plane per degree: the same tile the other way
+__global__ void __launch_bounds__(256)
+update_kernel(float* __restrict__ param, const float* __restrict__ o, int64_t pairs, int dp1, float keep, float step) {
+    extern __shared__ float tile[];
+    const int width = tile_width(dp1), odd = dp1 | 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t tiles = (pairs + width - 1) / width;
+    for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
+        const int64_t p0 = t * width;
+        const int n = (int)(pairs - p0 < width ? pairs - p0 : width), count = n * dp1;
+        __syncthreads();
+        for (int d = warp; d < dp1; d += 8) {
+            float x[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (lane + k * 32 < n) x[k] = o[d * pairs + p0 + lane + k * 32];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (lane + k * 32 < n) tile[(lane + k * 32) * odd + d] = x[k];
+        }
+        __syncthreads();
+        for (int e0 = threadIdx.x; e0 < count; e0 += 4 * 256) {
+            float p[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (e0 + k * 256 < count) p[k] = param[p0 * dp1 + e0 + k * 256];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int e = e0 + k * 256;
+                if (e < count) param[p0 * dp1 + e] = fmaf(-step, tile[e / dp1 * odd + e % dp1], keep * p[k]);
+            }
+        }
     }
 }
 
-// X_0 planes of one matrix tile: 32 x 32 elements, transposed on the way where the matrix is tall
-template <typename Src>
+// the scales of matrix b from its partial sums, by one warp
+__device__ __forceinline__ void warp_scales(const double* partial, float eps, int growth, double* pow2, float* alpha, float* later) {
+    double t = 0.;
+    for (int k = threadIdx.x & 31; k < NORM_BLOCKS; k += 32) t += partial[k];
+#pragma unroll
+    for (int d = 16; d; d >>= 1) t += __shfl_down_sync(0xffffffffu, t, d);
+    if ((threadIdx.x & 31) == 0) scales_of(sqrt(t), eps, growth, pow2, alpha, later);
+}
+
+// X_0 planes where X's rows are the rows of the source: eight columns per thread
+template <typename T, int PLANES>
 __global__ void __launch_bounds__(256)
-pack_kernel(Src src, int64_t m, int64_t n, __half* __restrict__ x, float* __restrict__ alpha, const double* __restrict__ partial,
-            float eps, int growth, Shape sh) {
-    __shared__ float tile[32][33];
+pack_rows_kernel(const T* __restrict__ g, const Plane pl, __half* __restrict__ x, float* __restrict__ alpha, const double* __restrict__ partial,
+                 float eps, int growth, Shape sh) {
     __shared__ double pow2;
-    const int64_t b = blockIdx.z, r0 = blockIdx.y * 32, c0 = blockIdx.x * 32;
-    if (threadIdx.x == 0) {
-        float al, later;
-        double t = 0.;
-        for (int k = 0; k < NORM_BLOCKS; ++k) t += partial[b * NORM_BLOCKS + k];
-        scales_of(sqrt(t), eps, growth, &pow2, &al, &later);
-        if (blockIdx.x == 0 && blockIdx.y == 0) { alpha[b] = al; alpha[sh.batch + b] = later; }
-    }
+    __shared__ float scales[2];
+    const int64_t b = blockIdx.y;
+    if (threadIdx.x < 32) warp_scales(partial + b * NORM_BLOCKS, eps, growth, &pow2, &scales[0], &scales[1]);
     __syncthreads();
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    for (int k = ty; k < 32; k += 8)
-        if (r0 + k < m && c0 + tx < n) tile[k][tx] = (float)((double)src.load(b, r0 + k, c0 + tx) * pow2);
-    __syncthreads();
-    const bool tall = m > n;
-    const int64_t y0 = tall ? c0 : r0, x0 = tall ? r0 : c0;
-    __half* dst = x + b * sh.planes * sh.x_slab();
-    for (int k = ty; k < 32; k += 8)
-        if (y0 + k < sh.s && x0 + tx < sh.l) {
-            __half hi, lo;
-            split_half(tall ? tile[tx][k] : tile[k][tx], hi, lo);
-            const int64_t at = (y0 + k) * sh.ls + x0 + tx;
-            dst[at] = hi;
-            if (sh.planes == 2) dst[at + sh.x_slab()] = lo;
-        }
-}
-
-// out[b][m][n] from o[b][s][l]
-template <typename T>
-__global__ void __launch_bounds__(256) unpack_kernel(const float* __restrict__ o, T* __restrict__ out, int64_t m, int64_t n, int64_t total) {
-    for (int64_t e = blockIdx.x * (int64_t)256 + threadIdx.x; e < total; e += (int64_t)gridDim.x * 256) {
-        const int64_t b = e / (m * n), w = e % (m * n), r = w / n, c = w % n;
-        out[e] = from_float<T>(m > n ? o[b * m * n + c * m + r] : o[e]);
+    if (blockIdx.x == 0 && threadIdx.x == 0) { alpha[b] = scales[0]; alpha[sh.batch + b] = scales[1]; }
+    const int64_t groups = sh.ls / 8, total = sh.s * groups;
+    __half* dst = x + b * PLANES * sh.x_slab();
+    for (int64_t w = blockIdx.x * (int64_t)256 + threadIdx.x; w < total; w += (int64_t)gridDim.x * 256) {
+        const int64_t r = w / groups, c = (w - r * groups) * 8;
+        float v[8];
+        load8(g + b * pl.batch + r * pl.pitch + c * pl.step, pl.step, pl.cols - c, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (float)((double)v[e] * pow2);
+        uint32_t hi[4], lo[4];
+        split8<PLANES>(v, hi, lo);
+        *reinterpret_cast<uint4*>(dst + w * 8) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        if (PLANES == 2) *reinterpret_cast<uint4*>(dst + w * 8 + sh.x_slab()) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
 }
 
-// param = keep * param - step * O
+// X_0 planes where X's rows are the source's columns: tiles of 32 source rows x 64 source columns turned in shared memory
+template <typename T, int PLANES>
 __global__ void __launch_bounds__(256)
-update_kernel(float* __restrict__ param, const float* __restrict__ o, int64_t in, int64_t out, int dp1, float keep, float step) {
-    const int64_t total = in * out * dp1;
-    for (int64_t e = blockIdx.x * (int64_t)256 + threadIdx.x; e < total; e += (int64_t)gridDim.x * 256) {
-        const int64_t d = e % dp1, w = e / dp1, i = w / out, c = w % out;
-        const float v = o[d * in * out + (in > out ? c * in + i : w)];
-        param[e] = fmaf(-step, v, keep * param[e]);
+pack_turned_kernel(const T* __restrict__ g, const Plane pl, __half* __restrict__ x, float* __restrict__ alpha, const double* __restrict__ partial,
+                   float eps, int growth, Shape sh) {
+    __shared__ float tile[64][33];                 // [source column = X row][source row = X column]
+    __shared__ double pow2;
+    __shared__ float scales[2];
+    const int64_t b = blockIdx.z, r0 = blockIdx.y * 32, c0 = blockIdx.x * 64;
+    if (threadIdx.x < 32) warp_scales(partial + b * NORM_BLOCKS, eps, growth, &pow2, &scales[0], &scales[1]);
+    __syncthreads();
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) { alpha[b] = scales[0]; alpha[sh.batch + b] = scales[1]; }
+    {
+        const int c = (threadIdx.x & 7) * 8, r = threadIdx.x >> 3;
+        float v[8];
+        if (r0 + r < pl.rows && c0 + c < pl.cols) load8(g + b * pl.batch + (r0 + r) * pl.pitch + (c0 + c) * pl.step, pl.step, pl.cols - c0 - c, v);
+        else
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) tile[c + e][r] = (float)((double)v[e] * pow2);
     }
-}
-
-unsigned blocks_for(int64_t n) {
-    int64_t b = ceil_div(n, 256);
-    return (unsigned)(b < 1 ? 1 : (b > 148 * 16 ? 148 * 16 : b));
+    __syncthreads();
+    const int row = threadIdx.x >> 2, col = (threadIdx.x & 3) * 8;          // 64 rows of X x 4 groups of 8 columns
+    if (c0 + row >= sh.s || r0 + col >= sh.ls) return;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = tile[row][col + e];
+    uint32_t hi[4], lo[4];
+    split8<PLANES>(v, hi, lo);
+    __half* dst = x + b * PLANES * sh.x_slab() + (c0 + row) * sh.ls + r0 + col;
+    *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    if (PLANES == 2) *reinterpret_cast<uint4*>(dst + sh.x_slab()) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
 }
 
 int64_t a256(int64_t b) { return round_up(b, 256); }
@@ -135,16 +248,18 @@ Shape shape_of(int64_t batch, int64_t m, int64_t n, int mode) {
     return sh;
 }
 
-Workspace layout_of(const Shape& sh) {
+// `update`: the Muon step's, which also holds u, one fp32 plane per degree (and later O in its place)
+Workspace layout_of(const Shape& sh, bool update) {
     Workspace w{};
-    if (small_supported(sh)) return w;           // one launch that keeps everything on chip
+    const int64_t ub = update ? a256(4 * (int64_t)sh.batch * sh.s * sh.l) : 0;
+    if (small_supported(sh)) { w.total = ub; return w; }           // one launch that keeps everything else on chip
     const int64_t xb = a256(2 * sh.x_slab() * sh.planes * sh.batch), ab = a256(2 * sh.a_slab() * sh.planes * sh.batch);
     int64_t at = 0;
     w.x0 = at; at += xb;
     w.x1 = at; at += xb;
     w.a = at; at += ab;
     w.p = at; at += ab;
-    w.o = at; at += a256(4 * (int64_t)sh.batch * sh.s * sh.l);
+    w.u = at; at += ub;
     w.partial = at; at += a256(8 * (int64_t)NORM_BLOCKS * sh.batch);
     w.alpha = at; at += a256(8 * (int64_t)sh.batch);
     w.total = at;
@@ -174,45 +289,61 @@ bool coefficients_ok(int64_t steps, float a, float b, float c, int* growth) {
     return true;
 }
 
-// steps on packed operands; leaves O in o [batch][s][l]
-int run_steps(char* ws, const Workspace& w, const Shape& sh, int64_t steps, float a, float b, float c, int32_t* status,
-              cudaStream_t s) {
+// steps on packed operands; leaves the result in o [batch][m][n]
+int run_steps(char* ws, const Workspace& w, const Shape& sh, const Steps& st, void* o, int dtype, bool tall, int32_t* status, cudaStream_t s) {
     __half* x[2] = {reinterpret_cast<__half*>(ws + w.x0), reinterpret_cast<__half*>(ws + w.x1)};
     __half* A = reinterpret_cast<__half*>(ws + w.a);
     __half* P = reinterpret_cast<__half*>(ws + w.p);
-    float* o = reinterpret_cast<float*>(ws + w.o);
     const float* alpha = reinterpret_cast<const float*>(ws + w.alpha);
-    for (int64_t k = 0; k < steps; ++k) {
+    for (int k = 0; k < st.n; ++k) {
         const float *later = alpha + sh.batch, *al = k == 0 ? alpha : later;
         int rc;
         if ((rc = launch_gram(x[k & 1], A, al, sh, status, s))) return rc;
-        if ((rc = launch_poly(A, P, a, b, c, sh, status, s))) return rc;
-        if ((rc = launch_apply(P, x[k & 1], k + 1 < steps ? x[(k + 1) & 1] : nullptr, o, al, later, sh, status, s))) return rc;
+        if ((rc = launch_poly(A, P, st.a, st.b, st.c, sh, status, s))) return rc;
+        if (k + 1 < st.n) rc = launch_apply(P, x[k & 1], x[(k + 1) & 1], al, later, sh, status, s);
+        else rc = launch_apply_last(P, x[k & 1], o, dtype, tall, al, sh, status, s);
+        if (rc) return rc;
     }
     return CHEBYKAN_OK;
 }
 
-template <typename Src>
-int launch_pack_planes(const Src& src, int64_t m, int64_t n, char* ws, const Workspace& w, const Shape& sh, float eps, int growth,
-                       cudaStream_t s) {
-    const dim3 grid((unsigned)ceil_div(n, 32), (unsigned)ceil_div(m, 32), (unsigned)sh.batch);
-    pack_kernel<<<grid, 256, 0, s>>>(src, m, n, reinterpret_cast<__half*>(ws + w.x0), reinterpret_cast<float*>(ws + w.alpha),
-                                     reinterpret_cast<const double*>(ws + w.partial), eps, growth, sh);
+// [batch][m][n] with the given strides, with the closer one inside
+Plane plane_of(int64_t m, int64_t n, int64_t sb, int64_t sr, int64_t sc, bool* swapped) {
+    *swapped = sr < sc;
+    return *swapped ? Plane{n, m, sc, sr, sb} : Plane{m, n, sr, sc, sb};
+}
+
+template <typename T, int PLANES>
+int pack_planes(const T* g, const Plane& pl, bool turned, char* ws, const Workspace& w, const Shape& sh, const Steps& st, cudaStream_t s) {
+    __half* x = reinterpret_cast<__half*>(ws + w.x0);
+    float* alpha = reinterpret_cast<float*>(ws + w.alpha);
+    const double* partial = reinterpret_cast<const double*>(ws + w.partial);
+    if (turned) {
+        const dim3 grid((unsigned)ceil_div(pl.cols, 64), (unsigned)ceil_div(pl.rows, 32), (unsigned)sh.batch);
+        pack_turned_kernel<T, PLANES><<<grid, 256, 0, s>>>(g, pl, x, alpha, partial, st.eps, st.growth, sh);
+    } else {
+        // about four groups per thread, so that the norm's partial sums are not added up by too many blocks
+        int64_t blocks = ceil_div((int64_t)sh.s * sh.ls / 8, 4 * 256);
+        pack_rows_kernel<T, PLANES><<<dim3((unsigned)blocks, (unsigned)sh.batch), 256, 0, s>>>(g, pl, x, alpha, partial, st.eps, st.growth, sh);
+    }
     return check_cuda(cudaGetLastError());
+}
+template <typename T>
+int pack(const T* g, const Plane& pl, bool turned, char* ws, const Workspace& w, const Shape& sh, const Steps& st, cudaStream_t s) {
+    return sh.planes == 2 ? pack_planes<T, 2>(g, pl, turned, ws, w, sh, st, s) : pack_planes<T, 1>(g, pl, turned, ws, w, sh, st, s);
 }
 
 template <typename T>
-int orthogonalize_typed(const void* g, int64_t sb, int64_t sr, int64_t sc, void* out, char* ws, const Workspace& w, const Shape& sh,
-                        int64_t m, int64_t n, int64_t steps, float a, float b, float c, float eps, int growth, int32_t* status, cudaStream_t s) {
-    const StridedSource<T> src{reinterpret_cast<const T*>(g), sb, sr, sc};
-    norm_kernel<T><<<dim3(NORM_BLOCKS, (unsigned)sh.batch), 256, 0, s>>>(src, m, n, reinterpret_cast<double*>(ws + w.partial));
+int orthogonalize_typed(const void* g, int dtype, int64_t sb, int64_t sr, int64_t sc, void* out, char* ws, const Workspace& w,
+                        const Shape& sh, int64_t m, int64_t n, const Steps& st, int32_t* status, cudaStream_t s) {
+    bool swapped;
+    const Plane pl = plane_of(m, n, sb, sr, sc, &swapped);
+    const T* src = reinterpret_cast<const T*>(g);
+    norm_kernel<T><<<dim3(NORM_BLOCKS, (unsigned)sh.batch), 256, 0, s>>>(src, pl, reinterpret_cast<double*>(ws + w.partial));
     int rc = check_cuda(cudaGetLastError());
     if (rc) return rc;
-    if ((rc = launch_pack_planes(src, m, n, ws, w, sh, eps, growth, s))) return rc;
-    if ((rc = run_steps(ws, w, sh, steps, a, b, c, status, s))) return rc;
-    const int64_t total = sh.batch * m * n;
-    unpack_kernel<T><<<blocks_for(total), 256, 0, s>>>(reinterpret_cast<const float*>(ws + w.o), reinterpret_cast<T*>(out), m, n, total);
-    return check_cuda(cudaGetLastError());
+    if ((rc = pack(src, pl, swapped != (m > n), ws, w, sh, st, s))) return rc;
+    return run_steps(ws, w, sh, st, out, dtype, m > n, status, s);
 }
 
 bool ns_mode(int mode) { return mode == CHEBYKAN_MODE_FP32X3 || mode == CHEBYKAN_MODE_TF32; }
@@ -230,7 +361,7 @@ extern "C" {
 int64_t chebykan_orthogonalize_workspace_bytes(int64_t batch, int64_t m, int64_t n, int mode) {
     if (!shape_fits(batch, m, n) || !known_mode(mode)) return CHEBYKAN_EINVAL;
     if (!ns_mode(mode)) return CHEBYKAN_EUNSUPPORTED;
-    return layout_of(shape_of(batch, m, n, mode)).total;
+    return layout_of(shape_of(batch, m, n, mode), false).total;
 }
 
 int chebykan_orthogonalize(const void* g, int64_t stride_batch, int64_t stride_row, int64_t stride_col, int dtype, void* out,
@@ -249,23 +380,23 @@ int chebykan_orthogonalize(const void* g, int64_t stride_batch, int64_t stride_r
     int rc = check_device();
     if (rc) return rc;
     const Shape sh = shape_of(batch, m, n, mode);
+    const Steps st{(int)steps, a, b, c, eps, growth};
     cudaStream_t s = (cudaStream_t)stream;
     if (small_supported(sh))
-        return launch_small_orthogonalize(g, dtype, stride_batch, stride_row, stride_col, out, m, n, sh,
-                                          {(int)steps, a, b, c, eps, growth}, status, s);
-    const Workspace w = layout_of(sh);
+        return launch_small_orthogonalize(g, dtype, stride_batch, stride_row, stride_col, out, m, n, sh, st, status, s);
+    const Workspace w = layout_of(sh, false);
     char* ws = reinterpret_cast<char*>(workspace);
     if (dtype == CHEBYKAN_DTYPE_FP32)
-        return orthogonalize_typed<float>(g, stride_batch, stride_row, stride_col, out, ws, w, sh, m, n, steps, a, b, c, eps, growth, status, s);
+        return orthogonalize_typed<float>(g, dtype, stride_batch, stride_row, stride_col, out, ws, w, sh, m, n, st, status, s);
     if (dtype == CHEBYKAN_DTYPE_BF16)
-        return orthogonalize_typed<__nv_bfloat16>(g, stride_batch, stride_row, stride_col, out, ws, w, sh, m, n, steps, a, b, c, eps, growth, status, s);
-    return orthogonalize_typed<__half>(g, stride_batch, stride_row, stride_col, out, ws, w, sh, m, n, steps, a, b, c, eps, growth, status, s);
+        return orthogonalize_typed<__nv_bfloat16>(g, dtype, stride_batch, stride_row, stride_col, out, ws, w, sh, m, n, st, status, s);
+    return orthogonalize_typed<__half>(g, dtype, stride_batch, stride_row, stride_col, out, ws, w, sh, m, n, st, status, s);
 }
 
 int64_t chebykan_muon_workspace_bytes(int64_t in, int64_t out, int64_t deg, int mode) {
     if (in < 1 || out < 1 || deg < 0 || deg > 127 || !known_mode(mode) || !shape_fits(deg + 1, in, out)) return CHEBYKAN_EINVAL;
     if (!ns_mode(mode)) return CHEBYKAN_EUNSUPPORTED;
-    return layout_of(shape_of(deg + 1, in, out, mode)).total;
+    return layout_of(shape_of(deg + 1, in, out, mode), true).total;
 }
 
 int chebykan_muon_step(float* param, const float* grad, float* buf, void* workspace, int64_t workspace_bytes, int64_t in,
@@ -284,20 +415,26 @@ int chebykan_muon_step(float* param, const float* grad, float* buf, void* worksp
     if (rc) return rc;
     const int dp1 = (int)deg + 1;
     const Shape sh = shape_of(dp1, in, out, mode);
-    cudaStream_t s = (cudaStream_t)stream;
-    if (small_supported(sh))
-        return launch_small_muon(param, grad, buf, in, out, dp1, 1.f - lr * weight_decay, lr * update_scale, momentum, nesterov,
-                                 grad_scale, sh, {(int)steps, a, b, c, eps, growth}, status, s);
-    const Workspace w = layout_of(sh);
+    const Steps st{(int)steps, a, b, c, eps, growth};
+    const Workspace w = layout_of(sh, true);
     char* ws = reinterpret_cast<char*>(workspace);
-    momentum_kernel<<<NORM_BLOCKS, 256, 0, s>>>(grad, buf, in * out * dp1, dp1, momentum, nesterov, grad_scale,
-                                                reinterpret_cast<double*>(ws + w.partial));
+    float* u = reinterpret_cast<float*>(ws + w.u);
+    cudaStream_t s = (cudaStream_t)stream;
+    const bool small = small_supported(sh);
+    const int64_t pairs = in * out, tiles = ceil_div(pairs, tile_width(dp1));
+    const int smem = (dp1 | 1) * tile_width(dp1) * 4;
+    // a block of the norm's partial sums each, also where it has no tile
+    const unsigned blocks = (unsigned)(small && tiles < NORM_BLOCKS ? tiles : NORM_BLOCKS);
+    momentum_kernel<<<blocks, 256, smem, s>>>(grad, buf, u, pairs, dp1, momentum, nesterov, grad_scale,
+                                              small ? nullptr : reinterpret_cast<double*>(ws + w.partial));
     if ((rc = check_cuda(cudaGetLastError()))) return rc;
-    const MomentumSource src{grad, buf, out, dp1, momentum, grad_scale, nesterov};
-    if ((rc = launch_pack_planes(src, in, out, ws, w, sh, eps, growth, s))) return rc;
-    if ((rc = run_steps(ws, w, sh, steps, a, b, c, status, s))) return rc;
-    update_kernel<<<blocks_for(in * out * dp1), 256, 0, s>>>(param, reinterpret_cast<const float*>(ws + w.o), in, out, dp1,
-                                                             1.f - lr * weight_decay, lr * update_scale);
+    const float keep = 1.f - lr * weight_decay, step = lr * update_scale;
+    if (small) return launch_small_update(param, u, in, out, dp1, keep, step, sh, st, status, s);
+    if ((rc = pack(u, Plane{in, out, out, 1, pairs}, in > out, ws, w, sh, st, s))) return rc;
+    // the packed operands have taken u's place: O goes there
+    if ((rc = run_steps(ws, w, sh, st, u, CHEBYKAN_DTYPE_FP32, in > out, status, s))) return rc;
+    const int64_t update_blocks = tiles < 148 * 4 ? tiles : 148 * 4;
+    update_kernel<<<(unsigned)update_blocks, 256, smem, s>>>(param, u, pairs, dp1, keep, step);
     return check_cuda(cudaGetLastError());
 }
 

@@ -29,42 +29,52 @@ struct Shape {
 };
 
 struct Workspace {        // byte offsets of the buffers
-    int64_t x0, x1, a, p, o, partial, alpha, total;
+    int64_t x0, x1, a, p, u, partial, alpha, total;
 };
 
 // per-matrix partial sums of squares written by the norm kernels
-constexpr int NORM_BLOCKS = 64;
+constexpr int NORM_BLOCKS = 296;
 
-__device__ __forceinline__ void split_half(float v, __half& hi, __half& lo) {
-    hi = __float2half_rn(v);
-    lo = __float2half_rn(v - __half2float(hi));
+__device__ __forceinline__ uint32_t half2_bits(float x, float y) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
 }
-
-// ---- where a matrix's elements come from ----------------------------------------------------------------------
-// u(i, r, c) of matrix i.  Strided: a tensor of any strides and type.  Momentum: the degree slices of a coefficient
-// gradient [in][out][deg+1] after the momentum update (buf already holds the new value).
-template <typename T>
-struct StridedSource {
-    const T* g;
-    int64_t sb, sr, sc;
-    __device__ __forceinline__ float load(int64_t i, int64_t r, int64_t c) const {
-        return (float)g[i * sb + r * sr + c * sc];
+// Heads and tails of eight values as packed fp16.  The head is the value rounded to 11 bits by the splitting of Veltkamp and
+// Dekker (c = 8193 v, head = c - (c - v)), which stays in fp32 and leaves two values per conversion instruction; a
+// conversion each way per value is what an epilogue would otherwise spend most of its time on.  Below fp16's normal range
+// the head is rounded once more, by at most 2^-25, as the tail is.
+template <int PLANES>
+__device__ __forceinline__ void split8(const float (&x)[8], uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+    if (PLANES == 1) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) hi[e] = half2_bits(x[2 * e], x[2 * e + 1]);
+        return;
     }
-};
-struct MomentumSource {
-    const float *grad, *buf;
-    int64_t out;
-    int dp1;
-    float momentum, gs;
-    int nesterov;
-    __device__ __forceinline__ float at(int64_t e) const {
-        const float m = buf[e];
-        if (!nesterov) return m;
-        const float g = grad[e] * gs;
-        return fmaf(momentum, m - g, g);
+    float h[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float c = __fmul_rn(x[e], 8193.f);
+        h[e] = __fsub_rn(c, __fsub_rn(c, x[e]));
     }
-    __device__ __forceinline__ float load(int64_t i, int64_t r, int64_t c) const { return at((r * out + c) * dp1 + i); }
-};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        hi[e] = half2_bits(h[2 * e], h[2 * e + 1]);
+        lo[e] = half2_bits(x[2 * e] - h[2 * e], x[2 * e + 1] - h[2 * e + 1]);
+    }
+}
+// values of eight packed heads (and tails)
+template <int PLANES>
+__device__ __forceinline__ void join8(const uint32_t (&hi)[4], const uint32_t (&lo)[4], float (&x)[8]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        float2 v = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
+        if (PLANES == 2) {
+            const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&lo[e]));
+            v.x += t.x; v.y += t.y;
+        }
+        x[2 * e] = v.x; x[2 * e + 1] = v.y;
+    }
+}
 
 // power of two that puts the norm into [2^14, 2^15), the factor that is left of 1 / max(norm, eps), and the scale of the
 // later X: growth bounds log2 of what the steps multiply a small X by, and below eps 2^-growth that leaves X under 1,
@@ -94,10 +104,12 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(f
 int launch_gram(const __half* x, __half* a, const float* alpha, const Shape& sh, int32_t* status, cudaStream_t s);
 // P = ca I + cb A + cc A A
 int launch_poly(const __half* a, __half* p, float ca, float cb, float cc, const Shape& sh, int32_t* status, cudaStream_t s);
-// X' = P X as planes (x_next, stored over alpha_next[b]), or as fp32 [batch][s][l] (o) where x_next is null
-int launch_apply(const __half* p, const __half* x, __half* x_next, float* o, const float* alpha, const float* alpha_next,
-                 const Shape& sh, int32_t* status, cudaStream_t s);
-
+// X' = P X as planes, stored over alpha_next[b]
+int launch_apply(const __half* p, const __half* x, __half* x_next, const float* alpha, const float* alpha_next, const Shape& sh,
+                 int32_t* status, cudaStream_t s);
+// the last step: P X, transposed back if the matrix is tall, to o [batch][m][n] of `dtype`
+int launch_apply_last(const __half* p, const __half* x, void* o, int dtype, bool tall, const float* alpha, const Shape& sh,
+                      int32_t* status, cudaStream_t s);
 
 // ---- whole calls for small matrices in one launch (ns_small.cu) ----
 struct Steps {
@@ -108,8 +120,9 @@ struct Steps {
 bool small_supported(const Shape& sh);
 int launch_small_orthogonalize(const void* g, int dtype, int64_t sb, int64_t sr, int64_t sc, void* out, int64_t m, int64_t n, const Shape& sh,
                                const Steps& st, int32_t* status, cudaStream_t s);
-int launch_small_muon(float* param, const float* grad, float* buf, int64_t in, int64_t out, int dp1, float keep, float step, float momentum,
-                      int nesterov, float gs, const Shape& sh, const Steps& st, int32_t* status, cudaStream_t s);
+// from the updates u[dp1][in][out] to param = keep * param - step * O
+int launch_small_update(float* param, const float* u, int64_t in, int64_t out, int dp1, float keep, float step, const Shape& sh,
+                        const Steps& st, int32_t* status, cudaStream_t s);
 
 }  // namespace ns
 }  // namespace chebykan

@@ -1,5 +1,5 @@
-// Newton-Schulz orthogonalisation and the whole Muon step of small matrices (shorter side up to 128, longer up to 2048) in
-// one launch.
+// Newton-Schulz orthogonalisation of small matrices (shorter side up to 128, longer up to 2048) in one launch, and with it
+// the weights' update of a Muon step.
 //
 // A matrix of this size is a few microseconds of reading and no arithmetic to speak of, but 3 * steps products that wait
 // for one another: as launches of their own each costs a launch, a pipeline's start and its drain (about 9 us; 150 us for
@@ -23,7 +23,7 @@ namespace ns {
 namespace {
 using namespace tc;
 
-constexpr int THREADS = 256;
+constexpr int THREADS = 512, GROUPS = THREADS / 128;       // GROUPS warps per 32 lanes of tensor memory share the columns
 constexpr int PANEL = 128 * 128;                 // 128 rows of 64 fp16 columns
 constexpr int MAX_CLUSTER = 8, MAX_SLICE = 256;
 enum { ST_GRAM = 31, ST_POLY = 32, ST_APPLY = 33 };
@@ -59,47 +59,31 @@ __device__ __forceinline__ double ld_cluster_f64(uint32_t addr) {
 __device__ __forceinline__ uint32_t chunk_at(int row, int col) {
     return (uint32_t)((col >> 6) * PANEL + row * 128 + ((((col & 63) >> 3) ^ (row & 7)) << 4));
 }
-__device__ __forceinline__ uint32_t half2_bits(__half x, __half y) {
-    return (uint32_t)__half_as_ushort(x) | ((uint32_t)__half_as_ushort(y) << 16);
-}
-
 // ---- the two uses: where elements come from and where results go.  Elements are addressed by their offset; what a batch of
 // them needs from memory is fetched before any of it is used, so that the latencies overlap. ----
 template <typename T>
 struct OrthogonalizeIo {
-    StridedSource<T> src;
+    const T* g;
+    int64_t sb, sr, sc;
     T* out;
     int64_t m, n;
-    struct Raw { T g; };
     struct Old {};
-    __device__ __forceinline__ int64_t in_at(int64_t b, int64_t r, int64_t c) const { return b * src.sb + r * src.sr + c * src.sc; }
-    __device__ __forceinline__ Raw fetch(int64_t e) const { return {src.g[e]}; }
-    __device__ __forceinline__ double first(int64_t, const Raw& v) const { return (double)(float)v.g; }
-    __device__ __forceinline__ float again(const Raw& v) const { return (float)v.g; }
+    __device__ __forceinline__ int64_t in_at(int64_t b, int64_t r, int64_t c) const { return b * sb + r * sr + c * sc; }
+    __device__ __forceinline__ float fetch(int64_t e) const { return (float)g[e]; }
     __device__ __forceinline__ int64_t out_at(int64_t b, int64_t r, int64_t c) const { return (b * m + r) * n + c; }
     __device__ __forceinline__ Old fetch_out(int64_t) const { return {}; }
     __device__ __forceinline__ void store(int64_t e, const Old&, float v) const { out[e] = from_float<T>(v); }
 };
-struct MuonIo {
+struct UpdateIo {
     float* param;
-    const float* grad;
-    float* buf;
-    int64_t out;
-    int dp1, nesterov;
-    float momentum, gs, keep, step;
-    struct Raw { float g, m; };
+    const float* u;
+    int64_t in, out;
+    int dp1;
+    float keep, step;
     struct Old { float p; };
-    __device__ __forceinline__ int64_t in_at(int64_t b, int64_t r, int64_t c) const { return (r * out + c) * dp1 + b; }
-    __device__ __forceinline__ Raw fetch(int64_t e) const { return {grad[e] * gs, buf[e]}; }
-    __device__ __forceinline__ float update(float g, float m) const { return nesterov ? fmaf(momentum, m - g, g) : m; }
-    // the first visit moves the momentum; the second, by the same thread, finds it moved
-    __device__ __forceinline__ double first(int64_t e, const Raw& v) const {
-        const float m = fmaf(1.f - momentum, v.g - v.m, v.m);
-        buf[e] = m;
-        return (double)update(v.g, m);
-    }
-    __device__ __forceinline__ float again(const Raw& v) const { return update(v.g, v.m); }
-    __device__ __forceinline__ int64_t out_at(int64_t b, int64_t r, int64_t c) const { return in_at(b, r, c); }
+    __device__ __forceinline__ int64_t in_at(int64_t b, int64_t r, int64_t c) const { return (b * in + r) * out + c; }
+    __device__ __forceinline__ float fetch(int64_t e) const { return u[e]; }
+    __device__ __forceinline__ int64_t out_at(int64_t b, int64_t r, int64_t c) const { return (r * out + c) * dp1 + b; }
     __device__ __forceinline__ Old fetch_out(int64_t e) const { return {param[e]}; }
     __device__ __forceinline__ void store(int64_t e, const Old& old, float v) const { param[e] = fmaf(-step, v, keep * old.p); }
 };
@@ -110,12 +94,12 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io io, const Ge
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
     uint8_t* tail = gen + g.x_bytes + g.a_bytes;
-    double* red = reinterpret_cast<double*>(tail);                               // [8], and the CTA's sum in [8]
-    float* scales = reinterpret_cast<float*>(tail + 80);                         // alpha of X_0 and of the later X
-    double* pow2 = reinterpret_cast<double*>(tail + 88);
-    const uint32_t bar = base + (uint32_t)(g.x_bytes + g.a_bytes) + 96;
-    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(tail + 104);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 108);
+    double* red = reinterpret_cast<double*>(tail);                               // a sum per warp, and the CTA's in [16]
+    float* scales = reinterpret_cast<float*>(tail + 144);                         // alpha of X_0 and of the later X
+    double* pow2 = reinterpret_cast<double*>(tail + 152);
+    const uint32_t bar = base + (uint32_t)(g.x_bytes + g.a_bytes) + 160;
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(tail + 168);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 172);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)cluster_ctarank();
@@ -144,29 +128,24 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io io, const Ge
         if (g.tall) { c = e / g.s; r = e - c * g.s; } else { r = e / cols; c = e - r * cols; }
     };
     constexpr int U = 8;
-    // f(place in the slice, offset in memory, what was fetched) for this thread's elements, U fetches in flight
+    // f(place in the slice, value) for this thread's elements, U loads in flight
     auto elements = [&](auto f) {
         for (int e0 = threadIdx.x; e0 < count; e0 += U * THREADS) {
             int r[U], c[U];
-            int64_t at[U];
-            typename Io::Raw raw[U];
+            float v[U];
 #pragma unroll
             for (int u = 0; u < U; ++u)
                 if (e0 + u * THREADS < count) {
                     place(e0 + u * THREADS, r[u], c[u]);
-                    at[u] = g.tall ? io.in_at(b, col0 + c[u], r[u]) : io.in_at(b, r[u], col0 + c[u]);
-                    raw[u] = io.fetch(at[u]);
+                    v[u] = io.fetch(g.tall ? io.in_at(b, col0 + c[u], r[u]) : io.in_at(b, r[u], col0 + c[u]));
                 }
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                if (e0 + u * THREADS < count) f(r[u], c[u], at[u], raw[u]);
+                if (e0 + u * THREADS < count) f(r[u], c[u], v[u]);
         }
     };
     double sum = 0.;
-    elements([&](int, int, int64_t at, const typename Io::Raw& raw) {
-        const double v = io.first(at, raw);
-        sum += v * v;
-    });
+    elements([&](int, int, float v) { sum = fma((double)v, (double)v, sum); });
     for (uint32_t at = threadIdx.x * 16; at < (uint32_t)(g.x_bytes + g.a_bytes); at += THREADS * 16)
         *reinterpret_cast<uint4*>(gen + at) = make_uint4(0, 0, 0, 0);           // rows and columns of padding
 #pragma unroll
@@ -176,15 +155,15 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io io, const Ge
     if (threadIdx.x == 0) {
         double t = 0.;
         for (int w = 0; w < THREADS / 32; ++w) t += red[w];
-        red[8] = t;
+        red[16] = t;
     }
     __syncthreads();
     if (g.cluster > 1) cluster_sync_all();
     if (threadIdx.x == 0) {
-        double t = red[8];
+        double t = red[16];
         if (g.cluster > 1) {
             t = 0.;
-            for (int k = 0; k < g.cluster; ++k) t += ld_cluster_f64(mapa_cluster(base + (uint32_t)(g.x_bytes + g.a_bytes) + 64, (uint32_t)k));
+            for (int k = 0; k < g.cluster; ++k) t += ld_cluster_f64(mapa_cluster(base + (uint32_t)(g.x_bytes + g.a_bytes) + 128, (uint32_t)k));
         }
         scales_of(sqrt(t), st.eps, st.growth, pow2, &scales[0], &scales[1]);
     }
@@ -194,12 +173,12 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io io, const Ge
     const uint32_t tmem = *tmem_slot;
     {
         const double p2 = *pow2;
-        elements([&](int r, int c, int64_t, const typename Io::Raw& raw) {
-            __half hi, lo;
-            split_half((float)((double)io.again(raw) * p2), hi, lo);
+        elements([&](int r, int c, float v) {
+            v = (float)((double)v * p2);
+            const __half hi = __float2half_rn(v);
             uint8_t* at = gen + chunk_at(r, c) + 2 * (c & 7);
             *reinterpret_cast<__half*>(at) = hi;
-            if (PLANES == 2) *reinterpret_cast<__half*>(at + x_plane) = lo;
+            if (PLANES == 2) *reinterpret_cast<__half*>(at + x_plane) = __float2half_rn(v - __half2float(hi));
         });
     }
 
@@ -213,28 +192,26 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io io, const Ge
         __syncthreads();
         if (warp == 0) {
             tc_fence_after();
-            if (elected) {
-                const uint32_t idesc = (1u << 4) | ((mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
-                for (int k = 0; k < ksteps; ++k) {
-                    const uint32_t kmaj = (uint32_t)((k >> 2) * PANEL + (k & 3) * 32);
-                    uint64_t l[PLANES], r[PLANES];
-#pragma unroll
-                    for (int p = 0; p < PLANES; ++p) {
-                        l[p] = make_smem_desc(left + (uint32_t)(p * left_plane) + kmaj);
-                        if (mn)
-                            r[p] = (make_smem_desc(right + (uint32_t)(p * right_plane) + (uint32_t)(k * 2048)) & ~((uint64_t)0x3fff << 16)) |
-                                   ((uint64_t)(PANEL >> 4) << 16);
-                        else
-                            r[p] = make_smem_desc(right + (uint32_t)(p * right_plane) + kmaj);
-                    }
-                    umma<CHEBYKAN_MODE_BF16>(tmem, l[0], r[0], idesc, k > 0);
+            // the whole warp runs the loop and one lane issues (see elect_one_sync); only the low words of descriptors move
+            const uint32_t idesc = (1u << 4) | ((mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+            const uint64_t ld = make_smem_desc(left), rd = make_smem_desc(right);
+            const uint32_t l_hi = (uint32_t)(ld >> 32), l_lo = (uint32_t)ld, l_tail = (uint32_t)(left_plane >> 4);
+            // MN-major: columns 64 apart are a panel apart
+            const uint32_t r_hi = (uint32_t)(rd >> 32), r_tail = (uint32_t)(right_plane >> 4);
+            const uint32_t r_lo = mn ? ((uint32_t)rd & 0xffffu) | ((uint32_t)(PANEL >> 4) << 16) : (uint32_t)rd;
+#pragma unroll 4
+            for (int k = 0; k < ksteps; ++k) {
+                const uint32_t kmaj = (uint32_t)((k >> 2) * (PANEL >> 4) + (k & 3) * 2), kr = mn ? (uint32_t)(k * 128) : kmaj;
+                if (elected) {
+                    const uint64_t l0 = desc_from_words(l_lo + kmaj, l_hi), r0 = desc_from_words(r_lo + kr, r_hi);
+                    umma<CHEBYKAN_MODE_BF16>(tmem, l0, r0, idesc, k > 0);
                     if (PLANES == 2) {
-                        umma<CHEBYKAN_MODE_BF16>(tmem + g.acc, l[0], r[PLANES - 1], idesc, k > 0);
-                        umma<CHEBYKAN_MODE_BF16>(tmem + g.acc, l[PLANES - 1], r[0], idesc, 1u);
+                        umma<CHEBYKAN_MODE_BF16>(tmem + g.acc, l0, desc_from_words(r_lo + kr + r_tail, r_hi), idesc, k > 0);
+                        umma<CHEBYKAN_MODE_BF16>(tmem + g.acc, desc_from_words(l_lo + kmaj + l_tail, l_hi), r0, idesc, 1u);
                     }
                 }
-                umma_commit(bar);
             }
+            if (elected) umma_commit(bar);
             __syncwarp();
         }
         mbar_wait(bar, phase, abort_flag, status, code);
@@ -242,11 +219,11 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io io, const Ge
         __syncwarp();
         tc_fence_after();
     };
-    const int q = warp & 3, half = warp >> 2;          // lanes of tensor memory, and which of two interleaved column groups
+    const int q = warp & 3, group = warp >> 2;         // lanes of tensor memory, and which of the interleaved column groups
     const int row = q * 32 + lane;
     // visits the accumulator's columns 16 at a time: f(first column, values)
     auto columns = [&](int n, auto f) {
-        for (int c = half * 16; c < n; c += 32) {
+        for (int c = group * 16; c < n; c += GROUPS * 16) {
             __syncwarp();                               // the loads are warp-collective
             uint32_t v[16], w[16];
             const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)c;
@@ -260,15 +237,12 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io io, const Ge
         }
     };
     auto put = [&](uint32_t dst, int plane, int r, int c, const float (&x)[8]) {       // 8 columns of a row, both planes
-        __half hi[8], lo[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) split_half(x[e], hi[e], lo[e]);
+        uint32_t hi[4], lo[4];
+        split8<PLANES>(x, hi, lo);
         const uint32_t at = dst + chunk_at(r, c);
-        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(half2_bits(hi[0], hi[1])), "r"(half2_bits(hi[2], hi[3])),
-                     "r"(half2_bits(hi[4], hi[5])), "r"(half2_bits(hi[6], hi[7])) : "memory");
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
         if (PLANES == 2)
-            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at + (uint32_t)plane), "r"(half2_bits(lo[0], lo[1])),
-                         "r"(half2_bits(lo[2], lo[3])), "r"(half2_bits(lo[4], lo[5])), "r"(half2_bits(lo[6], lo[7])) : "memory");
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at + (uint32_t)plane), "r"(lo[0]), "r"(lo[1]), "r"(lo[2]), "r"(lo[3]) : "memory");
     };
 
     const int cols16 = (cols + 15) & ~15;
@@ -300,46 +274,69 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io io, const Ge
             tc_fence_before();
             __syncthreads();
             cluster_sync_all();
-            // this CTA's band of rows, 8 columns per thread; a band of at most 64 rows x 16 groups is 4 per thread.  Rows
+            // this CTA's band of rows, 8 columns per thread; a band of at most 64 rows x 16 groups is 2 per thread.  Rows
             // from s to s16 become zero: the next product reads them, and the partial sums have been lying there.
+            constexpr int W = 1024 / THREADS;
             const int band = (g.s16 + g.cluster - 1) / g.cluster, r0 = rank * band;
             const int nrow = g.s16 - r0 < band ? (g.s16 - r0 > 0 ? g.s16 - r0 : 0) : band;
             const int groups = g.s16 / 8, todo = nrow * groups;
-            float y[4][8];
+            float y[W][8];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
+            for (int u = 0; u < W; ++u) {
                 const int w = threadIdx.x + u * THREADS;
                 if (w < todo) {
+                    const bool inside = r0 + w / groups < g.s;
                     const uint32_t at = as + (uint32_t)((r0 + w / groups) * pitch + w % groups * 32);
+                    float4 v[MAX_CLUSTER][2];                        // all in flight at once, added in rank order
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) y[u][e] = 0.f;
-                    for (int p = 0; p < g.cluster && r0 + w / groups < g.s; ++p) {
-                        const uint32_t from = mapa_cluster(at, (uint32_t)p);
-                        const float4 v0 = ld_cluster_f4(from), v1 = ld_cluster_f4(from + 16);
-                        y[u][0] += v0.x; y[u][1] += v0.y; y[u][2] += v0.z; y[u][3] += v0.w;
-                        y[u][4] += v1.x; y[u][5] += v1.y; y[u][6] += v1.z; y[u][7] += v1.w;
-                    }
+                    for (int p = 0; p < MAX_CLUSTER; ++p)
+                        if (p < g.cluster) {
+                            const uint32_t from = mapa_cluster(at, (uint32_t)p);
+                            v[p][0] = ld_cluster_f4(from);
+                            v[p][1] = ld_cluster_f4(from + 16);
+                        }
+                    float4 a0 = v[0][0], a1 = v[0][1];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) y[u][e] = r0 + w / groups < g.s ? y[u][e] * fa : 0.f;
+                    for (int p = 1; p < MAX_CLUSTER; ++p)
+                        if (p < g.cluster) {
+                            a0.x += v[p][0].x; a0.y += v[p][0].y; a0.z += v[p][0].z; a0.w += v[p][0].w;
+                            a1.x += v[p][1].x; a1.y += v[p][1].y; a1.z += v[p][1].z; a1.w += v[p][1].w;
+                        }
+                    const float sum8[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w};
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y[u][e] = inside ? sum8[e] * fa : 0.f;
                 }
             }
             cluster_sync_all();              // all partial sums are read: the buffer becomes A
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
+            for (int u = 0; u < W; ++u) {
                 const int w = threadIdx.x + u * THREADS;
                 if (w < todo) put(as, a_plane, r0 + w / groups, w % groups * 8, y[u]);
             }
             cluster_sync_all();
             // the other bands; nobody overwrites its own before the barrier below is complete
-            for (int w = threadIdx.x; w < g.s16 * groups; w += THREADS) {
-                const int r = w / groups, owner = r / band;
-                if (owner == rank) continue;
-                const uint32_t at = as + chunk_at(r, w % groups * 8), from = mapa_cluster(at, (uint32_t)owner);
+            {
+                constexpr int FETCH = 128 * 16 / THREADS;
+                float4 v[FETCH][PLANES];
+                uint32_t at[FETCH];
 #pragma unroll
-                for (int p = 0; p < PLANES; ++p) {
-                    const float4 v = ld_cluster_f4(from + (uint32_t)(p * a_plane));
-                    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at + (uint32_t)(p * a_plane)), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+                for (int u = 0; u < FETCH; ++u) {
+                    const int w = threadIdx.x + u * THREADS, r = w / groups, owner = r / band;
+                    at[u] = 0;
+                    if (w < g.s16 * groups && owner != rank) {
+                        at[u] = as + chunk_at(r, w % groups * 8);
+                        const uint32_t from = mapa_cluster(at[u], (uint32_t)owner);
+#pragma unroll
+                        for (int p = 0; p < PLANES; ++p) v[u][p] = ld_cluster_f4(from + (uint32_t)(p * a_plane));
+                    }
                 }
+#pragma unroll
+                for (int u = 0; u < FETCH; ++u)
+                    if (at[u] != 0)
+#pragma unroll
+                        for (int p = 0; p < PLANES; ++p)
+                            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at[u] + (uint32_t)(p * a_plane)), "f"(v[u][p].x), "f"(v[u][p].y),
+                                         "f"(v[u][p].z), "f"(v[u][p].w) : "memory");
             }
             __syncwarp();
             cluster_arrive();
@@ -356,12 +353,11 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io io, const Ge
                 asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(at));
                 if (PLANES == 2)
                     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(t[0]), "=r"(t[1]), "=r"(t[2]), "=r"(t[3]) : "r"(at + (uint32_t)a_plane));
-                float y[8];
+                float a[8], y[8];
+                join8<PLANES>(h, t, a);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    float a = __half2float(__ushort_as_half((unsigned short)(h[e >> 1] >> (16 * (e & 1)))));
-                    if (PLANES == 2) a += __half2float(__ushort_as_half((unsigned short)(t[e >> 1] >> (16 * (e & 1)))));
-                    y[e] = fmaf(st.b * exp2f((float)(P_EXP - A_EXP)), a, x[j + e] * (st.c * exp2f((float)(P_EXP - 2 * A_EXP))));
+                    y[e] = fmaf(st.b * exp2f((float)(P_EXP - A_EXP)), a[e], x[j + e] * (st.c * exp2f((float)(P_EXP - 2 * A_EXP))));
                     if (c + j + e == row) y[e] += st.a * exp2f((float)P_EXP);
                 }
                 put(as, a_plane, row, c + j, y);
@@ -439,7 +435,7 @@ int launch(const Io& io, const Geometry& g, int64_t batch, const Steps& st, int3
     cfg.gridDim = dim3((unsigned)(batch * g.cluster)); cfg.blockDim = dim3(THREADS);
     // A CTA that waits for tensor memory may not hold up a cluster whose other CTAs are waited for: kernels with clusters
     // take more than half of an SM's shared memory, so that no two of them share one.
-    size_t smem = (size_t)(g.x_bytes + g.a_bytes + 128 + 1024);
+    size_t smem = (size_t)(g.x_bytes + g.a_bytes + 256 + 1024);
     if (g.cluster > 1 && smem < 116 * 1024) smem = 116 * 1024;
     cfg.dynamicSmemBytes = smem; cfg.stream = s;
     cudaLaunchAttribute attr[1];
@@ -455,7 +451,7 @@ int launch_planes(const Io& io, const Geometry& g, int64_t batch, const Steps& s
 template <typename T>
 int orthogonalize_typed(const void* g, int64_t sb, int64_t sr, int64_t sc, void* out, int64_t m, int64_t n, const Shape& sh, const Steps& st,
                         int32_t* status, cudaStream_t s) {
-    const OrthogonalizeIo<T> io{{reinterpret_cast<const T*>(g), sb, sr, sc}, reinterpret_cast<T*>(out), m, n};
+    const OrthogonalizeIo<T> io{reinterpret_cast<const T*>(g), sb, sr, sc, reinterpret_cast<T*>(out), m, n};
     return launch_planes(io, geometry(sh, m > n), sh.batch, st, status, s);
 }
 }  // namespace
@@ -468,9 +464,9 @@ int launch_small_orthogonalize(const void* g, int dtype, int64_t sb, int64_t sr,
     if (dtype == CHEBYKAN_DTYPE_BF16) return orthogonalize_typed<__nv_bfloat16>(g, sb, sr, sc, out, m, n, sh, st, status, s);
     return orthogonalize_typed<__half>(g, sb, sr, sc, out, m, n, sh, st, status, s);
 }
-int launch_small_muon(float* param, const float* grad, float* buf, int64_t in, int64_t out, int dp1, float keep, float step, float momentum,
-                      int nesterov, float gs, const Shape& sh, const Steps& st, int32_t* status, cudaStream_t s) {
-    const MuonIo io{param, grad, buf, out, dp1, nesterov, momentum, gs, keep, step};
+int launch_small_update(float* param, const float* u, int64_t in, int64_t out, int dp1, float keep, float step, const Shape& sh,
+                        const Steps& st, int32_t* status, cudaStream_t s) {
+    const UpdateIo io{param, u, in, out, dp1, keep, step};
     return launch_planes(io, geometry(sh, in > out), dp1, st, status, s);
 }
 
