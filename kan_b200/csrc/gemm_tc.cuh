@@ -35,7 +35,7 @@ struct Config {
     static constexpr int L_PANEL = 128 * 128, R_PANEL = BN / CG * 128;
     static constexpr int STAGE = PLANES * (L_PANEL + R_PANEL);
     static constexpr int STAGES = (200 * 1024) / STAGE > 8 ? 8 : (200 * 1024) / STAGE;
-    static constexpr int KCHUNK = PP == 3 ? 4 : (1 << 30);
+    static constexpr int KCHUNK = PP == 3 ? 2 : (1 << 30);
     static constexpr int ACC_COLS = PP == 3 ? 2 * BN : BN;     // columns of one accumulator buffer
     static constexpr int TMEM_COLS = 2 * ACC_COLS;
     static constexpr int BARS = 2 * STAGES + 5;

@@ -30,41 +30,84 @@ __device__ __forceinline__ float load1(const float* p) { return *p; }
 __device__ __forceinline__ float load1(const __half* p) { return __half2float(*p); }
 __device__ __forceinline__ float load1(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 
-__device__ __forceinline__ int quantise(float v, float inv) {
-    const int q = __float2int_rn(v * inv);
-    return q > 127 ? 127 : (q < -127 ? -127 : q);
+// eight values from p (values past `left` are zero): 16-byte loads where the rows allow
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int left, bool vec, float (&v)[8]) {
+    if (vec && left >= 8) {
+        alignas(16) T t[8];
+        *reinterpret_cast<uint4*>(t) = *reinterpret_cast<const uint4*>(p);
+        if (sizeof(T) == 4) *reinterpret_cast<uint4*>(t + 8 - 16 / sizeof(T)) = *reinterpret_cast<const uint4*>(p + 8 - 16 / sizeof(T));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = load1(t + e);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = e < left ? load1(p + e) : 0.f;
+    }
 }
 
-// One group of G threads per row (G = 32: eight rows per block; 256: a row per block), four inputs per thread at a time.
-// Pass 1 finds the row's largest |T_d|, pass 2 evaluates the row again and writes it.
-template <typename T, int G>
+// round(v * inv) for four values with |v * inv| < 128, as bytes: adding 1.5 * 2^23 leaves the rounded integer (ties to
+// even) in the low bits of the sum, whose lowest bytes a byte permutation collects.  A conversion instruction per value
+// has a quarter of the throughput.
+__device__ __forceinline__ uint32_t quantise4(const float (&v)[8], int at, float inv) {
+    uint32_t b[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) b[e] = __float_as_uint(fmaf(v[at + e], inv, 12582912.f));
+    return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+}
+
+// A row per group of G threads, eight neighbouring inputs per thread and chunk.  The first pass finds the row's largest
+// |T_d|, the second evaluates the recurrence again and writes it; tanh, by far the dearer part, is kept in registers in
+// between (CHUNKS per thread; 0: rows longer than that evaluate it twice).
+// Bound by issue slots and memory alike: 32768 x 2048, degree 4 moves 268 MB in and 268 MB out.
+template <typename T, int G, int CHUNKS>
 __global__ void __launch_bounds__(256)
-basis_kernel(const T* __restrict__ x, int8_t* __restrict__ q, float* __restrict__ scale, int64_t B, int in, int pad, int deg) {
-    constexpr int ROWS = 256 / G;
+basis_kernel(const T* __restrict__ x, int8_t* __restrict__ q, float* __restrict__ scale, int64_t B, int in, int pad, int deg, int vec) {
+    constexpr int ROWS = 256 / G, KEEP = CHUNKS ? CHUNKS : 1;
     __shared__ float red[8];
     const int lane = threadIdx.x % G;
     const int64_t row = blockIdx.x * (int64_t)ROWS + threadIdx.x / G;
     const bool live = row < B;
     const T* src = x + row * in;
+    const int chunks = CHUNKS ? CHUNKS : (pad + 8 * G - 1) / (8 * G);
+    float t[KEEP][8];
     float top = 0.f;
-    if (live)
-        for (int i0 = 4 * lane; i0 < in; i0 += 4 * G)
-            for (int e = 0; e < 4 && i0 + e < in; ++e) {
-                const float t = tanh_of(load1(src + i0 + e));
-                float a = t, b = 1.f;
-                top = t == t ? fmaxf(top, fabsf(a)) : __int_as_float(0x7f800000);      // a NaN wins
-                for (int d = 2; d <= deg; ++d) {
-                    const float n = fmaf(2.f * t, a, -b);
-                    b = a; a = n;
-                    top = fmaxf(top, fabsf(a));
-                }
+    bool nan = false;
+#pragma unroll
+    for (int c = 0; c < chunks; ++c) {
+        float (&tc)[8] = t[CHUNKS ? c : 0];
+        const int i0 = (c * G + lane) * 8;
+        if (live && i0 < in) {
+            load8(src + i0, in - i0, vec, tc);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                tc[e] = tanh_of(tc[e]);
+                nan = nan || tc[e] != tc[e];
             }
+            // from degree 2 on inputs past the row's end would count as T_2(0) = -1
+            const int n = in - i0 < 8 ? in - i0 : 8;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < n) {
+                    float a = tc[e], b = 1.f;
+                    const float tt = 2.f * a;
+                    top = fmaxf(top, fabsf(a));
+                    for (int d = 2; d <= deg; ++d) {
+                        const float next = fmaf(tt, a, -b);
+                        b = a; a = next;
+                        top = fmaxf(top, fabsf(a));
+                    }
+                }
+        }
+    }
+    if (nan) top = __int_as_float(0x7f800000);
 #pragma unroll
     for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
     if (G > 32) {
         if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
         __syncthreads();
-        for (int w = 0; w < 8; ++w) top = fmaxf(top, red[w]);
+        const int w0 = threadIdx.x / G * (G / 32);
+#pragma unroll
+        for (int w = 0; w < G / 32; ++w) top = fmaxf(top, red[w0 + w]);
     }
     if (!live) return;
     const bool bad = top > 3.f;                    // |T_d| <= 1 up to rounding
@@ -72,23 +115,35 @@ basis_kernel(const T* __restrict__ x, int8_t* __restrict__ q, float* __restrict_
     const float inv = (bad || s == 0.f) ? 0.f : __fdiv_rn(1.f, s);
     if (lane == 0) scale[row] = s;
     int8_t* dst = q + row * (int64_t)deg * pad;
-    for (int i0 = 4 * lane; i0 < pad; i0 += 4 * G) {
-        float tt[4], a[4], b[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float t = (i0 + e < in && !bad) ? tanh_of(load1(src + i0 + e)) : 0.f;
-            tt[e] = 2.f * t; a[e] = t; b[e] = 1.f;
+    for (int c = 0; c < chunks; ++c) {
+        float (&tc)[8] = t[CHUNKS ? c : 0];
+        const int i0 = (c * G + lane) * 8;
+        if (i0 >= pad) continue;
+        const int n = in - i0;                     // inputs of the chunk; the rest of the padded row is zero
+        if (CHUNKS == 0 && n > 0) {
+            load8(src + i0, n, vec, tc);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) tc[e] = tanh_of(tc[e]);
+        }
+        float a[8], b[8];
+        uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
+        if (bad) keep0 = keep1 = 0;
+        else if (n < 8) {
+            keep0 = n <= 0 ? 0 : (n >= 4 ? keep0 : (1u << (8 * n)) - 1u);
+            keep1 = n <= 4 ? 0 : (1u << (8 * (n - 4))) - 1u;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            a[e] = tc[e]; b[e] = 1.f;
+            tc[e] *= 2.f;
         }
         for (int d = 1; d <= deg; ++d) {
-            uint32_t w = 0;
+            *reinterpret_cast<uint2*>(dst + (int64_t)(d - 1) * pad + i0) = make_uint2(quantise4(a, 0, inv) & keep0, quantise4(a, 4, inv) & keep1);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (i0 + e < in) w |= (uint32_t)(quantise(a[e], inv) & 255) << (8 * e);
-            *reinterpret_cast<uint32_t*>(dst + (int64_t)(d - 1) * pad + i0) = w;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float n = fmaf(tt[e], a[e], -b[e]);
-                b[e] = a[e]; a[e] = n;
+            for (int e = 0; e < 8; ++e) {
+                const float next = fmaf(tc[e], a[e], -b[e]);
+                b[e] = a[e]; a[e] = next;
             }
         }
     }
@@ -136,15 +191,23 @@ pack_kernel(const float* __restrict__ c, int8_t* __restrict__ wq, float* __restr
         }
 }
 
+template <typename T, int G, int CHUNKS>
+int launch_basis_one(const T* x, int8_t* q, float* scale, int64_t B, int64_t in, int64_t deg, cudaStream_t s) {
+    const int vec = (in * sizeof(T)) % 16 == 0;
+    basis_kernel<T, G, CHUNKS><<<(unsigned)ceil_div(B, 256 / G), 256, 0, s>>>(x, q, scale, B, (int)in, (int)in_pad(in), (int)deg, vec);
+    return check_cuda(cudaGetLastError());
+}
+// the narrowest group that needs at most two chunks per thread: more rows per block, fewer idle threads at a row's end
 template <typename T>
 int launch_basis_typed(const void* x, int8_t* q, float* scale, int64_t B, int64_t in, int64_t deg, cudaStream_t s) {
-    const int pad = (int)in_pad(in);
     const T* xt = reinterpret_cast<const T*>(x);
-    if (in <= 256)
-        basis_kernel<T, 32><<<(unsigned)ceil_div(B, 8), 256, 0, s>>>(xt, q, scale, B, (int)in, pad, (int)deg);
-    else
-        basis_kernel<T, 256><<<(unsigned)B, 256, 0, s>>>(xt, q, scale, B, (int)in, pad, (int)deg);
-    return check_cuda(cudaGetLastError());
+    const int64_t pad = in_pad(in);
+    if (pad <= 256) return launch_basis_one<T, 32, 1>(xt, q, scale, B, in, deg, s);
+    if (pad <= 512) return launch_basis_one<T, 32, 2>(xt, q, scale, B, in, deg, s);
+    if (pad <= 1024) return launch_basis_one<T, 64, 2>(xt, q, scale, B, in, deg, s);
+    if (pad <= 2048) return launch_basis_one<T, 256, 1>(xt, q, scale, B, in, deg, s);
+    if (pad <= 4096) return launch_basis_one<T, 256, 2>(xt, q, scale, B, in, deg, s);
+    return launch_basis_one<T, 256, 0>(xt, q, scale, B, in, deg, s);
 }
 
 int launch_basis(const void* x, int dtype, int8_t* q, float* scale, int64_t B, int64_t in, int64_t deg, cudaStream_t s) {

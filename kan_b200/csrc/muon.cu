@@ -80,15 +80,23 @@ __global__ void __launch_bounds__(256) norm_kernel(const T* __restrict__ g, cons
 // Momentum of the whole tensor, and the update u turned from [in*out][deg+1] to a plane per degree, through a tile in shared
 // memory (deg+1 made odd, so that a column of it meets every bank): both sides are contiguous.  With `partial` also the
 // sums of squares of each degree's u.
-// deg+1 up to 40: 256 elements of every degree in a tile, above: 64 (42 KB at most)
-__host__ __device__ constexpr int tile_width(int dp1) { return dp1 <= 40 ? 256 : 64; }
+// `width` elements of every degree: as many as 24 KB hold (so that several blocks share an SM), fewer where the tensor would
+// not give every SM two tiles
+int tile_width(int64_t pairs, int dp1) {
+    int width = 256;
+    while (width > 32 && ((dp1 | 1) * width * 4 > 24 * 1024 || ceil_div(pairs, width) < 2 * 148)) width /= 2;
+    return width;
+}
+// quotient by dp1 of numbers below 2^16 without a division
+__device__ __forceinline__ uint32_t divide(uint32_t e, uint32_t magic) { return __umulhi(e, magic); }
+uint32_t magic_of(int dp1) { return dp1 == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + dp1 - 1) / dp1); }
 
 __global__ void __launch_bounds__(256)
-momentum_kernel(const float* __restrict__ grad, float* __restrict__ buf, float* __restrict__ u, int64_t pairs, int dp1, float momentum,
-                int nesterov, float gs, double* __restrict__ partial) {
+momentum_kernel(const float* __restrict__ grad, float* __restrict__ buf, float* __restrict__ u, int64_t pairs, int dp1, int width,
+                uint32_t magic, float momentum, int nesterov, float gs, double* __restrict__ partial) {
     extern __shared__ float tile[];
     __shared__ double sums[128];
-    const int width = tile_width(dp1), odd = dp1 | 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int odd = dp1 | 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     for (int d = threadIdx.x; d < dp1; d += 256) sums[d] = 0.;
     const int64_t tiles = (pairs + width - 1) / width;
     for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
@@ -106,7 +114,8 @@ momentum_kernel(const float* __restrict__ grad, float* __restrict__ buf, float* 
                 if (e < count) {
                     m[k] = fmaf(1.f - momentum, g[k] - m[k], m[k]);
                     buf[p0 * dp1 + e] = m[k];
-                    tile[e / dp1 * odd + e % dp1] = nesterov ? fmaf(momentum, m[k] - g[k], g[k]) : m[k];
+                    const int w = magic ? (int)divide((uint32_t)e, magic) : e;
+                    tile[w * odd + e - w * dp1] = nesterov ? fmaf(momentum, m[k] - g[k], g[k]) : m[k];
                 }
             }
         }
@@ -133,9 +142,9 @@ momentum_kernel(const float* __restrict__ grad, float* __restrict__ buf, float* 
 
 // param = keep * param - step * O, O one plane per degree: the same tile the other way
 __global__ void __launch_bounds__(256)
-update_kernel(float* __restrict__ param, const float* __restrict__ o, int64_t pairs, int dp1, float keep, float step) {
+update_kernel(float* __restrict__ param, const float* __restrict__ o, int64_t pairs, int dp1, int width, uint32_t magic, float keep, float step) {
     extern __shared__ float tile[];
-    const int width = tile_width(dp1), odd = dp1 | 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int odd = dp1 | 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t tiles = (pairs + width - 1) / width;
     for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
         const int64_t p0 = t * width;
@@ -159,19 +168,22 @@ update_kernel(float* __restrict__ param, const float* __restrict__ o, int64_t pa
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const int e = e0 + k * 256;
-                if (e < count) param[p0 * dp1 + e] = fmaf(-step, tile[e / dp1 * odd + e % dp1], keep * p[k]);
+                if (e < count) {
+                    const int w = magic ? (int)divide((uint32_t)e, magic) : e;
+                    param[p0 * dp1 + e] = fmaf(-step, tile[w * odd + e - w * dp1], keep * p[k]);
+                }
             }
         }
     }
 }
 
-// the scales of matrix b from its partial sums, by one warp
-__device__ __forceinline__ void warp_scales(const double* partial, float eps, int growth, double* pow2, float* alpha, float* later) {
+// the scales of a matrix from its partial sums, by the block (thread 0 writes them; a barrier follows in the caller)
+__device__ __forceinline__ void block_scales(const double* partial, float eps, int growth, double* pow2, float* alpha, float* later) {
+    __shared__ double smem[8];
     double t = 0.;
-    for (int k = threadIdx.x & 31; k < NORM_BLOCKS; k += 32) t += partial[k];
-#pragma unroll
-    for (int d = 16; d; d >>= 1) t += __shfl_down_sync(0xffffffffu, t, d);
-    if ((threadIdx.x & 31) == 0) scales_of(sqrt(t), eps, growth, pow2, alpha, later);
+    for (int k = threadIdx.x; k < NORM_BLOCKS; k += 256) t += partial[k];
+    t = block_sum(t, smem);
+    if (threadIdx.x == 0) scales_of(sqrt(t), eps, growth, pow2, alpha, later);
 }
 
 // X_0 planes where X's rows are the rows of the source: eight columns per thread
@@ -182,7 +194,7 @@ pack_rows_kernel(const T* __restrict__ g, const Plane pl, __half* __restrict__ x
     __shared__ double pow2;
     __shared__ float scales[2];
     const int64_t b = blockIdx.y;
-    if (threadIdx.x < 32) warp_scales(partial + b * NORM_BLOCKS, eps, growth, &pow2, &scales[0], &scales[1]);
+    block_scales(partial + b * NORM_BLOCKS, eps, growth, &pow2, &scales[0], &scales[1]);
     __syncthreads();
     if (blockIdx.x == 0 && threadIdx.x == 0) { alpha[b] = scales[0]; alpha[sh.batch + b] = scales[1]; }
     const int64_t groups = sh.ls / 8, total = sh.s * groups;
@@ -209,7 +221,7 @@ pack_turned_kernel(const T* __restrict__ g, const Plane pl, __half* __restrict__
     __shared__ double pow2;
     __shared__ float scales[2];
     const int64_t b = blockIdx.z, r0 = blockIdx.y * 32, c0 = blockIdx.x * 64;
-    if (threadIdx.x < 32) warp_scales(partial + b * NORM_BLOCKS, eps, growth, &pow2, &scales[0], &scales[1]);
+    block_scales(partial + b * NORM_BLOCKS, eps, growth, &pow2, &scales[0], &scales[1]);
     __syncthreads();
     if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) { alpha[b] = scales[0]; alpha[sh.batch + b] = scales[1]; }
     {
@@ -421,11 +433,13 @@ int chebykan_muon_step(float* param, const float* grad, float* buf, void* worksp
     float* u = reinterpret_cast<float*>(ws + w.u);
     cudaStream_t s = (cudaStream_t)stream;
     const bool small = small_supported(sh);
-    const int64_t pairs = in * out, tiles = ceil_div(pairs, tile_width(dp1));
-    const int smem = (dp1 | 1) * tile_width(dp1) * 4;
+    const int64_t pairs = in * out;
+    const int width = tile_width(pairs, dp1), smem = (dp1 | 1) * width * 4;
+    const int64_t tiles = ceil_div(pairs, width);
+    const uint32_t magic = magic_of(dp1);
     // a block of the norm's partial sums each, also where it has no tile
     const unsigned blocks = (unsigned)(small && tiles < NORM_BLOCKS ? tiles : NORM_BLOCKS);
-    momentum_kernel<<<blocks, 256, smem, s>>>(grad, buf, u, pairs, dp1, momentum, nesterov, grad_scale,
+    momentum_kernel<<<blocks, 256, smem, s>>>(grad, buf, u, pairs, dp1, width, magic, momentum, nesterov, grad_scale,
                                               small ? nullptr : reinterpret_cast<double*>(ws + w.partial));
     if ((rc = check_cuda(cudaGetLastError()))) return rc;
     const float keep = 1.f - lr * weight_decay, step = lr * update_scale;
@@ -433,8 +447,7 @@ int chebykan_muon_step(float* param, const float* grad, float* buf, void* worksp
     if ((rc = pack(u, Plane{in, out, out, 1, pairs}, in > out, ws, w, sh, st, s))) return rc;
     // the packed operands have taken u's place: O goes there
     if ((rc = run_steps(ws, w, sh, st, u, CHEBYKAN_DTYPE_FP32, in > out, status, s))) return rc;
-    const int64_t update_blocks = tiles < 148 * 4 ? tiles : 148 * 4;
-    update_kernel<<<(unsigned)update_blocks, 256, smem, s>>>(param, u, pairs, dp1, keep, step);
+    update_kernel<<<(unsigned)(tiles < 148 * 8 ? tiles : 148 * 8), 256, smem, s>>>(param, u, pairs, dp1, width, magic, keep, step);
     return check_cuda(cudaGetLastError());
 }
 

@@ -33,7 +33,7 @@ struct Workspace {        // byte offsets of the buffers
 };
 
 // per-matrix partial sums of squares written by the norm kernels
-constexpr int NORM_BLOCKS = 296;
+constexpr int NORM_BLOCKS = 148 * 6;
 
 __device__ __forceinline__ uint32_t half2_bits(float x, float y) {
     const __half2 h = __floats2half2_rn(x, y);
