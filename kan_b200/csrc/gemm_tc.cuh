@@ -9,10 +9,10 @@
 //
 // CG = 2: a pair of CTAs works on 256 rows with cta_group::2, each staging its own 128 rows of L and half of R's columns,
 // which halves R's traffic out of L2 and the shared-memory reads per MMA.  The even CTA's thread issues the MMAs.
-// PP = 3: both operands come as two fp16 planes (head and tail) and three products are summed: head x head in one
-// accumulator, head x tail and tail x head in another, each over KCHUNK K blocks only.  The tensor pipe's fp32 sums
-// truncate, by about 2^-26 of the accumulator per MMA: short sums of their own, added up in registers by the epilogue
-// warps with round-to-nearest, keep the result at fp32 quality.
+// PP = 3: both operands come as two fp16 planes (head and tail) and three products are summed: head x head over KCHUNK K
+// blocks at a time, head x tail and tail x head over the whole of K in an accumulator of their own.  The tensor pipe's fp32
+// sums truncate, by about 2^-26 of the accumulator per MMA: short sums, added up in registers by the epilogue warps with
+// round-to-nearest, keep the result at fp32 quality, and the cross products are 2^11 times smaller to begin with.
 // Two accumulator buffers alternate, so an epilogue (or a chunk's addition) overlaps the next MMAs.
 // Every wait is bounded (see tc_common.cuh).
 #pragma once
@@ -36,8 +36,8 @@ struct Config {
     static constexpr int STAGE = PLANES * (L_PANEL + R_PANEL);
     static constexpr int STAGES = (200 * 1024) / STAGE > 8 ? 8 : (200 * 1024) / STAGE;
     static constexpr int KCHUNK = PP == 3 ? 2 : (1 << 30);
-    static constexpr int ACC_COLS = PP == 3 ? 2 * BN : BN;     // columns of one accumulator buffer
-    static constexpr int TMEM_COLS = 2 * ACC_COLS;
+    // two accumulators of BN columns that alternate chunk by chunk; PP = 3: behind them two for the cross products, tile by tile
+    static constexpr int TMEM_COLS = (PP == 3 ? 4 : 2) * BN;
     static constexpr int BARS = 2 * STAGES + 5;
     static constexpr int BAR_OFFSET = STAGES * STAGE;
     static constexpr int SMEM = BAR_OFFSET + BARS * 8 + 16 + 1024;
@@ -113,6 +113,22 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
           "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr) : "memory");
+}
+// v[0..BN) (+)= columns of an accumulator; the next 16 are on their way while 16 are added
+template <int BN, bool SET>
+__device__ __forceinline__ void add_columns(uint32_t taddr, float (&v)[BN]) {
+    uint32_t r[2][16];
+    tmem_ld16(taddr, r[0]);
+#pragma unroll
+    for (int c = 0; c < BN / 16; ++c) {
+        tmem_ld_wait();
+        if (c + 1 < BN / 16) tmem_ld16(taddr + (c + 1) * 16, r[(c + 1) & 1]);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const float x = __uint_as_float(r[c & 1][e]);
+            v[c * 16 + e] = SET ? x : v[c * 16 + e] + x;
+        }
+    }
 }
 // operand of [K][N] boxes: 64 columns per 128-byte row, rows are K; 8-row groups 1024 bytes apart, the next 64 columns
 // one box (64 rows, 8192 bytes) further
@@ -215,12 +231,13 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ C
             const uint32_t l_hi = (uint32_t)(l_desc >> 32), r_hi = (uint32_t)(r_desc >> 32);
             constexpr uint32_t L_TAIL = C::L_PANEL >> 4, R_TAIL = C::R_PANEL >> 4;
             constexpr uint32_t R_STEP = C::RMN ? 2048 >> 4 : 32 >> 4;      // 16 rows of K, or 32 bytes of a row
-            for (int64_t t = unit; t < g.total && alive; t += units)
+            uint32_t cross = tmem + 2 * BN;
+            for (int64_t t = unit; t < g.total && alive; t += units, cross ^= BN)
                 for (int kb0 = 0; kb0 < g.nkb && alive; kb0 += C::KCHUNK) {
                     const int kb1 = g.nkb - kb0 < C::KCHUNK ? g.nkb : kb0 + C::KCHUNK;
                     if (!__all_sync(0xffffffffu, mbar_wait(acc_empty(acc), acc_ph ^ 1u, abort_flag, status, ST_MMA_ACC))) { alive = false; break; }
                     tc_fence_after();
-                    const uint32_t d = tmem + (uint32_t)(acc * C::ACC_COLS);
+                    const uint32_t d = tmem + (uint32_t)(acc * BN);
                     for (int kb = kb0; kb < kb1; ++kb) {
                         if (!__all_sync(0xffffffffu, mbar_wait(full(s), ph, abort_flag, status, ST_MMA))) { alive = false; break; }
                         tc_fence_after();
@@ -233,8 +250,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ C
                                 const uint32_t la = l_lo + 2u * k, ra = r_lo + R_STEP * k;
                                 mma<C::KIND, CG>(d, desc_from_words(la, l_hi), desc_from_words(ra, r_hi), C::IDESC, k ? 1u : later);
                                 if constexpr (C::PP == 3) {
-                                    mma<C::KIND, CG>(d + BN, desc_from_words(la, l_hi), desc_from_words(ra + R_TAIL, r_hi), C::IDESC, k ? 1u : later);
-                                    mma<C::KIND, CG>(d + BN, desc_from_words(la + L_TAIL, l_hi), desc_from_words(ra, r_hi), C::IDESC, 1u);
+                                    mma<C::KIND, CG>(cross, desc_from_words(la, l_hi), desc_from_words(ra + R_TAIL, r_hi), C::IDESC, k ? 1u : (uint32_t)(kb != 0));
+                                    mma<C::KIND, CG>(cross, desc_from_words(la + L_TAIL, l_hi), desc_from_words(ra, r_hi), C::IDESC, 1u);
                                 }
                             }
                             if (CG == 2) umma2_commit_both(empty(s)); else umma_commit(empty(s));
@@ -257,7 +274,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ C
         }
     } else {
         const int q = warp & 3;               // quarter of the tensor memory's lanes that this warp may read
-        int acc = 0; uint32_t acc_ph = 0;
+        int acc = 0; uint32_t acc_ph = 0, cross_at = 2 * BN;
         bool alive = true;
         auto release = [&](int a) {
             tc_fence_before();
@@ -283,20 +300,15 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ C
                     const bool ok = mbar_wait(acc_full(acc), acc_ph, abort_flag, status, ST_EPILOGUE);
                     if (!__all_sync(0xffffffffu, ok)) { alive = false; break; }
                     tc_fence_after();
-                    const uint32_t ta = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * C::ACC_COLS);
-#pragma unroll
-                    for (int c = 0; c < BN / 16; ++c)
-                        if (c < 2 * nch) {
-                            uint32_t r0[16], r1[16];
-                            tmem_ld16(ta + c * 16, r0);
-                            tmem_ld16(ta + BN + c * 16, r1);
-                            tmem_ld_wait();
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) {
-                                const float part = __uint_as_float(r0[e]) + __uint_as_float(r1[e]);
-                                v[c * 16 + e] = kb0 == 0 ? part : v[c * 16 + e] + part;
-                            }
-                        }
+                    const uint32_t ta = tmem + ((uint32_t)(q * 32) << 16);
+                    if (kb0 == 0) add_columns<BN, true>(ta + (uint32_t)(acc * BN), v);
+                    else add_columns<BN, false>(ta + (uint32_t)(acc * BN), v);
+                    // Before the tile's last buffer is given back the cross products are read: the buffer they will be
+                    // summed in next, two tiles on, is started only after two more buffers were given back.
+                    if (kb0 + C::KCHUNK >= g.nkb) {
+                        add_columns<BN, false>(ta + cross_at, v);
+                        cross_at ^= BN;
+                    }
                     release(acc);
                     acc ^= 1;
                     if (acc == 0) acc_ph ^= 1u;
@@ -315,7 +327,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ C
                 const bool ok = mbar_wait(acc_full(acc), acc_ph, abort_flag, status, ST_EPILOGUE);
                 if (!__all_sync(0xffffffffu, ok)) { alive = false; break; }
                 tc_fence_after();
-                const uint32_t ta = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * C::ACC_COLS);
+                const uint32_t ta = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN);
                 // two register buffers: the load of the next 32 columns is in flight while these are written
                 uint32_t ra[32], rb[32];
                 tmem_ld32(ta, ra);
@@ -460,7 +472,7 @@ split_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ 
             const int kb1 = k_last - kb0 < C::KCHUNK ? k_last : kb0 + C::KCHUNK;
             if (!__all_sync(0xffffffffu, mbar_wait(acc_empty(acc), acc_ph ^ 1u, abort_flag, status, ST_MMA_ACC))) { alive = false; break; }
             tc_fence_after();
-            const uint32_t d = tmem + (uint32_t)(acc * C::ACC_COLS);
+            const uint32_t d = tmem + (uint32_t)(acc * BN);
             for (int kb = kb0; kb < kb1; ++kb) {
                 if (!__all_sync(0xffffffffu, mbar_wait(full(s), ph, abort_flag, status, ST_MMA))) { alive = false; break; }
                 tc_fence_after();
@@ -473,8 +485,8 @@ split_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ 
                         const uint32_t la = l_lo + 2u * k, ra = r_lo + R_STEP * k;
                         mma<C::KIND, 1>(d, desc_from_words(la, l_hi), desc_from_words(ra, r_hi), C::IDESC, k ? 1u : later);
                         if constexpr (C::PP == 3) {
-                            mma<C::KIND, 1>(d + BN, desc_from_words(la, l_hi), desc_from_words(ra + R_TAIL, r_hi), C::IDESC, k ? 1u : later);
-                            mma<C::KIND, 1>(d + BN, desc_from_words(la + L_TAIL, l_hi), desc_from_words(ra, r_hi), C::IDESC, 1u);
+                            mma<C::KIND, 1>(tmem + 2 * BN, desc_from_words(la, l_hi), desc_from_words(ra + R_TAIL, r_hi), C::IDESC, k ? 1u : (uint32_t)(kb != k_first));
+                            mma<C::KIND, 1>(tmem + 2 * BN, desc_from_words(la + L_TAIL, l_hi), desc_from_words(ra, r_hi), C::IDESC, 1u);
                         }
                     }
                     umma_commit(empty(s));
@@ -497,28 +509,15 @@ split_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ 
         const int q = warp & 3;
         int acc = 0; uint32_t acc_ph = 0;
         bool alive = true;
-        uint32_t v[BN];
+        float v[BN];
         for (int kb0 = k_first; kb0 < k_last; kb0 += C::KCHUNK) {
             const bool ok = mbar_wait(acc_full(acc), acc_ph, abort_flag, status, ST_EPILOGUE);
             if (!__all_sync(0xffffffffu, ok)) { alive = false; break; }
             tc_fence_after();
-            const uint32_t ta = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * C::ACC_COLS);
-#pragma unroll
-            for (int c = 0; c < BN / 32; ++c) {
-                uint32_t r0[32], r1[32];
-                tmem_ld32(ta + c * 32, r0);
-                if (C::PP == 3) tmem_ld32(ta + BN + c * 32, r1);
-                tmem_ld_wait();
-#pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    if constexpr (C::PP == 3) {
-                        const float part = __uint_as_float(r0[e]) + __uint_as_float(r1[e]);
-                        v[c * 32 + e] = __float_as_uint(kb0 == k_first ? part : __uint_as_float(v[c * 32 + e]) + part);
-                    } else {
-                        v[c * 32 + e] = r0[e];
-                    }
-                }
-            }
+            const uint32_t ta = tmem + ((uint32_t)(q * 32) << 16);
+            if (kb0 == k_first) add_columns<BN, true>(ta + (uint32_t)(acc * BN), v);      // integers: bits, never added here
+            else add_columns<BN, false>(ta + (uint32_t)(acc * BN), v);
+            if (C::PP == 3 && kb0 + C::KCHUNK >= k_last) add_columns<BN, false>(ta + 2 * BN, v);
             tc_fence_before();
             mbar_arrive(acc_empty(acc));
             acc ^= 1;
@@ -529,7 +528,8 @@ split_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ 
             const uint32_t dst = base + (uint32_t)((q * 32 + lane) * L::PITCH);
 #pragma unroll
             for (int e = 0; e < BN; e += 4)
-                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + e * 4), "r"(v[e]), "r"(v[e + 1]), "r"(v[e + 2]), "r"(v[e + 3]) : "memory");
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + e * 4), "r"(__float_as_uint(v[e])), "r"(__float_as_uint(v[e + 1])),
+                             "r"(__float_as_uint(v[e + 2])), "r"(__float_as_uint(v[e + 3])) : "memory");
         }
     }
     tc_fence_before();

@@ -16,6 +16,7 @@ using gemm::Tiles;
 struct EpiArgs {
     const float *q_scale, *w_scale, *bias;
     void* y;
+    int vec;                  // y's rows and the columns' scales allow 16-byte accesses
 };
 
 template <typename OUT>
@@ -32,23 +33,41 @@ struct Epilogue {
         const float qs = __ldg(p.q_scale + row);
         OUT* dst = reinterpret_cast<OUT*>(p.y) + (int64_t)row * g.N + col0;
         constexpr int V = 16 / (int)sizeof(OUT);          // values of a 16-byte store
-        const bool vec = g.N % V == 0;
+        if (col0 + NC <= g.N && p.vec) {
+            // every load of the columns' scales first: one after the other, each waited for, they would take longer than
+            // the tile's MMAs
+            float4 ws[NC / 4], bs[NC / 4];
 #pragma unroll
-        for (int c = 0; c < NC; c += V) {
-            alignas(16) OUT out[V];
+            for (int c = 0; c < NC / 4; ++c) ws[c] = __ldg(reinterpret_cast<const float4*>(p.w_scale + col0) + c);
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const int col = col0 + c + e;
-                if (col < g.N)
-                    out[e] = to_type<OUT>(fmaf((float)(int)r[c + e] * qs, __ldg(p.w_scale + col), p.bias ? __ldg(p.bias + col) : 0.f));
-            }
-            if (vec && col0 + c < g.N) {
+            for (int c = 0; c < NC / 4; ++c)
+                bs[c] = p.bias ? __ldg(reinterpret_cast<const float4*>(p.bias + col0) + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int c = 0; c < NC; c += V) {
+                alignas(16) OUT out[V];
+#pragma unroll
+                for (int e = 0; e < V; e += 4) {
+                    const int k = c + e;
+                    const float4 w = ws[k / 4], b = bs[k / 4];
+                    out[e] = to_type<OUT>(fmaf((float)(int)r[k] * qs, w.x, b.x));
+                    out[e + 1] = to_type<OUT>(fmaf((float)(int)r[k + 1] * qs, w.y, b.y));
+                    out[e + 2] = to_type<OUT>(fmaf((float)(int)r[k + 2] * qs, w.z, b.z));
+                    out[e + 3] = to_type<OUT>(fmaf((float)(int)r[k + 3] * qs, w.w, b.w));
+                }
                 *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(out);
-            } else {
-#pragma unroll
-                for (int e = 0; e < V; ++e)
-                    if (col0 + c + e < g.N) dst[c + e] = out[e];
             }
+        } else {
+            // ragged right edge, or rows of y that are not 16 bytes apart
+            float ws[NC], bs[NC];
+#pragma unroll
+            for (int e = 0; e < NC; ++e) {
+                const int col = col0 + e < g.N ? col0 + e : g.N - 1;
+                ws[e] = __ldg(p.w_scale + col);
+                bs[e] = p.bias ? __ldg(p.bias + col) : 0.f;
+            }
+#pragma unroll
+            for (int e = 0; e < NC; ++e)
+                if (col0 + e < g.N) dst[e] = to_type<OUT>(fmaf((float)(int)r[e] * qs, ws[e], bs[e]));
         }
     }
 };
@@ -154,7 +173,7 @@ int launch_typed(const Product& p, int32_t* status, cudaStream_t s) {
         return check_cuda(cudaGetLastError());
     }
     if (p.M <= 8) return launch_rows<OUT>(p, s);
-    const EpiArgs args{p.q_scale, p.w_scale, p.bias, p.y};
+    const EpiArgs args{p.q_scale, p.w_scale, p.bias, p.y, p.N % (16 / (int64_t)sizeof(OUT)) == 0 && aligned16(p.w_scale) && aligned16(p.bias)};
     using Pair = gemm::Config<gemm::I8, 1, 2, 256, false>;
     using Narrow = gemm::Config<gemm::I8, 1, 1, 64, false>;
     using Wide = gemm::Config<gemm::I8, 1, 1, 128, false>;
