@@ -5,7 +5,8 @@
 //   warp 0     TMA: one stage = 128 bytes of K of the tile's L rows (128 per CTA) and of R, 128-byte swizzle, no multicast.
 //              R is either [N][K] (K-major) or [K][N] (boxes of 64 K rows x 64 columns, read through an MN-major descriptor)
 //   warp 1     MMA: one elected lane issues tcgen05.mma and the commits that free stages and publish accumulators
-//   warps 2-5  epilogue: tcgen05.ld, then the epilogue's emit() on 32 columns of a row at a time
+//   warps 2-9  epilogue: tcgen05.ld, then the epilogue's emit() on 32 columns of a row at a time; two warps share a quarter of
+//              tensor memory's lanes, half of the columns each
 //
 // CG = 2: a pair of CTAs works on 256 rows with cta_group::2, each staging its own 128 rows of L and half of R's columns,
 // which halves R's traffic out of L2 and the shared-memory reads per MMA.  The even CTA's thread issues the MMAs.
@@ -47,7 +48,7 @@ struct Config {
     static_assert(TMEM_COLS <= 512 && (TMEM_COLS & (TMEM_COLS - 1)) == 0, "accumulators must fit tensor memory");
     static_assert(KIND == F16 || (PP == 1 && !RMN), "integer products have one plane and K-major operands");
 };
-constexpr int THREADS = 192;
+constexpr int THREADS = 320, EPI_THREADS = 256;
 enum { ST_LOAD = 21, ST_MMA = 22, ST_MMA_ACC = 23, ST_EPILOGUE = 24 };
 
 struct Tiles {
@@ -159,7 +160,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ C
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
-        for (int a = 0; a < 2; ++a) { mbar_init(acc_full(a), 1); mbar_init(acc_empty(a), 128 * CG); }
+        for (int a = 0; a < 2; ++a) { mbar_init(acc_full(a), 1); mbar_init(acc_empty(a), EPI_THREADS * CG); }
         mbar_init(drain, 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -274,6 +275,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ C
         }
     } else {
         const int q = warp & 3;               // quarter of the tensor memory's lanes that this warp may read
+        constexpr int EB = BN / 2;            // columns of its half
+        const int half0 = (warp - 2) / 4 * EB;
         int acc = 0; uint32_t acc_ph = 0, cross_at = 2 * BN;
         bool alive = true;
         auto release = [&](int a) {
@@ -284,29 +287,31 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ C
         for (int64_t t = unit; t < g.total && alive; t += units) {
             int b, m0, n0;
             decode<C::BM, BN>(g, t, b, m0, n0);
+            n0 += half0;
             const int row = m0 + (int)rank * 128 + q * 32 + lane;
             // symmetric results: the warp's 32 x 32 block also goes to its transposed place where no tile computes that
             auto mirrored = [&](int col0) {
                 return g.sym && (row / BN + 1) * BN <= col0 / C::BM * C::BM;
             };
             int ncols = g.N - n0;
-            if (ncols > BN) ncols = BN;
-            const int nch = (ncols + 31) >> 5;
-            typename Epi::template Fetched<32> fa, fb;
-            Epi::template fetch<32>(args, g, b, row, n0, fa);      // in flight while the MMAs run
+            if (ncols > EB) ncols = EB;
+            const int nch = ncols > 0 ? (ncols + 31) >> 5 : 0;
             if constexpr (C::PP == 3) {
-                float v[BN];
+                typename Epi::template Fetched<32> f[EB / 32];      // on their way while the MMAs run
+#pragma unroll
+                for (int c = 0; c < EB / 32; ++c) Epi::template fetch<32>(args, g, b, row, n0 + c * 32, f[c]);
+                float v[EB];
                 for (int kb0 = 0; kb0 < g.nkb; kb0 += C::KCHUNK) {
                     const bool ok = mbar_wait(acc_full(acc), acc_ph, abort_flag, status, ST_EPILOGUE);
                     if (!__all_sync(0xffffffffu, ok)) { alive = false; break; }
                     tc_fence_after();
-                    const uint32_t ta = tmem + ((uint32_t)(q * 32) << 16);
-                    if (kb0 == 0) add_columns<BN, true>(ta + (uint32_t)(acc * BN), v);
-                    else add_columns<BN, false>(ta + (uint32_t)(acc * BN), v);
+                    const uint32_t ta = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)half0;
+                    if (kb0 == 0) add_columns<EB, true>(ta + (uint32_t)(acc * BN), v);
+                    else add_columns<EB, false>(ta + (uint32_t)(acc * BN), v);
                     // Before the tile's last buffer is given back the cross products are read: the buffer they will be
                     // summed in next, two tiles on, is started only after two more buffers were given back.
                     if (kb0 + C::KCHUNK >= g.nkb) {
-                        add_columns<BN, false>(ta + cross_at, v);
+                        add_columns<EB, false>(ta + cross_at, v);
                         cross_at ^= BN;
                     }
                     release(acc);
@@ -315,22 +320,24 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ C
                 }
                 if (!alive) break;
 #pragma unroll
-                for (int c = 0; c < BN / 32; ++c)
+                for (int c = 0; c < EB / 32; ++c)
                     if (c < nch) {
                         uint32_t r[32];
 #pragma unroll
                         for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(v[c * 32 + e]);
-                        if (c + 1 < BN / 32) Epi::template fetch<32>(args, g, b, row, n0 + (c + 1) * 32, c & 1 ? fa : fb);
-                        Epi::template emit<32>(args, g, b, row, n0 + c * 32, r, mirrored(n0 + c * 32), c & 1 ? fb : fa);
+                        Epi::template emit<32>(args, g, b, row, n0 + c * 32, r, mirrored(n0 + c * 32), f[c]);
                     }
             } else {
+                typename Epi::template Fetched<32> fa, fb;
+                Epi::template fetch<32>(args, g, b, row, n0, fa);
                 const bool ok = mbar_wait(acc_full(acc), acc_ph, abort_flag, status, ST_EPILOGUE);
                 if (!__all_sync(0xffffffffu, ok)) { alive = false; break; }
                 tc_fence_after();
-                const uint32_t ta = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN);
+                const uint32_t ta = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN + half0);
                 // two register buffers: the load of the next 32 columns is in flight while these are written
                 uint32_t ra[32], rb[32];
-                tmem_ld32(ta, ra);
+                if (nch > 0) tmem_ld32(ta, ra);
+                else release(acc);
 #pragma unroll 1
                 for (int c = 0; c < nch; c += 2) {
                     tmem_ld_wait();
@@ -411,7 +418,7 @@ split_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ 
     const int rank = (int)cluster_ctarank();
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
-        for (int a = 0; a < 2; ++a) { mbar_init(acc_full(a), 1); mbar_init(acc_empty(a), 128); }
+        for (int a = 0; a < 2; ++a) { mbar_init(acc_full(a), 1); mbar_init(acc_empty(a), EPI_THREADS); }
         mbar_init(drain, 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -509,15 +516,17 @@ split_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ 
         const int q = warp & 3;
         int acc = 0; uint32_t acc_ph = 0;
         bool alive = true;
-        float v[BN];
+        constexpr int EB = BN / 2;
+        const int half0 = (warp - 2) / 4 * EB;
+        float v[EB];
         for (int kb0 = k_first; kb0 < k_last; kb0 += C::KCHUNK) {
             const bool ok = mbar_wait(acc_full(acc), acc_ph, abort_flag, status, ST_EPILOGUE);
             if (!__all_sync(0xffffffffu, ok)) { alive = false; break; }
             tc_fence_after();
-            const uint32_t ta = tmem + ((uint32_t)(q * 32) << 16);
-            if (kb0 == k_first) add_columns<BN, true>(ta + (uint32_t)(acc * BN), v);      // integers: bits, never added here
-            else add_columns<BN, false>(ta + (uint32_t)(acc * BN), v);
-            if (C::PP == 3 && kb0 + C::KCHUNK >= k_last) add_columns<BN, false>(ta + 2 * BN, v);
+            const uint32_t ta = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)half0;
+            if (kb0 == k_first) add_columns<EB, true>(ta + (uint32_t)(acc * BN), v);      // integers: bits, never added here
+            else add_columns<EB, false>(ta + (uint32_t)(acc * BN), v);
+            if (C::PP == 3 && kb0 + C::KCHUNK >= k_last) add_columns<EB, false>(ta + 2 * BN, v);
             tc_fence_before();
             mbar_arrive(acc_empty(acc));
             acc ^= 1;
@@ -525,9 +534,9 @@ split_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ 
         }
         if (alive) {
             // the last accumulator is complete, so every MMA has read its stages and the ring is free for the partial tile
-            const uint32_t dst = base + (uint32_t)((q * 32 + lane) * L::PITCH);
+            const uint32_t dst = base + (uint32_t)((q * 32 + lane) * L::PITCH + half0 * 4);
 #pragma unroll
-            for (int e = 0; e < BN; e += 4)
+            for (int e = 0; e < EB; e += 4)
                 asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + e * 4), "r"(__float_as_uint(v[e])), "r"(__float_as_uint(v[e + 1])),
                              "r"(__float_as_uint(v[e + 2])), "r"(__float_as_uint(v[e + 3])) : "memory");
         }
