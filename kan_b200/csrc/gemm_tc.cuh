@@ -1,20 +1,24 @@
 // D[M][N] = L[M][K] R on tcgen05, for 16-bit floating and 8-bit integer operands: the pipeline shared by the products of
-// the Newton-Schulz steps and of the 8-bit forward.  What happens to the accumulator is the epilogue's, a template argument: emit() takes NC
-// columns of a row, fetch() asks one step earlier for what emit() will read from memory.
+// the Newton-Schulz steps and of the 8-bit forward.  What happens to the accumulator is the epilogue's, a template argument:
+// emit() takes 32 columns of a row per lane, fetch() asks one step earlier for what emit() will read from memory.
 //
 //   warp 0     TMA: one stage = 128 bytes of K of the tile's L rows (128 per CTA) and of R, 128-byte swizzle, no multicast.
 //              R is either [N][K] (K-major) or [K][N] (boxes of 64 K rows x 64 columns, read through an MN-major descriptor)
 //   warp 1     MMA: one elected lane issues tcgen05.mma and the commits that free stages and publish accumulators
-//   warps 2-9  epilogue: tcgen05.ld, then the epilogue's emit() on 32 columns of a row at a time; two warps share a quarter of
-//              tensor memory's lanes, half of the columns each
+//   warps 2-9  epilogue: tcgen05.ld, then emit(); two warps share a quarter of tensor memory's lanes, half of the columns each
 //
 // CG = 2: a pair of CTAs works on 256 rows with cta_group::2, each staging its own 128 rows of L and half of R's columns,
 // which halves R's traffic out of L2 and the shared-memory reads per MMA.  The even CTA's thread issues the MMAs.
-// PP = 3: both operands come as two fp16 planes (head and tail) and three products are summed: head x head over KCHUNK K
-// blocks at a time, head x tail and tail x head over the whole of K in an accumulator of their own.  The tensor pipe's fp32
-// sums truncate, by about 2^-26 of the accumulator per MMA: short sums, added up in registers by the epilogue warps with
-// round-to-nearest, keep the result at fp32 quality, and the cross products are 2^11 times smaller to begin with.
-// Two accumulator buffers alternate, so an epilogue (or a chunk's addition) overlaps the next MMAs.
+// PP = 3: both operands come as two fp16 planes (head and tail) and three products are summed.  The tensor pipe's fp32 sums
+// truncate, by about 2^-26 of the accumulator per MMA, so the accumulator of head x head takes one K block (4 MMAs) at a
+// time and the epilogue warps add the blocks up in registers, rounding to nearest, while the MMAs of head x tail and
+// tail x head run; those are 2^11 times smaller and stay in an accumulator of their own for the whole of K.
+// BN = 256 with pairs: per K block of 64 an SM's shared memory then takes 64 KB and gives 96 KB in the 1536 cycles of 12 MMAs
+// (104 of its 128 bytes per cycle); with BN = 128 it would be 160 bytes per cycle, which held the products at 3/4 of the
+// pipe's rate.
+// PP = 1: two accumulators alternate, so a tile's epilogue overlaps the next tile's MMAs.
+// Symmetric operands (LSYM, RSYM) are stored only in the 256 x 256 blocks on and above the diagonal: a block below it is
+// loaded from its mirror image and read through the other major-ness, which is a bit of the instruction descriptor.
 // Every wait is bounded (see tc_common.cuh).
 #pragma once
 #include "tc_common.cuh"
@@ -25,28 +29,28 @@ using namespace tc;
 
 enum Kind { F16 = 0, I8 = 1 };
 
-template <Kind KIND_, int PP_, int CG_, int BN_, bool RMN_>
+template <Kind KIND_, int PP_, int CG_, int BN_, bool RMN_, bool LSYM_ = false, bool RSYM_ = false>
 struct Config {
     static constexpr Kind KIND = KIND_;
     static constexpr int PP = PP_, CG = CG_, BN = BN_;
-    static constexpr bool RMN = RMN_;
+    static constexpr bool RMN = RMN_, LSYM = LSYM_, RSYM = RSYM_;
     static constexpr int PLANES = PP == 3 ? 2 : 1;
     static constexpr int BM = 128 * CG;                        // rows of a tile
     static constexpr int KE = KIND == I8 ? 128 : 64;           // K elements per stage (128 bytes)
     static constexpr int L_PANEL = 128 * 128, R_PANEL = BN / CG * 128;
     static constexpr int STAGE = PLANES * (L_PANEL + R_PANEL);
-    static constexpr int STAGES = (200 * 1024) / STAGE > 8 ? 8 : (200 * 1024) / STAGE;
-    static constexpr int KCHUNK = PP == 3 ? 2 : (1 << 30);
-    // two accumulators of BN columns that alternate chunk by chunk; PP = 3: behind them two for the cross products, tile by tile
-    static constexpr int TMEM_COLS = (PP == 3 ? 4 : 2) * BN;
+    static constexpr int STAGES = (192 * 1024) / STAGE > 8 ? 8 : (192 * 1024) / STAGE;
+    static constexpr int TMEM_COLS = 2 * BN;                   // two accumulators; PP = 3: heads, cross products
     static constexpr int BARS = 2 * STAGES + 5;
-    static constexpr int BAR_OFFSET = STAGES * STAGE;
+    static constexpr int OUT_OFFSET = STAGES * STAGE;          // 4 KB per epilogue warp
+    static constexpr int BAR_OFFSET = OUT_OFFSET + 8 * 4096;
     static constexpr int SMEM = BAR_OFFSET + BARS * 8 + 16 + 1024;
     static constexpr uint32_t IDESC = KIND == I8
         ? (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24)
         : (1u << 4) | ((RMN ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
     static_assert(TMEM_COLS <= 512 && (TMEM_COLS & (TMEM_COLS - 1)) == 0, "accumulators must fit tensor memory");
-    static_assert(KIND == F16 || (PP == 1 && !RMN), "integer products have one plane and K-major operands");
+    static_assert(KIND == F16 || (PP == 1 && !RMN && !LSYM && !RSYM), "integer products have one plane and K-major operands");
+    static_assert(!(RMN && RSYM), "a symmetric right operand is K-major");
 };
 constexpr int THREADS = 320, EPI_THREADS = 256;
 enum { ST_LOAD = 21, ST_MMA = 22, ST_MMA_ACC = 23, ST_EPILOGUE = 24 };
@@ -56,9 +60,12 @@ struct Tiles {
     int nkb;              // K blocks of a tile
     int ntm, ntn;         // tile rows and columns
     int per_batch;        // tiles of one matrix
-    int sym;              // only tiles that reach the diagonal or lie above it
+    int sym;              // only the 256 x 256 blocks on and above the diagonal
     int64_t total;
 };
+
+// whether element (i, j) of a symmetric matrix is stored
+__host__ __device__ __forceinline__ bool stored(int i, int j) { return j / 256 >= i / 256; }
 
 // position of tile t: matrix b, first row, first column
 template <int BM, int BN>
@@ -72,14 +79,14 @@ __device__ __forceinline__ void decode(const Tiles& g, int64_t t, int& b, int& m
     }
     int tm = 0;
     for (;; ++tm) {
-        const int first = tm * BM / BN, count = g.ntn - first;
+        const int first = tm * BM / 256 * (256 / BN), count = g.ntn - first;
         if (r < count) { m0 = tm * BM; n0 = (first + r) * BN; return; }
         r -= count;
     }
 }
 inline int sym_tiles(int ntm, int ntn, int bm, int bn) {
     int n = 0;
-    for (int tm = 0; tm < ntm; ++tm) n += ntn - tm * bm / bn;
+    for (int tm = 0; tm < ntm; ++tm) n += ntn - tm * bm / 256 * (256 / bn);
     return n;
 }
 
@@ -131,16 +138,53 @@ __device__ __forceinline__ void add_columns(uint32_t taddr, float (&v)[BN]) {
         }
     }
 }
-// operand of [K][N] boxes: 64 columns per 128-byte row, rows are K; 8-row groups 1024 bytes apart, the next 64 columns
-// one box (64 rows, 8192 bytes) further
-__device__ __forceinline__ uint64_t mn_desc(uint32_t addr) {
-    return (make_smem_desc(addr) & ~((uint64_t)0x3fff << 16)) | ((uint64_t)(8192 >> 4) << 16);
+// ---- writing a warp's 32 rows x 32 columns, through its 4 KB of shared memory so that lanes write along rows ----
+__device__ __forceinline__ void st_shared_v4(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+// each lane holds a row's 32 values; rows are `pitch` elements apart from dst on, `rows` x `cols` of them exist.  vec: the
+// row's start and pitch are multiples of 16 bytes
+template <typename OUT>
+__device__ __forceinline__ void store_rows(uint32_t buf, const OUT (&v)[32], OUT* dst, int64_t pitch, int rows, int cols, bool vec) {
+    constexpr int ROW = 32 * (int)sizeof(OUT), CHUNKS = ROW / 16, V = 16 / (int)sizeof(OUT);
+    const int lane = threadIdx.x & 31;
+    // 16-byte chunks are permuted within a row so that neither side's eight lanes meet in a bank
+    auto place = [&](int r, int c) { return buf + (uint32_t)(r * ROW + ((CHUNKS == 8 ? c ^ (r & 7) : c ^ ((r >> 1) & 3)) << 4)); };
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(v);
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) st_shared_v4(place(lane, c), w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) {
+        const int r = (i * 32 + lane) / CHUNKS, c = (i * 32 + lane) % CHUNKS;
+        alignas(16) uint32_t x[4];
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(place(r, c)));
+        if (r < rows) {
+            OUT* to = dst + r * pitch + c * V;
+            if (vec && c * V + V <= cols) {
+                *reinterpret_cast<uint4*>(to) = make_uint4(x[0], x[1], x[2], x[3]);
+            } else {
+                const OUT* e = reinterpret_cast<const OUT*>(x);
+#pragma unroll
+                for (int k = 0; k < V; ++k)
+                    if (c * V + k < cols) to[k] = e[k];
+            }
+        }
+    }
+    __syncwarp();
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+__device__ __forceinline__ void store_3d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];"
+                 ::"l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(src) : "memory");
 }
 
 template <class C, class Epi>
 __global__ void __launch_bounds__(THREADS, 1)
 gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ CUtensorMap map_r, const Tiles g,
-            const typename Epi::Args args, int32_t* status) {
+             const __grid_constant__ typename Epi::Args args, int32_t* status) {
     constexpr int CG = C::CG, BN = C::BN, S = C::STAGES, PLANES = C::PLANES;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -200,16 +244,25 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ C
                         if (CG == 2) load_3d_pair(to, map, c0, c1, z, bar);
                         else load_3d(to, map, c0, c1, z, bar);
                     };
+                    const int k0 = kb * C::KE;
+                    // 128 (or 64) rows from r0 of a symmetric matrix against its columns from k0: two boxes, or their mirror images
+                    auto load_sym = [&](uint32_t to, const CUtensorMap* map, int r0, int rows, int z) {
+                        const bool direct = stored(r0, k0);
+                        for (int q = 0; q < rows; q += 64) load(to + q * 128, map, direct ? k0 : r0 + q, direct ? r0 + q : k0, z);
+                    };
 #pragma unroll
                     for (int p = 0; p < PLANES; ++p) {
                         const int z = b * PLANES + p;
-                        load(dst + p * C::L_PANEL, &map_l, kb * C::KE, row, z);
+                        if (C::LSYM) load_sym(dst + p * C::L_PANEL, &map_l, row, 128, z);
+                        else load(dst + p * C::L_PANEL, &map_l, k0, row, z);
                         const uint32_t rd = dst + PLANES * C::L_PANEL + p * C::R_PANEL;
                         if (C::RMN) {
 #pragma unroll
-                            for (int q = 0; q < BN / CG / 64; ++q) load(rd + q * 8192, &map_r, col + q * 64, kb * C::KE, z);
+                            for (int q = 0; q < BN / CG / 64; ++q) load(rd + q * 8192, &map_r, col + q * 64, k0, z);
+                        } else if (C::RSYM) {
+                            load_sym(rd, &map_r, col, BN / CG, z);
                         } else {
-                            load(rd, &map_r, kb * C::KE, col, z);
+                            load(rd, &map_r, k0, col, z);
                         }
                     }
                     if (++s == S) { s = 0; ph ^= 1u; }
@@ -225,46 +278,73 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ C
         if (rank == 0) {
             const bool elected = elect_one_sync();
             int s = 0; uint32_t ph = 0;
-            int acc = 0; uint32_t acc_ph = 0;
+            int acc = 0; uint32_t acc_ph = 0, cross_ph = 0;
             bool alive = true;
-            const uint64_t l_desc = make_smem_desc(base);
-            const uint64_t r_desc = C::RMN ? mn_desc(base + PLANES * C::L_PANEL) : make_smem_desc(base + PLANES * C::L_PANEL);
+            // descriptors of the first stage; only low words move.  K-major: a step of 16 (32) columns is 32 bytes; MN-major: 16
+            // rows of 128 bytes, and the next 64 columns a box further (bits 16-29)
+            const uint64_t l_desc = make_smem_desc(base), r_desc = make_smem_desc(base + PLANES * C::L_PANEL);
             const uint32_t l_hi = (uint32_t)(l_desc >> 32), r_hi = (uint32_t)(r_desc >> 32);
             constexpr uint32_t L_TAIL = C::L_PANEL >> 4, R_TAIL = C::R_PANEL >> 4;
-            constexpr uint32_t R_STEP = C::RMN ? 2048 >> 4 : 32 >> 4;      // 16 rows of K, or 32 bytes of a row
-            uint32_t cross = tmem + 2 * BN;
-            for (int64_t t = unit; t < g.total && alive; t += units, cross ^= BN)
-                for (int kb0 = 0; kb0 < g.nkb && alive; kb0 += C::KCHUNK) {
-                    const int kb1 = g.nkb - kb0 < C::KCHUNK ? g.nkb : kb0 + C::KCHUNK;
-                    if (!__all_sync(0xffffffffu, mbar_wait(acc_empty(acc), acc_ph ^ 1u, abort_flag, status, ST_MMA_ACC))) { alive = false; break; }
-                    tc_fence_after();
-                    const uint32_t d = tmem + (uint32_t)(acc * BN);
-                    for (int kb = kb0; kb < kb1; ++kb) {
-                        if (!__all_sync(0xffffffffu, mbar_wait(full(s), ph, abort_flag, status, ST_MMA))) { alive = false; break; }
-                        tc_fence_after();
-                        const uint32_t off = (uint32_t)((s * C::STAGE) >> 4);
-                        const uint32_t l_lo = (uint32_t)l_desc + off, r_lo = (uint32_t)r_desc + off;
-                        const uint32_t later = (uint32_t)(kb != kb0);
+            constexpr uint32_t KSTEP = 32 >> 4, MNSTEP = 2048 >> 4, MNBOX = (8192u >> 4) << 16, LBO = 0x3fffu << 16;
+            const uint32_t l_k = (uint32_t)l_desc, l_mn = ((uint32_t)l_desc & ~LBO) | MNBOX;
+            const uint32_t r_k = (uint32_t)r_desc, r_mn = ((uint32_t)r_desc & ~LBO) | MNBOX;
+            auto wait_all = [&](uint32_t bar, uint32_t parity, int code) {
+                if (!__all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, code))) alive = false;
+                tc_fence_after();
+                return alive;
+            };
+            auto commit = [&](uint32_t bar) {
+                if (elected) { if (CG == 2) umma2_commit_both(bar); else umma_commit(bar); }
+                __syncwarp();
+            };
+            for (int64_t t = unit; t < g.total && alive; t += units) {
+                int b, m0 = 0, n0 = 0;
+                if (C::LSYM || C::RSYM) decode<C::BM, BN>(g, t, b, m0, n0);
+                if (C::PP == 1 && !wait_all(acc_empty(acc), acc_ph ^ 1u, ST_MMA_ACC)) break;
+                const uint32_t d = C::PP == 1 ? tmem + (uint32_t)(acc * BN) : tmem, cross = tmem + BN;
+                for (int kb = 0; kb < g.nkb; ++kb) {
+                    if (C::PP == 3 && !wait_all(acc_empty(0), acc_ph ^ 1u, ST_MMA_ACC)) break;
+                    if (!wait_all(full(s), ph, ST_MMA)) break;
+                    const uint32_t off = (uint32_t)((s * C::STAGE) >> 4);
+                    const bool lmn = C::LSYM && !stored(m0, kb * C::KE);
+                    const bool rmn = C::RMN || (C::RSYM && !stored(n0, kb * C::KE));
+                    const uint32_t l_lo = (lmn ? l_mn : l_k) + off, r_lo = (rmn ? r_mn : r_k) + off;
+                    const uint32_t l_step = lmn ? MNSTEP : KSTEP, r_step = rmn ? MNSTEP : KSTEP;
+                    const uint32_t idesc = C::IDESC | (lmn ? 1u << 15 : 0u) | (rmn ? 1u << 16 : 0u);
+                    if (elected) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            mma<C::KIND, CG>(d, desc_from_words(l_lo + l_step * k, l_hi), desc_from_words(r_lo + r_step * k, r_hi), idesc,
+                                             k ? 1u : (uint32_t)(C::PP == 1 && kb != 0));
+                    }
+                    if (C::PP == 3) {
+                        commit(acc_full(0));                       // drained while the cross products run
+                        acc_ph ^= 1u;
+                        if (kb == 0) {
+                            if (!wait_all(acc_empty(1), cross_ph ^ 1u, ST_MMA_ACC)) break;
+                            cross_ph ^= 1u;
+                        }
                         if (elected) {
 #pragma unroll
                             for (int k = 0; k < 4; ++k) {
-                                const uint32_t la = l_lo + 2u * k, ra = r_lo + R_STEP * k;
-                                mma<C::KIND, CG>(d, desc_from_words(la, l_hi), desc_from_words(ra, r_hi), C::IDESC, k ? 1u : later);
-                                if constexpr (C::PP == 3) {
-                                    mma<C::KIND, CG>(cross, desc_from_words(la, l_hi), desc_from_words(ra + R_TAIL, r_hi), C::IDESC, k ? 1u : (uint32_t)(kb != 0));
-                                    mma<C::KIND, CG>(cross, desc_from_words(la + L_TAIL, l_hi), desc_from_words(ra, r_hi), C::IDESC, 1u);
-                                }
+                                const uint32_t la = l_lo + l_step * k, ra = r_lo + r_step * k;
+                                mma<C::KIND, CG>(cross, desc_from_words(la, l_hi), desc_from_words(ra + R_TAIL, r_hi), idesc, k ? 1u : (uint32_t)(kb != 0));
+                                mma<C::KIND, CG>(cross, desc_from_words(la + L_TAIL, l_hi), desc_from_words(ra, r_hi), idesc, 1u);
                             }
-                            if (CG == 2) umma2_commit_both(empty(s)); else umma_commit(empty(s));
                         }
-                        __syncwarp();
-                        if (++s == S) { s = 0; ph ^= 1u; }
                     }
-                    if (alive && elected) { if (CG == 2) umma2_commit_both(acc_full(acc)); else umma_commit(acc_full(acc)); }
-                    __syncwarp();
+                    commit(empty(s));
+                    if (++s == S) { s = 0; ph ^= 1u; }
+                }
+                if (!alive) break;
+                if (C::PP == 3) {
+                    commit(acc_full(1));
+                } else {
+                    commit(acc_full(acc));
                     acc ^= 1;
                     if (acc == 0) acc_ph ^= 1u;
                 }
+            }
             if (!alive && elected) {
                 // wait (bounded) until the MMAs already issued have retired
                 if (CG == 2) umma2_commit(drain); else umma_commit(drain);
@@ -277,63 +357,57 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ C
         const int q = warp & 3;               // quarter of the tensor memory's lanes that this warp may read
         constexpr int EB = BN / 2;            // columns of its half
         const int half0 = (warp - 2) / 4 * EB;
-        int acc = 0; uint32_t acc_ph = 0, cross_at = 2 * BN;
+        const uint32_t buf = base + C::OUT_OFFSET + (uint32_t)((warp - 2) * 4096);
+        int acc = 0; uint32_t acc_ph = 0, cross_ph = 0;
         bool alive = true;
+        auto wait_all = [&](uint32_t bar, uint32_t parity) {
+            if (!__all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, ST_EPILOGUE))) alive = false;
+            tc_fence_after();
+            return alive;
+        };
         auto release = [&](int a) {
             tc_fence_before();
             if (CG == 2 && rank != 0) mbar_arrive_cluster(mapa_cluster(acc_empty(a), 0));
             else mbar_arrive(acc_empty(a));
         };
+        const uint32_t lanes = (uint32_t)(q * 32) << 16;
         for (int64_t t = unit; t < g.total && alive; t += units) {
             int b, m0, n0;
             decode<C::BM, BN>(g, t, b, m0, n0);
             n0 += half0;
-            const int row = m0 + (int)rank * 128 + q * 32 + lane;
-            // symmetric results: the warp's 32 x 32 block also goes to its transposed place where no tile computes that
-            auto mirrored = [&](int col0) {
-                return g.sym && (row / BN + 1) * BN <= col0 / C::BM * C::BM;
-            };
+            const int row0 = m0 + (int)rank * 128 + q * 32;
             int ncols = g.N - n0;
             if (ncols > EB) ncols = EB;
-            const int nch = ncols > 0 ? (ncols + 31) >> 5 : 0;
+            const int nch = ncols > 0 && row0 < g.M ? (ncols + 31) >> 5 : 0;
+            typename Epi::Fetched fa, fb;
             if constexpr (C::PP == 3) {
-                typename Epi::template Fetched<32> f[EB / 32];      // on their way while the MMAs run
-#pragma unroll
-                for (int c = 0; c < EB / 32; ++c) Epi::template fetch<32>(args, g, b, row, n0 + c * 32, f[c]);
                 float v[EB];
-                for (int kb0 = 0; kb0 < g.nkb; kb0 += C::KCHUNK) {
-                    const bool ok = mbar_wait(acc_full(acc), acc_ph, abort_flag, status, ST_EPILOGUE);
-                    if (!__all_sync(0xffffffffu, ok)) { alive = false; break; }
-                    tc_fence_after();
-                    const uint32_t ta = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)half0;
-                    if (kb0 == 0) add_columns<EB, true>(ta + (uint32_t)(acc * BN), v);
-                    else add_columns<EB, false>(ta + (uint32_t)(acc * BN), v);
-                    // Before the tile's last buffer is given back the cross products are read: the buffer they will be
-                    // summed in next, two tiles on, is started only after two more buffers were given back.
-                    if (kb0 + C::KCHUNK >= g.nkb) {
-                        add_columns<EB, false>(ta + cross_at, v);
-                        cross_at ^= BN;
-                    }
-                    release(acc);
-                    acc ^= 1;
-                    if (acc == 0) acc_ph ^= 1u;
+                for (int kb = 0; kb < g.nkb; ++kb) {
+                    if (!wait_all(acc_full(0), acc_ph)) break;
+                    acc_ph ^= 1u;
+                    if (kb == 0) add_columns<EB, true>(tmem + lanes + (uint32_t)half0, v);
+                    else add_columns<EB, false>(tmem + lanes + (uint32_t)half0, v);
+                    release(0);
                 }
                 if (!alive) break;
+                Epi::fetch(args, g, b, row0 + lane, n0, fa);
+                if (!wait_all(acc_full(1), cross_ph)) break;
+                cross_ph ^= 1u;
+                add_columns<EB, false>(tmem + lanes + (uint32_t)(BN + half0), v);
+                release(1);
 #pragma unroll
                 for (int c = 0; c < EB / 32; ++c)
                     if (c < nch) {
                         uint32_t r[32];
 #pragma unroll
                         for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(v[c * 32 + e]);
-                        Epi::template emit<32>(args, g, b, row, n0 + c * 32, r, mirrored(n0 + c * 32), f[c]);
+                        if (c + 1 < EB / 32) Epi::fetch(args, g, b, row0 + lane, n0 + (c + 1) * 32, c & 1 ? fa : fb);
+                        Epi::emit(args, g, b, row0, n0 + c * 32, r, c & 1 ? fb : fa, buf);
                     }
             } else {
-                typename Epi::template Fetched<32> fa, fb;
-                Epi::template fetch<32>(args, g, b, row, n0, fa);
-                const bool ok = mbar_wait(acc_full(acc), acc_ph, abort_flag, status, ST_EPILOGUE);
-                if (!__all_sync(0xffffffffu, ok)) { alive = false; break; }
-                tc_fence_after();
-                const uint32_t ta = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN + half0);
+                Epi::fetch(args, g, b, row0 + lane, n0, fa);
+                if (!wait_all(acc_full(acc), acc_ph)) break;
+                const uint32_t ta = tmem + lanes + (uint32_t)(acc * BN + half0);
                 // two register buffers: the load of the next 32 columns is in flight while these are written
                 uint32_t ra[32], rb[32];
                 if (nch > 0) tmem_ld32(ta, ra);
@@ -343,26 +417,27 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ C
                     tmem_ld_wait();
                     if (c + 1 < nch) {
                         tmem_ld32(ta + (c + 1) * 32, rb);
-                        Epi::template fetch<32>(args, g, b, row, n0 + (c + 1) * 32, fb);
+                        Epi::fetch(args, g, b, row0 + lane, n0 + (c + 1) * 32, fb);
                     } else {
                         release(acc);
                     }
-                    Epi::template emit<32>(args, g, b, row, n0 + c * 32, ra, mirrored(n0 + c * 32), fa);
+                    Epi::emit(args, g, b, row0, n0 + c * 32, ra, fa, buf);
                     if (c + 1 < nch) {
                         tmem_ld_wait();
                         if (c + 2 < nch) {
                             tmem_ld32(ta + (c + 2) * 32, ra);
-                            Epi::template fetch<32>(args, g, b, row, n0 + (c + 2) * 32, fa);
+                            Epi::fetch(args, g, b, row0 + lane, n0 + (c + 2) * 32, fa);
                         } else {
                             release(acc);
                         }
-                        Epi::template emit<32>(args, g, b, row, n0 + (c + 1) * 32, rb, mirrored(n0 + (c + 1) * 32), fb);
+                        Epi::emit(args, g, b, row0, n0 + (c + 1) * 32, rb, fb, buf);
                     }
                 }
                 acc ^= 1;
                 if (acc == 0) acc_ph ^= 1u;
             }
         }
+        if (Epi::BULK && lane == 0) bulk_wait_all();
     }
 
     tc_fence_before();
@@ -379,7 +454,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ C
 }
 
 // ---- few tiles: the K range of a tile split over the CTAs of a cluster ------------------------------------------------
-// One tile of 128 x BN per cluster of SPLIT CTAs (SPLIT a run-time power of two up to 8).  Every CTA sums its share of the
+// Integer products.  One tile of 128 x BN per cluster of SPLIT CTAs (SPLIT a run-time power of two up to 8).  Every CTA sums its share of the
 // K blocks in tensor memory, leaves the partial tile in its shared memory, and after a cluster barrier adds up 128 / SPLIT
 // rows of all partials through distributed shared memory, in rank order, and writes them: one launch, no scratch, no
 // atomics, the same result every time.
@@ -391,26 +466,24 @@ struct SplitSmem {
     static constexpr int PITCH = (C::BN + 4) * 4;                   // bytes of a partial row: 16-byte stores of 8 rows meet no bank twice
     static constexpr int PARTIAL = 128 * PITCH;
     static constexpr int RING = C::STAGES * C::STAGE > PARTIAL ? C::STAGES * C::STAGE : PARTIAL;
-    static constexpr int BARS = 2 * C::STAGES + 5;
+    static constexpr int BARS = 2 * C::STAGES + 2;
     static constexpr int TOTAL = RING + BARS * 8 + 16 + 1024;
 };
 
 template <class C, class Epi>
 __global__ void __launch_bounds__(THREADS, 1)
 split_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ CUtensorMap map_r, const Tiles g,
-             const typename Epi::Args args, int split, int32_t* status) {
-    static_assert(C::CG == 1, "one CTA per accumulator");
+             const __grid_constant__ typename Epi::Args args, int split, int32_t* status) {
+    static_assert(C::KIND == I8 && C::CG == 1, "integer sums, one CTA per accumulator");
     using L = SplitSmem<C>;
-    constexpr int BN = C::BN, S = C::STAGES, PLANES = C::PLANES;
+    constexpr int BN = C::BN, S = C::STAGES;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
     const uint32_t bars = base + L::RING;
     auto full = [&](int s) { return bars + 8u * s; };
     auto empty = [&](int s) { return bars + 8u * (S + s); };
-    auto acc_full = [&](int a) { return bars + 8u * (2 * S + a); };
-    auto acc_empty = [&](int a) { return bars + 8u * (2 * S + 2 + a); };
-    const uint32_t drain = bars + 8u * (2 * S + 4);
+    const uint32_t done = bars + 8u * (2 * S), drain = done + 8u;
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + L::RING + L::BARS * 8);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + L::RING + L::BARS * 8 + 4);
 
@@ -418,7 +491,7 @@ split_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ 
     const int rank = (int)cluster_ctarank();
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
-        for (int a = 0; a < 2; ++a) { mbar_init(acc_full(a), 1); mbar_init(acc_empty(a), EPI_THREADS); }
+        mbar_init(done, 1);
         mbar_init(drain, 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -446,18 +519,8 @@ split_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ 
                 if (!mbar_wait(empty(s), ph ^ 1u, abort_flag, status, ST_LOAD)) { alive = false; break; }
                 const uint32_t dst = base + s * C::STAGE;
                 mbar_arrive_expect_tx(full(s), (uint32_t)C::STAGE);
-#pragma unroll
-                for (int p = 0; p < PLANES; ++p) {
-                    const int z = b * PLANES + p;
-                    load_3d(dst + p * C::L_PANEL, &map_l, kb * C::KE, m0, z, full(s));
-                    const uint32_t rd = dst + PLANES * C::L_PANEL + p * C::R_PANEL;
-                    if (C::RMN) {
-#pragma unroll
-                        for (int q = 0; q < BN / 64; ++q) load_3d(rd + q * 8192, &map_r, n0 + q * 64, kb * C::KE, z, full(s));
-                    } else {
-                        load_3d(rd, &map_r, kb * C::KE, n0, z, full(s));
-                    }
-                }
+                load_3d(dst, &map_l, kb * C::KE, m0, 0, full(s));
+                load_3d(dst + C::L_PANEL, &map_r, kb * C::KE, n0, 0, full(s));
                 if (++s == S) { s = 0; ph ^= 1u; }
             }
             if (!alive) {
@@ -468,44 +531,25 @@ split_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ 
     } else if (warp == 1) {
         const bool elected = elect_one_sync();
         int s = 0; uint32_t ph = 0;
-        int acc = 0; uint32_t acc_ph = 0;
         bool alive = true;
-        const uint64_t l_desc = make_smem_desc(base);
-        const uint64_t r_desc = C::RMN ? mn_desc(base + PLANES * C::L_PANEL) : make_smem_desc(base + PLANES * C::L_PANEL);
+        const uint64_t l_desc = make_smem_desc(base), r_desc = make_smem_desc(base + C::L_PANEL);
         const uint32_t l_hi = (uint32_t)(l_desc >> 32), r_hi = (uint32_t)(r_desc >> 32);
-        constexpr uint32_t L_TAIL = C::L_PANEL >> 4, R_TAIL = C::R_PANEL >> 4;
-        constexpr uint32_t R_STEP = C::RMN ? 2048 >> 4 : 32 >> 4;
-        for (int kb0 = k_first; kb0 < k_last && alive; kb0 += C::KCHUNK) {
-            const int kb1 = k_last - kb0 < C::KCHUNK ? k_last : kb0 + C::KCHUNK;
-            if (!__all_sync(0xffffffffu, mbar_wait(acc_empty(acc), acc_ph ^ 1u, abort_flag, status, ST_MMA_ACC))) { alive = false; break; }
+        for (int kb = k_first; kb < k_last; ++kb) {
+            if (!__all_sync(0xffffffffu, mbar_wait(full(s), ph, abort_flag, status, ST_MMA))) { alive = false; break; }
             tc_fence_after();
-            const uint32_t d = tmem + (uint32_t)(acc * BN);
-            for (int kb = kb0; kb < kb1; ++kb) {
-                if (!__all_sync(0xffffffffu, mbar_wait(full(s), ph, abort_flag, status, ST_MMA))) { alive = false; break; }
-                tc_fence_after();
-                const uint32_t off = (uint32_t)((s * C::STAGE) >> 4);
-                const uint32_t l_lo = (uint32_t)l_desc + off, r_lo = (uint32_t)r_desc + off;
-                const uint32_t later = (uint32_t)(kb != kb0);
-                if (elected) {
+            const uint32_t off = (uint32_t)((s * C::STAGE) >> 4);
+            if (elected) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const uint32_t la = l_lo + 2u * k, ra = r_lo + R_STEP * k;
-                        mma<C::KIND, 1>(d, desc_from_words(la, l_hi), desc_from_words(ra, r_hi), C::IDESC, k ? 1u : later);
-                        if constexpr (C::PP == 3) {
-                            mma<C::KIND, 1>(tmem + 2 * BN, desc_from_words(la, l_hi), desc_from_words(ra + R_TAIL, r_hi), C::IDESC, k ? 1u : (uint32_t)(kb != k_first));
-                            mma<C::KIND, 1>(tmem + 2 * BN, desc_from_words(la + L_TAIL, l_hi), desc_from_words(ra, r_hi), C::IDESC, 1u);
-                        }
-                    }
-                    umma_commit(empty(s));
-                }
-                __syncwarp();
-                if (++s == S) { s = 0; ph ^= 1u; }
+                for (int k = 0; k < 4; ++k)
+                    mma<C::KIND, 1>(tmem, desc_from_words((uint32_t)l_desc + off + 2u * k, l_hi), desc_from_words((uint32_t)r_desc + off + 2u * k, r_hi),
+                                    C::IDESC, k ? 1u : (uint32_t)(kb != k_first));
+                umma_commit(empty(s));
             }
-            if (alive && elected) umma_commit(acc_full(acc));
             __syncwarp();
-            acc ^= 1;
-            if (acc == 0) acc_ph ^= 1u;
+            if (++s == S) { s = 0; ph ^= 1u; }
         }
+        if (alive && elected) umma_commit(done);
+        __syncwarp();
         if (!alive && elected) {
             umma_commit(drain);
             const uint64_t t0 = globaltimer_ns();
@@ -514,31 +558,20 @@ split_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ 
         __syncwarp();
     } else {
         const int q = warp & 3;
-        int acc = 0; uint32_t acc_ph = 0;
-        bool alive = true;
         constexpr int EB = BN / 2;
         const int half0 = (warp - 2) / 4 * EB;
-        float v[EB];
-        for (int kb0 = k_first; kb0 < k_last; kb0 += C::KCHUNK) {
-            const bool ok = mbar_wait(acc_full(acc), acc_ph, abort_flag, status, ST_EPILOGUE);
-            if (!__all_sync(0xffffffffu, ok)) { alive = false; break; }
+        if (__all_sync(0xffffffffu, mbar_wait(done, 0, abort_flag, status, ST_EPILOGUE))) {
             tc_fence_after();
-            const uint32_t ta = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)half0;
-            if (kb0 == k_first) add_columns<EB, true>(ta + (uint32_t)(acc * BN), v);      // integers: bits, never added here
-            else add_columns<EB, false>(ta + (uint32_t)(acc * BN), v);
-            if (C::PP == 3 && kb0 + C::KCHUNK >= k_last) add_columns<EB, false>(ta + 2 * BN, v);
-            tc_fence_before();
-            mbar_arrive(acc_empty(acc));
-            acc ^= 1;
-            if (acc == 0) acc_ph ^= 1u;
-        }
-        if (alive) {
-            // the last accumulator is complete, so every MMA has read its stages and the ring is free for the partial tile
+            // the accumulator is complete, so every MMA has read its stages and the ring is free for the partial tile
             const uint32_t dst = base + (uint32_t)((q * 32 + lane) * L::PITCH + half0 * 4);
 #pragma unroll
-            for (int e = 0; e < EB; e += 4)
-                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + e * 4), "r"(__float_as_uint(v[e])), "r"(__float_as_uint(v[e + 1])),
-                             "r"(__float_as_uint(v[e + 2])), "r"(__float_as_uint(v[e + 3])) : "memory");
+            for (int c = 0; c < EB / 32; ++c) {
+                uint32_t v[32];
+                tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(half0 + c * 32), v);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 32; e += 4) st_shared_v4(dst + (c * 32 + e) * 4, v[e], v[e + 1], v[e + 2], v[e + 3]);
+            }
         }
     }
     tc_fence_before();
@@ -559,19 +592,11 @@ split_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ 
                 ld_cluster_v4(from + 16, r1);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    if constexpr (C::KIND == I8) {
-                        sum[e] = k ? sum[e] + r0[e] : r0[e];
-                        sum[4 + e] = k ? sum[4 + e] + r1[e] : r1[e];
-                    } else {
-                        sum[e] = k ? __float_as_uint(__uint_as_float(sum[e]) + __uint_as_float(r0[e])) : r0[e];
-                        sum[4 + e] = k ? __float_as_uint(__uint_as_float(sum[4 + e]) + __uint_as_float(r1[e])) : r1[e];
-                    }
+                    sum[e] = k ? sum[e] + r0[e] : r0[e];
+                    sum[4 + e] = k ? sum[4 + e] + r1[e] : r1[e];
                 }
             }
-            const int row = m0 + lrow;
-            typename Epi::template Fetched<8> f;
-            Epi::template fetch<8>(args, g, b, row, n0 + col, f);
-            Epi::template emit<8>(args, g, b, row, n0 + col, sum, g.sym && (row / BN + 1) * BN <= (n0 + col) / C::BM * C::BM, f);
+            Epi::emit8(args, g, m0 + lrow, n0 + col, sum);
         }
     }
     __syncthreads();
@@ -612,9 +637,9 @@ int launch_split(const CUtensorMap& map_l, const CUtensorMap& map_r, const Tiles
 }
 
 // map of `slabs` row-major matrices [rows][cols], rows pitch_bytes and matrices slab_bytes apart, read in boxes of
-// box_cols x box_rows with 128-byte swizzle; what lies outside a matrix reads as zero
+// box_cols x box_rows (stores: written, clipped to the matrix); what lies outside a matrix reads as zero
 inline int make_map(CUtensorMap* map, Kind kind, const void* base, int64_t cols, int64_t rows, int64_t slabs, int64_t pitch_bytes,
-                    int64_t slab_bytes, int box_cols, int box_rows) {
+                    int64_t slab_bytes, int box_cols, int box_rows, CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
     EncodeTiledFn encode = get_encode_fn();
     if (!encode) return CHEBYKAN_ECUDA;
     const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)slabs};
@@ -623,7 +648,7 @@ inline int make_map(CUtensorMap* map, Kind kind, const void* base, int64_t cols,
     const cuuint32_t one[3] = {1, 1, 1};
     const CUresult r = encode(map, kind == I8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
                               const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                              swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) { set_last_cuda_error((int)r); return CHEBYKAN_ECUDA; }
     return CHEBYKAN_OK;
 }

@@ -22,52 +22,56 @@ struct EpiArgs {
 template <typename OUT>
 struct Epilogue {
     using Args = EpiArgs;
-    struct Nothing {};
-    template <int NC> using Fetched = Nothing;
+    static constexpr bool BULK = false;
+    struct Fetched {};
+    static __device__ __forceinline__ void fetch(const Args&, const Tiles&, int, int, int, Fetched&) {}
+
+    // the scales and biases of NC columns: every load first; one after the other, each waited for, they would take longer than
+    // the tile's MMAs
     template <int NC>
-    static __device__ __forceinline__ void fetch(const Args&, const Tiles&, int, int, int, Nothing&) {}
-    template <int NC>
-    static __device__ __forceinline__ void emit(const Args& p, const Tiles& g, int, int row, int col0, uint32_t (&r)[NC], bool,
-                                                const Nothing&) {
-        if (row >= g.M) return;
-        const float qs = __ldg(p.q_scale + row);
-        OUT* dst = reinterpret_cast<OUT*>(p.y) + (int64_t)row * g.N + col0;
-        constexpr int V = 16 / (int)sizeof(OUT);          // values of a 16-byte store
+    static __device__ __forceinline__ void columns(const Args& p, const Tiles& g, int col0, float (&ws)[NC], float (&bs)[NC]) {
         if (col0 + NC <= g.N && p.vec) {
-            // every load of the columns' scales first: one after the other, each waited for, they would take longer than
-            // the tile's MMAs
-            float4 ws[NC / 4], bs[NC / 4];
 #pragma unroll
-            for (int c = 0; c < NC / 4; ++c) ws[c] = __ldg(reinterpret_cast<const float4*>(p.w_scale + col0) + c);
+            for (int c = 0; c < NC; c += 4) *reinterpret_cast<float4*>(ws + c) = __ldg(reinterpret_cast<const float4*>(p.w_scale + col0 + c));
 #pragma unroll
-            for (int c = 0; c < NC / 4; ++c)
-                bs[c] = p.bias ? __ldg(reinterpret_cast<const float4*>(p.bias + col0) + c) : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int c = 0; c < NC; c += V) {
-                alignas(16) OUT out[V];
-#pragma unroll
-                for (int e = 0; e < V; e += 4) {
-                    const int k = c + e;
-                    const float4 w = ws[k / 4], b = bs[k / 4];
-                    out[e] = to_type<OUT>(fmaf((float)(int)r[k] * qs, w.x, b.x));
-                    out[e + 1] = to_type<OUT>(fmaf((float)(int)r[k + 1] * qs, w.y, b.y));
-                    out[e + 2] = to_type<OUT>(fmaf((float)(int)r[k + 2] * qs, w.z, b.z));
-                    out[e + 3] = to_type<OUT>(fmaf((float)(int)r[k + 3] * qs, w.w, b.w));
-                }
-                *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(out);
-            }
+            for (int c = 0; c < NC; c += 4)
+                *reinterpret_cast<float4*>(bs + c) = p.bias ? __ldg(reinterpret_cast<const float4*>(p.bias + col0 + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
         } else {
-            // ragged right edge, or rows of y that are not 16 bytes apart
-            float ws[NC], bs[NC];
 #pragma unroll
             for (int e = 0; e < NC; ++e) {
                 const int col = col0 + e < g.N ? col0 + e : g.N - 1;
                 ws[e] = __ldg(p.w_scale + col);
                 bs[e] = p.bias ? __ldg(p.bias + col) : 0.f;
             }
+        }
+    }
+    static __device__ __forceinline__ void emit(const Args& p, const Tiles& g, int, int row0, int col0, uint32_t (&r)[32], const Fetched&, uint32_t buf) {
+        const int row = row0 + (threadIdx.x & 31);
+        alignas(16) float ws[32], bs[32];
+        columns(p, g, col0, ws, bs);
+        const float qs = row < g.M ? __ldg(p.q_scale + row) : 0.f;
+        alignas(16) OUT out[32];
 #pragma unroll
-            for (int e = 0; e < NC; ++e)
-                if (col0 + e < g.N) dst[e] = to_type<OUT>(fmaf((float)(int)r[e] * qs, ws[e], bs[e]));
+        for (int e = 0; e < 32; ++e) out[e] = to_type<OUT>(fmaf((float)(int)r[e] * qs, ws[e], bs[e]));
+        gemm::store_rows(buf, out, reinterpret_cast<OUT*>(p.y) + (int64_t)row0 * g.N + col0, g.N, g.M - row0, g.N - col0, p.vec);
+    }
+    // 8 columns of one row, from the kernel that splits K
+    static __device__ __forceinline__ void emit8(const Args& p, const Tiles& g, int row, int col0, const uint32_t (&r)[8]) {
+        alignas(16) float ws[8], bs[8];
+        columns(p, g, col0, ws, bs);
+        const float qs = __ldg(p.q_scale + row);
+        OUT* dst = reinterpret_cast<OUT*>(p.y) + (int64_t)row * g.N + col0;
+        alignas(16) OUT out[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) out[e] = to_type<OUT>(fmaf((float)(int)r[e] * qs, ws[e], bs[e]));
+        if (p.vec && col0 + 8 <= g.N) {
+#pragma unroll
+            for (int c = 0; c < 8; c += 16 / (int)sizeof(OUT))
+                *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(out + c);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (col0 + e < g.N) dst[e] = out[e];
         }
     }
 };

@@ -2,7 +2,8 @@
 //   A = X X^T            both operands are X's rows; symmetric
 //   P = a I + b A + c A A      both operands are A's rows (A is symmetric); symmetric
 //   X' = P X             P's rows against X as it lies, [K][N]: no transposed copy of X exists
-// The symmetric two compute the tiles on and above the diagonal and write each block to both places.
+// Of the symmetric two only the 256 x 256 blocks on and above the diagonal are computed and stored; the products that read
+// them take a block below the diagonal from its mirror image.
 #include <type_traits>
 #include "gemm_tc.cuh"
 #include "newton_schulz.cuh"
@@ -14,38 +15,31 @@ using gemm::Tiles;
 
 enum { GRAM = 0, POLY = 1, APPLY = 2, LAST = 3 };       // LAST: the final APPLY, to the caller's layout and type
 
-struct EpiArgs {
+struct alignas(64) EpiArgs {
+    CUtensorMap map;          // planes of the result: boxes of 32 x 32
     const __half* a;          // POLY: A's planes
-    __half* out;              // planes
     void* o;                  // LAST: [batch][m][n]
     int tall;                 // LAST: o is the transposed result
     const float *alpha, *alpha_next;
-    int pitch;                // of out (and of a)
+    int pitch;                // of a
     int64_t slab;
     float ca, cb, cc;
 };
 
-// 8 columns of A's row, fetched ahead of the accumulator's
-template <int NC, int PLANES>
-struct Ahead {
-    uint4 hi[NC / 8], lo[PLANES == 2 ? NC / 8 : 1];
-};
-struct Nothing {};
-
 template <int KIND, int PLANES, typename OUT = float>
 struct Epilogue {
     using Args = EpiArgs;
-    template <int NC>
-    using Fetched = typename std::conditional<KIND == POLY, Ahead<NC, PLANES>, Nothing>::type;
+    static constexpr bool BULK = KIND != LAST;
+    struct Ahead { uint4 hi[4], lo[PLANES == 2 ? 4 : 1]; };       // 32 columns of A's row
+    struct Nothing {};
+    using Fetched = typename std::conditional<KIND == POLY, Ahead, Nothing>::type;
 
-    // what emit() reads from memory, for the caller to ask for early
-    template <int NC>
-    static __device__ __forceinline__ void fetch(const Args& p, const Tiles& g, int b, int row, int col0, Fetched<NC>& f) {
+    static __device__ __forceinline__ void fetch(const Args& p, const Tiles& g, int b, int row, int col0, Fetched& f) {
         if constexpr (KIND == POLY) {
             if (row >= g.M) return;
             const __half* a = p.a + (int64_t)b * PLANES * p.slab + (int64_t)row * p.pitch + col0;
 #pragma unroll
-            for (int c = 0; c < NC / 8; ++c)
+            for (int c = 0; c < 4; ++c)
                 if (col0 + c * 8 < g.N) {
                     f.hi[c] = *reinterpret_cast<const uint4*>(a + c * 8);
                     if (PLANES == 2) f.lo[c] = *reinterpret_cast<const uint4*>(a + c * 8 + p.slab);
@@ -53,76 +47,62 @@ struct Epilogue {
         }
     }
 
-    // NC consecutive columns of one row
-    template <int NC>
-    static __device__ __forceinline__ void emit(const Args& p, const Tiles& g, int b, int row, int col0, uint32_t (&r)[NC], bool mirror,
-                                                const Fetched<NC>& f) {
+    // 32 columns from col0 of the rows from row0, one per lane; buf: the warp's 4 KB
+    static __device__ __forceinline__ void emit(const Args& p, const Tiles& g, int b, int row0, int col0, uint32_t (&r)[32], const Fetched& f,
+                                                uint32_t buf) {
+        const int lane = threadIdx.x & 31, row = row0 + lane;
         float factor;
         if (KIND == GRAM) { const float al = p.alpha[b]; factor = al * al * exp2f((float)A_EXP); }
         else if (KIND == POLY) factor = p.cc * exp2f(-2.f * A_EXP + P_EXP);
         else if (KIND == APPLY) factor = exp2f(-(float)P_EXP) * p.alpha[b] / p.alpha_next[b];
         else factor = exp2f(-(float)P_EXP) * p.alpha[b];
-        if (row >= g.M) return;
         if constexpr (KIND == LAST) {
             OUT* o = reinterpret_cast<OUT*>(p.o) + (int64_t)b * g.M * g.N;
             if (p.tall) {                       // the warp's lanes hold consecutive rows, which are o's columns
+                if (row < g.M)
 #pragma unroll
-                for (int e = 0; e < NC; ++e)
-                    if (col0 + e < g.N) o[(int64_t)(col0 + e) * g.M + row] = from_float<OUT>(__uint_as_float(r[e]) * factor);
+                    for (int e = 0; e < 32; ++e)
+                        if (col0 + e < g.N) o[(int64_t)(col0 + e) * g.M + row] = from_float<OUT>(__uint_as_float(r[e]) * factor);
                 return;
             }
-            OUT* dst = o + (int64_t)row * g.N + col0;
-            constexpr int V = 16 / (int)sizeof(OUT);
-            const bool vec = g.N % V == 0;
+            alignas(16) OUT v[32];
 #pragma unroll
-            for (int c = 0; c < NC; c += V) {
-                alignas(16) OUT v[V];
-#pragma unroll
-                for (int e = 0; e < V; ++e) v[e] = from_float<OUT>(__uint_as_float(r[c + e]) * factor);
-                if (vec) {
-                    if (col0 + c < g.N) *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(v);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < V; ++e)
-                        if (col0 + c + e < g.N) dst[c + e] = v[e];
-                }
-            }
-            return;
+            for (int e = 0; e < 32; ++e) v[e] = from_float<OUT>(__uint_as_float(r[e]) * factor);
+            gemm::store_rows(buf, v, o + (int64_t)row0 * g.N + col0, g.N, g.M - row0, g.N - col0, g.N % (16 / (int)sizeof(OUT)) == 0);
         } else {
-            const int64_t slab0 = (int64_t)b * PLANES * p.slab, at = slab0 + (int64_t)row * p.pitch + col0;
-            // eight columns (16 bytes of a plane) at a time; a row's last group may run into its padding, which nothing reads
+            // both planes of 32 x 32 into shared memory, 64-byte rows with the 16-byte chunks permuted as the map's swizzle has
+            // it (chunk ^ bits 1-2 of the row), and from there by TMA, which clips what lies outside the matrix
+            if (lane == 0) gemm::bulk_wait_read();
+            __syncwarp();
 #pragma unroll
-            for (int c = 0; c < NC; c += 8) {
-                if (col0 + c >= g.N) break;
+            for (int c = 0; c < 4; ++c) {
                 float v[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(r[c + e]) * factor;
+                for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(r[c * 8 + e]) * factor;
                 if constexpr (KIND == POLY) {
                     float a[8];
-                    const uint32_t ah[4] = {f.hi[c / 8].x, f.hi[c / 8].y, f.hi[c / 8].z, f.hi[c / 8].w};
+                    const uint32_t ah[4] = {f.hi[c].x, f.hi[c].y, f.hi[c].z, f.hi[c].w};
                     uint32_t al[4] = {};
-                    if (PLANES == 2) { al[0] = f.lo[c / 8].x; al[1] = f.lo[c / 8].y; al[2] = f.lo[c / 8].z; al[3] = f.lo[c / 8].w; }
+                    if (PLANES == 2) { al[0] = f.lo[c].x; al[1] = f.lo[c].y; al[2] = f.lo[c].z; al[3] = f.lo[c].w; }
                     join8<PLANES>(ah, al, a);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         v[e] = fmaf(p.cb * exp2f((float)(P_EXP - A_EXP)), a[e], v[e]);
-                        if (col0 + c + e == row) v[e] += p.ca * exp2f((float)P_EXP);
+                        if (col0 + c * 8 + e == row) v[e] += p.ca * exp2f((float)P_EXP);
                     }
                 }
                 uint32_t hi[4], lo[4];
                 split8<PLANES>(v, hi, lo);
-                *reinterpret_cast<uint4*>(p.out + at + c) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                if (PLANES == 2) *reinterpret_cast<uint4*>(p.out + at + c + p.slab) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                if (KIND != APPLY && mirror) {
-                    // the warp's lanes hold consecutive rows: 64 bytes of one row of the transposed block
-                    unsigned short* to = reinterpret_cast<unsigned short*>(p.out) + slab0 + (int64_t)(col0 + c) * p.pitch + row;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (col0 + c + e < g.N) {
-                            to[(int64_t)e * p.pitch] = (unsigned short)(hi[e >> 1] >> (16 * (e & 1)));
-                            if (PLANES == 2) to[(int64_t)e * p.pitch + p.slab] = (unsigned short)(lo[e >> 1] >> (16 * (e & 1)));
-                        }
-                }
+                const uint32_t at = buf + (uint32_t)(lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4));
+                gemm::st_shared_v4(at, hi[0], hi[1], hi[2], hi[3]);
+                if (PLANES == 2) gemm::st_shared_v4(at + 2048, lo[0], lo[1], lo[2], lo[3]);
+            }
+            gemm::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                gemm::store_3d(&p.map, buf, col0, row0, b * PLANES);
+                if (PLANES == 2) gemm::store_3d(&p.map, buf + 2048, col0, row0, b * PLANES + 1);
+                gemm::bulk_commit();
             }
         }
     }
@@ -135,54 +115,67 @@ struct Operands {
     int batch;
 };
 
+// pairs: tiles of 256 x 256; single CTAs: 128 x 128
+template <int KIND, int PP, int CG>
+using Shape2 = gemm::Config<gemm::F16, PP, CG, CG == 2 ? 256 : 128, KIND == APPLY || KIND == LAST, KIND != GRAM, KIND == POLY>;
+
 template <int KIND, int PP, int CG, typename OUT>
-int run(const Operands& o, const EpiArgs& args, int32_t* status, cudaStream_t s) {
-    constexpr bool MN = KIND == APPLY || KIND == LAST;
-    using C = gemm::Config<gemm::F16, PP, CG, PP == 3 ? 128 : 256, MN>;
+int run(const Operands& o, __half* out, int64_t out_pitch, int64_t out_slab, EpiArgs& args, int32_t* status, cudaStream_t s) {
+    using C = Shape2<KIND, PP, CG>;
     CUtensorMap ml, mr;
     const int64_t slabs = (int64_t)o.batch * C::PLANES;
-    int rc = gemm::make_map(&ml, gemm::F16, o.left, o.K, o.M, slabs, 2 * o.pitch_l, 2 * o.slab_l, C::KE, 128);
+    int rc = gemm::make_map(&ml, gemm::F16, o.left, o.K, o.M, slabs, 2 * o.pitch_l, 2 * o.slab_l, 64, C::LSYM ? 64 : 128);
     if (rc) return rc;
-    if (MN) rc = gemm::make_map(&mr, gemm::F16, o.right, o.N, o.K, slabs, 2 * o.pitch_r, 2 * o.slab_r, 64, 64);
-    else rc = gemm::make_map(&mr, gemm::F16, o.right, o.K, o.N, slabs, 2 * o.pitch_r, 2 * o.slab_r, C::KE, C::BN / CG);
+    if (C::RMN) rc = gemm::make_map(&mr, gemm::F16, o.right, o.N, o.K, slabs, 2 * o.pitch_r, 2 * o.slab_r, 64, 64);
+    else rc = gemm::make_map(&mr, gemm::F16, o.right, o.K, o.N, slabs, 2 * o.pitch_r, 2 * o.slab_r, 64, C::RSYM ? 64 : C::BN / CG);
     if (rc) return rc;
-    return gemm::launch<C, Epilogue<KIND, C::PLANES, OUT>>(ml, mr, gemm::tiles_of<C>(o.M, o.N, o.K, o.batch, !MN), args, status, s);
+    if (KIND != LAST) {
+        rc = gemm::make_map(&args.map, gemm::F16, out, o.N, o.M, slabs, 2 * out_pitch, 2 * out_slab, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
+        if (rc) return rc;
+    }
+    return gemm::launch<C, Epilogue<KIND, C::PLANES, OUT>>(ml, mr, gemm::tiles_of<C>(o.M, o.N, o.K, o.batch, KIND == GRAM || KIND == POLY), args,
+                                                          status, s);
 }
 
-// CTA pairs (tiles of 256 rows) where there are enough of them to occupy every SM; single CTAs otherwise
+// pairs where there are enough of their tiles to occupy every SM; single CTAs otherwise
 template <int KIND, int PP, typename OUT>
-int choose(const Operands& o, const EpiArgs& args, int32_t* status, cudaStream_t s) {
-    constexpr bool MN = KIND == APPLY || KIND == LAST;
-    using Pair = gemm::Config<gemm::F16, PP, 2, PP == 3 ? 128 : 256, MN>;
-    if (gemm::tiles_of<Pair>(o.M, o.N, o.K, o.batch, !MN).total >= 74) return run<KIND, PP, 2, OUT>(o, args, status, s);
-    return run<KIND, PP, 1, OUT>(o, args, status, s);
+int choose(const Operands& o, __half* out, int64_t out_pitch, int64_t out_slab, EpiArgs& args, int32_t* status, cudaStream_t s) {
+    if (gemm::tiles_of<Shape2<KIND, PP, 2>>(o.M, o.N, o.K, o.batch, KIND == GRAM || KIND == POLY).total >= 74)
+        return run<KIND, PP, 2, OUT>(o, out, out_pitch, out_slab, args, status, s);
+    return run<KIND, PP, 1, OUT>(o, out, out_pitch, out_slab, args, status, s);
 }
 template <int KIND, typename OUT = float>
-int product(const Shape& sh, const Operands& o, const EpiArgs& args, int32_t* status, cudaStream_t s) {
-    return sh.planes == 2 ? choose<KIND, 3, OUT>(o, args, status, s) : choose<KIND, 1, OUT>(o, args, status, s);
+int product(const Shape& sh, const Operands& o, __half* out, int64_t out_pitch, int64_t out_slab, EpiArgs& args, int32_t* status, cudaStream_t s) {
+    return sh.planes == 2 ? choose<KIND, 3, OUT>(o, out, out_pitch, out_slab, args, status, s)
+                          : choose<KIND, 1, OUT>(o, out, out_pitch, out_slab, args, status, s);
 }
 }  // namespace
 
 int launch_gram(const __half* x, __half* a, const float* alpha, const Shape& sh, int32_t* status, cudaStream_t s) {
-    const EpiArgs args{nullptr, a, nullptr, 0, alpha, nullptr, sh.ss, sh.a_slab(), 0, 0, 0};
-    return product<GRAM>(sh, {x, x, sh.s, sh.s, sh.l, sh.ls, sh.ls, sh.x_slab(), sh.x_slab(), sh.batch}, args, status, s);
+    EpiArgs args{};
+    args.alpha = alpha;
+    return product<GRAM>(sh, {x, x, sh.s, sh.s, sh.l, sh.ls, sh.ls, sh.x_slab(), sh.x_slab(), sh.batch}, a, sh.ss, sh.a_slab(), args, status, s);
 }
 int launch_poly(const __half* a, __half* q, float ca, float cb, float cc, const Shape& sh, int32_t* status, cudaStream_t s) {
-    const EpiArgs args{a, q, nullptr, 0, nullptr, nullptr, sh.ss, sh.a_slab(), ca, cb, cc};
-    return product<POLY>(sh, {a, a, sh.s, sh.s, sh.s, sh.ss, sh.ss, sh.a_slab(), sh.a_slab(), sh.batch}, args, status, s);
+    EpiArgs args{};
+    args.a = a; args.pitch = sh.ss; args.slab = sh.a_slab();
+    args.ca = ca; args.cb = cb; args.cc = cc;
+    return product<POLY>(sh, {a, a, sh.s, sh.s, sh.s, sh.ss, sh.ss, sh.a_slab(), sh.a_slab(), sh.batch}, q, sh.ss, sh.a_slab(), args, status, s);
 }
 int launch_apply(const __half* q, const __half* x, __half* x_next, const float* alpha, const float* alpha_next, const Shape& sh,
                  int32_t* status, cudaStream_t s) {
-    const EpiArgs args{nullptr, x_next, nullptr, 0, alpha, alpha_next, sh.ls, sh.x_slab(), 0, 0, 0};
-    return product<APPLY>(sh, {q, x, sh.s, sh.l, sh.s, sh.ss, sh.ls, sh.a_slab(), sh.x_slab(), sh.batch}, args, status, s);
+    EpiArgs args{};
+    args.alpha = alpha; args.alpha_next = alpha_next;
+    return product<APPLY>(sh, {q, x, sh.s, sh.l, sh.s, sh.ss, sh.ls, sh.a_slab(), sh.x_slab(), sh.batch}, x_next, sh.ls, sh.x_slab(), args, status, s);
 }
 int launch_apply_last(const __half* q, const __half* x, void* o, int dtype, bool tall, const float* alpha, const Shape& sh,
                       int32_t* status, cudaStream_t s) {
-    const EpiArgs args{nullptr, nullptr, o, tall, alpha, nullptr, sh.ls, sh.x_slab(), 0, 0, 0};
+    EpiArgs args{};
+    args.o = o; args.tall = tall; args.alpha = alpha;
     const Operands p{q, x, sh.s, sh.l, sh.s, sh.ss, sh.ls, sh.a_slab(), sh.x_slab(), sh.batch};
-    if (dtype == CHEBYKAN_DTYPE_FP32) return product<LAST, float>(sh, p, args, status, s);
-    if (dtype == CHEBYKAN_DTYPE_BF16) return product<LAST, __nv_bfloat16>(sh, p, args, status, s);
-    return product<LAST, __half>(sh, p, args, status, s);
+    if (dtype == CHEBYKAN_DTYPE_FP32) return product<LAST, float>(sh, p, nullptr, 0, 0, args, status, s);
+    if (dtype == CHEBYKAN_DTYPE_BF16) return product<LAST, __nv_bfloat16>(sh, p, nullptr, 0, 0, args, status, s);
+    return product<LAST, __half>(sh, p, nullptr, 0, 0, args, status, s);
 }
 
 }  // namespace ns
