@@ -1,6 +1,7 @@
 // D[M][N] = L[M][K] R on tcgen05, for 16-bit floating and 8-bit integer operands: the pipeline shared by the products of
 // the Newton-Schulz steps and of the 8-bit forward.  What happens to the accumulator is the epilogue's, a template argument:
-// emit() takes 32 columns of a row per lane, fetch() asks one step earlier for what emit() will read from memory.
+// emit() takes 32 columns of a row per lane, fetch() asks one step earlier for what emit() will read from memory.  (PP = 3
+// sums in registers anyway: there the sums start from init() and take the accumulators times scale(), and put() writes.)
 //
 //   warp 0     TMA: one stage = 128 bytes of K of the tile's L rows (128 per CTA) and of R, 128-byte swizzle, no multicast.
 //              R is either [N][K] (K-major) or [K][N] (boxes of 64 K rows x 64 columns, read through an MN-major descriptor)
@@ -122,9 +123,9 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
           "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr) : "memory");
 }
-// v[0..BN) (+)= columns of an accumulator; the next 16 are on their way while 16 are added
+// v[0..BN) (+)= scale * columns of an accumulator; the next 16 are on their way while 16 are added
 template <int BN, bool SET>
-__device__ __forceinline__ void add_columns(uint32_t taddr, float (&v)[BN]) {
+__device__ __forceinline__ void add_columns(uint32_t taddr, float scale, float (&v)[BN]) {
     uint32_t r[2][16];
     tmem_ld16(taddr, r[0]);
 #pragma unroll
@@ -134,7 +135,7 @@ __device__ __forceinline__ void add_columns(uint32_t taddr, float (&v)[BN]) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
             const float x = __uint_as_float(r[c & 1][e]);
-            v[c * 16 + e] = SET ? x : v[c * 16 + e] + x;
+            v[c * 16 + e] = SET ? x * scale : fmaf(x, scale, v[c * 16 + e]);
         }
     }
 }
@@ -379,32 +380,32 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ C
             int ncols = g.N - n0;
             if (ncols > EB) ncols = EB;
             const int nch = ncols > 0 && row0 < g.M ? (ncols + 31) >> 5 : 0;
-            typename Epi::Fetched fa, fb;
             if constexpr (C::PP == 3) {
+                const float scale = Epi::scale(args, b);
                 float v[EB];
+                if (Epi::INIT) Epi::init(args, g, b, row0 + lane, n0, v);      // while the first MMAs run
                 for (int kb = 0; kb < g.nkb; ++kb) {
                     if (!wait_all(acc_full(0), acc_ph)) break;
                     acc_ph ^= 1u;
-                    if (kb == 0) add_columns<EB, true>(tmem + lanes + (uint32_t)half0, v);
-                    else add_columns<EB, false>(tmem + lanes + (uint32_t)half0, v);
+                    if (!Epi::INIT && kb == 0) add_columns<EB, true>(tmem + lanes + (uint32_t)half0, scale, v);
+                    else add_columns<EB, false>(tmem + lanes + (uint32_t)half0, scale, v);
                     release(0);
                 }
                 if (!alive) break;
-                Epi::fetch(args, g, b, row0 + lane, n0, fa);
                 if (!wait_all(acc_full(1), cross_ph)) break;
                 cross_ph ^= 1u;
-                add_columns<EB, false>(tmem + lanes + (uint32_t)(BN + half0), v);
+                add_columns<EB, false>(tmem + lanes + (uint32_t)(BN + half0), scale, v);
                 release(1);
 #pragma unroll
                 for (int c = 0; c < EB / 32; ++c)
                     if (c < nch) {
-                        uint32_t r[32];
+                        float x[32];
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(v[c * 32 + e]);
-                        if (c + 1 < EB / 32) Epi::fetch(args, g, b, row0 + lane, n0 + (c + 1) * 32, c & 1 ? fa : fb);
-                        Epi::emit(args, g, b, row0, n0 + c * 32, r, c & 1 ? fb : fa, buf);
+                        for (int e = 0; e < 32; ++e) x[e] = v[c * 32 + e];
+                        Epi::put(args, g, b, row0, n0 + c * 32, x, buf);
                     }
             } else {
+                typename Epi::Fetched fa, fb;
                 Epi::fetch(args, g, b, row0 + lane, n0, fa);
                 if (!wait_all(acc_full(acc), acc_ph)) break;
                 const uint32_t ta = tmem + lanes + (uint32_t)(acc * BN + half0);

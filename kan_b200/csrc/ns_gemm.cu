@@ -47,27 +47,57 @@ struct Epilogue {
         }
     }
 
+    // what the accumulator is multiplied with
+    static __device__ __forceinline__ float scale(const Args& p, int b) {
+        if (KIND == GRAM) { const float al = p.alpha[b]; return al * al * exp2f((float)A_EXP); }
+        if (KIND == POLY) return p.cc * exp2f(-2.f * A_EXP + P_EXP);
+        if (KIND == APPLY) return exp2f(-(float)P_EXP) * p.alpha[b] / p.alpha_next[b];
+        return exp2f(-(float)P_EXP) * p.alpha[b];
+    }
+    // POLY: what the product is added to, ca I + cb A, for eight columns
+    static __device__ __forceinline__ void addend(const Args& p, int row, int col0, const uint32_t (&ah)[4], const uint32_t (&al)[4], float (&v)[8]) {
+        float a[8];
+        join8<PLANES>(ah, al, a);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            v[e] = p.cb * exp2f((float)(P_EXP - A_EXP)) * a[e];
+            if (col0 + e == row) v[e] += p.ca * exp2f((float)P_EXP);
+        }
+    }
+    static constexpr bool INIT = KIND == POLY;
+    template <int NC>
+    static __device__ __forceinline__ void init(const Args& p, const Tiles& g, int b, int row, int col0, float (&v)[NC]) {
+        const __half* a = p.a + (int64_t)b * PLANES * p.slab + (int64_t)row * p.pitch + col0;
+#pragma unroll
+        for (int c = 0; c < NC; c += 8) {
+            uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
+            if (row < g.M && col0 + c < g.N) {
+                hi = *reinterpret_cast<const uint4*>(a + c);
+                if (PLANES == 2) lo = *reinterpret_cast<const uint4*>(a + c + p.slab);
+            }
+            const uint32_t ah[4] = {hi.x, hi.y, hi.z, hi.w}, al[4] = {lo.x, lo.y, lo.z, lo.w};
+            float x[8];
+            addend(p, row, col0 + c, ah, al, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[c + e] = x[e];
+        }
+    }
+
     // 32 columns from col0 of the rows from row0, one per lane; buf: the warp's 4 KB
-    static __device__ __forceinline__ void emit(const Args& p, const Tiles& g, int b, int row0, int col0, uint32_t (&r)[32], const Fetched& f,
-                                                uint32_t buf) {
+    static __device__ __forceinline__ void put(const Args& p, const Tiles& g, int b, int row0, int col0, const float (&x)[32], uint32_t buf) {
         const int lane = threadIdx.x & 31, row = row0 + lane;
-        float factor;
-        if (KIND == GRAM) { const float al = p.alpha[b]; factor = al * al * exp2f((float)A_EXP); }
-        else if (KIND == POLY) factor = p.cc * exp2f(-2.f * A_EXP + P_EXP);
-        else if (KIND == APPLY) factor = exp2f(-(float)P_EXP) * p.alpha[b] / p.alpha_next[b];
-        else factor = exp2f(-(float)P_EXP) * p.alpha[b];
         if constexpr (KIND == LAST) {
             OUT* o = reinterpret_cast<OUT*>(p.o) + (int64_t)b * g.M * g.N;
             if (p.tall) {                       // the warp's lanes hold consecutive rows, which are o's columns
                 if (row < g.M)
 #pragma unroll
                     for (int e = 0; e < 32; ++e)
-                        if (col0 + e < g.N) o[(int64_t)(col0 + e) * g.M + row] = from_float<OUT>(__uint_as_float(r[e]) * factor);
+                        if (col0 + e < g.N) o[(int64_t)(col0 + e) * g.M + row] = from_float<OUT>(x[e]);
                 return;
             }
             alignas(16) OUT v[32];
 #pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] = from_float<OUT>(__uint_as_float(r[e]) * factor);
+            for (int e = 0; e < 32; ++e) v[e] = from_float<OUT>(x[e]);
             gemm::store_rows(buf, v, o + (int64_t)row0 * g.N + col0, g.N, g.M - row0, g.N - col0, g.N % (16 / (int)sizeof(OUT)) == 0);
         } else {
             // both planes of 32 x 32 into shared memory, 64-byte rows with the 16-byte chunks permuted as the map's swizzle has
@@ -76,21 +106,7 @@ struct Epilogue {
             __syncwarp();
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                float v[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(r[c * 8 + e]) * factor;
-                if constexpr (KIND == POLY) {
-                    float a[8];
-                    const uint32_t ah[4] = {f.hi[c].x, f.hi[c].y, f.hi[c].z, f.hi[c].w};
-                    uint32_t al[4] = {};
-                    if (PLANES == 2) { al[0] = f.lo[c].x; al[1] = f.lo[c].y; al[2] = f.lo[c].z; al[3] = f.lo[c].w; }
-                    join8<PLANES>(ah, al, a);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        v[e] = fmaf(p.cb * exp2f((float)(P_EXP - A_EXP)), a[e], v[e]);
-                        if (col0 + c * 8 + e == row) v[e] += p.ca * exp2f((float)P_EXP);
-                    }
-                }
+                const float v[8] = {x[c * 8], x[c * 8 + 1], x[c * 8 + 2], x[c * 8 + 3], x[c * 8 + 4], x[c * 8 + 5], x[c * 8 + 6], x[c * 8 + 7]};
                 uint32_t hi[4], lo[4];
                 split8<PLANES>(v, hi, lo);
                 const uint32_t at = buf + (uint32_t)(lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4));
@@ -105,6 +121,26 @@ struct Epilogue {
                 gemm::bulk_commit();
             }
         }
+    }
+    static __device__ __forceinline__ void emit(const Args& p, const Tiles& g, int b, int row0, int col0, uint32_t (&r)[32], const Fetched& f,
+                                                uint32_t buf) {
+        const float factor = scale(p, b);
+        float x[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) x[e] = __uint_as_float(r[e]) * factor;
+        if constexpr (KIND == POLY) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const uint32_t ah[4] = {f.hi[c].x, f.hi[c].y, f.hi[c].z, f.hi[c].w};
+                uint32_t al[4] = {};
+                if (PLANES == 2) { al[0] = f.lo[c].x; al[1] = f.lo[c].y; al[2] = f.lo[c].z; al[3] = f.lo[c].w; }
+                float v[8];
+                addend(p, row0 + (threadIdx.x & 31), col0 + c * 8, ah, al, v);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[c * 8 + e] += v[e];
+            }
+        }
+        put(p, g, b, row0, col0, x, buf);
     }
 };
 
