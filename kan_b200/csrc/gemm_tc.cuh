@@ -36,6 +36,7 @@ struct Config {
     static constexpr int PP = PP_, CG = CG_, BN = BN_;
     static constexpr bool RMN = RMN_, LSYM = LSYM_, RSYM = RSYM_;
     static constexpr int PLANES = PP == 3 ? 2 : 1;
+    static constexpr bool HALVES = KIND == F16 && CG == 2;     // the last tiles may be cut in two (see Tiles)
     static constexpr int BM = 128 * CG;                        // rows of a tile
     static constexpr int KE = KIND == I8 ? 128 : 64;           // K elements per stage (128 bytes)
     static constexpr int L_PANEL = 128 * 128, R_PANEL = BN / CG * 128;
@@ -62,28 +63,35 @@ struct Tiles {
     int ntm, ntn;         // tile rows and columns
     int per_batch;        // tiles of one matrix
     int sym;              // only the 256 x 256 blocks on and above the diagonal
-    int64_t total;
+    // Tiles from `whole` on are cut into two of half the width: what is left after the last full wave, where the halves fit
+    // into one.  90 tiles on 74 pairs then take about 1.6 tiles' time instead of 2.  total counts the halves.
+    int64_t whole, total;
 };
 
 // whether element (i, j) of a symmetric matrix is stored
 __host__ __device__ __forceinline__ bool stored(int i, int j) { return j / 256 >= i / 256; }
 
-// position of tile t: matrix b, first row, first column
+// position of tile t: matrix b, first row, first column; true for half a tile
 template <int BM, int BN>
-__device__ __forceinline__ void decode(const Tiles& g, int64_t t, int& b, int& m0, int& n0) {
+__device__ __forceinline__ bool decode(const Tiles& g, int64_t t, int& b, int& m0, int& n0) {
+    const bool half = t >= g.whole;
+    const int second = half ? (int)(t - g.whole) & 1 : 0;
+    if (half) t = g.whole + ((t - g.whole) >> 1);
     b = (int)(t / g.per_batch);
     int r = (int)(t - (int64_t)b * g.per_batch);
     if (!g.sym) {
         m0 = r / g.ntn * BM;
         n0 = r % g.ntn * BN;
-        return;
+    } else {
+        int tm = 0;
+        for (;; ++tm) {
+            const int first = tm * BM / 256 * (256 / BN), count = g.ntn - first;
+            if (r < count) { m0 = tm * BM; n0 = (first + r) * BN; break; }
+            r -= count;
+        }
     }
-    int tm = 0;
-    for (;; ++tm) {
-        const int first = tm * BM / 256 * (256 / BN), count = g.ntn - first;
-        if (r < count) { m0 = tm * BM; n0 = (first + r) * BN; return; }
-        r -= count;
-    }
+    n0 += second * (BN / 2);
+    return half;
 }
 inline int sym_tiles(int ntm, int ntn, int bm, int bn) {
     int n = 0;
@@ -233,13 +241,15 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ C
             bool alive = true;
             for (int64_t t = unit; t < g.total && alive; t += units) {
                 int b, m0, n0;
-                decode<C::BM, BN>(g, t, b, m0, n0);
-                const int row = m0 + (int)rank * 128, col = n0 + (int)rank * (BN / CG);
+                const bool half = decode<C::BM, BN>(g, t, b, m0, n0);
+                const int width = (half ? BN / 2 : BN) / CG;             // this CTA's share of R's columns
+                const int row = m0 + (int)rank * 128, col = n0 + (int)rank * width;
+                const uint32_t bytes = (uint32_t)(PLANES * CG * (C::L_PANEL + width * 128));
                 for (int kb = 0; kb < g.nkb; ++kb) {
                     if (!mbar_wait(empty(s), ph ^ 1u, abort_flag, status, ST_LOAD)) { alive = false; break; }
                     const uint32_t dst = base + s * C::STAGE;
                     uint32_t bar = full(s);
-                    if (rank == 0) mbar_arrive_expect_tx(bar, (uint32_t)(C::STAGE * CG));
+                    if (rank == 0) mbar_arrive_expect_tx(bar, bytes);
                     if (CG == 2) bar = mapa_cluster(bar, 0);
                     auto load = [&](uint32_t to, const CUtensorMap* map, int c0, int c1, int z) {
                         if (CG == 2) load_3d_pair(to, map, c0, c1, z, bar);
@@ -258,10 +268,11 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ C
                         else load(dst + p * C::L_PANEL, &map_l, k0, row, z);
                         const uint32_t rd = dst + PLANES * C::L_PANEL + p * C::R_PANEL;
                         if (C::RMN) {
-#pragma unroll
-                            for (int q = 0; q < BN / CG / 64; ++q) load(rd + q * 8192, &map_r, col + q * 64, k0, z);
+                            for (int q = 0; q < width; q += 64) load(rd + q * 128, &map_r, col + q, k0, z);
                         } else if (C::RSYM) {
-                            load_sym(rd, &map_r, col, BN / CG, z);
+                            load_sym(rd, &map_r, col, width, z);
+                        } else if (C::KIND == F16) {
+                            for (int q = 0; q < width; q += 64) load(rd + q * 128, &map_r, k0, col + q, z);
                         } else {
                             load(rd, &map_r, k0, col, z);
                         }
@@ -300,7 +311,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ C
             };
             for (int64_t t = unit; t < g.total && alive; t += units) {
                 int b, m0 = 0, n0 = 0;
-                if (C::LSYM || C::RSYM) decode<C::BM, BN>(g, t, b, m0, n0);
+                const bool half = decode<C::BM, BN>(g, t, b, m0, n0);
+                const uint32_t idesc0 = half ? C::IDESC - ((uint32_t)(BN >> 4) << 17) : C::IDESC;       // N halved
                 if (C::PP == 1 && !wait_all(acc_empty(acc), acc_ph ^ 1u, ST_MMA_ACC)) break;
                 const uint32_t d = C::PP == 1 ? tmem + (uint32_t)(acc * BN) : tmem, cross = tmem + BN;
                 for (int kb = 0; kb < g.nkb; ++kb) {
@@ -311,7 +323,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ C
                     const bool rmn = C::RMN || (C::RSYM && !stored(n0, kb * C::KE));
                     const uint32_t l_lo = (lmn ? l_mn : l_k) + off, r_lo = (rmn ? r_mn : r_k) + off;
                     const uint32_t l_step = lmn ? MNSTEP : KSTEP, r_step = rmn ? MNSTEP : KSTEP;
-                    const uint32_t idesc = C::IDESC | (lmn ? 1u << 15 : 0u) | (rmn ? 1u << 16 : 0u);
+                    const uint32_t idesc = idesc0 | (lmn ? 1u << 15 : 0u) | (rmn ? 1u << 16 : 0u);
                     if (elected) {
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
@@ -356,8 +368,6 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ C
         }
     } else {
         const int q = warp & 3;               // quarter of the tensor memory's lanes that this warp may read
-        constexpr int EB = BN / 2;            // columns of its half
-        const int half0 = (warp - 2) / 4 * EB;
         const uint32_t buf = base + C::OUT_OFFSET + (uint32_t)((warp - 2) * 4096);
         int acc = 0; uint32_t acc_ph = 0, cross_ph = 0;
         bool alive = true;
@@ -372,18 +382,20 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ C
             else mbar_arrive(acc_empty(a));
         };
         const uint32_t lanes = (uint32_t)(q * 32) << 16;
+        constexpr int EB = BN / 2;            // columns of this warp (half of them mean nothing in half a tile)
         for (int64_t t = unit; t < g.total && alive; t += units) {
             int b, m0, n0;
-            decode<C::BM, BN>(g, t, b, m0, n0);
+            const int width = decode<C::BM, BN>(g, t, b, m0, n0) ? EB / 2 : EB;
+            const int half0 = (warp - 2) / 4 * width;
             n0 += half0;
             const int row0 = m0 + (int)rank * 128 + q * 32;
             int ncols = g.N - n0;
-            if (ncols > EB) ncols = EB;
+            if (ncols > width) ncols = width;
             const int nch = ncols > 0 && row0 < g.M ? (ncols + 31) >> 5 : 0;
             if constexpr (C::PP == 3) {
                 const float scale = Epi::scale(args, b);
                 float v[EB];
-                if (Epi::INIT) Epi::init(args, g, b, row0 + lane, n0, v);      // while the first MMAs run
+                if (Epi::INIT) Epi::init(args, g, b, row0, n0, v, buf);      // while the first MMAs run
                 for (int kb = 0; kb < g.nkb; ++kb) {
                     if (!wait_all(acc_full(0), acc_ph)) break;
                     acc_ph ^= 1u;
@@ -663,7 +675,7 @@ Tiles tiles_of(int M, int N, int K, int batch, bool sym) {
     g.ntn = (int)ceil_div(N, C::BN);
     g.sym = sym;
     g.per_batch = sym ? sym_tiles(g.ntm, g.ntn, C::BM, C::BN) : g.ntm * g.ntn;
-    g.total = (int64_t)g.per_batch * batch;
+    g.whole = g.total = (int64_t)g.per_batch * batch;
     return g;
 }
 
@@ -697,9 +709,15 @@ int launch(const CUtensorMap& map_l, const CUtensorMap& map_r, const Tiles& g, c
         }
         max_units[dev] = n;
     }
-    const int64_t units = g.total < max_units[dev] ? g.total : max_units[dev];
+    Tiles h = g;
+    const int64_t left = g.total % max_units[dev];
+    if (C::HALVES && left > 0 && 2 * left <= max_units[dev]) {
+        h.whole = g.total - left;
+        h.total = h.whole + 2 * left;
+    }
+    const int64_t units = h.total < max_units[dev] ? h.total : max_units[dev];
     cfg.gridDim = dim3((unsigned)(units * C::CG));
-    return check_cuda(cudaLaunchKernelEx(&cfg, kernel, map_l, map_r, g, args, status));
+    return check_cuda(cudaLaunchKernelEx(&cfg, kernel, map_l, map_r, h, args, status));
 }
 
 }  // namespace gemm

@@ -65,21 +65,49 @@ struct Epilogue {
         }
     }
     static constexpr bool INIT = KIND == POLY;
+    // A's 32 x NC block: lanes read along rows (a row per lane would touch 32 lines per load) and meet their rows in buf
     template <int NC>
-    static __device__ __forceinline__ void init(const Args& p, const Tiles& g, int b, int row, int col0, float (&v)[NC]) {
-        const __half* a = p.a + (int64_t)b * PLANES * p.slab + (int64_t)row * p.pitch + col0;
+    static __device__ __forceinline__ void init(const Args& p, const Tiles& g, int b, int row0, int col0, float (&v)[NC], uint32_t buf) {
+        const int lane = threadIdx.x & 31, ch = lane & 3;
+        const __half* a = p.a + (int64_t)b * PLANES * p.slab + (int64_t)row0 * p.pitch + col0;
+        if (lane == 0) gemm::bulk_wait_read();
+        __syncwarp();
+        auto place = [&](int plane, int r, int c) { return buf + (uint32_t)(plane * 2048 + r * 64 + ((c ^ ((r >> 1) & 3)) << 4)); };
+        uint4 x[2][4 * PLANES];
+        auto ask = [&](int c, uint4 (&to)[4 * PLANES]) {
 #pragma unroll
-        for (int c = 0; c < NC; c += 8) {
-            uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
-            if (row < g.M && col0 + c < g.N) {
-                hi = *reinterpret_cast<const uint4*>(a + c);
-                if (PLANES == 2) lo = *reinterpret_cast<const uint4*>(a + c + p.slab);
+            for (int i = 0; i < 4; ++i) {
+                const int r = i * 8 + (lane >> 2);
+                const bool in = row0 + r < g.M && col0 + c + ch * 8 < g.N;
+#pragma unroll
+                for (int q = 0; q < PLANES; ++q)
+                    to[i * PLANES + q] = in ? *reinterpret_cast<const uint4*>(a + (int64_t)r * p.pitch + c + ch * 8 + q * p.slab) : make_uint4(0, 0, 0, 0);
             }
-            const uint32_t ah[4] = {hi.x, hi.y, hi.z, hi.w}, al[4] = {lo.x, lo.y, lo.z, lo.w};
-            float x[8];
-            addend(p, row, col0 + c, ah, al, x);
+        };
+        ask(0, x[0]);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[c + e] = x[e];
+        for (int c = 0; c < NC; c += 32) {
+            if (c + 32 < NC) ask(c + 32, x[(c / 32 + 1) & 1]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int q = 0; q < PLANES; ++q) {
+                    const uint4 w = x[(c / 32) & 1][i * PLANES + q];
+                    gemm::st_shared_v4(place(q, i * 8 + (lane >> 2), ch), w.x, w.y, w.z, w.w);
+                }
+            __syncwarp();
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                uint32_t ah[4], al[4] = {};
+                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(ah[0]), "=r"(ah[1]), "=r"(ah[2]), "=r"(ah[3]) : "r"(place(0, lane, k)));
+                if (PLANES == 2)
+                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(al[0]), "=r"(al[1]), "=r"(al[2]), "=r"(al[3]) : "r"(place(1, lane, k)));
+                float y[8];
+                addend(p, row0 + lane, col0 + c + k * 8, ah, al, y);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[c + k * 8 + e] = y[e];
+            }
+            __syncwarp();
         }
     }
 
@@ -163,7 +191,7 @@ int run(const Operands& o, __half* out, int64_t out_pitch, int64_t out_slab, Epi
     int rc = gemm::make_map(&ml, gemm::F16, o.left, o.K, o.M, slabs, 2 * o.pitch_l, 2 * o.slab_l, 64, C::LSYM ? 64 : 128);
     if (rc) return rc;
     if (C::RMN) rc = gemm::make_map(&mr, gemm::F16, o.right, o.N, o.K, slabs, 2 * o.pitch_r, 2 * o.slab_r, 64, 64);
-    else rc = gemm::make_map(&mr, gemm::F16, o.right, o.K, o.N, slabs, 2 * o.pitch_r, 2 * o.slab_r, 64, C::RSYM ? 64 : C::BN / CG);
+    else rc = gemm::make_map(&mr, gemm::F16, o.right, o.K, o.N, slabs, 2 * o.pitch_r, 2 * o.slab_r, 64, 64);
     if (rc) return rc;
     if (KIND != LAST) {
         rc = gemm::make_map(&args.map, gemm::F16, out, o.N, o.M, slabs, 2 * out_pitch, 2 * out_slab, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
