@@ -160,6 +160,32 @@ struct TableRec {
     }
 };
 
+// ---- kernels of one call that follow one another (programmatic dependent launch) ----
+// A kernel launched with launch_after() may be scheduled once every block of the kernel before it has called
+// let_next_start(): its blocks take the SMs as they fall free and set themselves up, and then wait in wait_for_previous()
+// until that kernel has completed and its writes are visible.  Everything that reads or writes device memory comes after
+// the wait, except reads of data that no kernel of the same call writes.  Without the launch attribute both do nothing.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+template <typename... Params, typename... Args>
+cudaError_t launch_after(bool after, void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, int cluster,
+                         const Args&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid; cfg.blockDim = block; cfg.dynamicSmemBytes = smem; cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    unsigned n = 0;
+    if (after) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster > 0) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = (unsigned)cluster; attr[n].val.clusterDim.y = 1; attr[n++].val.clusterDim.z = 1;
+    }
+    cfg.attrs = attr; cfg.numAttrs = n;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // thread-local record of the last CUDA error seen by an entry point
 void set_last_cuda_error(int e);
 inline int check_cuda(cudaError_t e) {

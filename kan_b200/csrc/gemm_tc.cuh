@@ -234,6 +234,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ C
     if (CG == 2) cluster_sync_all();      // the peer's barriers exist before anything arrives on them
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    let_next_start();
+    wait_for_previous();
 
     if (warp == 0) {
         if (lane == 0) {
@@ -518,6 +520,8 @@ split_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ 
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    let_next_start();
+    wait_for_previous();
 
     int b, m0, n0;
     decode<C::BM, BN>(g, blockIdx.x / split, b, m0, n0);
@@ -629,7 +633,7 @@ inline int split_of(const Tiles& g, int sms = 148) {
 
 template <class C, class Epi>
 int launch_split(const CUtensorMap& map_l, const CUtensorMap& map_r, const Tiles& g, const typename Epi::Args& args, int split,
-                 int32_t* status, cudaStream_t s) {
+                 int32_t* status, cudaStream_t s, bool after) {
     static bool ready[64] = {false};
     int dev = 0;
     cudaGetDevice(&dev);
@@ -640,13 +644,8 @@ int launch_split(const CUtensorMap& map_l, const CUtensorMap& map_r, const Tiles
         if (rc) return rc;
         ready[dev] = true;
     }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(g.total * split)); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = SplitSmem<C>::TOTAL; cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)split; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr; cfg.numAttrs = 1;
-    return check_cuda(cudaLaunchKernelEx(&cfg, kernel, map_l, map_r, g, args, split, status));
+    return check_cuda(launch_after(after, kernel, dim3((unsigned)(g.total * split)), dim3(THREADS), SplitSmem<C>::TOTAL, s, split, map_l, map_r, g,
+                                   args, split, status));
 }
 
 // map of `slabs` row-major matrices [rows][cols], rows pitch_bytes and matrices slab_bytes apart, read in boxes of
@@ -679,21 +678,15 @@ Tiles tiles_of(int M, int N, int K, int batch, bool sym) {
     return g;
 }
 
-// persistent launch, one CTA (or pair) per SM (or two)
+// persistent launch, one CTA (or pair) per SM (or two); after: see launch_after
 template <class C, class Epi>
 int launch(const CUtensorMap& map_l, const CUtensorMap& map_r, const Tiles& g, const typename Epi::Args& args, int32_t* status,
-           cudaStream_t s) {
+           cudaStream_t s, bool after) {
     static int max_units[64] = {0};
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64) return CHEBYKAN_EINVAL;
     auto kernel = gemm_kernel<C, Epi>;
-    cudaLaunchConfig_t cfg = {};
-    cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = C::SMEM; cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = C::CG; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr; cfg.numAttrs = 1;
     if (max_units[dev] == 0) {
         int rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
         if (rc) return rc;
@@ -701,7 +694,12 @@ int launch(const CUtensorMap& map_l, const CUtensorMap& map_r, const Tiles& g, c
         cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
         n = sms / C::CG;
         if (C::CG == 2) {
-            cfg.gridDim = dim3((unsigned)(sms & ~1));
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3((unsigned)(sms & ~1)); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = C::SMEM;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = C::CG; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+            cfg.attrs = attr; cfg.numAttrs = 1;
             int clusters = 0;
             if ((rc = check_cuda(cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg)))) return rc;
             if (clusters < 1) return CHEBYKAN_ECUDA;
@@ -716,8 +714,7 @@ int launch(const CUtensorMap& map_l, const CUtensorMap& map_r, const Tiles& g, c
         h.total = h.whole + 2 * left;
     }
     const int64_t units = h.total < max_units[dev] ? h.total : max_units[dev];
-    cfg.gridDim = dim3((unsigned)(units * C::CG));
-    return check_cuda(cudaLaunchKernelEx(&cfg, kernel, map_l, map_r, h, args, status));
+    return check_cuda(launch_after(after, kernel, dim3((unsigned)(units * C::CG)), dim3(THREADS), C::SMEM, s, C::CG, map_l, map_r, h, args, status));
 }
 
 }  // namespace gemm

@@ -68,6 +68,7 @@ basis_kernel(const T* __restrict__ x, int8_t* __restrict__ q, float* __restrict_
     const int64_t row = blockIdx.x * (int64_t)ROWS + threadIdx.x / G;
     const bool live = row < B;
     const T* src = x + row * in;
+    let_next_start();
     const int chunks = CHUNKS ? CHUNKS : (pad + 8 * G - 1) / (8 * G);
     float t[KEEP][8];
     float top = 0.f;
@@ -276,7 +277,7 @@ int chebykan_int8_matmul(const int8_t* q, int64_t ldq, const float* q_scale, con
     if (workspace_bytes < need || (need > 0 && !workspace)) return CHEBYKAN_EWORKSPACE;
     int rc = check_device();
     if (rc) return rc;
-    return launch_matmul({q, q_scale, wq, w_scale, bias, y, dtype, M, N, K, ldq, ldw}, workspace, status, (cudaStream_t)stream);
+    return launch_matmul({q, q_scale, wq, w_scale, bias, y, dtype, M, N, K, ldq, ldw}, workspace, status, (cudaStream_t)stream, false);
 }
 
 int64_t chebykan_int8_fwd_workspace_bytes(int64_t B, int64_t in, int64_t out, int64_t deg) {
@@ -303,7 +304,7 @@ int chebykan_int8_fwd(const void* x, int x_dtype, const int8_t* wq, const float*
     float* scale = reinterpret_cast<float*>(ws + a256(B * K));
     if ((rc = launch_basis(x, x_dtype, q, scale, B, in, deg, (cudaStream_t)stream))) return rc;
     return launch_matmul({q, scale, wq, w_scale, bias, y, y_dtype, B, out, K, K, K}, ws + a256(B * K) + a256(B * 4), status,
-                         (cudaStream_t)stream);
+                         (cudaStream_t)stream, true);
 }
 
 }  // extern "C"

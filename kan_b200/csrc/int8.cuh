@@ -30,7 +30,8 @@ template <> __device__ __forceinline__ __nv_bfloat16 to_type<__nv_bfloat16>(floa
 
 // bytes of scratch the product needs, and the product itself
 int64_t matmul_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t ldq, int64_t ldw);
-int launch_matmul(const Product& p, void* ws, int32_t* status, cudaStream_t s);
+// `after`: the kernel before it in the stream writes q and lets it start early (launch_after)
+int launch_matmul(const Product& p, void* ws, int32_t* status, cudaStream_t s, bool after);
 
 }  // namespace int8
 }  // namespace chebykan

@@ -77,46 +77,58 @@ struct Epilogue {
 };
 
 // ---- up to 8 rows ---------------------------------------------------------------------------------------------------
-// A warp per output column: lanes take 16 bytes of the column's weights each, eight loads in flight, against the same
-// bytes of every row (from the caches).  Bytes past K are zero.
-__device__ __forceinline__ int4 load16(const int8_t* p, int64_t k, int64_t K) {
-    if (k + 16 <= K) return __ldg(reinterpret_cast<const int4*>(p + k));
-    int w[4] = {0, 0, 0, 0};
-    for (int e = 0; e < 16 && k + e < K; ++e) w[e >> 2] |= (int)((uint32_t)(uint8_t)p[k + e] << (8 * (e & 3)));
-    return make_int4(w[0], w[1], w[2], w[3]);
-}
+// A warp per output column: lanes take 16 bytes of the column's weights each, U loads in flight, against the same bytes of
+// every row (from the caches).  The first weights are asked for before the rows' producer is waited for.
 template <typename OUT, int ROWS>
 __global__ void __launch_bounds__(256) row_kernel(const Product p) {
     const int lane = threadIdx.x & 31;
     const int64_t o = blockIdx.x * (int64_t)8 + (threadIdx.x >> 5);
     if (o >= p.N) return;
     const int8_t* w = p.wq + o * p.ldw;
+    const int whole = (int)(p.K / 16);                 // 16-byte pieces; the rest is one lane's, byte by byte
     int acc[ROWS] = {};
-    constexpr int U = ROWS <= 2 ? 8 : 4;
-    for (int64_t k0 = lane * 16; k0 < p.K; k0 += U * 512) {
-        int4 wv[U];
+    constexpr int U = ROWS <= 2 ? 16 : 8;
+    int4 wv[U];
+    auto weights = [&](int c0) {
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (k0 + u * 512 < p.K) wv[u] = load16(w, k0 + u * 512, p.K);
+        for (int u = 0; u < U; ++u) {
+            wv[u] = make_int4(0, 0, 0, 0);
+            if (c0 + u * 32 < whole) wv[u] = __ldg(reinterpret_cast<const int4*>(w) + c0 + u * 32);
+        }
+    };
+    weights(lane);
+    const float ws = __ldg(p.w_scale + o), bias = p.bias ? __ldg(p.bias + o) : 0.f;
+    wait_for_previous();
+    for (int c0 = lane; c0 < whole;) {
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (k0 + u * 512 < p.K)
+        for (int r = 0; r < ROWS; ++r)
+            if (r < p.M) {
+                const int4* q = reinterpret_cast<const int4*>(p.q + r * p.ldq);
+                int4 v[U];
 #pragma unroll
-                for (int r = 0; r < ROWS; ++r)
-                    if (r < p.M) {
-                        const int4 v = load16(p.q + r * p.ldq, k0 + u * 512, p.K);
-                        acc[r] = __dp4a(v.x, wv[u].x, __dp4a(v.y, wv[u].y, __dp4a(v.z, wv[u].z, __dp4a(v.w, wv[u].w, acc[r]))));
-                    }
+                for (int u = 0; u < U; ++u) {
+                    v[u] = make_int4(0, 0, 0, 0);
+                    if (c0 + u * 32 < whole) v[u] = q[c0 + u * 32];
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    acc[r] = __dp4a(v[u].x, wv[u].x, __dp4a(v[u].y, wv[u].y, __dp4a(v[u].z, wv[u].z, __dp4a(v[u].w, wv[u].w, acc[r]))));
+            }
+        c0 += U * 32;
+        if (c0 < whole) weights(c0);
     }
+    if (lane == 0)
+        for (int64_t k = (int64_t)whole * 16; k < p.K; ++k)
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r)
+                if (r < p.M) acc[r] += (int)p.q[r * p.ldq + k] * (int)w[k];
 #pragma unroll
     for (int r = 0; r < ROWS; ++r)
 #pragma unroll
         for (int d = 16; d; d >>= 1) acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], d);
 #pragma unroll
     for (int r = 0; r < ROWS; ++r)
-        if (lane == r && r < p.M)
-            reinterpret_cast<OUT*>(p.y)[r * p.N + o] =
-                to_type<OUT>(fmaf((float)acc[r] * p.q_scale[r], p.w_scale[o], p.bias ? p.bias[o] : 0.f));
+        if (lane == r && r < p.M) reinterpret_cast<OUT*>(p.y)[r * p.N + o] = to_type<OUT>(fmaf((float)acc[r] * p.q_scale[r], ws, bias));
 }
 
 // no columns at all: the sums are zero
@@ -140,13 +152,9 @@ __global__ void __launch_bounds__(256) pad_kernel(const int8_t* __restrict__ src
 }
 
 template <typename OUT>
-int launch_rows(const Product& p, cudaStream_t s) {
-    const unsigned grid = (unsigned)ceil_div(p.N, 8);
-    if (p.M == 1) row_kernel<OUT, 1><<<grid, 256, 0, s>>>(p);
-    else if (p.M == 2) row_kernel<OUT, 2><<<grid, 256, 0, s>>>(p);
-    else if (p.M <= 4) row_kernel<OUT, 4><<<grid, 256, 0, s>>>(p);
-    else row_kernel<OUT, 8><<<grid, 256, 0, s>>>(p);
-    return check_cuda(cudaGetLastError());
+int launch_rows(const Product& p, cudaStream_t s, bool after) {
+    auto kernel = p.M == 1 ? row_kernel<OUT, 1> : p.M == 2 ? row_kernel<OUT, 2> : p.M <= 4 ? row_kernel<OUT, 4> : row_kernel<OUT, 8>;
+    return check_cuda(launch_after(after, kernel, dim3((unsigned)ceil_div(p.N, 8)), dim3(256), 0, s, 0, p));
 }
 
 template <class C>
@@ -156,27 +164,27 @@ int maps_of(const Product& p, CUtensorMap* mq, CUtensorMap* mw) {
 }
 
 template <class C, typename OUT>
-int run_split(const Product& p, const Tiles& g, const EpiArgs& args, int32_t* status, cudaStream_t s) {
+int run_split(const Product& p, const Tiles& g, const EpiArgs& args, int32_t* status, cudaStream_t s, bool after) {
     CUtensorMap mq, mw;
     const int rc = maps_of<C>(p, &mq, &mw);
     if (rc) return rc;
-    return gemm::launch_split<C, Epilogue<OUT>>(mq, mw, g, args, gemm::split_of(g), status, s);
+    return gemm::launch_split<C, Epilogue<OUT>>(mq, mw, g, args, gemm::split_of(g), status, s, after);
 }
 template <class C, typename OUT>
-int run_persistent(const Product& p, const EpiArgs& args, int32_t* status, cudaStream_t s) {
+int run_persistent(const Product& p, const EpiArgs& args, int32_t* status, cudaStream_t s, bool after) {
     CUtensorMap mq, mw;
     const int rc = maps_of<C>(p, &mq, &mw);
     if (rc) return rc;
-    return gemm::launch<C, Epilogue<OUT>>(mq, mw, gemm::tiles_of<C>((int)p.M, (int)p.N, (int)p.K, 1, false), args, status, s);
+    return gemm::launch<C, Epilogue<OUT>>(mq, mw, gemm::tiles_of<C>((int)p.M, (int)p.N, (int)p.K, 1, false), args, status, s, after);
 }
 
 template <typename OUT>
-int launch_typed(const Product& p, int32_t* status, cudaStream_t s) {
+int launch_typed(const Product& p, int32_t* status, cudaStream_t s, bool after) {
     if (p.K == 0) {
         empty_kernel<OUT><<<(unsigned)(ceil_div(p.M * p.N, 256) < 148 * 8 ? ceil_div(p.M * p.N, 256) : 148 * 8), 256, 0, s>>>(p);
         return check_cuda(cudaGetLastError());
     }
-    if (p.M <= 8) return launch_rows<OUT>(p, s);
+    if (p.M <= 8) return launch_rows<OUT>(p, s, after);
     const EpiArgs args{p.q_scale, p.w_scale, p.bias, p.y, p.N % (16 / (int64_t)sizeof(OUT)) == 0 && aligned16(p.w_scale) && aligned16(p.bias)};
     using Pair = gemm::Config<gemm::I8, 1, 2, 256, false>;
     using Narrow = gemm::Config<gemm::I8, 1, 1, 64, false>;
@@ -184,9 +192,9 @@ int launch_typed(const Product& p, int32_t* status, cudaStream_t s) {
     // tiles of 128 x 64 as long as that leaves SMs idle, of 128 x 128 up to one each, pairs on 256 x 256 beyond
     const int M = (int)p.M, N = (int)p.N, K = (int)p.K;
     const Tiles narrow = gemm::tiles_of<Narrow>(M, N, K, 1, false), wide = gemm::tiles_of<Wide>(M, N, K, 1, false);
-    if (narrow.total <= 148) return run_split<Narrow, OUT>(p, narrow, args, status, s);
-    if (wide.total <= 148) return run_split<Wide, OUT>(p, wide, args, status, s);
-    return run_persistent<Pair, OUT>(p, args, status, s);
+    if (narrow.total <= 148) return run_split<Narrow, OUT>(p, narrow, args, status, s, after);
+    if (wide.total <= 148) return run_split<Wide, OUT>(p, wide, args, status, s, after);
+    return run_persistent<Pair, OUT>(p, args, status, s, after);
 }
 
 int64_t a256(int64_t b) { return round_up(b, 256); }
@@ -197,7 +205,7 @@ int64_t matmul_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t ldq, int
     return (ldq % 16 ? a256(M * pitch) : 0) + (ldw % 16 ? a256(N * pitch) : 0);
 }
 
-int launch_matmul(const Product& given, void* ws, int32_t* status, cudaStream_t s) {
+int launch_matmul(const Product& given, void* ws, int32_t* status, cudaStream_t s, bool after) {
     Product p = given;
     const int64_t pitch = round_up(p.K, 16);
     int8_t* at = reinterpret_cast<int8_t*>(ws);
@@ -211,9 +219,9 @@ int launch_matmul(const Product& given, void* ws, int32_t* status, cudaStream_t 
     int rc;
     if ((rc = pad(p.q, p.ldq, p.M))) return rc;
     if ((rc = pad(p.wq, p.ldw, p.N))) return rc;
-    if (p.dtype == CHEBYKAN_DTYPE_FP32) return launch_typed<float>(p, status, s);
-    if (p.dtype == CHEBYKAN_DTYPE_BF16) return launch_typed<__nv_bfloat16>(p, status, s);
-    return launch_typed<__half>(p, status, s);
+    if (p.dtype == CHEBYKAN_DTYPE_FP32) return launch_typed<float>(p, status, s, after);
+    if (p.dtype == CHEBYKAN_DTYPE_BF16) return launch_typed<__nv_bfloat16>(p, status, s, after);
+    return launch_typed<__half>(p, status, s, after);
 }
 
 }  // namespace int8

@@ -55,6 +55,7 @@ __device__ __forceinline__ void load8(const T* p, int64_t step, int64_t left, fl
 template <typename T>
 __global__ void __launch_bounds__(256) norm_kernel(const T* __restrict__ g, const Plane pl, double* __restrict__ partial) {
     __shared__ double smem[8];
+    let_next_start();
     const T* src = g + blockIdx.y * pl.batch;
     const int64_t groups = (pl.cols + 7) / 8, total = pl.rows * groups, stride = (int64_t)gridDim.x * 256;
     double v = 0.;
@@ -96,6 +97,7 @@ momentum_kernel(const float* __restrict__ grad, float* __restrict__ buf, float* 
                 uint32_t magic, float momentum, int nesterov, float gs, double* __restrict__ partial) {
     extern __shared__ float tile[];
     __shared__ double sums[128];
+    let_next_start();
     const int odd = dp1 | 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     for (int d = threadIdx.x; d < dp1; d += 256) sums[d] = 0.;
     const int64_t tiles = (pairs + width - 1) / width;
@@ -103,21 +105,35 @@ momentum_kernel(const float* __restrict__ grad, float* __restrict__ buf, float* 
         const int64_t p0 = t * width;
         const int count = (int)((pairs - p0 < width ? pairs - p0 : width) * dp1);
         __syncthreads();                           // the tile is free
-        for (int e0 = threadIdx.x; e0 < count; e0 += 4 * 256) {
-            float g[4], m[4];
+        const float* gt = grad + p0 * dp1;
+        float* bt = buf + p0 * dp1;
+        auto one = [&](int e, float g, float m) {
+            g *= gs;
+            m = fmaf(1.f - momentum, g - m, m);
+            const int w = magic ? (int)divide((uint32_t)e, magic) : e;
+            tile[w * odd + e - w * dp1] = nesterov ? fmaf(momentum, m - g, g) : m;
+            return m;
+        };
+        // tiles start on multiples of 32 elements, so on 16 bytes; three vectors of both arrays in flight per thread
+        for (int e0 = threadIdx.x * 4; e0 < (count & ~3); e0 += 3 * 1024) {
+            float4 g[3], m[3];
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (e0 + k * 256 < count) { g[k] = grad[p0 * dp1 + e0 + k * 256] * gs; m[k] = buf[p0 * dp1 + e0 + k * 256]; }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int e = e0 + k * 256;
-                if (e < count) {
-                    m[k] = fmaf(1.f - momentum, g[k] - m[k], m[k]);
-                    buf[p0 * dp1 + e] = m[k];
-                    const int w = magic ? (int)divide((uint32_t)e, magic) : e;
-                    tile[w * odd + e - w * dp1] = nesterov ? fmaf(momentum, m[k] - g[k], g[k]) : m[k];
+            for (int k = 0; k < 3; ++k)
+                if (e0 + k * 1024 < (count & ~3)) {
+                    g[k] = *reinterpret_cast<const float4*>(gt + e0 + k * 1024);
+                    m[k] = *reinterpret_cast<const float4*>(bt + e0 + k * 1024);
                 }
+#pragma unroll
+            for (int k = 0; k < 3; ++k) {
+                const int e = e0 + k * 1024;
+                if (e < (count & ~3))
+                    *reinterpret_cast<float4*>(bt + e) = make_float4(one(e, g[k].x, m[k].x), one(e + 1, g[k].y, m[k].y),
+                                                                     one(e + 2, g[k].z, m[k].z), one(e + 3, g[k].w, m[k].w));
             }
+        }
+        if ((int)threadIdx.x < (count & 3)) {
+            const int e = (count & ~3) + threadIdx.x;
+            bt[e] = one(e, gt[e], bt[e]);
         }
         __syncthreads();
         const int n = count / dp1;
@@ -144,6 +160,7 @@ momentum_kernel(const float* __restrict__ grad, float* __restrict__ buf, float* 
 __global__ void __launch_bounds__(256)
 update_kernel(float* __restrict__ param, const float* __restrict__ o, int64_t pairs, int dp1, int width, uint32_t magic, float keep, float step) {
     extern __shared__ float tile[];
+    wait_for_previous();
     const int odd = dp1 | 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t tiles = (pairs + width - 1) / width;
     for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
@@ -160,19 +177,26 @@ update_kernel(float* __restrict__ param, const float* __restrict__ o, int64_t pa
                 if (lane + k * 32 < n) tile[(lane + k * 32) * odd + d] = x[k];
         }
         __syncthreads();
-        for (int e0 = threadIdx.x; e0 < count; e0 += 4 * 256) {
-            float p[4];
+        float* pt = param + p0 * dp1;
+        auto one = [&](int e, float p) {
+            const int w = magic ? (int)divide((uint32_t)e, magic) : e;
+            return fmaf(-step, tile[w * odd + e - w * dp1], keep * p);
+        };
+        for (int e0 = threadIdx.x * 4; e0 < (count & ~3); e0 += 3 * 1024) {
+            float4 p[3];
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (e0 + k * 256 < count) p[k] = param[p0 * dp1 + e0 + k * 256];
+            for (int k = 0; k < 3; ++k)
+                if (e0 + k * 1024 < (count & ~3)) p[k] = *reinterpret_cast<const float4*>(pt + e0 + k * 1024);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int e = e0 + k * 256;
-                if (e < count) {
-                    const int w = magic ? (int)divide((uint32_t)e, magic) : e;
-                    param[p0 * dp1 + e] = fmaf(-step, tile[w * odd + e - w * dp1], keep * p[k]);
-                }
+            for (int k = 0; k < 3; ++k) {
+                const int e = e0 + k * 1024;
+                if (e < (count & ~3))
+                    *reinterpret_cast<float4*>(pt + e) = make_float4(one(e, p[k].x), one(e + 1, p[k].y), one(e + 2, p[k].z), one(e + 3, p[k].w));
             }
+        }
+        if ((int)threadIdx.x < (count & 3)) {
+            const int e = (count & ~3) + threadIdx.x;
+            pt[e] = one(e, pt[e]);
         }
     }
 }
@@ -194,6 +218,8 @@ pack_rows_kernel(const T* __restrict__ g, const Plane pl, __half* __restrict__ x
     __shared__ double pow2;
     __shared__ float scales[2];
     const int64_t b = blockIdx.y;
+    let_next_start();
+    wait_for_previous();
     block_scales(partial + b * NORM_BLOCKS, eps, growth, &pow2, &scales[0], &scales[1]);
     __syncthreads();
     if (blockIdx.x == 0 && threadIdx.x == 0) { alpha[b] = scales[0]; alpha[sh.batch + b] = scales[1]; }
@@ -221,6 +247,8 @@ pack_turned_kernel(const T* __restrict__ g, const Plane pl, __half* __restrict__
     __shared__ double pow2;
     __shared__ float scales[2];
     const int64_t b = blockIdx.z, r0 = blockIdx.y * 32, c0 = blockIdx.x * 64;
+    let_next_start();
+    wait_for_previous();
     block_scales(partial + b * NORM_BLOCKS, eps, growth, &pow2, &scales[0], &scales[1]);
     __syncthreads();
     if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) { alpha[b] = scales[0]; alpha[sh.batch + b] = scales[1]; }
@@ -332,13 +360,13 @@ int pack_planes(const T* g, const Plane& pl, bool turned, char* ws, const Worksp
     const double* partial = reinterpret_cast<const double*>(ws + w.partial);
     if (turned) {
         const dim3 grid((unsigned)ceil_div(pl.cols, 64), (unsigned)ceil_div(pl.rows, 32), (unsigned)sh.batch);
-        pack_turned_kernel<T, PLANES><<<grid, 256, 0, s>>>(g, pl, x, alpha, partial, st.eps, st.growth, sh);
+        return check_cuda(launch_after(true, pack_turned_kernel<T, PLANES>, grid, dim3(256), 0, s, 0, g, pl, x, alpha, partial, st.eps, st.growth, sh));
     } else {
         // about four groups per thread, so that the norm's partial sums are not added up by too many blocks
         int64_t blocks = ceil_div((int64_t)sh.s * sh.ls / 8, 4 * 256);
-        pack_rows_kernel<T, PLANES><<<dim3((unsigned)blocks, (unsigned)sh.batch), 256, 0, s>>>(g, pl, x, alpha, partial, st.eps, st.growth, sh);
+        return check_cuda(launch_after(true, pack_rows_kernel<T, PLANES>, dim3((unsigned)blocks, (unsigned)sh.batch), dim3(256), 0, s, 0, g, pl, x, alpha,
+                                       partial, st.eps, st.growth, sh));
     }
-    return check_cuda(cudaGetLastError());
 }
 template <typename T>
 int pack(const T* g, const Plane& pl, bool turned, char* ws, const Workspace& w, const Shape& sh, const Steps& st, cudaStream_t s) {
@@ -447,8 +475,8 @@ int chebykan_muon_step(float* param, const float* grad, float* buf, void* worksp
     if ((rc = pack(u, Plane{in, out, out, 1, pairs}, in > out, ws, w, sh, st, s))) return rc;
     // the packed operands have taken u's place: O goes there
     if ((rc = run_steps(ws, w, sh, st, u, CHEBYKAN_DTYPE_FP32, in > out, status, s))) return rc;
-    update_kernel<<<(unsigned)(tiles < 148 * 8 ? tiles : 148 * 8), 256, smem, s>>>(param, u, pairs, dp1, width, magic, keep, step);
-    return check_cuda(cudaGetLastError());
+    return check_cuda(launch_after(true, update_kernel, dim3((unsigned)(tiles < 148 * 8 ? tiles : 148 * 8)), dim3(256), smem, s, 0, param, u, pairs, dp1,
+                                   width, magic, keep, step));
 }
 
 }  // extern "C"

@@ -198,7 +198,7 @@ int run(const Operands& o, __half* out, int64_t out_pitch, int64_t out_slab, Epi
         if (rc) return rc;
     }
     return gemm::launch<C, Epilogue<KIND, C::PLANES, OUT>>(ml, mr, gemm::tiles_of<C>(o.M, o.N, o.K, o.batch, KIND == GRAM || KIND == POLY), args,
-                                                          status, s);
+                                                          status, s, true);
 }
 
 // pairs where there are enough of their tiles to occupy every SM; single CTAs otherwise

@@ -121,7 +121,9 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io io, const Ge
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
 
-    // ---- norm (and momentum), then X_0 ----
+    wait_for_previous();
+
+    // ---- norm, then X_0 ----
     // elements in the order of the matrix's own columns, so that reads are coalesced whichever side is the shorter
     const int count = g.s * cols;
     auto place = [&](int e, int& r, int& c) {
@@ -419,7 +421,7 @@ Geometry geometry(const Shape& sh, bool tall) {
 }
 
 template <class Io, int PLANES>
-int launch(const Io& io, const Geometry& g, int64_t batch, const Steps& st, int32_t* status, cudaStream_t s) {
+int launch(const Io& io, const Geometry& g, int64_t batch, const Steps& st, int32_t* status, cudaStream_t s, bool after) {
     constexpr int MOST = 2 * (MAX_SLICE / 64) * PANEL + 128 * 132 * 4 + 2048;
     static bool ready[64] = {false};
     int dev = 0;
@@ -431,28 +433,21 @@ int launch(const Io& io, const Geometry& g, int64_t batch, const Steps& st, int3
         if (rc) return rc;
         ready[dev] = true;
     }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(batch * g.cluster)); cfg.blockDim = dim3(THREADS);
     // A CTA that waits for tensor memory may not hold up a cluster whose other CTAs are waited for: kernels with clusters
     // take more than half of an SM's shared memory, so that no two of them share one.
     size_t smem = (size_t)(g.x_bytes + g.a_bytes + 256 + 1024);
     if (g.cluster > 1 && smem < 116 * 1024) smem = 116 * 1024;
-    cfg.dynamicSmemBytes = smem; cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)g.cluster; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr; cfg.numAttrs = 1;
-    return check_cuda(cudaLaunchKernelEx(&cfg, kernel, io, g, st, status));
+    return check_cuda(launch_after(after, kernel, dim3((unsigned)(batch * g.cluster)), dim3(THREADS), smem, s, g.cluster, io, g, st, status));
 }
 template <class Io>
-int launch_planes(const Io& io, const Geometry& g, int64_t batch, const Steps& st, int32_t* status, cudaStream_t s) {
-    return g.planes == 2 ? launch<Io, 2>(io, g, batch, st, status, s) : launch<Io, 1>(io, g, batch, st, status, s);
+int launch_planes(const Io& io, const Geometry& g, int64_t batch, const Steps& st, int32_t* status, cudaStream_t s, bool after) {
+    return g.planes == 2 ? launch<Io, 2>(io, g, batch, st, status, s, after) : launch<Io, 1>(io, g, batch, st, status, s, after);
 }
 template <typename T>
 int orthogonalize_typed(const void* g, int64_t sb, int64_t sr, int64_t sc, void* out, int64_t m, int64_t n, const Shape& sh, const Steps& st,
                         int32_t* status, cudaStream_t s) {
     const OrthogonalizeIo<T> io{reinterpret_cast<const T*>(g), sb, sr, sc, reinterpret_cast<T*>(out), m, n};
-    return launch_planes(io, geometry(sh, m > n), sh.batch, st, status, s);
+    return launch_planes(io, geometry(sh, m > n), sh.batch, st, status, s, false);
 }
 }  // namespace
 
@@ -467,7 +462,7 @@ int launch_small_orthogonalize(const void* g, int dtype, int64_t sb, int64_t sr,
 int launch_small_update(float* param, const float* u, int64_t in, int64_t out, int dp1, float keep, float step, const Shape& sh,
                         const Steps& st, int32_t* status, cudaStream_t s) {
     const UpdateIo io{param, u, in, out, dp1, keep, step};
-    return launch_planes(io, geometry(sh, in > out), dp1, st, status, s);
+    return launch_planes(io, geometry(sh, in > out), dp1, st, status, s, true);
 }
 
 }  // namespace ns
