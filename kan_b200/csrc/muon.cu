@@ -423,7 +423,7 @@ int chebykan_orthogonalize(const void* g, int64_t stride_batch, int64_t stride_r
     const Steps st{(int)steps, a, b, c, eps, growth};
     cudaStream_t s = (cudaStream_t)stream;
     if (small_supported(sh))
-        return launch_small_orthogonalize(g, dtype, stride_batch, stride_row, stride_col, out, m, n, sh, st, status, s);
+        return launch_small(g, dtype, stride_batch, stride_row, stride_col, out, m, n, sh, st, status, s, false);
     const Workspace w = layout_of(sh, false);
     char* ws = reinterpret_cast<char*>(workspace);
     if (dtype == CHEBYKAN_DTYPE_FP32)
@@ -471,10 +471,14 @@ int chebykan_muon_step(float* param, const float* grad, float* buf, void* worksp
                                               small ? nullptr : reinterpret_cast<double*>(ws + w.partial));
     if ((rc = check_cuda(cudaGetLastError()))) return rc;
     const float keep = 1.f - lr * weight_decay, step = lr * update_scale;
-    if (small) return launch_small_update(param, u, in, out, dp1, keep, step, sh, st, status, s);
-    if ((rc = pack(u, Plane{in, out, out, 1, pairs}, in > out, ws, w, sh, st, s))) return rc;
-    // the packed operands have taken u's place: O goes there
-    if ((rc = run_steps(ws, w, sh, st, u, CHEBYKAN_DTYPE_FP32, in > out, status, s))) return rc;
+    // O takes u's place
+    if (small) {
+        rc = launch_small(u, CHEBYKAN_DTYPE_FP32, pairs, out, 1, u, in, out, sh, st, status, s, true);
+    } else {
+        if ((rc = pack(u, Plane{in, out, out, 1, pairs}, in > out, ws, w, sh, st, s))) return rc;
+        rc = run_steps(ws, w, sh, st, u, CHEBYKAN_DTYPE_FP32, in > out, status, s);
+    }
+    if (rc) return rc;
     return check_cuda(launch_after(true, update_kernel, dim3((unsigned)(tiles < 148 * 8 ? tiles : 148 * 8)), dim3(256), smem, s, 0, param, u, pairs, dp1,
                                    width, magic, keep, step));
 }

@@ -118,11 +118,9 @@ struct Steps {
     int growth;
 };
 bool small_supported(const Shape& sh);
-int launch_small_orthogonalize(const void* g, int dtype, int64_t sb, int64_t sr, int64_t sc, void* out, int64_t m, int64_t n, const Shape& sh,
-                               const Steps& st, int32_t* status, cudaStream_t s);
-// from the updates u[dp1][in][out] to param = keep * param - step * O
-int launch_small_update(float* param, const float* u, int64_t in, int64_t out, int dp1, float keep, float step, const Shape& sh,
-                        const Steps& st, int32_t* status, cudaStream_t s);
+// out may be g's own memory; after: see launch_after
+int launch_small(const void* g, int dtype, int64_t sb, int64_t sr, int64_t sc, void* out, int64_t m, int64_t n, const Shape& sh,
+                 const Steps& st, int32_t* status, cudaStream_t s, bool after);
 
 }  // namespace ns
 }  // namespace chebykan

@@ -1,5 +1,4 @@
-// Newton-Schulz orthogonalisation of small matrices (shorter side up to 128, longer up to 2048) in one launch, and with it
-// the weights' update of a Muon step.
+// Newton-Schulz orthogonalisation of small matrices (shorter side up to 128, longer up to 2048) in one launch.
 //
 // A matrix of this size is a few microseconds of reading and no arithmetic to speak of, but 3 * steps products that wait
 // for one another: as launches of their own each costs a launch, a pipeline's start and its drain (about 9 us; 150 us for
@@ -7,8 +6,8 @@
 // CTA holds a slice of up to 256 columns of X, rows padded to 128, as fp16 planes in 64-column panels of 128-byte swizzled
 // rows, which serve as they lie as both operands of A = X X^T (K-major) and as the right operand of P X (MN-major).  A and P
 // share one buffer: a row of P is formed from the same row of A by the thread that then overwrites it.
-//   A  = X X^T   each CTA over its columns; with several CTAs the fp32 partial results are added in rank order through
-//                distributed shared memory, each CTA reducing a band of rows, which the others then fetch
+//   A  = X X^T   each CTA over its columns; with several CTAs the fp32 partial results of a row go to the CTA
+//                that owns its band, which adds them in rank order and sends the finished row to all
 //   P  = a I + b A + c A A    every CTA for itself
 //   X' = P X     on the CTA's own columns
 // Products are tcgen05.mma (cta_group::1, M = 128) issued by one elected lane; between two of them all eight warps turn the
@@ -28,12 +27,16 @@ constexpr int PANEL = 128 * 128;                 // 128 rows of 64 fp16 columns
 constexpr int MAX_CLUSTER = 8, MAX_SLICE = 256;
 enum { ST_GRAM = 31, ST_POLY = 32, ST_APPLY = 33 };
 
+constexpr int MOST_SMEM = 224 * 1024;            // of operands and inbox; a little more for barriers and alignment
+
 struct Geometry {
     int s, l;
     int cluster, slice;      // CTAs per matrix, columns per CTA (a multiple of 16)
     int s16, acc;            // rows rounded up to 16; columns of one accumulator
     int planes, tall;
-    int x_bytes, a_bytes;    // shared memory: X planes, and the buffer of A / P / partial sums
+    int band;                // rows of A that a CTA of a cluster sums
+    int x_bytes, a_bytes;    // shared memory: X planes, and A / P with the inbox of partial sums
+    int inbox;               // its offset in the latter: behind A, or on A where there is no room for both
 };
 
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
@@ -45,10 +48,8 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-    return v;
+__device__ __forceinline__ void st_cluster_v4(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 __device__ __forceinline__ double ld_cluster_f64(uint32_t addr) {
     double v;
@@ -59,37 +60,15 @@ __device__ __forceinline__ double ld_cluster_f64(uint32_t addr) {
 __device__ __forceinline__ uint32_t chunk_at(int row, int col) {
     return (uint32_t)((col >> 6) * PANEL + row * 128 + ((((col & 63) >> 3) ^ (row & 7)) << 4));
 }
-// ---- the two uses: where elements come from and where results go.  Elements are addressed by their offset; what a batch of
-// them needs from memory is fetched before any of it is used, so that the latencies overlap. ----
 template <typename T>
-struct OrthogonalizeIo {
-    const T* g;
+struct Io {
+    const T* g;                   // element (b, r, c) at b*sb + r*sr + c*sc
     int64_t sb, sr, sc;
-    T* out;
+    T* out;                       // [batch][m][n]; may be g's own memory: a CTA has read its columns before it writes them
     int64_t m, n;
-    struct Old {};
-    __device__ __forceinline__ int64_t in_at(int64_t b, int64_t r, int64_t c) const { return b * sb + r * sr + c * sc; }
-    __device__ __forceinline__ float fetch(int64_t e) const { return (float)g[e]; }
-    __device__ __forceinline__ int64_t out_at(int64_t b, int64_t r, int64_t c) const { return (b * m + r) * n + c; }
-    __device__ __forceinline__ Old fetch_out(int64_t) const { return {}; }
-    __device__ __forceinline__ void store(int64_t e, const Old&, float v) const { out[e] = from_float<T>(v); }
 };
-struct UpdateIo {
-    float* param;
-    const float* u;
-    int64_t in, out;
-    int dp1;
-    float keep, step;
-    struct Old { float p; };
-    __device__ __forceinline__ int64_t in_at(int64_t b, int64_t r, int64_t c) const { return (b * in + r) * out + c; }
-    __device__ __forceinline__ float fetch(int64_t e) const { return u[e]; }
-    __device__ __forceinline__ int64_t out_at(int64_t b, int64_t r, int64_t c) const { return (r * out + c) * dp1 + b; }
-    __device__ __forceinline__ Old fetch_out(int64_t e) const { return {param[e]}; }
-    __device__ __forceinline__ void store(int64_t e, const Old& old, float v) const { param[e] = fmaf(-step, v, keep * old.p); }
-};
-
-template <class Io, int PLANES>
-__global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io io, const Geometry g, const Steps st, int32_t* status) {
+template <typename T, int PLANES>
+__global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io<T> io, const Geometry g, const Steps st, int32_t* status) {
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
@@ -121,6 +100,7 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io io, const Ge
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
 
+    let_next_start();
     wait_for_previous();
 
     // ---- norm, then X_0 ----
@@ -139,7 +119,7 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io io, const Ge
             for (int u = 0; u < U; ++u)
                 if (e0 + u * THREADS < count) {
                     place(e0 + u * THREADS, r[u], c[u]);
-                    v[u] = io.fetch(g.tall ? io.in_at(b, col0 + c[u], r[u]) : io.in_at(b, r[u], col0 + c[u]));
+                    v[u] = (float)io.g[b * io.sb + (g.tall ? (col0 + c[u]) * io.sr + r[u] * io.sc : r[u] * io.sr + (col0 + c[u]) * io.sc)];
                 }
 #pragma unroll
             for (int u = 0; u < U; ++u)
@@ -248,6 +228,7 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io io, const Ge
     };
 
     const int cols16 = (cols + 15) & ~15;
+    if (g.cluster > 1) { __syncwarp(); cluster_arrive(); }      // every wait below has its arrival a phase earlier
     for (int k = 0; k < st.n; ++k) {
         const float al = scales[k ? 1 : 0];
         // A = X X^T
@@ -265,87 +246,63 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io io, const Ge
                 }
             });
         } else {
-            // partial sums, rows (s16 + 4) floats apart: 16-byte accesses of 8 rows meet no bank twice
-            const int pitch = (g.s16 + 4) * 4;
+            // Each CTA sums a band of rows: the partial sums of a row go straight to the CTA that owns it, which adds them in
+            // rank order and sends the finished row to every CTA.  Remote stores need no answer, so an exchange costs its two
+            // barriers and little else; fetching from the others instead cost four times as much.
+            const int pitch = (g.s16 + 4) * 4;          // 16-byte accesses of 8 rows meet no bank twice
+            const uint32_t inbox = as + (uint32_t)g.inbox;
+            cluster_wait();                             // everybody's P (which an inbox may lie on) has been used
             columns(g.s16, [&](int c, const float (&x)[16]) {
                 if (row >= g.s) return;
+                const int owner = row / g.band;
+                const uint32_t to = mapa_cluster(inbox + (uint32_t)((rank * g.band + row - owner * g.band) * pitch + c * 4), (uint32_t)owner);
 #pragma unroll
-                for (int j = 0; j < 16; j += 4)
-                    *reinterpret_cast<float4*>(gen + g.x_bytes + row * pitch + (c + j) * 4) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+                for (int j = 0; j < 16; j += 4) st_cluster_v4(to + j * 4, __float_as_uint(x[j]), __float_as_uint(x[j + 1]), __float_as_uint(x[j + 2]), __float_as_uint(x[j + 3]));
             });
             tc_fence_before();
-            __syncthreads();
+            __syncwarp();
             cluster_sync_all();
-            // this CTA's band of rows, 8 columns per thread; a band of at most 64 rows x 16 groups is 2 per thread.  Rows
-            // from s to s16 become zero: the next product reads them, and the partial sums have been lying there.
+            // 8 columns per thread; a band of at most 64 rows x 16 groups is 2 per thread.  Rows from s to s16 become zero:
+            // the next product reads them.
             constexpr int W = 1024 / THREADS;
-            const int band = (g.s16 + g.cluster - 1) / g.cluster, r0 = rank * band;
-            const int nrow = g.s16 - r0 < band ? (g.s16 - r0 > 0 ? g.s16 - r0 : 0) : band;
-            const int groups = g.s16 / 8, todo = nrow * groups;
+            const int r0 = rank * g.band, groups = g.s16 / 8;
+            const int nrow = g.s16 - r0 < g.band ? (g.s16 - r0 > 0 ? g.s16 - r0 : 0) : g.band, todo = nrow * groups;
             float y[W][8];
 #pragma unroll
             for (int u = 0; u < W; ++u) {
                 const int w = threadIdx.x + u * THREADS;
-                if (w < todo) {
-                    const bool inside = r0 + w / groups < g.s;
-                    const uint32_t at = as + (uint32_t)((r0 + w / groups) * pitch + w % groups * 32);
-                    float4 v[MAX_CLUSTER][2];                        // all in flight at once, added in rank order
 #pragma unroll
-                    for (int p = 0; p < MAX_CLUSTER; ++p)
-                        if (p < g.cluster) {
-                            const uint32_t from = mapa_cluster(at, (uint32_t)p);
-                            v[p][0] = ld_cluster_f4(from);
-                            v[p][1] = ld_cluster_f4(from + 16);
-                        }
-                    float4 a0 = v[0][0], a1 = v[0][1];
+                for (int e = 0; e < 8; ++e) y[u][e] = 0.f;
+                if (w < todo && r0 + w / groups < g.s)
+                    for (int p = 0; p < g.cluster; ++p) {
+                        const float* from = reinterpret_cast<const float*>(gen + g.x_bytes + g.inbox + (p * g.band + w / groups) * pitch + w % groups * 32);
 #pragma unroll
-                    for (int p = 1; p < MAX_CLUSTER; ++p)
-                        if (p < g.cluster) {
-                            a0.x += v[p][0].x; a0.y += v[p][0].y; a0.z += v[p][0].z; a0.w += v[p][0].w;
-                            a1.x += v[p][1].x; a1.y += v[p][1].y; a1.z += v[p][1].z; a1.w += v[p][1].w;
-                        }
-                    const float sum8[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w};
+                        for (int e = 0; e < 8; ++e) y[u][e] += from[e];
+                    }
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) y[u][e] = inside ? sum8[e] * fa : 0.f;
-                }
+                for (int e = 0; e < 8; ++e) y[u][e] *= fa;
             }
-            cluster_sync_all();              // all partial sums are read: the buffer becomes A
+            if (g.inbox == 0) cluster_sync_all();       // every inbox is read: the buffer becomes A
 #pragma unroll
             for (int u = 0; u < W; ++u) {
                 const int w = threadIdx.x + u * THREADS;
-                if (w < todo) put(as, a_plane, r0 + w / groups, w % groups * 8, y[u]);
-            }
-            cluster_sync_all();
-            // the other bands; nobody overwrites its own before the barrier below is complete
-            {
-                constexpr int FETCH = 128 * 16 / THREADS;
-                float4 v[FETCH][PLANES];
-                uint32_t at[FETCH];
-#pragma unroll
-                for (int u = 0; u < FETCH; ++u) {
-                    const int w = threadIdx.x + u * THREADS, r = w / groups, owner = r / band;
-                    at[u] = 0;
-                    if (w < g.s16 * groups && owner != rank) {
-                        at[u] = as + chunk_at(r, w % groups * 8);
-                        const uint32_t from = mapa_cluster(at[u], (uint32_t)owner);
-#pragma unroll
-                        for (int p = 0; p < PLANES; ++p) v[u][p] = ld_cluster_f4(from + (uint32_t)(p * a_plane));
+                if (w < todo) {
+                    uint32_t hi[4], lo[4];
+                    split8<PLANES>(y[u], hi, lo);
+                    const uint32_t at = as + chunk_at(r0 + w / groups, w % groups * 8);
+                    for (int p = 0; p < g.cluster; ++p) {
+                        const uint32_t to = mapa_cluster(at, (uint32_t)p);
+                        st_cluster_v4(to, hi[0], hi[1], hi[2], hi[3]);
+                        if (PLANES == 2) st_cluster_v4(to + (uint32_t)a_plane, lo[0], lo[1], lo[2], lo[3]);
                     }
                 }
-#pragma unroll
-                for (int u = 0; u < FETCH; ++u)
-                    if (at[u] != 0)
-#pragma unroll
-                        for (int p = 0; p < PLANES; ++p)
-                            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at[u] + (uint32_t)(p * a_plane)), "f"(v[u][p].x), "f"(v[u][p].y),
-                                         "f"(v[u][p].z), "f"(v[u][p].w) : "memory");
             }
+            asm volatile("fence.proxy.async;" ::: "memory");
             __syncwarp();
-            cluster_arrive();
+            cluster_sync_all();
         }
         // P = a I + b A + c A A
         product(as, a_plane, as, a_plane, false, g.s16 / 16, g.s16, ST_POLY);
-        if (g.cluster > 1) cluster_wait();
         columns(g.s16, [&](int c, const float (&x)[16]) {
             if (row >= g.s) return;
 #pragma unroll
@@ -367,20 +324,18 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io io, const Ge
         });
         // X' = P X
         product(as, a_plane, xs, x_plane, true, g.s16 / 16, cols16, ST_APPLY);
+        if (g.cluster > 1) cluster_arrive();            // P has been used
         const bool last = k + 1 == st.n;
         const float fx = exp2f(-(float)P_EXP) * al / (last ? 1.f : scales[1]);
         columns(cols16, [&](int c, const float (&x)[16]) {
             if (row >= g.s) return;
             if (last) {
-                typename Io::Old old[16];
-                const int64_t at = g.tall ? io.out_at(b, col0 + c, row) : io.out_at(b, row, col0 + c);
-                const int64_t pitch = g.tall ? io.out_at(b, 1, 0) - io.out_at(b, 0, 0) : io.out_at(b, 0, 1) - io.out_at(b, 0, 0);
+                // tall: lanes (rows) are neighbours in memory, else the 16 columns are
+                T* to = io.out + b * io.m * io.n + (g.tall ? (int64_t)(col0 + c) * io.n + row : (int64_t)row * io.n + col0 + c);
+                const int64_t pitch = g.tall ? io.n : 1;
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
-                    if (c + e < cols) old[e] = io.fetch_out(at + e * pitch);
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    if (c + e < cols) io.store(at + e * pitch, old[e], x[e] * fx);
+                    if (c + e < cols) to[e * pitch] = from_float<T>(x[e] * fx);
             } else {
 #pragma unroll
                 for (int j = 0; j < 16; j += 8) {
@@ -395,7 +350,7 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io io, const Ge
 
     tc_fence_before();
     __syncthreads();
-    if (g.cluster > 1) cluster_sync_all();
+    if (g.cluster > 1) cluster_wait();                  // the last arrival's
     if (warp == 0) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(tmem_cols) : "memory");
@@ -415,19 +370,30 @@ Geometry geometry(const Shape& sh, bool tall) {
     g.acc = 32;
     while (g.acc < g.s16 || g.acc < g.slice) g.acc *= 2;
     g.x_bytes = sh.planes * (int)ceil_div(g.slice, 64) * PANEL;
-    const int operand = sh.planes * (int)ceil_div(g.s16, 64) * PANEL, partial = (int)round_up(128 * (g.s16 + 4) * 4, 1024);
-    g.a_bytes = g.cluster > 1 && partial > operand ? partial : operand;
+    const int operand = sh.planes * (int)ceil_div(g.s16, 64) * PANEL;
+    g.a_bytes = operand;
+    g.inbox = 0;
+    g.band = (int)ceil_div(g.s16, g.cluster);
+    if (g.cluster > 1) {
+        const int box = (int)round_up((int64_t)g.cluster * g.band * (g.s16 + 4) * 4, 1024);
+        if (g.x_bytes + operand + box <= MOST_SMEM) {
+            g.inbox = operand;
+            g.a_bytes = operand + box;
+        } else if (box > operand) {
+            g.a_bytes = box;
+        }
+    }
     return g;
 }
 
-template <class Io, int PLANES>
-int launch(const Io& io, const Geometry& g, int64_t batch, const Steps& st, int32_t* status, cudaStream_t s, bool after) {
-    constexpr int MOST = 2 * (MAX_SLICE / 64) * PANEL + 128 * 132 * 4 + 2048;
+template <typename T, int PLANES>
+int launch(const Io<T>& io, const Geometry& g, int64_t batch, const Steps& st, int32_t* status, cudaStream_t s, bool after) {
+    constexpr int MOST = MOST_SMEM + 2048;
     static bool ready[64] = {false};
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64) return CHEBYKAN_EINVAL;
-    auto kernel = small_kernel<Io, PLANES>;
+    auto kernel = small_kernel<T, PLANES>;
     if (!ready[dev]) {
         const int rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST));
         if (rc) return rc;
@@ -439,30 +405,22 @@ int launch(const Io& io, const Geometry& g, int64_t batch, const Steps& st, int3
     if (g.cluster > 1 && smem < 116 * 1024) smem = 116 * 1024;
     return check_cuda(launch_after(after, kernel, dim3((unsigned)(batch * g.cluster)), dim3(THREADS), smem, s, g.cluster, io, g, st, status));
 }
-template <class Io>
-int launch_planes(const Io& io, const Geometry& g, int64_t batch, const Steps& st, int32_t* status, cudaStream_t s, bool after) {
-    return g.planes == 2 ? launch<Io, 2>(io, g, batch, st, status, s, after) : launch<Io, 1>(io, g, batch, st, status, s, after);
-}
 template <typename T>
-int orthogonalize_typed(const void* g, int64_t sb, int64_t sr, int64_t sc, void* out, int64_t m, int64_t n, const Shape& sh, const Steps& st,
-                        int32_t* status, cudaStream_t s) {
-    const OrthogonalizeIo<T> io{reinterpret_cast<const T*>(g), sb, sr, sc, reinterpret_cast<T*>(out), m, n};
-    return launch_planes(io, geometry(sh, m > n), sh.batch, st, status, s, false);
+int launch_typed(const void* g, int64_t sb, int64_t sr, int64_t sc, void* out, int64_t m, int64_t n, const Shape& sh, const Steps& st,
+                 int32_t* status, cudaStream_t s, bool after) {
+    const Io<T> io{reinterpret_cast<const T*>(g), sb, sr, sc, reinterpret_cast<T*>(out), m, n};
+    const Geometry geo = geometry(sh, m > n);
+    return sh.planes == 2 ? launch<T, 2>(io, geo, sh.batch, st, status, s, after) : launch<T, 1>(io, geo, sh.batch, st, status, s, after);
 }
 }  // namespace
 
 bool small_supported(const Shape& sh) { return sh.s <= 128 && sh.l <= MAX_CLUSTER * MAX_SLICE; }
 
-int launch_small_orthogonalize(const void* g, int dtype, int64_t sb, int64_t sr, int64_t sc, void* out, int64_t m, int64_t n, const Shape& sh,
-                               const Steps& st, int32_t* status, cudaStream_t s) {
-    if (dtype == CHEBYKAN_DTYPE_FP32) return orthogonalize_typed<float>(g, sb, sr, sc, out, m, n, sh, st, status, s);
-    if (dtype == CHEBYKAN_DTYPE_BF16) return orthogonalize_typed<__nv_bfloat16>(g, sb, sr, sc, out, m, n, sh, st, status, s);
-    return orthogonalize_typed<__half>(g, sb, sr, sc, out, m, n, sh, st, status, s);
-}
-int launch_small_update(float* param, const float* u, int64_t in, int64_t out, int dp1, float keep, float step, const Shape& sh,
-                        const Steps& st, int32_t* status, cudaStream_t s) {
-    const UpdateIo io{param, u, in, out, dp1, keep, step};
-    return launch_planes(io, geometry(sh, in > out), dp1, st, status, s, true);
+int launch_small(const void* g, int dtype, int64_t sb, int64_t sr, int64_t sc, void* out, int64_t m, int64_t n, const Shape& sh,
+                 const Steps& st, int32_t* status, cudaStream_t s, bool after) {
+    if (dtype == CHEBYKAN_DTYPE_FP32) return launch_typed<float>(g, sb, sr, sc, out, m, n, sh, st, status, s, after);
+    if (dtype == CHEBYKAN_DTYPE_BF16) return launch_typed<__nv_bfloat16>(g, sb, sr, sc, out, m, n, sh, st, status, s, after);
+    return launch_typed<__half>(g, sb, sr, sc, out, m, n, sh, st, status, s, after);
 }
 
 }  // namespace ns
