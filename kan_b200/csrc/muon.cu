@@ -315,11 +315,26 @@ bool shape_fits(int64_t batch, int64_t m, int64_t n) {
 bool coefficients_ok(int64_t steps, float a, float b, float c, int* growth) {
     double top = 1., log_growth = 0.;
     for (int64_t k = 0; k < steps; ++k) {
+        // P = a + b y + c y^2 and the new value x P over y = x^2 in [0, top^2]: the ends, P's vertex, and where
+        // d(x P)/dx = a + 3 b y + 5 c y^2 vanishes
+        const double A = a, B = b, C = c, Y = top * top;
+        double at[5] = {0., Y, -1., -1., -1.};
+        if (C != 0.) {
+            at[2] = -B / (2 * C);
+            const double disc = 9 * B * B - 20 * A * C;
+            if (disc >= 0.) {
+                at[3] = (-3 * B + sqrt(disc)) / (10 * C);
+                at[4] = (-3 * B - sqrt(disc)) / (10 * C);
+            }
+        } else if (B != 0.) {
+            at[3] = -A / (3 * B);
+        }
         double next = 0., pmax = 0.;
-        for (int i = 0; i <= 512; ++i) {
-            const double x = top * i / 512., p = a + x * x * (b + c * x * x);
-            if (!(fabs(p * x) <= 7.) || !(fabs(p) <= 4000.)) return false;      // NaN included
-            next = fmax(next, fabs(p * x));
+        for (double y : at) {
+            if (!(y >= 0. && y <= Y)) continue;
+            const double p = A + y * (B + C * y), v = fabs(p) * sqrt(y);
+            if (!(v <= 7.) || !(fabs(p) <= 4000.)) return false;      // NaN included
+            next = fmax(next, v);
             pmax = fmax(pmax, fabs(p));
         }
         log_growth += log2(fmax(pmax, 1.));

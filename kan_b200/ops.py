@@ -6,6 +6,7 @@ sm_100a kernels of libchebykan_b200.so.  Nothing here computes on the CPU.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 
 import torch
@@ -481,43 +482,59 @@ def _require_any(t: torch.Tensor, name: str, dtype=None, device=None, contiguous
             raise RuntimeError(f"{name} must be 16-byte aligned")
 
 
-def _vector(t: torch.Tensor, name: str, size: int, device) -> int:
-    """Address of an fp32 vector of `size` elements."""
-    _require_any(t, name, torch.float32, device)
-    if t.numel() != size:
-        raise RuntimeError(f"{name} must have {size} elements")
-    return t.data_ptr()
+def _vector(t: torch.Tensor, name: str, size: int, idx: int) -> int:
+    """Address of an fp32 vector of `size` elements on device `idx`."""
+    if type(t) in _TENSORS and t.dtype is torch.float32 and t.get_device() == idx and t.numel() == size and t.is_contiguous():
+        p = t.data_ptr()
+        if not p & 15:
+            return p
+    _require_any(t, name, torch.float32, torch.device("cuda", idx))       # says what is wrong with it
+    raise RuntimeError(f"{name} must have {size} elements")
 
 
-def _result(out: torch.Tensor | None, shape, dtype, device) -> torch.Tensor:
-    """`out` checked, or a new tensor of `dtype`."""
+_TENSORS = (torch.Tensor, torch.nn.Parameter)
+
+
+def _result(out: torch.Tensor | None, shape, dtype, like: torch.Tensor) -> torch.Tensor:
+    """`out` checked, or a new tensor of `dtype` on the device of `like`."""
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    _require_any(out, "out", None, device)
+        return like.new_empty(shape, dtype=dtype)
+    _require_any(out, "out", None, like.device)
     if out.shape != shape:
         raise RuntimeError(f"out must have shape {list(shape)}")
     return out
 
 
-def _scratch(nbytes: int, what: str, device):
+@functools.lru_cache(maxsize=1024)
+def _bytes_for(query: str, *args) -> int:
+    """A workspace query of the library; its answers depend on the arguments alone."""
+    n = getattr(_lib.load(), query)(*args)
+    _lib.check(n, query)
+    return n
+
+
+def _scratch(nbytes: int, like: torch.Tensor):
     """(tensor, address) of a workspace; (None, None) for one of no bytes, which small calls then need not allocate."""
-    if nbytes <= 0:
-        _lib.check(nbytes, what)
+    if nbytes == 0:
         return None, None
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    ws = like.new_empty(nbytes, dtype=torch.uint8)
     return ws, ws.data_ptr()
 
 
-def _launch(name: str, device, *args) -> None:
-    """Library call `name`(*args, status, stream) on the current stream of `device`.  The smallest of these operators run
+_calls = {}        # (name, device index) -> (function, address of the device's status word)
+
+
+def _launch(name: str, idx: int, *args) -> None:
+    """Library call `name`(*args, status, stream) on the current stream of device `idx`.  The smallest of these operators run
     for a few microseconds, so the device is only switched where it has to be and no context manager is entered."""
-    idx = device.index
-    fn = getattr(_lib.load(), name)
+    call = _calls.get((name, idx))
+    if call is None:
+        call = _calls[name, idx] = getattr(_lib.load(), name), status_tensor(torch.device("cuda", idx)).data_ptr()
     if torch._C._cuda_getDevice() == idx and not _NVTX:
-        rc = fn(*args, status_tensor(device).data_ptr(), torch._C._cuda_getCurrentRawStream(idx))
+        rc = call[0](*args, call[1], torch._C._cuda_getCurrentRawStream(idx))
     else:
-        with _Range(name.replace("chebykan_", "chebykan.")), torch.cuda.device(device):
-            rc = fn(*args, status_tensor(device).data_ptr(), torch._C._cuda_getCurrentRawStream(idx))
+        with _Range(name.replace("chebykan_", "chebykan.")), torch.cuda.device(idx):
+            rc = call[0](*args, call[1], torch._C._cuda_getCurrentRawStream(idx))
     if rc:
         _lib.check(rc, name)
 
@@ -534,16 +551,16 @@ def orthogonalize(g: torch.Tensor, steps: int = 5, coefficients=NS_COEFFICIENTS,
     if g.dim() not in (2, 3):
         raise RuntimeError("g must have shape [m, n] or [batch, m, n]")
     dt = _dtype(g.dtype, "g")
-    out = _result(out, g.shape, g.dtype, g.device)
+    out = _result(out, g.shape, g.dtype, g)
     if out.dtype != g.dtype:
         raise RuntimeError("out must have the type of g")
     m = _mode(mode if mode is not None else ("tf32" if dt == _lib.DTYPE_BF16 else "fp32x3"))
     batch, rows, cols = (1, *g.shape) if g.dim() == 2 else g.shape
     sb, sr, sc = (0, *g.stride()) if g.dim() == 2 else g.stride()
-    ws_bytes = _lib.load().chebykan_orthogonalize_workspace_bytes(batch, rows, cols, m)
-    ws, ws_ptr = _scratch(ws_bytes, "chebykan_orthogonalize_workspace_bytes", g.device)
+    ws_bytes = _bytes_for("chebykan_orthogonalize_workspace_bytes", batch, rows, cols, m)
+    ws, ws_ptr = _scratch(ws_bytes, g)
     a, b, c = coefficients
-    _launch("chebykan_orthogonalize", g.device, g.data_ptr(), sb, sr, sc, dt, out.data_ptr(), ws_ptr, ws_bytes, batch, rows,
+    _launch("chebykan_orthogonalize", g.get_device(), g.data_ptr(), sb, sr, sc, dt, out.data_ptr(), ws_ptr, ws_bytes, batch, rows,
             cols, steps, a, b, c, eps, m)
     return out
 
@@ -578,10 +595,10 @@ def muon_step(param: torch.Tensor, grad: torch.Tensor, momentum_buffer: torch.Te
     n_in, n_out = param.shape[:2]
     degree = param.shape[2] - 1 if param.dim() == 3 else 0
     m = _mode(mode)
-    ws_bytes = _lib.load().chebykan_muon_workspace_bytes(n_in, n_out, degree, m)
-    ws, ws_ptr = _scratch(ws_bytes, "chebykan_muon_workspace_bytes", param.device)
+    ws_bytes = _bytes_for("chebykan_muon_workspace_bytes", n_in, n_out, degree, m)
+    ws, ws_ptr = _scratch(ws_bytes, param)
     a, b, c = coefficients
-    _launch("chebykan_muon_step", param.device, param.data_ptr(), grad.data_ptr(), momentum_buffer.data_ptr(), ws_ptr, ws_bytes,
+    _launch("chebykan_muon_step", param.get_device(), param.data_ptr(), grad.data_ptr(), momentum_buffer.data_ptr(), ws_ptr, ws_bytes,
             n_in, n_out, degree, lr, weight_decay, momentum, int(bool(nesterov)), muon_scale(param.shape, adjust), steps, a, b, c,
             eps, grad_scale, m)
 
@@ -632,6 +649,9 @@ def int8_basis(x: torch.Tensor, degree: int):
 
 def _require_int8(t: torch.Tensor, name: str, device=None) -> None:
     """int8 matrix on the GPU with adjacent columns; rows may be any distance apart."""
+    if (type(t) in _TENSORS and t.dtype is torch.int8 and t.is_cuda and (device is None or t.device == device) and t.dim() == 2
+            and t.is_contiguous() and not t.data_ptr() & 15):
+        return
     _require_any(t, name, torch.int8, device, contiguous=False)
     if t.dim() != 2:
         raise RuntimeError(f"{name} must be a matrix")
@@ -653,16 +673,17 @@ def int8_matmul(q: torch.Tensor, q_scale: torch.Tensor, wq: torch.Tensor, w_scal
     N = wq.shape[0]
     if wq.shape[1] != K:
         raise RuntimeError(f"q has {K} columns, wq {wq.shape[1]}")
-    device = q.device
-    qs, ws_, bs = (_vector(q_scale, "q_scale", M, device), _vector(w_scale, "w_scale", N, device),
-                   None if bias is None else _vector(bias, "bias", N, device))
-    out = _result(out, (M, N), out_dtype, device)
+    idx = q.get_device()
+    qs, ws_, bs = (_vector(q_scale, "q_scale", M, idx), _vector(w_scale, "w_scale", N, idx),
+                   None if bias is None else _vector(bias, "bias", N, idx))
+    out = _result(out, (M, N), out_dtype, q)
     # the pitch of a single row does not matter
-    ldq, ldw = (t.stride(0) if t.shape[0] > 1 else -(-K // 16) * 16 for t in (q, wq))
-    ws_bytes = _lib.load().chebykan_int8_matmul_workspace_bytes(M, N, K, ldq, ldw)
-    ws, ws_ptr = _scratch(ws_bytes, "chebykan_int8_matmul_workspace_bytes", device)
-    _launch("chebykan_int8_matmul", device, q.data_ptr(), ldq, qs, wq.data_ptr(), ldw, ws_, bs, out.data_ptr(),
-            _dtype(out.dtype, "out"), ws_ptr, ws_bytes, M, N, K)
+    ldq = q.stride(0) if M > 1 else -(-K // 16) * 16
+    ldw = wq.stride(0) if N > 1 else -(-K // 16) * 16
+    ws_bytes = _bytes_for("chebykan_int8_matmul_workspace_bytes", M, N, K, ldq, ldw)
+    ws, ws_ptr = _scratch(ws_bytes, q)
+    _launch("chebykan_int8_matmul", idx, q.data_ptr(), ldq, qs, wq.data_ptr(), ldw, ws_, bs, out.data_ptr(), _dtype(out.dtype, "out"),
+            ws_ptr, ws_bytes, M, N, K)
     return out
 
 
@@ -674,17 +695,17 @@ def int8_forward(x: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor, bias:
     if x.dim() != 2:
         raise RuntimeError("x must have shape [B, in]")
     B, n_in = x.shape
-    _require_any(wq, "wq", dtype=torch.int8, device=x.device)
+    _require_any(wq, "wq", torch.int8, x.device)
     if wq.dim() != 2 or wq.shape[1] != int8_width(n_in, degree):
         raise RuntimeError(f"wq must have shape [out, {int8_width(n_in, degree)}] for {n_in} inputs and degree {degree}")
     N = wq.shape[0]
-    device = x.device
-    ws_, bs = _vector(w_scale, "w_scale", N, device), None if bias is None else _vector(bias, "bias", N, device)
-    out = _result(out, (B, N), out_dtype, device)
-    ws_bytes = _lib.load().chebykan_int8_fwd_workspace_bytes(B, n_in, N, degree)
-    ws, ws_ptr = _scratch(ws_bytes, "chebykan_int8_fwd_workspace_bytes", device)
-    _launch("chebykan_int8_fwd", device, x.data_ptr(), _dtype(x.dtype, "x"), wq.data_ptr(), ws_, bs, out.data_ptr(),
-            _dtype(out.dtype, "out"), ws_ptr, ws_bytes, B, n_in, N, degree)
+    idx = x.get_device()
+    ws_, bs = _vector(w_scale, "w_scale", N, idx), None if bias is None else _vector(bias, "bias", N, idx)
+    out = _result(out, (B, N), out_dtype, x)
+    ws_bytes = _bytes_for("chebykan_int8_fwd_workspace_bytes", B, n_in, N, degree)
+    ws, ws_ptr = _scratch(ws_bytes, x)
+    _launch("chebykan_int8_fwd", idx, x.data_ptr(), _dtype(x.dtype, "x"), wq.data_ptr(), ws_, bs, out.data_ptr(), _dtype(out.dtype, "out"),
+            ws_ptr, ws_bytes, B, n_in, N, degree)
     return out
 
 
