@@ -11,19 +11,55 @@ namespace chebykan {
 namespace int8 {
 namespace {
 
-// tanh: a series below 0.3 (relative error below 1e-7), above it the exponential form, whose error is absolute: a row of
-// small inputs would show that, scaled up to 127 steps
-__device__ __forceinline__ float tanh_of(float x) {
-    if (fabsf(x) < 0.3f) {
-        const float z = x * x;
-        float p = -0.0088632355f;                 // -1382/155925
-        p = fmaf(p, z, 0.021869488f);             // 62/2835
-        p = fmaf(p, z, -0.053968254f);            // -17/315
-        p = fmaf(p, z, 0.13333333f);              // 2/15
-        p = fmaf(p, z, -0.33333333f);
-        return fmaf(x * z, p, x);
-    }
-    return tanh_fast(x);
+// ---- two fp32 values per instruction: the evaluation is bound by issue slots ----
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair(float x, float y) {
+    f32x2 d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
+    return d;
+}
+__device__ __forceinline__ void halves(f32x2 v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+// tanh of two values, 1 - 2 / (1 + 2^(2x log2 e)) as tanh_fast: about 2e-7 absolute.  SMALL adds an odd series below 0.3,
+// relative to 1e-7: a layer of degree 1 may see rows of small inputs only, which their scale blows up to 127 steps; from
+// degree 2 on every row's largest |T_d| is of the order of 1.
+template <bool SMALL>
+__device__ __forceinline__ f32x2 tanh2(f32x2 x) {
+    float z0, z1, e0, e1;
+    halves(mul2(x, pair(2.885390081777927f, 2.885390081777927f)), z0, z1);
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(z0));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(z1));
+    halves(add2(pair(e0, e1), pair(1.f, 1.f)), z0, z1);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(z0));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(z1));
+    const f32x2 t = fma2(pair(-2.f, -2.f), pair(e0, e1), pair(1.f, 1.f));
+    if (!SMALL) return t;
+    const f32x2 z = mul2(x, x);
+    f32x2 p = pair(-0.0088632355f, -0.0088632355f);           // -1382/155925
+    p = fma2(p, z, pair(0.021869488f, 0.021869488f));         // 62/2835
+    p = fma2(p, z, pair(-0.053968254f, -0.053968254f));       // -17/315
+    p = fma2(p, z, pair(0.13333333f, 0.13333333f));           // 2/15
+    p = fma2(p, z, pair(-0.33333333f, -0.33333333f));
+    float x0, x1, t0, t1, s0, s1;
+    halves(x, x0, x1);
+    halves(t, t0, t1);
+    halves(fma2(mul2(x, z), p, x), s0, s1);
+    return pair(fabsf(x0) < 0.3f ? s0 : t0, fabsf(x1) < 0.3f ? s1 : t1);
 }
 
 __device__ __forceinline__ float load1(const float* p) { return *p; }
@@ -48,18 +84,41 @@ __device__ __forceinline__ void load8(const T* p, int left, bool vec, float (&v)
 // round(v * inv) for four values with |v * inv| < 128, as bytes: adding 1.5 * 2^23 leaves the rounded integer (ties to
 // even) in the low bits of the sum, whose lowest bytes a byte permutation collects.  A conversion instruction per value
 // has a quarter of the throughput.
-__device__ __forceinline__ uint32_t quantise4(const float (&v)[8], int at, float inv) {
-    uint32_t b[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) b[e] = __float_as_uint(fmaf(v[at + e], inv, 12582912.f));
-    return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+__device__ __forceinline__ uint32_t quantise4(f32x2 v0, f32x2 v1, f32x2 inv) {
+    const f32x2 magic = pair(12582912.f, 12582912.f);
+    float b0, b1, b2, b3;
+    halves(fma2(v0, inv, magic), b0, b1);
+    halves(fma2(v1, inv, magic), b2, b3);
+    return __byte_perm(__byte_perm(__float_as_uint(b0), __float_as_uint(b1), 0x0040),
+                       __byte_perm(__float_as_uint(b2), __float_as_uint(b3), 0x0040), 0x5410);
 }
+
+// The recurrence as N_{d+1} = +-2t N_d + N_{d-1}: N_d = T_d up to a sign that goes + + - - with d, and no operand has to be
+// negated.  Steps to even degrees take -2t, to odd ones 2t.
+struct Recurrence {
+    f32x2 tt[4], ntt[4], a[4], b[4];
+    __device__ __forceinline__ void start(const f32x2 (&t)[4]) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            tt[e] = add2(t[e], t[e]);
+            ntt[e] = mul2(t[e], pair(-2.f, -2.f));
+            a[e] = t[e]; b[e] = pair(1.f, 1.f);
+        }
+    }
+    __device__ __forceinline__ void even() {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) b[e] = fma2(ntt[e], a[e], b[e]);
+    }
+    __device__ __forceinline__ void odd() {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] = fma2(tt[e], b[e], a[e]);
+    }
+};
 
 // A row per group of G threads, eight neighbouring inputs per thread and chunk.  The first pass finds the row's largest
 // |T_d|, the second evaluates the recurrence again and writes it; tanh, by far the dearer part, is kept in registers in
 // between (CHUNKS per thread; 0: rows longer than that evaluate it twice).
-// Bound by issue slots and memory alike: 32768 x 2048, degree 4 moves 268 MB in and 268 MB out.
-template <typename T, int G, int CHUNKS>
+template <typename T, int G, int CHUNKS, bool SMALL>
 __global__ void __launch_bounds__(256)
 basis_kernel(const T* __restrict__ x, int8_t* __restrict__ q, float* __restrict__ scale, int64_t B, int in, int pad, int deg, int vec) {
     constexpr int ROWS = 256 / G, KEEP = CHUNKS ? CHUNKS : 1;
@@ -70,37 +129,55 @@ basis_kernel(const T* __restrict__ x, int8_t* __restrict__ q, float* __restrict_
     const T* src = x + row * in;
     let_next_start();
     const int chunks = CHUNKS ? CHUNKS : (pad + 8 * G - 1) / (8 * G);
-    float t[KEEP][8];
+    f32x2 t[KEEP][4];
+    auto load = [&](int i0, f32x2 (&tc)[4]) {
+        float v[8];
+        load8(src + i0, in - i0, vec, v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) tc[e] = tanh2<SMALL>(pair(v[2 * e], v[2 * e + 1]));
+    };
     float top = 0.f;
-    bool nan = false;
+    f32x2 nan = pair(0.f, 0.f);                    // 0, or NaN once an input was one
 #pragma unroll
     for (int c = 0; c < chunks; ++c) {
-        float (&tc)[8] = t[CHUNKS ? c : 0];
+        f32x2 (&tc)[4] = t[CHUNKS ? c : 0];
         const int i0 = (c * G + lane) * 8;
         if (live && i0 < in) {
-            load8(src + i0, in - i0, vec, tc);
+            load(i0, tc);
+            Recurrence r;
+            r.start(tc);
+            float big[8];
+            auto look = [&](const f32x2 (&v)[4], bool first) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                tc[e] = tanh_of(tc[e]);
-                nan = nan || tc[e] != tc[e];
-            }
-            // from degree 2 on inputs past the row's end would count as T_2(0) = -1
-            const int n = in - i0 < 8 ? in - i0 : 8;
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (e < n) {
-                    float a = tc[e], b = 1.f;
-                    const float tt = 2.f * a;
-                    top = fmaxf(top, fabsf(a));
-                    for (int d = 2; d <= deg; ++d) {
-                        const float next = fmaf(tt, a, -b);
-                        b = a; a = next;
-                        top = fmaxf(top, fabsf(a));
-                    }
+                for (int e = 0; e < 4; ++e) {
+                    float v0, v1;
+                    halves(v[e], v0, v1);
+                    big[2 * e] = first ? fabsf(v0) : fmaxf(big[2 * e], fabsf(v0));
+                    big[2 * e + 1] = first ? fabsf(v1) : fmaxf(big[2 * e + 1], fabsf(v1));
                 }
+            };
+            look(r.a, true);
+            for (int d = 2; d <= deg; d += 2) {
+                r.even();
+                look(r.b, false);
+                if (d < deg) { r.odd(); look(r.a, false); }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) nan = fma2(tc[e], pair(0.f, 0.f), nan);
+            const int n = in - i0;
+            if (n >= 8) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = fmaxf(top, big[e]);
+            } else {                               // not the zeros past the row's end: T_2(0) = -1
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (e < n) top = fmaxf(top, big[e]);
+            }
         }
     }
-    if (nan) top = __int_as_float(0x7f800000);
+    float n0, n1;
+    halves(nan, n0, n1);
+    if (n0 != 0.f || n1 != 0.f || n0 != n0 || n1 != n1) top = __int_as_float(0x7f800000);
 #pragma unroll
     for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
     if (G > 32) {
@@ -115,37 +192,35 @@ basis_kernel(const T* __restrict__ x, int8_t* __restrict__ q, float* __restrict_
     const float s = bad ? __int_as_float(0x7fc00000) : __fdiv_rn(top, 127.f);
     const float inv = (bad || s == 0.f) ? 0.f : __fdiv_rn(1.f, s);
     if (lane == 0) scale[row] = s;
+    const f32x2 plus = pair(inv, inv), minus = pair(-inv, -inv);
     int8_t* dst = q + row * (int64_t)deg * pad;
 #pragma unroll
     for (int c = 0; c < chunks; ++c) {
-        float (&tc)[8] = t[CHUNKS ? c : 0];
+        f32x2 (&tc)[4] = t[CHUNKS ? c : 0];
         const int i0 = (c * G + lane) * 8;
         if (i0 >= pad) continue;
         const int n = in - i0;                     // inputs of the chunk; the rest of the padded row is zero
-        if (CHUNKS == 0 && n > 0) {
-            load8(src + i0, n, vec, tc);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) tc[e] = tanh_of(tc[e]);
-        }
-        float a[8], b[8];
+        if (CHUNKS == 0 && n > 0) load(i0, tc);
         uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
         if (bad) keep0 = keep1 = 0;
         else if (n < 8) {
             keep0 = n <= 0 ? 0 : (n >= 4 ? keep0 : (1u << (8 * n)) - 1u);
             keep1 = n <= 4 ? 0 : (1u << (8 * (n - 4))) - 1u;
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            a[e] = tc[e]; b[e] = 1.f;
-            tc[e] *= 2.f;
-        }
-        for (int d = 1; d <= deg; ++d) {
-            *reinterpret_cast<uint2*>(dst + (int64_t)(d - 1) * pad + i0) = make_uint2(quantise4(a, 0, inv) & keep0, quantise4(a, 4, inv) & keep1);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float next = fmaf(tc[e], a[e], -b[e]);
-                b[e] = a[e]; a[e] = next;
-            }
+        Recurrence r;
+        r.start(tc);
+        int8_t* to = dst + i0;
+        auto put = [&](const f32x2 (&v)[4], f32x2 by) {
+            *reinterpret_cast<uint2*>(to) = make_uint2(quantise4(v[0], v[1], by) & keep0, quantise4(v[2], v[3], by) & keep1);
+            to += pad;
+        };
+        // signs + + - - from degree 0 on
+        put(r.a, plus);
+        for (int d = 2; d <= deg; d += 2) {
+            const f32x2 by = d & 2 ? minus : plus;
+            r.even();
+            put(r.b, by);
+            if (d < deg) { r.odd(); put(r.a, by); }
         }
     }
 }
@@ -195,7 +270,8 @@ pack_kernel(const float* __restrict__ c, int8_t* __restrict__ wq, float* __restr
 template <typename T, int G, int CHUNKS>
 int launch_basis_one(const T* x, int8_t* q, float* scale, int64_t B, int64_t in, int64_t deg, cudaStream_t s) {
     const int vec = (in * sizeof(T)) % 16 == 0;
-    basis_kernel<T, G, CHUNKS><<<(unsigned)ceil_div(B, 256 / G), 256, 0, s>>>(x, q, scale, B, (int)in, (int)in_pad(in), (int)deg, vec);
+    auto kernel = deg == 1 ? basis_kernel<T, G, CHUNKS, true> : basis_kernel<T, G, CHUNKS, false>;
+    kernel<<<(unsigned)ceil_div(B, 256 / G), 256, 0, s>>>(x, q, scale, B, (int)in, (int)in_pad(in), (int)deg, vec);
     return check_cuda(cudaGetLastError());
 }
 // the narrowest group that needs at most two chunks per thread: more rows per block, fewer idle threads at a row's end
