@@ -70,29 +70,27 @@ struct Epilogue {
     static __device__ __forceinline__ void init(const Args& p, const Tiles& g, int b, int row0, int col0, float (&v)[NC], uint32_t buf) {
         const int lane = threadIdx.x & 31, ch = lane & 3;
         const __half* a = p.a + (int64_t)b * PLANES * p.slab + (int64_t)row0 * p.pitch + col0;
-        if (lane == 0) gemm::bulk_wait_read();
-        __syncwarp();
         auto place = [&](int plane, int r, int c) { return buf + (uint32_t)(plane * 2048 + r * 64 + ((c ^ ((r >> 1) & 3)) << 4)); };
-        uint4 x[2][4 * PLANES];
-        auto ask = [&](int c, uint4 (&to)[4 * PLANES]) {
+        uint4 x[NC / 32][4 * PLANES];           // the whole block in flight: v takes its registers block by block
+#pragma unroll
+        for (int c = 0; c < NC; c += 32)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int r = i * 8 + (lane >> 2);
                 const bool in = row0 + r < g.M && col0 + c + ch * 8 < g.N;
 #pragma unroll
                 for (int q = 0; q < PLANES; ++q)
-                    to[i * PLANES + q] = in ? *reinterpret_cast<const uint4*>(a + (int64_t)r * p.pitch + c + ch * 8 + q * p.slab) : make_uint4(0, 0, 0, 0);
+                    x[c / 32][i * PLANES + q] = in ? *reinterpret_cast<const uint4*>(a + (int64_t)r * p.pitch + c + ch * 8 + q * p.slab) : make_uint4(0, 0, 0, 0);
             }
-        };
-        ask(0, x[0]);
+        if (lane == 0) gemm::bulk_wait_read();
+        __syncwarp();
 #pragma unroll
         for (int c = 0; c < NC; c += 32) {
-            if (c + 32 < NC) ask(c + 32, x[(c / 32 + 1) & 1]);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int q = 0; q < PLANES; ++q) {
-                    const uint4 w = x[(c / 32) & 1][i * PLANES + q];
+                    const uint4 w = x[c / 32][i * PLANES + q];
                     gemm::st_shared_v4(place(q, i * 8 + (lane >> 2), ch), w.x, w.y, w.z, w.w);
                 }
             __syncwarp();
@@ -201,12 +199,20 @@ int run(const Operands& o, __half* out, int64_t out_pitch, int64_t out_slab, Epi
                                                           status, s, true);
 }
 
-// pairs where there are enough of their tiles to occupy every SM; single CTAs otherwise
+// Pairs or single CTAs, by the cycles that the waves of their tiles take per K block: a pair's 256 x 256 tile 512 (PP = 3:
+// 1536), which is the tensor pipe's; a CTA's 128 x 128 tile 512 (1250), which is shared memory's.  Pairs are the better the
+// more tiles there are; 16 + 16 rows of tiles of 777 x 1000 on 148 SMs run in one wave of pairs or two of single CTAs.
 template <int KIND, int PP, typename OUT>
 int choose(const Operands& o, __half* out, int64_t out_pitch, int64_t out_slab, EpiArgs& args, int32_t* status, cudaStream_t s) {
-    if (gemm::tiles_of<Shape2<KIND, PP, 2>>(o.M, o.N, o.K, o.batch, KIND == GRAM || KIND == POLY).total >= 74)
-        return run<KIND, PP, 2, OUT>(o, out, out_pitch, out_slab, args, status, s);
-    return run<KIND, PP, 1, OUT>(o, out, out_pitch, out_slab, args, status, s);
+    constexpr bool SYM = KIND == GRAM || KIND == POLY;
+    const int64_t pairs = gemm::tiles_of<Shape2<KIND, PP, 2>>(o.M, o.N, o.K, o.batch, SYM).total;
+    const int64_t singles = gemm::tiles_of<Shape2<KIND, PP, 1>>(o.M, o.N, o.K, o.batch, SYM).total;
+    const int64_t rest = pairs % 74;
+    // half tiles in the last wave (see Tiles) count as 0.6
+    const double pair_waves = pairs / 74 + (rest == 0 ? 0. : (pairs > 74 && 2 * rest <= 74 ? 0.6 : 1.));
+    const double pair_time = pair_waves * (PP == 3 ? 1536 : 512), single_time = (double)ceil_div(singles, 148) * (PP == 3 ? 1250 : 512);
+    return pair_time < single_time ? run<KIND, PP, 2, OUT>(o, out, out_pitch, out_slab, args, status, s)
+                                   : run<KIND, PP, 1, OUT>(o, out, out_pitch, out_slab, args, status, s);
 }
 template <int KIND, typename OUT = float>
 int product(const Shape& sh, const Operands& o, __half* out, int64_t out_pitch, int64_t out_slab, EpiArgs& args, int32_t* status, cudaStream_t s) {
