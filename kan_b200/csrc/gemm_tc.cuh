@@ -11,10 +11,10 @@
 // CG = 2: a pair of CTAs works on 256 rows with cta_group::2, each staging its own 128 rows of L and half of R's columns,
 // which halves R's traffic out of L2 and the shared-memory reads per MMA.  The even CTA's thread issues the MMAs.
 // PP = 3: both operands come as two fp16 planes (head and tail) and three products are summed.  The tensor pipe's fp32 sums
-// truncate, by about 2^-26 of the accumulator per MMA, so the accumulator of head x head takes two K blocks (8 MMAs) at a
-// time and the epilogue warps add these up in registers, rounding to nearest, while the MMAs of head x tail and tail x head
-// run; those are 2^11 times smaller and stay in an accumulator of their own for the whole of K.  (With one K block at a
-// time the addition, about 1250 cycles with its hand-overs, takes longer than the 8 MMAs that hide it.)
+// truncate, by about 2^-26 of the accumulator per MMA, so the accumulator of head x head takes one K block (4 MMAs) at a
+// time and the epilogue warps add the blocks up in registers, rounding to nearest (580 cycles), while the MMAs of
+// head x tail and tail x head run (1024); those are 2^11 times smaller and stay in an accumulator of their own for the
+// whole of K.  Two K blocks at a time were no faster and lost half a digit.
 // BN = 256 with pairs: per K block of 64 an SM's shared memory then takes 64 KB and gives 96 KB in the 1536 cycles of 12 MMAs
 // (104 of its 128 bytes per cycle); with BN = 128 it would be 160 bytes per cycle, which held the products at 3/4 of the
 // pipe's rate.
@@ -43,7 +43,6 @@ struct Config {
     static constexpr int L_PANEL = 128 * 128, R_PANEL = BN / CG * 128;
     static constexpr int STAGE = PLANES * (L_PANEL + R_PANEL);
     static constexpr int STAGES = (192 * 1024) / STAGE > 8 ? 8 : (192 * 1024) / STAGE;
-    static constexpr int CHUNK = 1;
     static constexpr int TMEM_COLS = 2 * BN;                   // two accumulators; PP = 3: heads, cross products
     static constexpr int BARS = 2 * STAGES + 5;
     static constexpr int OUT_OFFSET = STAGES * STAGE;          // 4 KB per epilogue warp
@@ -345,7 +344,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ C
                         next_stage();
                     }
                 } else {
-                    auto tails = [&](const Operand& o, int stage, bool start) {
+                    auto tails = [&](const Operand& o, bool start) {
                         if (elected) {
 #pragma unroll
                             for (int k = 0; k < 4; ++k) {
@@ -354,32 +353,21 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ C
                                 mma<C::KIND, CG>(cross, desc_from_words(la + L_TAIL, l_hi), desc_from_words(ra, r_hi), o.idesc, 1u);
                             }
                         }
-                        commit(empty(stage));
                     };
-                    for (int kb = 0; kb < g.nkb; kb += C::CHUNK) {
+                    for (int kb = 0; kb < g.nkb; ++kb) {
                         if (!wait_all(acc_empty(0), acc_ph ^ 1u, ST_MMA_ACC)) break;
                         if (!wait_all(full(s), ph, ST_MMA)) break;
-                        const Operand o0 = operands(kb);
-                        const int s0 = s;
-                        heads(o0, true);
-                        next_stage();
-                        const bool two = C::CHUNK == 2 && kb + 1 < g.nkb;
-                        Operand o1 = o0;
-                        const int s1 = s;
-                        if (two) {
-                            if (!wait_all(full(s), ph, ST_MMA)) break;
-                            o1 = operands(kb + 1);
-                            heads(o1, false);
-                            next_stage();
-                        }
+                        const Operand o = operands(kb);
+                        heads(o, true);
                         commit(acc_full(0));                       // added up while the cross products run
                         acc_ph ^= 1u;
                         if (kb == 0) {
                             if (!wait_all(acc_empty(1), cross_ph ^ 1u, ST_MMA_ACC)) break;
                             cross_ph ^= 1u;
                         }
-                        tails(o0, s0, kb == 0);
-                        if (two) tails(o1, s1, false);
+                        tails(o, kb == 0);
+                        commit(empty(s));
+                        next_stage();
                     }
                 }
                 if (!alive) break;
@@ -429,7 +417,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ C
                 const float scale = Epi::scale(args, b);
                 float v[EB];
                 if (Epi::INIT) Epi::init(args, g, b, row0, n0, v, buf);      // while the first MMAs run
-                for (int kb = 0; kb < g.nkb; kb += C::CHUNK) {
+                for (int kb = 0; kb < g.nkb; ++kb) {
                     if (!wait_all(acc_full(0), acc_ph)) break;
                     acc_ph ^= 1u;
                     if (!Epi::INIT && kb == 0) add_columns<EB, true>(tmem + lanes + (uint32_t)half0, scale, v);

@@ -306,6 +306,12 @@ bool product_ok(int64_t M, int64_t N, int64_t K, int64_t ldq, int64_t ldw) {
            ldq <= ((int64_t)1 << 32) && ldw <= ((int64_t)1 << 32);
 }
 int64_t a256(int64_t b) { return round_up(b, 256); }
+// rows worked on at a time: 1 GiB of quantised rows at most (4096 rows if they are longer than that)
+int64_t chunk_rows(int64_t B, int64_t K) {
+    int64_t rows = ((int64_t)1 << 30) / K / 256 * 256;
+    if (rows < 4096) rows = 4096;
+    return B < rows ? B : rows;
+}
 
 }  // namespace
 }  // namespace int8
@@ -358,8 +364,8 @@ int chebykan_int8_matmul(const int8_t* q, int64_t ldq, const float* q_scale, con
 
 int64_t chebykan_int8_fwd_workspace_bytes(int64_t B, int64_t in, int64_t out, int64_t deg) {
     if (!layer_ok(B, in, out, deg)) return CHEBYKAN_EINVAL;
-    const int64_t K = in_pad(in) * deg;
-    return a256(B * K) + a256(B * 4) + a256(matmul_workspace_bytes(B, out, K, K, K));
+    const int64_t K = in_pad(in) * deg, rows = chunk_rows(B, K);
+    return a256(rows * K) + a256(rows * 4);
 }
 
 int chebykan_int8_fwd(const void* x, int x_dtype, const int8_t* wq, const float* w_scale, const float* bias, void* y, int y_dtype,
@@ -374,13 +380,20 @@ int chebykan_int8_fwd(const void* x, int x_dtype, const int8_t* wq, const float*
     if (workspace_bytes < need) return CHEBYKAN_EWORKSPACE;
     int rc = check_device();
     if (rc) return rc;
-    const int64_t K = in_pad(in) * deg;
+    const int64_t K = in_pad(in) * deg, rows = chunk_rows(B, K);
+    const int64_t x_size = x_dtype == CHEBYKAN_DTYPE_FP32 ? 4 : 2, y_size = y_dtype == CHEBYKAN_DTYPE_FP32 ? 4 : 2;
     char* ws = reinterpret_cast<char*>(workspace);
     int8_t* q = reinterpret_cast<int8_t*>(ws);
-    float* scale = reinterpret_cast<float*>(ws + a256(B * K));
-    if ((rc = launch_basis(x, x_dtype, q, scale, B, in, deg, (cudaStream_t)stream))) return rc;
-    return launch_matmul({q, scale, wq, w_scale, bias, y, y_dtype, B, out, K, K, K}, ws + a256(B * K) + a256(B * 4), status,
-                         (cudaStream_t)stream, true);
+    float* scale = reinterpret_cast<float*>(ws + a256(rows * K));
+    for (int64_t r = 0; r < B; r += rows) {        // rows is a multiple of 256 where there is more than one turn: pointers stay aligned
+        const int64_t n = B - r < rows ? B - r : rows;
+        const char* xr = reinterpret_cast<const char*>(x) + r * in * x_size;
+        char* yr = reinterpret_cast<char*>(y) + r * out * y_size;
+        if ((rc = launch_basis(xr, x_dtype, q, scale, n, in, deg, (cudaStream_t)stream))) return rc;
+        // rows of q and wq are K bytes apart, a multiple of 16: the product needs no scratch
+        if ((rc = launch_matmul({q, scale, wq, w_scale, bias, yr, y_dtype, n, out, K, K, K}, nullptr, status, (cudaStream_t)stream, true))) return rc;
+    }
+    return CHEBYKAN_OK;
 }
 
 }  // extern "C"

@@ -179,11 +179,11 @@ struct Operands {
 
 // pairs: tiles of 256 x 256; single CTAs: 128 x 128
 template <int KIND, int PP, int CG>
-using Shape2 = gemm::Config<gemm::F16, PP, CG, CG == 2 ? 256 : 128, KIND == APPLY || KIND == LAST, KIND != GRAM, KIND == POLY>;
+using TileShape = gemm::Config<gemm::F16, PP, CG, CG == 2 ? 256 : 128, KIND == APPLY || KIND == LAST, KIND != GRAM, KIND == POLY>;
 
 template <int KIND, int PP, int CG, typename OUT>
 int run(const Operands& o, __half* out, int64_t out_pitch, int64_t out_slab, EpiArgs& args, int32_t* status, cudaStream_t s) {
-    using C = Shape2<KIND, PP, CG>;
+    using C = TileShape<KIND, PP, CG>;
     CUtensorMap ml, mr;
     const int64_t slabs = (int64_t)o.batch * C::PLANES;
     int rc = gemm::make_map(&ml, gemm::F16, o.left, o.K, o.M, slabs, 2 * o.pitch_l, 2 * o.slab_l, 64, C::LSYM ? 64 : 128);
@@ -205,8 +205,8 @@ int run(const Operands& o, __half* out, int64_t out_pitch, int64_t out_slab, Epi
 template <int KIND, int PP, typename OUT>
 int choose(const Operands& o, __half* out, int64_t out_pitch, int64_t out_slab, EpiArgs& args, int32_t* status, cudaStream_t s) {
     constexpr bool SYM = KIND == GRAM || KIND == POLY;
-    const int64_t pairs = gemm::tiles_of<Shape2<KIND, PP, 2>>(o.M, o.N, o.K, o.batch, SYM).total;
-    const int64_t singles = gemm::tiles_of<Shape2<KIND, PP, 1>>(o.M, o.N, o.K, o.batch, SYM).total;
+    const int64_t pairs = gemm::tiles_of<TileShape<KIND, PP, 2>>(o.M, o.N, o.K, o.batch, SYM).total;
+    const int64_t singles = gemm::tiles_of<TileShape<KIND, PP, 1>>(o.M, o.N, o.K, o.batch, SYM).total;
     const int64_t rest = pairs % 74;
     // half tiles in the last wave (see Tiles) count as 0.6
     const double pair_waves = pairs / 74 + (rest == 0 ? 0. : (pairs > 74 && 2 * rest <= 74 ? 0.6 : 1.));

@@ -11,8 +11,8 @@
 //   P  = a I + b A + c A A    every CTA for itself
 //   X' = P X     on the CTA's own columns
 // Products are tcgen05.mma (cta_group::1, M = 128) issued by one elected lane; between two of them all eight warps turn the
-// accumulator into the next operand.  Sums run over at most 256 columns, so the tensor pipe's truncation stays below 1e-6
-// (see gemm_tc.cuh).
+// accumulator into the next operand.  Heads are summed over at most 128 columns of K in an
+// accumulator: the tensor pipe's sums truncate (see gemm_tc.cuh).
 #include <math.h>
 #include "newton_schulz.cuh"
 #include "tc_common.cuh"
@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io<T> io, const
     const int cols = g.l - col0 < g.slice ? g.l - col0 : g.slice;               // at least 1
     const uint32_t xs = base, as = base + (uint32_t)g.x_bytes;
     const int x_plane = g.x_bytes / PLANES, a_plane = (g.s16 + 63) / 64 * PANEL;
-    const uint32_t tmem_cols = (uint32_t)(PLANES * g.acc);
+    const uint32_t tmem_cols = PLANES == 2 ? 512u : (uint32_t)g.acc;
 
     if (threadIdx.x == 0) {
         mbar_init(bar, 1);
@@ -167,8 +167,14 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io<T> io, const
     // ---- one product: operands in shared memory, rows of 128; returns with the accumulator readable by every thread ----
     const bool elected = warp == 0 && elect_one_sync();
     uint32_t phase = 0;
-    // left: K-major panels from `left`; right: the same, or X as [K][N].  ksteps of 16, n columns
+    // left: K-major panels from `left`; right: the same, or X as [K][N].  ksteps of 16, n columns.  PLANES = 2: heads in one
+    // accumulator or, to keep sums short (they truncate), the first and the second half of K in two; cross products in another
+    uint32_t second = 0, cross = 0;                     // their columns for the product at hand; 0: no second
     auto product = [&](uint32_t left, int left_plane, uint32_t right, int right_plane, bool mn, int ksteps, int n, int code) {
+        if (PLANES == 2) {
+            second = n <= 128 && ksteps > 4 ? 128u : 0u;
+            cross = 256u;
+        }
         fence_proxy_async_smem();
         tc_fence_before();
         __syncthreads();
@@ -181,15 +187,16 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io<T> io, const
             // MN-major: columns 64 apart are a panel apart
             const uint32_t r_hi = (uint32_t)(rd >> 32), r_tail = (uint32_t)(right_plane >> 4);
             const uint32_t r_lo = mn ? ((uint32_t)rd & 0xffffu) | ((uint32_t)(PANEL >> 4) << 16) : (uint32_t)rd;
+            const int turn = second ? (ksteps + 1) / 2 : ksteps;
 #pragma unroll 4
             for (int k = 0; k < ksteps; ++k) {
                 const uint32_t kmaj = (uint32_t)((k >> 2) * (PANEL >> 4) + (k & 3) * 2), kr = mn ? (uint32_t)(k * 128) : kmaj;
                 if (elected) {
                     const uint64_t l0 = desc_from_words(l_lo + kmaj, l_hi), r0 = desc_from_words(r_lo + kr, r_hi);
-                    umma<CHEBYKAN_MODE_BF16>(tmem, l0, r0, idesc, k > 0);
+                    umma<CHEBYKAN_MODE_BF16>(tmem + (k < turn ? 0u : second), l0, r0, idesc, k != 0 && k != turn);
                     if (PLANES == 2) {
-                        umma<CHEBYKAN_MODE_BF16>(tmem + g.acc, l0, desc_from_words(r_lo + kr + r_tail, r_hi), idesc, k > 0);
-                        umma<CHEBYKAN_MODE_BF16>(tmem + g.acc, desc_from_words(l_lo + kmaj + l_tail, l_hi), r0, idesc, 1u);
+                        umma<CHEBYKAN_MODE_BF16>(tmem + cross, l0, desc_from_words(r_lo + kr + r_tail, r_hi), idesc, k > 0);
+                        umma<CHEBYKAN_MODE_BF16>(tmem + cross, desc_from_words(l_lo + kmaj + l_tail, l_hi), r0, idesc, 1u);
                     }
                 }
             }
@@ -210,11 +217,17 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io<T> io, const
             uint32_t v[16], w[16];
             const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)c;
             tmem_ld16(at, v);
-            if (PLANES == 2) tmem_ld16(at + g.acc, w);
+            if (PLANES == 2) tmem_ld16(at + cross, w);
             tmem_ld_wait();
             float x[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) x[e] = __uint_as_float(v[e]) + (PLANES == 2 ? __uint_as_float(w[e]) : 0.f);
+            if (PLANES == 2 && second) {
+                tmem_ld16(at + second, v);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[e] += __uint_as_float(v[e]);
+            }
             f(c, x);
         }
     };

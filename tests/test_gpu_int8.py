@@ -158,6 +158,19 @@ def test_forward(B, n_in, n_out, degree):
     ops.check_status()
 
 
+def test_forward_of_more_rows_than_the_workspace_holds():
+    # 16 * 127 * 64 = 130048 bytes per quantised row: 8192 rows fill the workspace, the rest is a second turn
+    B, n_in, degree = 8500, 1024, 127
+    assert ops._lib.load().chebykan_int8_fwd_workspace_bytes(B, n_in, 8, degree) < 1.1e9
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    x = torch.randn(B, n_in, generator=gen, device="cuda").bfloat16()
+    wq = random_int8(8, ops.int8_width(n_in, degree), gen)
+    ws = torch.rand(8, generator=gen, device="cuda")
+    y = ops.int8_forward(x, wq, ws, None, degree, out_dtype=torch.bfloat16)
+    for rows in (slice(0, 40), slice(8180, 8210), slice(8470, 8500)):
+        assert torch.equal(y[rows], ops.int8_forward(x[rows].contiguous(), wq, ws, None, degree, out_dtype=torch.bfloat16))
+
+
 def test_forward_in_a_graph_on_another_stream():
     x, c, _ = make_case(200, 48, 72, 5, seed=6)
     wq, ws, bias = ops.int8_pack_coeffs(c.cuda())

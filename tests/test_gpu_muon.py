@@ -40,7 +40,7 @@ def randn(*shape, seed=0, dtype=torch.float32, scale=1.0):
 
 
 SHAPES = [(1, 1, 1), (1, 1, 37), (1, 37, 1), (2, 3, 5), (1, 10, 64), (33, 64, 64), (5, 784, 64), (3, 127, 129), (2, 128, 128), (2, 113, 2048), (2, 1300, 97), (40, 50, 400),
-          (1, 129, 257), (3, 777, 1000), (2, 256, 1100), (1, 1024, 1024), (1, 2048, 640)]
+          (1, 129, 257), (3, 777, 1000), (1, 20, 5000), (2, 3000, 100), (1, 1, 5000), (2, 256, 1100), (1, 1024, 1024), (1, 2048, 640)]
 
 
 @pytest.mark.parametrize("shape", SHAPES)
