@@ -327,13 +327,14 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ C
                     return Operand{(lmn ? l_mn : l_k) + off, (rmn ? r_mn : r_k) + off, lmn ? MNSTEP : KSTEP, rmn ? MNSTEP : KSTEP,
                                    idesc0 | (lmn ? 1u << 15 : 0u) | (rmn ? 1u << 16 : 0u)};
                 };
+                // operands are formed by the whole warp, in uniform registers, and only the MMA itself is one lane's
+                auto issue = [&](uint32_t dst, uint32_t l, uint32_t r, uint32_t id, uint32_t accumulate) {
+                    const uint64_t ld = desc_from_words(l, l_hi), rd = desc_from_words(r, r_hi);
+                    if (elected) mma<C::KIND, CG>(dst, ld, rd, id, accumulate);
+                };
                 auto heads = [&](const Operand& o, bool start) {
-                    if (elected) {
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            mma<C::KIND, CG>(d, desc_from_words(o.l + o.lstep * k, l_hi), desc_from_words(o.r + o.rstep * k, r_hi), o.idesc,
-                                             k ? 1u : (uint32_t)!start);
-                    }
+                    for (int k = 0; k < 4; ++k) issue(d, o.l + o.lstep * k, o.r + o.rstep * k, o.idesc, k ? 1u : (uint32_t)!start);
                 };
                 auto next_stage = [&]() { if (++s == S) { s = 0; ph ^= 1u; } };
                 if constexpr (C::PP == 1) {
@@ -345,13 +346,11 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ C
                     }
                 } else {
                     auto tails = [&](const Operand& o, bool start) {
-                        if (elected) {
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                const uint32_t la = o.l + o.lstep * k, ra = o.r + o.rstep * k;
-                                mma<C::KIND, CG>(cross, desc_from_words(la, l_hi), desc_from_words(ra + R_TAIL, r_hi), o.idesc, k ? 1u : (uint32_t)!start);
-                                mma<C::KIND, CG>(cross, desc_from_words(la + L_TAIL, l_hi), desc_from_words(ra, r_hi), o.idesc, 1u);
-                            }
+                        for (int k = 0; k < 4; ++k) {
+                            const uint32_t la = o.l + o.lstep * k, ra = o.r + o.rstep * k;
+                            issue(cross, la, ra + R_TAIL, o.idesc, k ? 1u : (uint32_t)!start);
+                            issue(cross, la + L_TAIL, ra, o.idesc, 1u);
                         }
                     };
                     for (int kb = 0; kb < g.nkb; ++kb) {
@@ -574,13 +573,12 @@ split_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ 
             if (!__all_sync(0xffffffffu, mbar_wait(full(s), ph, abort_flag, status, ST_MMA))) { alive = false; break; }
             tc_fence_after();
             const uint32_t off = (uint32_t)((s * C::STAGE) >> 4);
-            if (elected) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    mma<C::KIND, 1>(tmem, desc_from_words((uint32_t)l_desc + off + 2u * k, l_hi), desc_from_words((uint32_t)r_desc + off + 2u * k, r_hi),
-                                    C::IDESC, k ? 1u : (uint32_t)(kb != k_first));
-                umma_commit(empty(s));
+            for (int k = 0; k < 4; ++k) {
+                const uint64_t ld = desc_from_words((uint32_t)l_desc + off + 2u * k, l_hi), rd = desc_from_words((uint32_t)r_desc + off + 2u * k, r_hi);
+                if (elected) mma<C::KIND, 1>(tmem, ld, rd, C::IDESC, k ? 1u : (uint32_t)(kb != k_first));
             }
+            if (elected) umma_commit(empty(s));
             __syncwarp();
             if (++s == S) { s = 0; ph ^= 1u; }
         }

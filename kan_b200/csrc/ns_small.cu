@@ -10,7 +10,10 @@
 //                that owns its band, which adds them in rank order and sends the finished row to all
 //   P  = a I + b A + c A A    every CTA for itself
 //   X' = P X     on the CTA's own columns
-// Products are tcgen05.mma (cta_group::1, M = 128) issued by one elected lane; between two of them all eight warps turn the
+// With at most 64 rows (NARROW) the tail plane lies in the panels' second 64 rows.  Then M = 64, which halves what an MMA reads
+// of its left operand (a product of this size is bound by that: some 80 cycles per MMA of M = 128, whatever N), and one MMA
+// multiplies head x head and head x tail side by side, as N = 128.
+// Products are tcgen05.mma (cta_group::1) issued by one elected lane; between two of them all eight warps turn the
 // accumulator into the next operand.  Heads are summed over at most 128 columns of K in an
 // accumulator: the tensor pipe's sums truncate (see gemm_tc.cuh).
 #include <math.h>
@@ -67,7 +70,7 @@ struct Io {
     T* out;                       // [batch][m][n]; may be g's own memory: a CTA has read its columns before it writes them
     int64_t m, n;
 };
-template <typename T, int PLANES>
+template <typename T, int PLANES, bool NARROW>
 __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io<T> io, const Geometry g, const Steps st, int32_t* status) {
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -86,7 +89,8 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io<T> io, const
     const int col0 = rank * g.slice;
     const int cols = g.l - col0 < g.slice ? g.l - col0 : g.slice;               // at least 1
     const uint32_t xs = base, as = base + (uint32_t)g.x_bytes;
-    const int x_plane = g.x_bytes / PLANES, a_plane = (g.s16 + 63) / 64 * PANEL;
+    constexpr bool STACK = NARROW && PLANES == 2;
+    const int x_plane = NARROW ? PANEL / 2 : g.x_bytes / PLANES, a_plane = NARROW ? PANEL / 2 : (g.s16 + 63) / 64 * PANEL;
     const uint32_t tmem_cols = PLANES == 2 ? 512u : (uint32_t)g.acc;
 
     if (threadIdx.x == 0) {
@@ -110,24 +114,26 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io<T> io, const
         if (g.tall) { c = e / g.s; r = e - c * g.s; } else { r = e / cols; c = e - r * cols; }
     };
     constexpr int U = 8;
-    // f(place in the slice, value) for this thread's elements, U loads in flight
-    auto elements = [&](auto f) {
-        for (int e0 = threadIdx.x; e0 < count; e0 += U * THREADS) {
-            int r[U], c[U];
-            float v[U];
+    // this thread's next U elements from the e0-th on: their places in the slice and values, all loads in flight
+    struct Batch { int r[U], c[U]; float v[U]; };
+    auto fetch = [&](int e0, Batch& t) {
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (e0 + u * THREADS < count) {
-                    place(e0 + u * THREADS, r[u], c[u]);
-                    v[u] = (float)io.g[b * io.sb + (g.tall ? (col0 + c[u]) * io.sr + r[u] * io.sc : r[u] * io.sr + (col0 + c[u]) * io.sc)];
-                }
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (e0 + u * THREADS < count) f(r[u], c[u], v[u]);
-        }
+        for (int u = 0; u < U; ++u)
+            if (e0 + u * THREADS < count) {
+                place(e0 + u * THREADS, t.r[u], t.c[u]);
+                t.v[u] = (float)io.g[b * io.sb + (g.tall ? (col0 + t.c[u]) * io.sr + t.r[u] * io.sc : t.r[u] * io.sr + (col0 + t.c[u]) * io.sc)];
+            }
     };
     double sum = 0.;
-    elements([&](int, int, float v) { sum = fma((double)v, (double)v, sum); });
+    Batch batch;                                        // the first, kept for X_0: it is all there is of a matrix of 4096 elements
+    for (int e0 = threadIdx.x; e0 < count; e0 += U * THREADS) {
+        Batch t;
+        fetch(e0, t);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (e0 + u * THREADS < count) sum = fma((double)t.v[u], (double)t.v[u], sum);
+        if (e0 == (int)threadIdx.x) batch = t;
+    }
     for (uint32_t at = threadIdx.x * 16; at < (uint32_t)(g.x_bytes + g.a_bytes); at += THREADS * 16)
         *reinterpret_cast<uint4*>(gen + at) = make_uint4(0, 0, 0, 0);           // rows and columns of padding
 #pragma unroll
@@ -155,13 +161,18 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io<T> io, const
     const uint32_t tmem = *tmem_slot;
     {
         const double p2 = *pow2;
-        elements([&](int r, int c, float v) {
-            v = (float)((double)v * p2);
-            const __half hi = __float2half_rn(v);
-            uint8_t* at = gen + chunk_at(r, c) + 2 * (c & 7);
-            *reinterpret_cast<__half*>(at) = hi;
-            if (PLANES == 2) *reinterpret_cast<__half*>(at + x_plane) = __float2half_rn(v - __half2float(hi));
-        });
+        for (int e0 = threadIdx.x; e0 < count; e0 += U * THREADS) {
+            if (e0 != (int)threadIdx.x) fetch(e0, batch);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (e0 + u * THREADS < count) {
+                    const float v = (float)((double)batch.v[u] * p2);
+                    const __half hi = __float2half_rn(v);
+                    uint8_t* at = gen + chunk_at(batch.r[u], batch.c[u]) + 2 * (batch.c[u] & 7);
+                    *reinterpret_cast<__half*>(at) = hi;
+                    if (PLANES == 2) *reinterpret_cast<__half*>(at + x_plane) = __float2half_rn(v - __half2float(hi));
+                }
+        }
     }
 
     // ---- one product: operands in shared memory, rows of 128; returns with the accumulator readable by every thread ----
@@ -169,34 +180,51 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io<T> io, const
     uint32_t phase = 0;
     // left: K-major panels from `left`; right: the same, or X as [K][N].  ksteps of 16, n columns.  PLANES = 2: heads in one
     // accumulator or, to keep sums short (they truncate), the first and the second half of K in two; cross products in another
-    uint32_t second = 0, cross = 0;                     // their columns for the product at hand; 0: no second
+    uint32_t second = 0;                                // its column for the product at hand; 0: there is none
+    constexpr uint32_t CROSS = STACK ? 64 : 256;        // from a head column to its cross product's
     auto product = [&](uint32_t left, int left_plane, uint32_t right, int right_plane, bool mn, int ksteps, int n, int code) {
-        if (PLANES == 2) {
-            second = n <= 128 && ksteps > 4 ? 128u : 0u;
-            cross = 256u;
-        }
+        if (PLANES == 2) second = ksteps > 4 && (STACK || n <= 128) ? (STACK ? 256u : 128u) : 0u;
         fence_proxy_async_smem();
         tc_fence_before();
         __syncthreads();
         if (warp == 0) {
             tc_fence_after();
             // the whole warp runs the loop and one lane issues (see elect_one_sync); only the low words of descriptors move
-            const uint32_t idesc = (1u << 4) | ((mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+            auto idesc_of = [&](int cols) {
+                return (1u << 4) | ((mn ? 1u : 0u) << 16) | ((uint32_t)(cols >> 3) << 17) | ((NARROW ? 64u : 128u) >> 4 << 24);
+            };
             const uint64_t ld = make_smem_desc(left), rd = make_smem_desc(right);
             const uint32_t l_hi = (uint32_t)(ld >> 32), l_lo = (uint32_t)ld, l_tail = (uint32_t)(left_plane >> 4);
-            // MN-major: columns 64 apart are a panel apart
+            // MN-major: columns 64 apart are a panel apart; stacked, a panel's tails follow its heads half a panel on
             const uint32_t r_hi = (uint32_t)(rd >> 32), r_tail = (uint32_t)(right_plane >> 4);
-            const uint32_t r_lo = mn ? ((uint32_t)rd & 0xffffu) | ((uint32_t)(PANEL >> 4) << 16) : (uint32_t)rd;
+            const uint32_t box = (uint32_t)((STACK ? PANEL / 2 : PANEL) >> 4) << 16;
+            const uint32_t r_lo = mn ? ((uint32_t)rd & 0xffffu) | box : (uint32_t)rd;
             const int turn = second ? (ksteps + 1) / 2 : ksteps;
+            const int panels = STACK && mn ? (n + 63) / 64 : 1;
+            const uint32_t idesc = idesc_of(n), idesc64 = idesc_of(64), idesc128 = idesc_of(128), idesc256 = idesc_of(256);
 #pragma unroll 4
             for (int k = 0; k < ksteps; ++k) {
                 const uint32_t kmaj = (uint32_t)((k >> 2) * (PANEL >> 4) + (k & 3) * 2), kr = mn ? (uint32_t)(k * 128) : kmaj;
-                if (elected) {
-                    const uint64_t l0 = desc_from_words(l_lo + kmaj, l_hi), r0 = desc_from_words(r_lo + kr, r_hi);
-                    umma<CHEBYKAN_MODE_BF16>(tmem + (k < turn ? 0u : second), l0, r0, idesc, k != 0 && k != turn);
+                const uint32_t go = (uint32_t)(k != 0 && k != turn), d = tmem + (k < turn ? 0u : second);
+                // operands are formed by the whole warp, in uniform registers, and only the MMA itself is one lane's
+                auto issue = [&](uint32_t dst, uint32_t l, uint32_t r, uint32_t id, uint32_t accumulate) {
+                    const uint64_t ldesc = desc_from_words(l, l_hi), rdesc = desc_from_words(r, r_hi);
+                    if (elected) umma<CHEBYKAN_MODE_BF16>(dst, ldesc, rdesc, id, accumulate);
+                };
+                const uint32_t l0 = l_lo + kmaj, r0 = r_lo + kr;
+                if (STACK) {
+                    // [heads | cross] in 64 columns each, panel by panel
+                    for (int p = 0; p < panels; p += 2) {
+                        const uint32_t at = r0 + (uint32_t)(p * (PANEL >> 4)), dp = d + (uint32_t)(p * 128);
+                        issue(dp, l0, at, p + 1 < panels ? idesc256 : idesc128, go);
+                        issue(dp + 64, l0 + l_tail, at, idesc64, 1u);
+                        if (p + 1 < panels) issue(dp + 192, l0 + l_tail, at + (uint32_t)(PANEL >> 4), idesc64, 1u);
+                    }
+                } else {
+                    issue(d, l0, r0, idesc, go);
                     if (PLANES == 2) {
-                        umma<CHEBYKAN_MODE_BF16>(tmem + cross, l0, desc_from_words(r_lo + kr + r_tail, r_hi), idesc, k > 0);
-                        umma<CHEBYKAN_MODE_BF16>(tmem + cross, desc_from_words(l_lo + kmaj + l_tail, l_hi), r0, idesc, 1u);
+                        issue(tmem + CROSS, l0, r0 + r_tail, idesc, k > 0);
+                        issue(tmem + CROSS, l0 + l_tail, r0, idesc, 1u);
                     }
                 }
             }
@@ -209,24 +237,26 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io<T> io, const
         tc_fence_after();
     };
     const int q = warp & 3, group = warp >> 2;         // lanes of tensor memory, and which of the interleaved column groups
-    const int row = q * 32 + lane;
+    // M = 64 fills 16 lanes of each quarter
+    const int row = NARROW ? (lane < 16 ? q * 16 + lane : 1 << 20) : q * 32 + lane;
     // visits the accumulator's columns 16 at a time: f(first column, values)
     auto columns = [&](int n, auto f) {
         for (int c = group * 16; c < n; c += GROUPS * 16) {
             __syncwarp();                               // the loads are warp-collective
             uint32_t v[16], w[16];
-            const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)c;
+            const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(STACK ? (c >> 6) * 128 + (c & 63) : c);
             tmem_ld16(at, v);
-            if (PLANES == 2) tmem_ld16(at + cross, w);
+            if (PLANES == 2) tmem_ld16(at + CROSS, w);
             tmem_ld_wait();
             float x[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) x[e] = __uint_as_float(v[e]) + (PLANES == 2 ? __uint_as_float(w[e]) : 0.f);
             if (PLANES == 2 && second) {
                 tmem_ld16(at + second, v);
+                if (STACK) tmem_ld16(at + second + CROSS, w);
                 tmem_ld_wait();
 #pragma unroll
-                for (int e = 0; e < 16; ++e) x[e] += __uint_as_float(v[e]);
+                for (int e = 0; e < 16; ++e) x[e] += __uint_as_float(v[e]) + (STACK ? __uint_as_float(w[e]) : 0.f);
             }
             f(c, x);
         }
@@ -382,8 +412,9 @@ Geometry geometry(const Shape& sh, bool tall) {
     g.s16 = (int)round_up(sh.s, 16);
     g.acc = 32;
     while (g.acc < g.s16 || g.acc < g.slice) g.acc *= 2;
-    g.x_bytes = sh.planes * (int)ceil_div(g.slice, 64) * PANEL;
-    const int operand = sh.planes * (int)ceil_div(g.s16, 64) * PANEL;
+    const int layers = g.s16 <= 64 ? 1 : sh.planes;            // panels per 64 columns (see NARROW)
+    g.x_bytes = layers * (int)ceil_div(g.slice, 64) * PANEL;
+    const int operand = layers * (int)ceil_div(g.s16, 64) * PANEL;
     g.a_bytes = operand;
     g.inbox = 0;
     g.band = (int)ceil_div(g.s16, g.cluster);
@@ -399,14 +430,14 @@ Geometry geometry(const Shape& sh, bool tall) {
     return g;
 }
 
-template <typename T, int PLANES>
+template <typename T, int PLANES, bool NARROW>
 int launch(const Io<T>& io, const Geometry& g, int64_t batch, const Steps& st, int32_t* status, cudaStream_t s, bool after) {
     constexpr int MOST = MOST_SMEM + 2048;
     static bool ready[64] = {false};
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64) return CHEBYKAN_EINVAL;
-    auto kernel = small_kernel<T, PLANES>;
+    auto kernel = small_kernel<T, PLANES, NARROW>;
     if (!ready[dev]) {
         const int rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST));
         if (rc) return rc;
@@ -423,7 +454,9 @@ int launch_typed(const void* g, int64_t sb, int64_t sr, int64_t sc, void* out, i
                  int32_t* status, cudaStream_t s, bool after) {
     const Io<T> io{reinterpret_cast<const T*>(g), sb, sr, sc, reinterpret_cast<T*>(out), m, n};
     const Geometry geo = geometry(sh, m > n);
-    return sh.planes == 2 ? launch<T, 2>(io, geo, sh.batch, st, status, s, after) : launch<T, 1>(io, geo, sh.batch, st, status, s, after);
+    if (geo.s16 <= 64)
+        return sh.planes == 2 ? launch<T, 2, true>(io, geo, sh.batch, st, status, s, after) : launch<T, 1, true>(io, geo, sh.batch, st, status, s, after);
+    return sh.planes == 2 ? launch<T, 2, false>(io, geo, sh.batch, st, status, s, after) : launch<T, 1, false>(io, geo, sh.batch, st, status, s, after);
 }
 }  // namespace
 
