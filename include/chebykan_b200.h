@@ -318,7 +318,8 @@ int chebykan_adam_step_graph(float* param, const float* grad, float* exp_avg,
  *
  * chebykan_orthogonalize: out = NS(G) for `batch` matrices G[m][n], by `steps` Newton-Schulz steps
  *     X_0 = G / max(|G|_F, eps);   A = X X^T;   X <- (a I + b A + c A^2) X
- * run on the shorter side (a matrix with m > n is worked on as its transpose).  The usual coefficients
+ * run on the shorter side (a matrix with m > n is worked on as its transpose; up to 128 x 2048 in one launch
+ * and without a workspace).  The usual coefficients
  * (3.4445, -4.7750, 2.0315) push every singular value that is not tiny into about [0.7, 1.2] in five steps.
  *   - g: element (i, r, c) at g[i*stride_batch + r*stride_row + c*stride_col] (element strides, >= 0), of
  *     `dtype`; out: [batch][m][n] contiguous, of `dtype`; it may not overlap g;
@@ -366,7 +367,8 @@ int chebykan_muon_step(float* param, const float* grad, float* buf, void* worksp
  * chebykan_int8_matmul: y[r][o] = (sum_k q[r][k] wq[o][k]) * q_scale[r] * w_scale[o] + bias[o], y contiguous
  *     [M][N] of `dtype`, bias may be NULL.  Rows of q / wq are ldq / ldw bytes apart.  The integer sum is exact:
  *     K <= 131071.  Row strides that are not a multiple of 16 cost a padded copy in the workspace.
- * chebykan_int8_fwd: the two in a row; the quantised rows live in the workspace.
+ * chebykan_int8_fwd: the two in a row; the quantised rows live in the workspace, 1 GiB of them at a time
+ *     (4096 rows where a row is longer than 256 KiB).
  */
 int chebykan_int8_pack_coeffs(const float* coeffs, int8_t* wq, float* w_scale, float* bias, int64_t in,
                               int64_t out, int64_t deg, void* stream);

@@ -117,7 +117,8 @@ struct Recurrence {
 
 // A row per group of G threads, eight neighbouring inputs per thread and chunk.  The first pass finds the row's largest
 // |T_d|, the second evaluates the recurrence again and writes it; tanh, by far the dearer part, is kept in registers in
-// between (CHUNKS per thread; 0: rows longer than that evaluate it twice).
+// between (CHUNKS per thread; 0: rows longer than that evaluate it twice).  32768 x 2048, degree 4: 138 us, 3.9 TB/s; groups of
+// 128 or 64 threads with two or four chunks each took 146 and 181 us, five blocks per SM (by spilling) 181 us.
 template <typename T, int G, int CHUNKS, bool SMALL>
 __global__ void __launch_bounds__(256)
 basis_kernel(const T* __restrict__ x, int8_t* __restrict__ q, float* __restrict__ scale, int64_t B, int in, int pad, int deg, int vec) {
