@@ -217,3 +217,32 @@ def test_train_with_muon_then_serve_in_8_bits():
     with pytest.raises(RuntimeError, match="inference"):
         served(x.clone().requires_grad_(True))
     ops.check_status()
+
+
+def test_matmul_on_two_streams_at_once():
+    cases = [case(*s, seed=3) for s in [(300, 500, 640), (20, 64, 4096), (2500, 1100, 300), (1, 700, 999)]]
+    want = [ops.int8_matmul(*c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = []
+    for turn in range(4):
+        for i, c in enumerate(cases):
+            with torch.cuda.stream(streams[(i + turn) % 2]):
+                got.append((i, ops.int8_matmul(*c)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i]) for i, y in got)
+    ops.check_status()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_forward_unaligned_rows_and_half_inputs(dtype):
+    # rows of 7 or 13 values start on any 2- or 4-byte boundary
+    for B, n_in in [(1, 7), (64, 13), (999, 7), (10, 1001)]:
+        x, c, _ = make_case(B, n_in, 21, 3, seed=8)
+        x = x.to(dtype).cuda()
+        wq, ws, bias = ops.int8_pack_coeffs(c.cuda())
+        q, scale = ops.int8_basis(x, 3)
+        y = ops.int8_forward(x, wq, ws, bias, 3)
+        check_product(y, q, scale, wq, ws, bias)
+        assert torch.equal(q, ops.int8_basis(x.float(), 3)[0])         # the type is converted exactly

@@ -190,3 +190,66 @@ def test_muon_graphed_training_step_matches_the_eager_one():
         assert torch.equal(p, q)
     step.close()
     ops.check_status()
+
+
+@pytest.mark.parametrize("shape", [(2, 300, 520), (3, 60, 900)])
+def test_orthogonalize_captured_and_replayed(shape):
+    a, b = randn(*shape, seed=20), randn(*shape, seed=21)
+    want = [ops.orthogonalize(a), ops.orthogonalize(b)]
+    static = a.clone()
+    torch.cuda.synchronize()
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    outs = []
+    for g in graphs:                                   # two graphs that live side by side
+        with torch.cuda.graph(g):
+            outs.append(ops.orthogonalize(static))
+    graphs[0].replay()
+    graphs[1].replay()
+    assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[0])
+    static.copy_(b)
+    graphs[1].replay()
+    graphs[0].replay()
+    assert torch.equal(outs[0], want[1]) and torch.equal(outs[1], want[1])
+
+
+def test_calls_on_two_streams_at_once():
+    inputs = [randn(2, 400, 700, seed=s) for s in range(4)] + [randn(5, 50, 600, seed=s) for s in range(4)]
+    want = [ops.orthogonalize(g) for g in inputs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = {}
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for turn in range(3):
+        for i, g in enumerate(inputs):
+            with torch.cuda.stream(streams[(i + turn) % 2]):
+                got[i, turn] = ops.orthogonalize(g)
+    for s in streams:
+        torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i]) for (i, _), o in got.items())
+    ops.check_status()
+
+
+def test_muon_step_of_a_large_tensor_in_a_graph():
+    shape = (200, 260, 3)
+    p, g, m = randn(*shape, seed=22, scale=0.01), randn(*shape, seed=23), randn(*shape, seed=24)
+    q, n = p.clone(), m.clone()
+    ops.muon_step(p.clone(), g, m.clone(), lr=0.1)
+    torch.cuda.synchronize()
+    graph_ = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph_):
+        ops.muon_step(p, g, m, lr=0.1)
+    for _ in range(3):
+        graph_.replay()
+        ops.muon_step(q, g, n, lr=0.1)
+    assert torch.equal(p, q) and torch.equal(m, n)
+
+
+def test_every_degree_count_of_the_turning_kernels():
+    # deg + 1 from 1 to 128 through the tiles that turn [in*out][deg+1] into planes, with a ragged last tile
+    for dp1 in (1, 2, 3, 7, 8, 16, 31, 32, 33, 40, 41, 64, 65, 100, 127, 128):
+        shape = (9, 11, dp1)
+        p, g, m = randn(*shape, seed=25, scale=0.01), randn(*shape, seed=26), randn(*shape, seed=27)
+        want = muon64(p, g, m, 0.5, 0.1, 0.95, True, (11 / 9) ** 0.5)
+        ops.muon_step(p, g, m, lr=0.5)
+        assert rel(p, want[0]) <= FP32_TOL and rel(m, want[1]) <= 1e-6, dp1
