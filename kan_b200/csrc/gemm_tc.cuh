@@ -145,9 +145,10 @@ __device__ __forceinline__ void add_columns(uint32_t taddr, float scale, float (
         tmem_ld_wait();
         if (c + 1 < BN / 16) tmem_ld16(taddr + (c + 1) * 16, r[(c + 1) & 1]);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const float x = __uint_as_float(r[c & 1][e]);
-            v[c * 16 + e] = SET ? x * scale : fmaf(x, scale, v[c * 16 + e]);
+        for (int e = 0; e < 16; e += 2) {
+            const f32x2 x = pair_of(__uint_as_float(r[c & 1][e]), __uint_as_float(r[c & 1][e + 1]));
+            const int i = c * 16 + e;
+            halves(SET ? mul2(x, pair_of(scale, scale)) : fma2(x, pair_of(scale, scale), pair_of(v[i], v[i + 1])), v[i], v[i + 1]);
         }
     }
 }

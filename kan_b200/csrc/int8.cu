@@ -11,55 +11,31 @@ namespace chebykan {
 namespace int8 {
 namespace {
 
-// ---- two fp32 values per instruction: the evaluation is bound by issue slots ----
-typedef unsigned long long f32x2;
-__device__ __forceinline__ f32x2 pair(float x, float y) {
-    f32x2 d;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
-    return d;
-}
-__device__ __forceinline__ void halves(f32x2 v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-    f32x2 d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
-    f32x2 d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
-    f32x2 d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-
 // tanh of two values, 1 - 2 / (1 + 2^(2x log2 e)) as tanh_fast: about 2e-7 absolute.  SMALL adds an odd series below 0.3,
 // relative to 1e-7: a layer of degree 1 may see rows of small inputs only, which their scale blows up to 127 steps; from
 // degree 2 on every row's largest |T_d| is of the order of 1.
 template <bool SMALL>
 __device__ __forceinline__ f32x2 tanh2(f32x2 x) {
     float z0, z1, e0, e1;
-    halves(mul2(x, pair(2.885390081777927f, 2.885390081777927f)), z0, z1);
+    halves(mul2(x, pair_of(2.885390081777927f, 2.885390081777927f)), z0, z1);
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(z0));
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(z1));
-    halves(add2(pair(e0, e1), pair(1.f, 1.f)), z0, z1);
+    halves(add2(pair_of(e0, e1), pair_of(1.f, 1.f)), z0, z1);
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(z0));
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(z1));
-    const f32x2 t = fma2(pair(-2.f, -2.f), pair(e0, e1), pair(1.f, 1.f));
+    const f32x2 t = fma2(pair_of(-2.f, -2.f), pair_of(e0, e1), pair_of(1.f, 1.f));
     if (!SMALL) return t;
     const f32x2 z = mul2(x, x);
-    f32x2 p = pair(-0.0088632355f, -0.0088632355f);           // -1382/155925
-    p = fma2(p, z, pair(0.021869488f, 0.021869488f));         // 62/2835
-    p = fma2(p, z, pair(-0.053968254f, -0.053968254f));       // -17/315
-    p = fma2(p, z, pair(0.13333333f, 0.13333333f));           // 2/15
-    p = fma2(p, z, pair(-0.33333333f, -0.33333333f));
+    f32x2 p = pair_of(-0.0088632355f, -0.0088632355f);           // -1382/155925
+    p = fma2(p, z, pair_of(0.021869488f, 0.021869488f));         // 62/2835
+    p = fma2(p, z, pair_of(-0.053968254f, -0.053968254f));       // -17/315
+    p = fma2(p, z, pair_of(0.13333333f, 0.13333333f));           // 2/15
+    p = fma2(p, z, pair_of(-0.33333333f, -0.33333333f));
     float x0, x1, t0, t1, s0, s1;
     halves(x, x0, x1);
     halves(t, t0, t1);
     halves(fma2(mul2(x, z), p, x), s0, s1);
-    return pair(fabsf(x0) < 0.3f ? s0 : t0, fabsf(x1) < 0.3f ? s1 : t1);
+    return pair_of(fabsf(x0) < 0.3f ? s0 : t0, fabsf(x1) < 0.3f ? s1 : t1);
 }
 
 __device__ __forceinline__ float load1(const float* p) { return *p; }
@@ -85,7 +61,7 @@ __device__ __forceinline__ void load8(const T* p, int left, bool vec, float (&v)
 // even) in the low bits of the sum, whose lowest bytes a byte permutation collects.  A conversion instruction per value
 // has a quarter of the throughput.
 __device__ __forceinline__ uint32_t quantise4(f32x2 v0, f32x2 v1, f32x2 inv) {
-    const f32x2 magic = pair(12582912.f, 12582912.f);
+    const f32x2 magic = pair_of(12582912.f, 12582912.f);
     float b0, b1, b2, b3;
     halves(fma2(v0, inv, magic), b0, b1);
     halves(fma2(v1, inv, magic), b2, b3);
@@ -101,8 +77,8 @@ struct Recurrence {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             tt[e] = add2(t[e], t[e]);
-            ntt[e] = mul2(t[e], pair(-2.f, -2.f));
-            a[e] = t[e]; b[e] = pair(1.f, 1.f);
+            ntt[e] = mul2(t[e], pair_of(-2.f, -2.f));
+            a[e] = t[e]; b[e] = pair_of(1.f, 1.f);
         }
     }
     __device__ __forceinline__ void even() {
@@ -135,10 +111,10 @@ basis_kernel(const T* __restrict__ x, int8_t* __restrict__ q, float* __restrict_
         float v[8];
         load8(src + i0, in - i0, vec, v);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) tc[e] = tanh2<SMALL>(pair(v[2 * e], v[2 * e + 1]));
+        for (int e = 0; e < 4; ++e) tc[e] = tanh2<SMALL>(pair_of(v[2 * e], v[2 * e + 1]));
     };
     float top = 0.f;
-    f32x2 nan = pair(0.f, 0.f);                    // 0, or NaN once an input was one
+    f32x2 nan = pair_of(0.f, 0.f);                    // 0, or NaN once an input was one
 #pragma unroll
     for (int c = 0; c < chunks; ++c) {
         f32x2 (&tc)[4] = t[CHUNKS ? c : 0];
@@ -164,7 +140,7 @@ basis_kernel(const T* __restrict__ x, int8_t* __restrict__ q, float* __restrict_
                 if (d < deg) { r.odd(); look(r.a, false); }
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) nan = fma2(tc[e], pair(0.f, 0.f), nan);
+            for (int e = 0; e < 4; ++e) nan = fma2(tc[e], pair_of(0.f, 0.f), nan);
             const int n = in - i0;
             if (n >= 8) {
 #pragma unroll
@@ -193,7 +169,7 @@ basis_kernel(const T* __restrict__ x, int8_t* __restrict__ q, float* __restrict_
     const float s = bad ? __int_as_float(0x7fc00000) : __fdiv_rn(top, 127.f);
     const float inv = (bad || s == 0.f) ? 0.f : __fdiv_rn(1.f, s);
     if (lane == 0) scale[row] = s;
-    const f32x2 plus = pair(inv, inv), minus = pair(-inv, -inv);
+    const f32x2 plus = pair_of(inv, inv), minus = pair_of(-inv, -inv);
     int8_t* dst = q + row * (int64_t)deg * pad;
 #pragma unroll
     for (int c = 0; c < chunks; ++c) {

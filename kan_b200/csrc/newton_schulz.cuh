@@ -50,16 +50,16 @@ __device__ __forceinline__ void split8(const float (&x)[8], uint32_t (&hi)[4], u
         for (int e = 0; e < 4; ++e) hi[e] = half2_bits(x[2 * e], x[2 * e + 1]);
         return;
     }
-    float h[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const float c = __fmul_rn(x[e], 8193.f);
-        h[e] = __fsub_rn(c, __fsub_rn(c, x[e]));
-    }
+    const f32x2 k = pair_of(8193.f, 8193.f), minus = pair_of(-1.f, -1.f);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        hi[e] = half2_bits(h[2 * e], h[2 * e + 1]);
-        lo[e] = half2_bits(x[2 * e] - h[2 * e], x[2 * e + 1] - h[2 * e + 1]);
+        const f32x2 v = pair_of(x[2 * e], x[2 * e + 1]), c = mul2(v, k);
+        const f32x2 h = fma2(fma2(v, minus, c), minus, c), t = fma2(h, minus, v);      // c - (c - v), v - h
+        float a, b;
+        halves(h, a, b);
+        hi[e] = half2_bits(a, b);
+        halves(t, a, b);
+        lo[e] = half2_bits(a, b);
     }
 }
 // values of eight packed heads (and tails)

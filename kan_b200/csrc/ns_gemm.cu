@@ -58,10 +58,13 @@ struct Epilogue {
     static __device__ __forceinline__ void addend(const Args& p, int row, int col0, const uint32_t (&ah)[4], const uint32_t (&al)[4], float (&v)[8]) {
         float a[8];
         join8<PLANES>(ah, al, a);
+        const float by = p.cb * exp2f((float)(P_EXP - A_EXP));
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            v[e] = p.cb * exp2f((float)(P_EXP - A_EXP)) * a[e];
-            if (col0 + e == row) v[e] += p.ca * exp2f((float)P_EXP);
+        for (int e = 0; e < 8; e += 2) halves(mul2(pair_of(a[e], a[e + 1]), pair_of(by, by)), v[e], v[e + 1]);
+        if (row >= col0 && row < col0 + 8) {                // the diagonal passes through
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (col0 + e == row) v[e] += p.ca * exp2f((float)P_EXP);
         }
     }
     static constexpr bool INIT = KIND == POLY;

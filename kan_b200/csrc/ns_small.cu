@@ -251,14 +251,20 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io<T> io, const
             if (PLANES == 2) tmem_ld16(at + CROSS, w);
             tmem_ld_wait();
             float x[16];
+            auto plus = [&](const uint32_t (&y)[16]) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) x[e] = __uint_as_float(v[e]) + (PLANES == 2 ? __uint_as_float(w[e]) : 0.f);
+                for (int e = 0; e < 16; e += 2)
+                    halves(add2(pair_of(x[e], x[e + 1]), pair_of(__uint_as_float(y[e]), __uint_as_float(y[e + 1]))), x[e], x[e + 1]);
+            };
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[e] = __uint_as_float(v[e]);
+            if (PLANES == 2) plus(w);
             if (PLANES == 2 && second) {
                 tmem_ld16(at + second, v);
                 if (STACK) tmem_ld16(at + second + CROSS, w);
                 tmem_ld_wait();
-#pragma unroll
-                for (int e = 0; e < 16; ++e) x[e] += __uint_as_float(v[e]) + (STACK ? __uint_as_float(w[e]) : 0.f);
+                plus(v);
+                if (STACK) plus(w);
             }
             f(c, x);
         }
@@ -271,6 +277,13 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io<T> io, const
         if (PLANES == 2)
             asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at + (uint32_t)plane), "r"(lo[0]), "r"(lo[1]), "r"(lo[2]), "r"(lo[3]) : "memory");
     };
+
+    auto times = [&](const float (&x)[16], int j, float by, float (&y)[8]) {
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) halves(mul2(pair_of(x[j + e], x[j + e + 1]), pair_of(by, by)), y[e], y[e + 1]);
+    };
+    // P's coefficients in the units of the stored numbers
+    const float pa = st.a * exp2f((float)P_EXP), pb = st.b * exp2f((float)(P_EXP - A_EXP)), pc = st.c * exp2f((float)(P_EXP - 2 * A_EXP));
 
     const int cols16 = (cols + 15) & ~15;
     if (g.cluster > 1) { __syncwarp(); cluster_arrive(); }      // every wait below has its arrival a phase earlier
@@ -285,8 +298,7 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io<T> io, const
 #pragma unroll
                 for (int j = 0; j < 16; j += 8) {
                     float y[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) y[e] = x[j + e] * fa;
+                    times(x, j, fa, y);
                     put(as, a_plane, row, c + j, y);
                 }
             });
@@ -359,10 +371,13 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io<T> io, const
                     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(t[0]), "=r"(t[1]), "=r"(t[2]), "=r"(t[3]) : "r"(at + (uint32_t)a_plane));
                 float a[8], y[8];
                 join8<PLANES>(h, t, a);
+                times(x, j, pc, y);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    y[e] = fmaf(st.b * exp2f((float)(P_EXP - A_EXP)), a[e], x[j + e] * (st.c * exp2f((float)(P_EXP - 2 * A_EXP))));
-                    if (c + j + e == row) y[e] += st.a * exp2f((float)P_EXP);
+                for (int e = 0; e < 8; e += 2) halves(fma2(pair_of(a[e], a[e + 1]), pair_of(pb, pb), pair_of(y[e], y[e + 1])), y[e], y[e + 1]);
+                if (row >= c + j && row < c + j + 8) {          // the diagonal passes through
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (c + j + e == row) y[e] += pa;
                 }
                 put(as, a_plane, row, c + j, y);
             }
@@ -385,8 +400,7 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const Io<T> io, const
 #pragma unroll
                 for (int j = 0; j < 16; j += 8) {
                     float y[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) y[e] = x[j + e] * fx;
+                    times(x, j, fx, y);
                     put(xs, x_plane, row, c + j, y);
                 }
             }
