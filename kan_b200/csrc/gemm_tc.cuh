@@ -168,20 +168,29 @@ __device__ __forceinline__ void store_rows(uint32_t buf, const OUT (&v)[32], OUT
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) st_shared_v4(place(lane, c), w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
     __syncwarp();
+    if (vec && cols >= 32) {
 #pragma unroll
-    for (int i = 0; i < CHUNKS; ++i) {
-        const int r = (i * 32 + lane) / CHUNKS, c = (i * 32 + lane) % CHUNKS;
-        alignas(16) uint32_t x[4];
-        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(place(r, c)));
-        if (r < rows) {
-            OUT* to = dst + r * pitch + c * V;
-            if (vec && c * V + V <= cols) {
-                *reinterpret_cast<uint4*>(to) = make_uint4(x[0], x[1], x[2], x[3]);
+        for (int i = 0; i < CHUNKS; ++i) {
+            const int r = (i * 32 + lane) / CHUNKS, c = (i * 32 + lane) % CHUNKS;
+            uint32_t x[4];
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(place(r, c)));
+            if (r < rows) *reinterpret_cast<uint4*>(dst + r * pitch + c * V) = make_uint4(x[0], x[1], x[2], x[3]);
+        }
+    } else {
+        // ragged right edge, or rows that are not 16 bytes apart: a column per lane, row after row
+        const uint32_t in = (uint32_t)(lane % V * (int)sizeof(OUT));
+        OUT* to = dst + lane;
+#pragma unroll 8
+        for (int r = 0; r < 32; ++r) {
+            const uint32_t at = place(r, lane / V) + in;
+            if constexpr (sizeof(OUT) == 4) {
+                uint32_t x;
+                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x) : "r"(at));
+                if (r < rows && lane < cols) *reinterpret_cast<uint32_t*>(to + r * pitch) = x;
             } else {
-                const OUT* e = reinterpret_cast<const OUT*>(x);
-#pragma unroll
-                for (int k = 0; k < V; ++k)
-                    if (c * V + k < cols) to[k] = e[k];
+                unsigned short x;
+                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(x) : "r"(at));
+                if (r < rows && lane < cols) *reinterpret_cast<unsigned short*>(to + r * pitch) = x;
             }
         }
     }

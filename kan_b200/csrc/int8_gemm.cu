@@ -3,9 +3,9 @@
 // The sum is exact in int32 whatever its order, so the kernels below give the same bits.  1 x 8192 -> 1024 5 us, 256 x 3136 -> 64
 // 8 us, 65536 x 8192 -> 1024 340 us.
 //
-//   up to 8 rows     row_kernel: bound by reading wq once; CUDA cores, four products per instruction
+//   few rows         row_kernel: bound by reading wq once; CUDA cores, four products per instruction
 //   few tiles        tcgen05 kind::i8, one tile per cluster, K split over its CTAs (gemm_tc.cuh)
-//   else             tcgen05 kind::i8, persistent pairs on 256 x 256 tiles
+//   else             tcgen05 kind::i8, persistent pairs on 256 x 256 tiles (256 x 128 or x 64 for fewer columns)
 #include "gemm_tc.cuh"
 #include "int8.cuh"
 
@@ -17,7 +17,7 @@ using gemm::Tiles;
 struct EpiArgs {
     const float *q_scale, *w_scale, *bias;
     void* y;
-    int vec;                  // y's rows and the columns' scales allow 16-byte accesses
+    int vec, vec_scales;      // whether y's rows, and the columns' scales, allow 16-byte accesses
 };
 
 template <typename OUT>
@@ -31,7 +31,7 @@ struct Epilogue {
     // the tile's MMAs
     template <int NC>
     static __device__ __forceinline__ void columns(const Args& p, const Tiles& g, int col0, float (&ws)[NC], float (&bs)[NC]) {
-        if (col0 + NC <= g.N && p.vec) {
+        if (col0 + NC <= g.N && p.vec_scales) {
 #pragma unroll
             for (int c = 0; c < NC; c += 4) *reinterpret_cast<float4*>(ws + c) = __ldg(reinterpret_cast<const float4*>(p.w_scale + col0 + c));
 #pragma unroll
@@ -77,7 +77,7 @@ struct Epilogue {
     }
 };
 
-// ---- up to 8 rows ---------------------------------------------------------------------------------------------------
+// ---- few rows -----------------------------------------------------------------------------------------------------
 // A warp per output column: lanes take 16 bytes of the column's weights each, U loads in flight, against the same bytes of
 // every row (from the caches).  The first weights are asked for before the rows' producer is waited for.
 template <typename OUT, int ROWS>
@@ -139,16 +139,30 @@ __global__ void __launch_bounds__(256) empty_kernel(const Product p) {
         reinterpret_cast<OUT*>(p.y)[e] = to_type<OUT>(fmaf(0.f * p.q_scale[e / p.N], p.w_scale[e % p.N], p.bias ? p.bias[e % p.N] : 0.f));
 }
 
-// rows of any byte pitch -> rows of a pitch that is a multiple of 16
+// rows of any byte pitch -> rows of a pitch that is a multiple of 16, 16 bytes per thread: the five aligned words around a
+// piece, shifted into place; words that reach out of the matrix are read byte by byte
 __global__ void __launch_bounds__(256) pad_kernel(const int8_t* __restrict__ src, int64_t ld, int8_t* __restrict__ dst, int64_t pitch, int64_t rows, int64_t K) {
-    const int64_t words = pitch / 4;
-    for (int64_t e = blockIdx.x * (int64_t)256 + threadIdx.x; e < rows * words; e += (int64_t)gridDim.x * 256) {
-        const int64_t r = e / words, k = e % words * 4;
-        uint32_t v = 0;
+    const int64_t pieces = pitch / 16, last = (rows - 1) * ld + K;      // bytes from src to the matrix's end
+    for (int64_t e = blockIdx.x * (int64_t)256 + threadIdx.x; e < rows * pieces; e += (int64_t)gridDim.x * 256) {
+        const int64_t r = e / pieces, k = (e - r * pieces) * 16, from = r * ld + k, aligned = from & ~(int64_t)3;
+        const uint32_t shift = (uint32_t)(from & 3) * 8;
+        uint32_t w[5];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (k + j < K) v |= (uint32_t)(uint8_t)src[r * ld + k + j] << (8 * j);
-        *reinterpret_cast<uint32_t*>(dst + r * pitch + k) = v;
+        for (int j = 0; j < 5; ++j) {
+            const int64_t at = aligned + 4 * j;
+            w[j] = 0;
+            if (at + 4 <= last) w[j] = *reinterpret_cast<const uint32_t*>(src + at);
+            else
+                for (int i = 0; i < 4 && at + i < last; ++i) w[j] |= (uint32_t)(uint8_t)src[at + i] << (8 * i);
+        }
+        uint32_t o[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            o[j] = __funnelshift_r(w[j], w[j + 1], shift);
+            const int64_t left = K - k - 4 * j;                         // the next row's bytes are not this one's padding
+            if (left < 4) o[j] &= left <= 0 ? 0u : (1u << (8 * left)) - 1u;
+        }
+        *reinterpret_cast<uint4*>(dst + r * pitch + k) = make_uint4(o[0], o[1], o[2], o[3]);
     }
 }
 
@@ -179,22 +193,33 @@ int run_persistent(const Product& p, const EpiArgs& args, int32_t* status, cudaS
     return gemm::launch<C, Epilogue<OUT>>(mq, mw, gemm::tiles_of<C>((int)p.M, (int)p.N, (int)p.K, 1, false), args, status, s, after);
 }
 
+// Few rows on the CUDA cores: every row adds to row_kernel's time, while a tile of up to 128 costs the same.  Measured (us,
+// row_kernel / split_kernel): 8192 -> 1024 with 2 rows 3.4 / 13, 4 rows 14 / 13.5, 8 rows 23 / 13.5; 2048 -> 8192 with 4 rows
+// 9.4 / 10.5, 8 rows 15 / 11; 512 -> 2048 with 8 rows 5.3 / 5.3.
+bool few_rows(int64_t M, int64_t K) { return M <= 4 || (M <= 8 && K <= 512); }
+
 template <typename OUT>
 int launch_typed(const Product& p, int32_t* status, cudaStream_t s, bool after) {
     if (p.K == 0) {
         empty_kernel<OUT><<<(unsigned)(ceil_div(p.M * p.N, 256) < 148 * 8 ? ceil_div(p.M * p.N, 256) : 148 * 8), 256, 0, s>>>(p);
         return check_cuda(cudaGetLastError());
     }
-    if (p.M <= 8) return launch_rows<OUT>(p, s, after);
-    const EpiArgs args{p.q_scale, p.w_scale, p.bias, p.y, p.N % (16 / (int64_t)sizeof(OUT)) == 0 && aligned16(p.w_scale) && aligned16(p.bias)};
+    if (few_rows(p.M, p.K)) return launch_rows<OUT>(p, s, after);
+    const EpiArgs args{p.q_scale, p.w_scale, p.bias, p.y, p.N % (16 / (int64_t)sizeof(OUT)) == 0,
+                       aligned16(p.w_scale) && aligned16(p.bias)};
     using Pair = gemm::Config<gemm::I8, 1, 2, 256, false>;
+    using Pair128 = gemm::Config<gemm::I8, 1, 2, 128, false>;
+    using Pair64 = gemm::Config<gemm::I8, 1, 2, 64, false>;
     using Narrow = gemm::Config<gemm::I8, 1, 1, 64, false>;
     using Wide = gemm::Config<gemm::I8, 1, 1, 128, false>;
-    // tiles of 128 x 64 as long as that leaves SMs idle, of 128 x 128 up to one each, pairs on 256 x 256 beyond
+    // tiles of 128 x 64 as long as that leaves SMs idle, of 128 x 128 up to one each; beyond, pairs on 256 rows and as many
+    // columns as there are, up to 256
     const int M = (int)p.M, N = (int)p.N, K = (int)p.K;
     const Tiles narrow = gemm::tiles_of<Narrow>(M, N, K, 1, false), wide = gemm::tiles_of<Wide>(M, N, K, 1, false);
     if (narrow.total <= 148) return run_split<Narrow, OUT>(p, narrow, args, status, s, after);
     if (wide.total <= 148) return run_split<Wide, OUT>(p, wide, args, status, s, after);
+    if (N <= 64) return run_persistent<Pair64, OUT>(p, args, status, s, after);
+    if (N <= 128) return run_persistent<Pair128, OUT>(p, args, status, s, after);
     return run_persistent<Pair, OUT>(p, args, status, s, after);
 }
 
@@ -212,7 +237,7 @@ int launch_matmul(const Product& given, void* ws, int32_t* status, cudaStream_t 
     int8_t* at = reinterpret_cast<int8_t*>(ws);
     auto pad = [&](const int8_t*& m, int64_t& ld, int64_t rows) -> int {
         if (ld % 16 == 0 || p.K == 0) return CHEBYKAN_OK;
-        const int64_t blocks = ceil_div(rows * pitch / 4, 256);
+        const int64_t blocks = ceil_div(rows * pitch / 16, 256);
         pad_kernel<<<(unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, s>>>(m, ld, at, pitch, rows, p.K);
         m = at; ld = pitch; at += a256(rows * pitch);
         return check_cuda(cudaGetLastError());

@@ -37,9 +37,9 @@ def case(M, N, K, seed=0):
             torch.rand(N, generator=gen, device="cuda") * 1e-3 + 1e-4, torch.randn(N, generator=gen, device="cuda"))
 
 
-SHAPES = [(1, 1, 1), (1, 5, 16), (1, 1024, 8192), (2, 7, 33), (3, 64, 100), (5, 10, 320), (8, 130, 272), (16, 100, 4096), (17, 65, 64),
+SHAPES = [(1, 1, 1), (1, 5, 16), (1, 1024, 8192), (2, 7, 33), (3, 64, 100), (5, 10, 320), (8, 130, 272), (4, 70, 1000), (6, 90, 2000), (7, 33, 515), (16, 100, 4096), (17, 65, 64),
           (33, 1, 48), (64, 1000, 256), (100, 129, 1040), (128, 128, 128), (129, 257, 144), (256, 64, 3136), (300, 300, 129),
-          (1000, 48, 16), (2000, 10, 64), (1024, 1024, 1024), (5000, 513, 272), (257, 2048, 8192)]
+          (1000, 48, 16), (2000, 10, 64), (1024, 1024, 1024), (5000, 513, 272), (20000, 100, 160), (20000, 20, 400), (9000, 301, 143), (257, 2048, 8192)]
 
 
 @pytest.mark.parametrize("shape", SHAPES)
