@@ -458,9 +458,10 @@ NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 
 
 def _dtype(dtype, name: str) -> int:
-    if dtype not in _DTYPES:
+    code = _DTYPES.get(dtype)
+    if code is None:
         raise RuntimeError(f"{name} must be float32, bfloat16 or float16, got {str(dtype).replace('torch.', '')}")
-    return _DTYPES[dtype]
+    return code
 
 
 def _require_any(t: torch.Tensor, name: str, dtype=None, device=None, contiguous: bool = True) -> None:
@@ -647,43 +648,42 @@ def int8_basis(x: torch.Tensor, degree: int):
     return q, scale
 
 
-def _require_int8(t: torch.Tensor, name: str, device=None) -> None:
-    """int8 matrix on the GPU with adjacent columns; rows may be any distance apart."""
-    if (type(t) in _TENSORS and t.dtype is torch.int8 and t.is_cuda and (device is None or t.device == device) and t.dim() == 2
-            and t.is_contiguous() and not t.data_ptr() & 15):
-        return
-    _require_any(t, name, torch.int8, device, contiguous=False)
+def _int8_matrix(t: torch.Tensor, name: str, idx: int | None):
+    """(address, rows, columns, row pitch) of an int8 matrix on device `idx` (None: any) with adjacent columns; rows may be
+    any distance apart, and the pitch of a single row does not matter."""
+    if (type(t) in _TENSORS and t.dtype is torch.int8 and t.is_cuda and (idx is None or t.get_device() == idx) and t.dim() == 2
+            and t.is_contiguous()):
+        p, (rows, cols) = t.data_ptr(), t.shape
+        if not p & 15:
+            return p, rows, cols, cols if rows > 1 else -(-cols // 16) * 16
+    _require_any(t, name, torch.int8, None if idx is None else torch.device("cuda", idx), contiguous=False)
     if t.dim() != 2:
         raise RuntimeError(f"{name} must be a matrix")
+    (rows, cols), (sr, sc) = t.shape, t.stride()
     if t.numel():
-        (rows, cols), (sr, sc) = t.shape, t.stride()
         if (cols > 1 and sc != 1) or (rows > 1 and sr < cols):
             raise RuntimeError(f"the rows of {name} must be contiguous and may not overlap")
         if t.data_ptr() % 16 != 0:
             raise RuntimeError(f"{name} must be 16-byte aligned")
+    return t.data_ptr(), rows, cols, max(sr, cols) if rows > 1 else -(-cols // 16) * 16
 
 
 def int8_matmul(q: torch.Tensor, q_scale: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor,
                 bias: torch.Tensor | None = None, out_dtype=torch.float32, out: torch.Tensor | None = None) -> torch.Tensor:
     """y[M, N] = (q[M, K] wq[N, K]^T) * q_scale[M] * w_scale[N] + bias[N] for int8 matrices; the integer sums are exact
     (K up to 131071).  Row strides that are multiples of 16 bytes are read in place, others through a padded copy."""
-    _require_int8(q, "q")
-    _require_int8(wq, "wq", q.device)
-    M, K = q.shape
-    N = wq.shape[0]
-    if wq.shape[1] != K:
-        raise RuntimeError(f"q has {K} columns, wq {wq.shape[1]}")
+    qp, M, K, ldq = _int8_matrix(q, "q", None)
     idx = q.get_device()
-    qs, ws_, bs = (_vector(q_scale, "q_scale", M, idx), _vector(w_scale, "w_scale", N, idx),
-                   None if bias is None else _vector(bias, "bias", N, idx))
+    wp, N, wk, ldw = _int8_matrix(wq, "wq", idx)
+    if wk != K:
+        raise RuntimeError(f"q has {K} columns, wq {wk}")
+    qs, ws_ = _vector(q_scale, "q_scale", M, idx), _vector(w_scale, "w_scale", N, idx)
+    bs = None if bias is None else _vector(bias, "bias", N, idx)
     out = _result(out, (M, N), out_dtype, q)
-    # the pitch of a single row does not matter
-    ldq = q.stride(0) if M > 1 else -(-K // 16) * 16
-    ldw = wq.stride(0) if N > 1 else -(-K // 16) * 16
     ws_bytes = _bytes_for("chebykan_int8_matmul_workspace_bytes", M, N, K, ldq, ldw)
-    ws, ws_ptr = _scratch(ws_bytes, q)
-    _launch("chebykan_int8_matmul", idx, q.data_ptr(), ldq, qs, wq.data_ptr(), ldw, ws_, bs, out.data_ptr(), _dtype(out.dtype, "out"),
-            ws_ptr, ws_bytes, M, N, K)
+    ws, ws_ptr = _scratch(ws_bytes, q) if ws_bytes else (None, None)
+    _launch("chebykan_int8_matmul", idx, qp, ldq, qs, wp, ldw, ws_, bs, out.data_ptr(), _dtype(out.dtype, "out"), ws_ptr, ws_bytes,
+            M, N, K)
     return out
 
 
@@ -691,21 +691,22 @@ def int8_forward(x: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor, bias:
                  out_dtype=torch.float32, out: torch.Tensor | None = None) -> torch.Tensor:
     """Forward of a Chebyshev layer from coefficients packed by ``int8_pack_coeffs``: y[B, out] of `out_dtype` from x[B, in]
     (fp32, bf16 or fp16).  ``int8_basis`` followed by ``int8_matmul`` in one call."""
-    _require_any(x, "x")
+    if not (type(x) in _TENSORS and x.is_cuda and x.is_contiguous() and not x.data_ptr() & 15):
+        _require_any(x, "x")
     if x.dim() != 2:
         raise RuntimeError("x must have shape [B, in]")
+    xt = _dtype(x.dtype, "x")
     B, n_in = x.shape
-    _require_any(wq, "wq", torch.int8, x.device)
-    if wq.dim() != 2 or wq.shape[1] != int8_width(n_in, degree):
-        raise RuntimeError(f"wq must have shape [out, {int8_width(n_in, degree)}] for {n_in} inputs and degree {degree}")
-    N = wq.shape[0]
     idx = x.get_device()
+    wp, N, K, ldw = _int8_matrix(wq, "wq", idx)
+    if K != int8_width(n_in, degree) or ldw != K:
+        raise RuntimeError(f"wq must be contiguous and have shape [out, {int8_width(n_in, degree)}] for {n_in} inputs and degree {degree}")
     ws_, bs = _vector(w_scale, "w_scale", N, idx), None if bias is None else _vector(bias, "bias", N, idx)
     out = _result(out, (B, N), out_dtype, x)
     ws_bytes = _bytes_for("chebykan_int8_fwd_workspace_bytes", B, n_in, N, degree)
     ws, ws_ptr = _scratch(ws_bytes, x)
-    _launch("chebykan_int8_fwd", idx, x.data_ptr(), _dtype(x.dtype, "x"), wq.data_ptr(), ws_, bs, out.data_ptr(), _dtype(out.dtype, "out"),
-            ws_ptr, ws_bytes, B, n_in, N, degree)
+    _launch("chebykan_int8_fwd", idx, x.data_ptr(), xt, wp, ws_, bs, out.data_ptr(), _dtype(out.dtype, "out"), ws_ptr, ws_bytes, B, n_in, N,
+            degree)
     return out
 
 
