@@ -91,20 +91,14 @@ struct Recurrence {
     }
 };
 
-// A row per group of G threads, eight neighbouring inputs per thread and chunk.  The first pass finds the row's largest
-// |T_d|, the second evaluates the recurrence again and writes it; tanh, by far the dearer part, is kept in registers in
-// between (CHUNKS per thread; 0: rows longer than that evaluate it twice).  32768 x 2048, degree 4: 138 us, 3.9 TB/s; groups of
-// 128 or 64 threads with two or four chunks each took 146 and 181 us, five blocks per SM (by spilling) 181 us.
+// One row by a group of G threads (lane: the thread's number in it), eight neighbouring inputs per thread and chunk.  The first
+// pass finds the row's largest |T_d|, the second evaluates the recurrence again and writes dst[deg][pad]; tanh, by far the
+// dearer part, is kept in registers in between (CHUNKS per thread; 0: rows longer than that evaluate it twice).  Every thread
+// of the block comes here, live or not; red: a float per warp.
 template <typename T, int G, int CHUNKS, bool SMALL>
-__global__ void __launch_bounds__(256)
-basis_kernel(const T* __restrict__ x, int8_t* __restrict__ q, float* __restrict__ scale, int64_t B, int in, int pad, int deg, int vec) {
-    constexpr int ROWS = 256 / G, KEEP = CHUNKS ? CHUNKS : 1;
-    __shared__ float red[8];
-    const int lane = threadIdx.x % G;
-    const int64_t row = blockIdx.x * (int64_t)ROWS + threadIdx.x / G;
-    const bool live = row < B;
-    const T* src = x + row * in;
-    let_next_start();
+__device__ __forceinline__ void quantise_row(const T* __restrict__ src, bool live, int lane, int in, int pad, int deg, int vec, float* red,
+                                             int8_t* dst, float* scale) {
+    constexpr int KEEP = CHUNKS ? CHUNKS : 1;
     const int chunks = CHUNKS ? CHUNKS : (pad + 8 * G - 1) / (8 * G);
     f32x2 t[KEEP][4];
     auto load = [&](int i0, f32x2 (&tc)[4]) {
@@ -168,16 +162,15 @@ basis_kernel(const T* __restrict__ x, int8_t* __restrict__ q, float* __restrict_
     const bool bad = top > 3.f;                    // |T_d| <= 1 up to rounding
     const float s = bad ? __int_as_float(0x7fc00000) : __fdiv_rn(top, 127.f);
     const float inv = (bad || s == 0.f) ? 0.f : __fdiv_rn(1.f, s);
-    if (lane == 0) scale[row] = s;
+    if (lane == 0) *scale = s;
     const f32x2 plus = pair_of(inv, inv), minus = pair_of(-inv, -inv);
-    int8_t* dst = q + row * (int64_t)deg * pad;
 #pragma unroll
     for (int c = 0; c < chunks; ++c) {
         f32x2 (&tc)[4] = t[CHUNKS ? c : 0];
         const int i0 = (c * G + lane) * 8;
         if (i0 >= pad) continue;
         const int n = in - i0;                     // inputs of the chunk; the rest of the padded row is zero
-        if (CHUNKS == 0 && n > 0) load(i0, tc);
+        if (CHUNKS == 0 && chunks > 1 && n > 0) load(i0, tc);
         uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
         if (bad) keep0 = keep1 = 0;
         else if (n < 8) {
@@ -198,6 +191,73 @@ basis_kernel(const T* __restrict__ x, int8_t* __restrict__ q, float* __restrict_
             r.even();
             put(r.b, by);
             if (d < deg) { r.odd(); put(r.a, by); }
+        }
+    }
+}
+
+// 256 / G rows per block.  32768 x 2048, degree 4: 138 us, 3.9 TB/s; groups of 128 or 64 threads with two or four chunks each
+// took 146 and 181 us, five blocks per SM (by spilling) 181 us.
+template <typename T, int G, int CHUNKS, bool SMALL>
+__global__ void __launch_bounds__(256)
+basis_kernel(const T* __restrict__ x, int8_t* __restrict__ q, float* __restrict__ scale, int64_t B, int in, int pad, int deg, int vec) {
+    __shared__ float red[8];
+    const int64_t row = blockIdx.x * (int64_t)(256 / G) + threadIdx.x / G;
+    let_next_start();
+    quantise_row<T, G, CHUNKS, SMALL>(x + row * in, row < B, threadIdx.x % G, in, pad, deg, vec, red, q + row * (int64_t)deg * pad, scale + row);
+}
+
+// The whole forward of a few rows in one launch: every block quantises the rows for itself, into shared memory, while the first
+// of its weights are on their way, and then takes columns as row_kernel does.  The same arithmetic, so the same bits, as the two
+// kernels, without the launch, the workspace and the wait between them.  In a graph 1 x 2048 -> 2048 of degree 4 takes 4.8 us (7.7
+// as two kernels), 4 x 2048 -> 2048 11.7 (20.7), 4 x 784 -> 64 of degree 8 7.9 (17.9); 2 x 2048 -> 2048 7.3 (5.1) and
+// 8 x 128 -> 4096 9.2 (8.6) lose what every call gains on the host.  Bound by latency: the rows' quantisation, 2 us, then one
+// trip to memory for the weights after the first.
+template <typename OUT, typename T, int ROWS, bool SMALL>
+__global__ void __launch_bounds__(256)
+few_rows_kernel(const T* __restrict__ x, const int8_t* __restrict__ wq, const float* __restrict__ w_scale, const float* __restrict__ bias,
+                OUT* __restrict__ y, int B, int N, int in, int pad, int deg, int vec) {
+    extern __shared__ int4 rows[];                     // [B][K / 16]
+    __shared__ float red[8], scale[ROWS];
+    const int lane = threadIdx.x & 31, step = (int)gridDim.x * 8, whole = deg * pad / 16;
+    constexpr int U = ROWS == 1 ? 16 : 8;
+    int4 wv[U];
+    auto weights = [&](int o, int c0) {
+        const int4* w = reinterpret_cast<const int4*>(wq) + (int64_t)o * whole;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            wv[u] = make_int4(0, 0, 0, 0);
+            if (c0 + u * 32 < whole) wv[u] = __ldg(w + c0 + u * 32);
+        }
+    };
+    int o = blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (o < N) weights(o, lane);
+    constexpr int G = 256 / ROWS;                      // all rows at once
+    const int row = threadIdx.x / G;
+    quantise_row<T, G, 0, SMALL>(x + (int64_t)row * in, row < B, threadIdx.x % G, in, pad, deg, vec, red,
+                                 reinterpret_cast<int8_t*>(rows + row * whole), scale + row);
+    __syncthreads();
+    for (; o < N; o += step) {
+        int acc[ROWS] = {};
+        for (int c0 = lane; c0 < whole;) {
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r)
+                if (r < B)
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+                        if (c0 + u * 32 < whole) {
+                            const int4 v = rows[r * whole + c0 + u * 32];
+                            acc[r] = __dp4a(v.x, wv[u].x, __dp4a(v.y, wv[u].y, __dp4a(v.z, wv[u].z, __dp4a(v.w, wv[u].w, acc[r]))));
+                        }
+            c0 += U * 32;
+            if (c0 < whole) weights(o, c0);
+        }
+        if (o + step < N) weights(o + step, lane);
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+#pragma unroll
+            for (int d = 16; d; d >>= 1) acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], d);
+            if (lane == r && r < B)
+                y[(int64_t)r * N + o] = to_type<OUT>(fmaf((float)acc[r] * scale[r], __ldg(w_scale + o), bias ? __ldg(bias + o) : 0.f));
         }
     }
 }
@@ -270,6 +330,27 @@ int launch_basis(const void* x, int dtype, int8_t* q, float* scale, int64_t B, i
     return launch_basis_typed<__half>(x, q, scale, B, in, deg, s);
 }
 
+template <typename OUT, typename T>
+int launch_few_rows(const void* x, const int8_t* wq, const float* w_scale, const float* bias, void* y, int64_t B, int64_t N, int64_t in,
+                    int64_t deg, cudaStream_t s) {
+    const int pad = (int)in_pad(in), vec = (in * sizeof(T)) % 16 == 0;
+    auto kernel = B == 1 ? (deg == 1 ? few_rows_kernel<OUT, T, 1, true> : few_rows_kernel<OUT, T, 1, false>)
+                : B == 2 ? (deg == 1 ? few_rows_kernel<OUT, T, 2, true> : few_rows_kernel<OUT, T, 2, false>)
+                : B <= 4 ? (deg == 1 ? few_rows_kernel<OUT, T, 4, true> : few_rows_kernel<OUT, T, 4, false>)
+                         : (deg == 1 ? few_rows_kernel<OUT, T, 8, true> : few_rows_kernel<OUT, T, 8, false>);
+    const int64_t blocks = ceil_div(N, 8);
+    kernel<<<(unsigned)(blocks < 2 * 148 ? blocks : 2 * 148), 256, (size_t)(B * deg * pad), s>>>(
+        reinterpret_cast<const T*>(x), wq, w_scale, bias, reinterpret_cast<OUT*>(y), (int)B, (int)N, (int)in, pad, (int)deg, vec);
+    return check_cuda(cudaGetLastError());
+}
+template <typename OUT>
+int launch_few_rows_to(const void* x, int x_dtype, const int8_t* wq, const float* w_scale, const float* bias, void* y, int64_t B, int64_t N,
+                       int64_t in, int64_t deg, cudaStream_t s) {
+    if (x_dtype == CHEBYKAN_DTYPE_FP32) return launch_few_rows<OUT, float>(x, wq, w_scale, bias, y, B, N, in, deg, s);
+    if (x_dtype == CHEBYKAN_DTYPE_BF16) return launch_few_rows<OUT, __nv_bfloat16>(x, wq, w_scale, bias, y, B, N, in, deg, s);
+    return launch_few_rows<OUT, __half>(x, wq, w_scale, bias, y, B, N, in, deg, s);
+}
+
 bool dtype_ok(int dtype) { return dtype >= CHEBYKAN_DTYPE_FP32 && dtype <= CHEBYKAN_DTYPE_FP16; }
 // row numbers are 32-bit inside the kernels, and a tile may reach past the last row
 constexpr int64_t MAX_ROWS = 0x7fffffff - 4096;
@@ -284,6 +365,7 @@ bool product_ok(int64_t M, int64_t N, int64_t K, int64_t ldq, int64_t ldw) {
 }
 int64_t a256(int64_t b) { return round_up(b, 256); }
 // rows worked on at a time: 1 GiB of quantised rows at most (4096 rows if they are longer than that)
+bool in_one_launch(int64_t B, int64_t K) { return few_rows(B, K) && B * K <= 46 * 1024; }      // the rows fit 48 KB of shared memory
 int64_t chunk_rows(int64_t B, int64_t K) {
     int64_t rows = ((int64_t)1 << 30) / K / 256 * 256;
     if (rows < 4096) rows = 4096;
@@ -342,6 +424,7 @@ int chebykan_int8_matmul(const int8_t* q, int64_t ldq, const float* q_scale, con
 int64_t chebykan_int8_fwd_workspace_bytes(int64_t B, int64_t in, int64_t out, int64_t deg) {
     if (!layer_ok(B, in, out, deg)) return CHEBYKAN_EINVAL;
     const int64_t K = in_pad(in) * deg, rows = chunk_rows(B, K);
+    if (in_one_launch(B, K)) return 0;
     return a256(rows * K) + a256(rows * 4);
 }
 
@@ -352,12 +435,18 @@ int chebykan_int8_fwd(const void* x, int x_dtype, const int8_t* wq, const float*
     if (need < 0) return (int)need;
     if (!dtype_ok(x_dtype) || !dtype_ok(y_dtype)) return CHEBYKAN_EINVAL;
     if (B == 0) return CHEBYKAN_OK;
-    if (!x || !wq || !w_scale || !y || !workspace || !status) return CHEBYKAN_EINVAL;
+    if (!x || !wq || !w_scale || !y || !status) return CHEBYKAN_EINVAL;
     if (!aligned16(x) || !aligned16(wq) || !aligned16(y) || !aligned16(workspace)) return CHEBYKAN_EALIGN;
-    if (workspace_bytes < need) return CHEBYKAN_EWORKSPACE;
+    if (workspace_bytes < need || (need > 0 && !workspace)) return CHEBYKAN_EWORKSPACE;
     int rc = check_device();
     if (rc) return rc;
     const int64_t K = in_pad(in) * deg, rows = chunk_rows(B, K);
+    if (need == 0) {
+        cudaStream_t s = (cudaStream_t)stream;
+        if (y_dtype == CHEBYKAN_DTYPE_FP32) return launch_few_rows_to<float>(x, x_dtype, wq, w_scale, bias, y, B, out, in, deg, s);
+        if (y_dtype == CHEBYKAN_DTYPE_BF16) return launch_few_rows_to<__nv_bfloat16>(x, x_dtype, wq, w_scale, bias, y, B, out, in, deg, s);
+        return launch_few_rows_to<__half>(x, x_dtype, wq, w_scale, bias, y, B, out, in, deg, s);
+    }
     const int64_t x_size = x_dtype == CHEBYKAN_DTYPE_FP32 ? 4 : 2, y_size = y_dtype == CHEBYKAN_DTYPE_FP32 ? 4 : 2;
     char* ws = reinterpret_cast<char*>(workspace);
     int8_t* q = reinterpret_cast<int8_t*>(ws);

@@ -193,11 +193,6 @@ int run_persistent(const Product& p, const EpiArgs& args, int32_t* status, cudaS
     return gemm::launch<C, Epilogue<OUT>>(mq, mw, gemm::tiles_of<C>((int)p.M, (int)p.N, (int)p.K, 1, false), args, status, s, after);
 }
 
-// Few rows on the CUDA cores: every row adds to row_kernel's time, while a tile of up to 128 costs the same.  Measured (us,
-// row_kernel / split_kernel): 8192 -> 1024 with 2 rows 3.4 / 13, 4 rows 14 / 13.5, 8 rows 23 / 13.5; 2048 -> 8192 with 4 rows
-// 9.4 / 10.5, 8 rows 15 / 11; 512 -> 2048 with 8 rows 5.3 / 5.3.
-bool few_rows(int64_t M, int64_t K) { return M <= 4 || (M <= 8 && K <= 512); }
-
 template <typename OUT>
 int launch_typed(const Product& p, int32_t* status, cudaStream_t s, bool after) {
     if (p.K == 0) {

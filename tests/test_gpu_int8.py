@@ -142,7 +142,8 @@ def test_pack(n_in, n_out, degree):
 
 
 @pytest.mark.parametrize("B,n_in,n_out,degree", [(1, 2048, 2048, 4), (1, 1, 1, 8), (5, 64, 10, 4), (257, 784, 64, 4), (130, 100, 200, 1),
-                                                 (1000, 64, 64, 32), (700, 1024, 1024, 8)])
+                                                 (2, 333, 700, 1), (3, 2048, 100, 4), (4, 1000, 3000, 2), (4, 3000, 100, 4),
+                                                 (8, 60, 1500, 5), (7, 128, 40, 4), (1000, 64, 64, 32), (700, 1024, 1024, 8)])
 def test_forward(B, n_in, n_out, degree):
     x, c, _ = make_case(B, n_in, n_out, degree, seed=4)
     wq, ws, bias = ops.int8_pack_coeffs(c.cuda())

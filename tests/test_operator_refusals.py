@@ -29,7 +29,8 @@ def test_workspace_queries(lib):
     assert lib.chebykan_int8_matmul_workspace_bytes(5, 0, 100, 100, 100) == -1
     assert lib.chebykan_int8_fwd_workspace_bytes(5, 64, 64, 0) == -1                          # degree 0: nothing to quantise
     assert lib.chebykan_int8_fwd_workspace_bytes(5, 2048, 64, 64) == -1                       # 2048 * 64 > 131071
-    assert lib.chebykan_int8_fwd_workspace_bytes(5, 64, 64, 4) >= 5 * 256
+    assert lib.chebykan_int8_fwd_workspace_bytes(50, 64, 64, 4) >= 50 * 256
+    assert lib.chebykan_int8_fwd_workspace_bytes(1, 2048, 64, 4) == 0        # a few rows: one launch without a workspace
 
 
 def orth(lib, **kw):
@@ -82,7 +83,8 @@ def test_int8_refuses(lib):
     assert lib.chebykan_int8_pack_coeffs(P, P + 4, P, P, 64, 64, 4, None) == -2
     assert lib.chebykan_int8_basis(P, 7, P, P, 5, 64, 4, None) == -1
     assert lib.chebykan_int8_basis(None, 0, P, P, 0, 64, 4, None) == 0
-    assert lib.chebykan_int8_fwd(P, 0, P, P, P, P, 0, P, 10, 5, 64, 64, 4, P, None) == -6
+    assert lib.chebykan_int8_fwd(P, 0, P, P, P, P, 0, P, 10, 50, 64, 64, 4, P, None) == -6
+    assert lib.chebykan_int8_fwd(P, 0, P, P, P, P, 0, None, 1 << 30, 50, 64, 64, 4, P, None) == -6
     assert lib.chebykan_int8_fwd(P, 0, P, P, P, P, 9, P, 1 << 30, 5, 64, 64, 4, P, None) == -1
 
 
