@@ -12,10 +12,11 @@ constexpr int64_t MAX_K = 131071;
 
 inline int64_t in_pad(int64_t in) { return round_up(in, 16); }
 
-// Few rows on the CUDA cores: every row adds to row_kernel's time, while a tile of up to 128 costs the same.  Measured (us,
-// row_kernel / split_kernel): 8192 -> 1024 with 2 rows 3.4 / 13, 4 rows 14 / 13.5, 8 rows 23 / 13.5; 2048 -> 8192 with 4 rows
-// 9.4 / 10.5, 8 rows 15 / 11; 512 -> 2048 with 8 rows 5.3 / 5.3.
-inline bool few_rows(int64_t M, int64_t K) { return M <= 4 || (M <= 8 && K <= 512); }
+// Few rows on the CUDA cores: every row adds to row_kernel's time, while a tile of up to 128 costs the same; four rows as
+// long as 48 KB of shared memory hold.  Measured (us, row_kernel / split_kernel): 8192 -> 1024 with 2 rows 3.4 / 13, 4 rows 5.2 / 13.5,
+// 8 rows 23 / 13.5; 2048 -> 8192 with 4 rows 7.9 / 10.5, 8 rows 15 / 11; 512 -> 2048 with 8 rows 5.3 / 5.3; 16000 -> 1024 with 4 rows
+// 25 / 17.
+inline bool few_rows(int64_t M, int64_t K) { return M <= 2 || (M <= 4 && M * K <= 48 * 1024) || (M <= 8 && K <= 512); }
 
 struct Product {
     const int8_t* q;          // [M][K], rows ldq bytes apart

@@ -80,11 +80,16 @@ struct Epilogue {
 // ---- few rows -----------------------------------------------------------------------------------------------------
 // A warp per output column: lanes take 16 bytes of the column's weights each, U loads in flight, against the same bytes of
 // every row (from the caches).  The first weights are asked for before the rows' producer is waited for.
-template <typename OUT, int ROWS>
+// STAGED: the block copies the rows into shared memory first, all at once: with four rows of 8192 the reads row after row took
+// 13.3 us (1024 outputs), staged 5.2; rows of 2048 (8192 outputs) 8.8 and 7.9.  Two rows (2.9 / 3.3) and eight short ones (512 ->
+// 2048 5.1 / 6.3) are faster from the caches.
+template <typename OUT, int ROWS, bool STAGED>
 __global__ void __launch_bounds__(256) row_kernel(const Product p) {
+    extern __shared__ int4 staged[];                   // [M][K / 16]
     const int lane = threadIdx.x & 31;
     const int64_t o = blockIdx.x * (int64_t)8 + (threadIdx.x >> 5);
-    if (o >= p.N) return;
+    if (!STAGED && o >= p.N) return;
+    const bool mine = o < p.N;
     const int8_t* w = p.wq + o * p.ldw;
     const int whole = (int)(p.K / 16);                 // 16-byte pieces; the rest is one lane's, byte by byte
     int acc[ROWS] = {};
@@ -97,14 +102,22 @@ __global__ void __launch_bounds__(256) row_kernel(const Product p) {
             if (c0 + u * 32 < whole) wv[u] = __ldg(reinterpret_cast<const int4*>(w) + c0 + u * 32);
         }
     };
-    weights(lane);
-    const float ws = __ldg(p.w_scale + o), bias = p.bias ? __ldg(p.bias + o) : 0.f;
+    if (mine) weights(lane);
+    const float ws = mine ? __ldg(p.w_scale + o) : 0.f, bias = mine && p.bias ? __ldg(p.bias + o) : 0.f;
     wait_for_previous();
+    if (STAGED) {
+        for (int r = 0; r < ROWS; ++r)
+            if (r < p.M)
+#pragma unroll 4
+                for (int c = threadIdx.x; c < whole; c += 256) staged[r * whole + c] = reinterpret_cast<const int4*>(p.q + r * p.ldq)[c];
+        __syncthreads();
+        if (!mine) return;
+    }
     for (int c0 = lane; c0 < whole;) {
 #pragma unroll
         for (int r = 0; r < ROWS; ++r)
             if (r < p.M) {
-                const int4* q = reinterpret_cast<const int4*>(p.q + r * p.ldq);
+                const int4* q = STAGED ? staged + r * whole : reinterpret_cast<const int4*>(p.q + r * p.ldq);
                 int4 v[U];
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
@@ -168,8 +181,13 @@ __global__ void __launch_bounds__(256) pad_kernel(const int8_t* __restrict__ src
 
 template <typename OUT>
 int launch_rows(const Product& p, cudaStream_t s, bool after) {
-    auto kernel = p.M == 1 ? row_kernel<OUT, 1> : p.M == 2 ? row_kernel<OUT, 2> : p.M <= 4 ? row_kernel<OUT, 4> : row_kernel<OUT, 8>;
-    return check_cuda(launch_after(after, kernel, dim3((unsigned)ceil_div(p.N, 8)), dim3(256), 0, s, 0, p));
+    const int64_t bytes = p.M * (p.K / 16) * 16;
+    const bool staged = p.M > 2 && p.M <= 4;           // few_rows: they fit
+    auto kernel = p.M == 1 ? row_kernel<OUT, 1, false>
+                : p.M == 2 ? row_kernel<OUT, 2, false>
+                : staged ? row_kernel<OUT, 4, true>
+                         : row_kernel<OUT, 8, false>;
+    return check_cuda(launch_after(after, kernel, dim3((unsigned)ceil_div(p.N, 8)), dim3(256), staged ? (size_t)bytes : 0, s, 0, p));
 }
 
 template <class C>

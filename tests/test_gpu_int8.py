@@ -39,7 +39,8 @@ def case(M, N, K, seed=0):
 
 SHAPES = [(1, 1, 1), (1, 5, 16), (1, 1024, 8192), (2, 7, 33), (3, 64, 100), (5, 10, 320), (8, 130, 272), (4, 70, 1000), (6, 90, 2000), (7, 33, 515), (16, 100, 4096), (17, 65, 64),
           (33, 1, 48), (64, 1000, 256), (100, 129, 1040), (128, 128, 128), (129, 257, 144), (256, 64, 3136), (300, 300, 129),
-          (1000, 48, 16), (2000, 10, 64), (1024, 1024, 1024), (5000, 513, 272), (20000, 100, 160), (20000, 20, 400), (9000, 301, 143), (257, 2048, 8192)]
+          (1000, 48, 16), (2000, 10, 64), (1024, 1024, 1024), (5000, 513, 272), (20000, 100, 160), (20000, 20, 400), (9000, 301, 143), (257, 2048, 8192),
+          (4, 33, 12288), (4, 33, 12289), (3, 40, 16384), (4, 1300, 2047)]
 
 
 @pytest.mark.parametrize("shape", SHAPES)
@@ -65,7 +66,7 @@ def test_matmul_longest_sum_is_exact(M):
     assert torch.equal(y, want.float().expand(M, N))
 
 
-@pytest.mark.parametrize("M", [1, 7, 200])
+@pytest.mark.parametrize("M", [1, 4, 7, 200])
 def test_matmul_strided_rows_offsets_and_guards(M):
     gen = torch.Generator(device="cuda").manual_seed(M)
     for K, pitch in [(100, 112), (100, 101), (48, 4096)]:
@@ -157,6 +158,23 @@ def test_forward(B, n_in, n_out, degree):
     if n_in * degree > 16:
         assert o.rel_l2(ops.int8_forward(x.cuda(), wq, ws, bias, degree).cpu(), o.forward(x, c)) <= 2e-2
     ops.check_status()
+
+
+@pytest.mark.parametrize("B,n_in,n_out,degree", [(1, 500, 70, 1), (2, 300, 1000, 4), (3, 40, 30, 3), (7, 100, 41, 5)])
+def test_forward_of_few_rows_writes_nothing_else_and_keeps_a_nan_to_its_row(B, n_in, n_out, degree):
+    gen = torch.Generator(device="cuda").manual_seed(B)
+    x = torch.randn(B, n_in, generator=gen, device="cuda")
+    wq, ws, bias = ops.int8_pack_coeffs(torch.randn(n_in, n_out, degree + 1, generator=gen, device="cuda"))
+    for xt in (x.clone(), x.bfloat16(), x.half()):
+        view, whole = guarded((B, n_out))
+        ops.int8_forward(xt, wq, ws, None, degree, out=view)
+        torch.cuda.synchronize()
+        assert_guards_intact(view, whole)
+        q, scale = ops.int8_basis(xt, degree)
+        assert torch.equal(view, ops.int8_matmul(q, scale, wq, ws))
+        xt[B - 1, n_in // 2] = float("nan")          # the guard check takes NaN for unwritten
+        y = ops.int8_forward(xt, wq, ws, None, degree)
+        assert bool(torch.isnan(y[B - 1]).all()) and torch.equal(y[:B - 1], view[:B - 1])
 
 
 def test_forward_of_more_rows_than_the_workspace_holds():
