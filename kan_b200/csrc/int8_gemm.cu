@@ -153,8 +153,18 @@ __global__ void __launch_bounds__(256) empty_kernel(const Product p) {
 }
 
 // rows of any byte pitch -> rows of a pitch that is a multiple of 16, 16 bytes per thread: the five aligned words around a
-// piece, shifted into place; words that reach out of the matrix are read byte by byte
-__global__ void __launch_bounds__(256) pad_kernel(const int8_t* __restrict__ src, int64_t ld, int8_t* __restrict__ dst, int64_t pitch, int64_t rows, int64_t K) {
+// piece, shifted into place; words that reach out of the matrix are read byte by byte.  One launch for both matrices
+// (blockIdx.y): 64 x 1001 -> 700 7.9 us, one after the other 9.2
+struct Padding {
+    const int8_t* src;
+    int8_t* dst;
+    int64_t ld, rows;
+};
+__global__ void __launch_bounds__(256) pad_kernel(const Padding first, const Padding second, int64_t pitch, int64_t K) {
+    const Padding m = blockIdx.y ? second : first;
+    const int8_t* __restrict__ src = m.src;
+    int8_t* __restrict__ dst = m.dst;
+    const int64_t ld = m.ld, rows = m.rows;
     const int64_t pieces = pitch / 16, last = (rows - 1) * ld + K;      // bytes from src to the matrix's end
     for (int64_t e = blockIdx.x * (int64_t)256 + threadIdx.x; e < rows * pieces; e += (int64_t)gridDim.x * 256) {
         const int64_t r = e / pieces, k = (e - r * pieces) * 16, from = r * ld + k, aligned = from & ~(int64_t)3;
@@ -248,16 +258,23 @@ int launch_matmul(const Product& given, void* ws, int32_t* status, cudaStream_t 
     Product p = given;
     const int64_t pitch = round_up(p.K, 16);
     int8_t* at = reinterpret_cast<int8_t*>(ws);
-    auto pad = [&](const int8_t*& m, int64_t& ld, int64_t rows) -> int {
-        if (ld % 16 == 0 || p.K == 0) return CHEBYKAN_OK;
-        const int64_t blocks = ceil_div(rows * pitch / 16, 256);
-        pad_kernel<<<(unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, s>>>(m, ld, at, pitch, rows, p.K);
+    Padding job[2];
+    int jobs = 0;
+    int64_t most = 0;
+    auto pad = [&](const int8_t*& m, int64_t& ld, int64_t rows) {
+        if (ld % 16 == 0 || p.K == 0) return;
+        job[jobs++] = {m, at, ld, rows};
+        if (rows > most) most = rows;
         m = at; ld = pitch; at += a256(rows * pitch);
-        return check_cuda(cudaGetLastError());
     };
-    int rc;
-    if ((rc = pad(p.q, p.ldq, p.M))) return rc;
-    if ((rc = pad(p.wq, p.ldw, p.N))) return rc;
+    pad(p.q, p.ldq, p.M);
+    pad(p.wq, p.ldw, p.N);
+    if (jobs > 0) {
+        const int64_t blocks = ceil_div(most * pitch / 16, 256);
+        pad_kernel<<<dim3((unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), (unsigned)jobs), 256, 0, s>>>(job[0], job[jobs - 1], pitch, p.K);
+        const int rc = check_cuda(cudaGetLastError());
+        if (rc) return rc;
+    }
     if (p.dtype == CHEBYKAN_DTYPE_FP32) return launch_typed<float>(p, status, s, after);
     if (p.dtype == CHEBYKAN_DTYPE_BF16) return launch_typed<__nv_bfloat16>(p, status, s, after);
     return launch_typed<__half>(p, status, s, after);
