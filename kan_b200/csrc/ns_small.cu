@@ -16,7 +16,7 @@
 // Products are tcgen05.mma (cta_group::1) issued by one elected lane; between two of them all eight warps turn the
 // accumulator into the next operand.  Heads are summed over at most 128 columns of K in an
 // accumulator: the tensor pipe's sums truncate (see gemm_tc.cuh).
-// Measured: 33 matrices of 64 x 64 27 us, five of 784 x 64 48 us, one of 64 x 10 17 us.  A product takes about 2200 cycles: 650 to
+// Measured: 33 matrices of 64 x 64 24 us, five of 784 x 64 47 us, one of 64 x 10 17 us.  A product takes about 2200 cycles: 650 to
 // issue, 170 to finish, 230 for the barriers and the rest to form the next operand.
 #include <math.h>
 #include "newton_schulz.cuh"
