@@ -189,6 +189,9 @@ __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
 // let_next_start(): its blocks take the SMs as they fall free and set themselves up, and then wait in wait_for_previous()
 // until that kernel has completed and its writes are visible.  Everything that reads or writes device memory comes after
 // the wait, except reads of data that no kernel of the same call writes.  Without the launch attribute both do nothing.
+// What the kernel before it writes may not be read by the non-coherent path (__ldg, or a `const T* __restrict__` argument,
+// from which the compiler may choose it): that path is for memory which nobody writes while the kernel is resident, and such
+// a kernel is resident before its input is written.  Plain pointers or __ldcg, after the wait.
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 template <typename... Params, typename... Args>

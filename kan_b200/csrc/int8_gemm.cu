@@ -50,7 +50,7 @@ struct Epilogue {
         const int row = row0 + (threadIdx.x & 31);
         alignas(16) float ws[32], bs[32];
         columns(p, g, col0, ws, bs);
-        const float qs = row < g.M ? __ldg(p.q_scale + row) : 0.f;
+        const float qs = row < g.M ? __ldcg(p.q_scale + row) : 0.f;       // see launch_after
         alignas(16) OUT out[32];
 #pragma unroll
         for (int e = 0; e < 32; ++e) out[e] = to_type<OUT>(fmaf((float)(int)r[e] * qs, ws[e], bs[e]));
@@ -60,7 +60,7 @@ struct Epilogue {
     static __device__ __forceinline__ void emit8(const Args& p, const Tiles& g, int row, int col0, const uint32_t (&r)[8]) {
         alignas(16) float ws[8], bs[8];
         columns(p, g, col0, ws, bs);
-        const float qs = __ldg(p.q_scale + row);
+        const float qs = __ldcg(p.q_scale + row);
         OUT* dst = reinterpret_cast<OUT*>(p.y) + (int64_t)row * g.N + col0;
         alignas(16) OUT out[8];
 #pragma unroll
@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(256) row_kernel(const Product p) {
         for (int d = 16; d; d >>= 1) acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], d);
 #pragma unroll
     for (int r = 0; r < ROWS; ++r)
-        if (lane == r && r < p.M) reinterpret_cast<OUT*>(p.y)[r * p.N + o] = to_type<OUT>(fmaf((float)acc[r] * p.q_scale[r], ws, bias));
+        if (lane == r && r < p.M) reinterpret_cast<OUT*>(p.y)[r * p.N + o] = to_type<OUT>(fmaf((float)acc[r] * __ldcg(p.q_scale + r), ws, bias));
 }
 
 // no columns at all: the sums are zero

@@ -159,7 +159,7 @@ momentum_kernel(const float* __restrict__ grad, float* __restrict__ buf, float* 
 
 // param = keep * param - step * O, O one plane per degree: the same tile the other way
 __global__ void __launch_bounds__(256)
-update_kernel(float* __restrict__ param, const float* __restrict__ o, int64_t pairs, int dp1, int width, uint32_t magic, float keep, float step) {
+update_kernel(float* param, const float* o, int64_t pairs, int dp1, int width, uint32_t magic, float keep, float step) {
     extern __shared__ float tile[];
     wait_for_previous();
     const int odd = dp1 | 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -172,7 +172,7 @@ update_kernel(float* __restrict__ param, const float* __restrict__ o, int64_t pa
             float x[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-                if (lane + k * 32 < n) x[k] = o[d * pairs + p0 + lane + k * 32];
+                if (lane + k * 32 < n) x[k] = __ldcg(o + d * pairs + p0 + lane + k * 32);     // see launch_after
 #pragma unroll
             for (int k = 0; k < 8; ++k)
                 if (lane + k * 32 < n) tile[(lane + k * 32) * odd + d] = x[k];
@@ -206,7 +206,7 @@ update_kernel(float* __restrict__ param, const float* __restrict__ o, int64_t pa
 __device__ __forceinline__ void block_scales(const double* partial, float eps, int growth, double* pow2, float* alpha, float* later) {
     __shared__ double smem[8];
     double t = 0.;
-    for (int k = threadIdx.x; k < NORM_BLOCKS; k += 256) t += partial[k];
+    for (int k = threadIdx.x; k < NORM_BLOCKS; k += 256) t += __ldcg(partial + k);
     t = block_sum(t, smem);
     if (threadIdx.x == 0) scales_of(sqrt(t), eps, growth, pow2, alpha, later);
 }
@@ -214,7 +214,7 @@ __device__ __forceinline__ void block_scales(const double* partial, float eps, i
 // X_0 planes where X's rows are the rows of the source: eight columns per thread
 template <typename T, int PLANES>
 __global__ void __launch_bounds__(256)
-pack_rows_kernel(const T* __restrict__ g, const Plane pl, __half* __restrict__ x, float* __restrict__ alpha, const double* __restrict__ partial,
+pack_rows_kernel(const T* g, const Plane pl, __half* x, float* alpha, const double* partial,
                  float eps, int growth, Shape sh) {
     __shared__ double pow2;
     __shared__ float scales[2];
@@ -242,7 +242,7 @@ pack_rows_kernel(const T* __restrict__ g, const Plane pl, __half* __restrict__ x
 // X_0 planes where X's rows are the source's columns: tiles of 32 source rows x 64 source columns turned in shared memory
 template <typename T, int PLANES>
 __global__ void __launch_bounds__(256)
-pack_turned_kernel(const T* __restrict__ g, const Plane pl, __half* __restrict__ x, float* __restrict__ alpha, const double* __restrict__ partial,
+pack_turned_kernel(const T* g, const Plane pl, __half* x, float* alpha, const double* partial,
                    float eps, int growth, Shape sh) {
     __shared__ float tile[64][33];                 // [source column = X row][source row = X column]
     __shared__ double pow2;

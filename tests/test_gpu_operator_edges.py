@@ -1,0 +1,40 @@
+"""Muon, orthogonalisation and 8-bit calls where they could go wrong at the edges: kernels that overlap their predecessor,
+tiny and huge values, tensors that are not the plain kind."""
+import pytest
+import torch
+
+from kan_b200 import ops
+from test_gpu_muon import muon64, randn, rel
+from _util import FP32_TOL
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("shape", [(100, 300, 3), (60, 1001, 2), (7, 2047, 4), (128, 1500), (33, 517, 9)])
+def test_muon_step_of_wide_small_matrices_in_a_row(shape):
+    # rows lie along memory and their ends fall anywhere in a sector, so the CTAs of a matrix write to shared ones, while the
+    # blocks of the update that follows are resident already
+    p, g, m = randn(*shape, seed=31, scale=0.01), randn(*shape, seed=32), torch.zeros(shape, device="cuda")
+    rows, cols = (shape[1], shape[0]) if len(shape) == 3 else shape
+    want, wm = p.double(), m.double()
+    for k in range(6):
+        g.copy_(randn(*shape, seed=40 + k))
+        want, wm = muon64(want, g, wm, 0.5, 0.1, 0.95, True, max(1.0, rows / cols) ** 0.5)
+        ops.muon_step(p, g, m, lr=0.5)
+    # each step adds an update of at most FP32_TOL relative error to weights that shrink; errors of six add up at most
+    assert rel(p, want) <= FP32_TOL * 6 and rel(m, wm) <= 1e-6
+    ops.check_status()
+
+
+@pytest.mark.parametrize("B,n_in,n_out,degree", [(40, 300, 90, 1), (3000, 64, 1100, 1), (20000, 40, 72, 1), (5, 900, 600, 1)])
+def test_int8_forward_in_a_row_takes_the_scales_of_its_own_rows(B, n_in, n_out, degree):
+    # the workspace is the same memory in every call: a scale left from the call before would show
+    gen = torch.Generator(device="cuda").manual_seed(B)
+    wq, ws, bias = ops.int8_pack_coeffs(torch.randn(n_in, n_out, degree + 1, generator=gen, device="cuda"))
+    xs = [torch.randn(B, n_in, generator=gen, device="cuda") * s for s in (1.0, 0.1, 3.0, 0.01)]
+    ys = [ops.int8_forward(x, wq, ws, bias, degree) for x in xs]
+    for x, y in zip(xs, ys):
+        q, scale = ops.int8_basis(x, degree)
+        torch.cuda.synchronize()
+        assert torch.equal(y, ops.int8_matmul(q, scale, wq, ws, bias))
+    ops.check_status()
