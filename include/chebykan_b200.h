@@ -39,6 +39,7 @@ extern "C" {
 #define CHEBYKAN_EWORKSPACE   -6  /* workspace / packed buffer too small            */
 #define CHEBYKAN_EDEVICE      -7  /* current device is not compute capability 10.x  */
 #define CHEBYKAN_ESTATIC      -8  /* problem needs more than the built-in 16 MiB scratch */
+#define CHEBYKAN_EOVERLAP     -9  /* a tensor that is written overlaps another argument */
 
 /* arithmetic mode of the contraction */
 #define CHEBYKAN_MODE_FP32 0  /* fp32 FFMA on CUDA cores, correctly rounded tanh   */
@@ -322,7 +323,8 @@ int chebykan_adam_step_graph(float* param, const float* grad, float* exp_avg,
  * and without a workspace).  The usual coefficients
  * (3.4445, -4.7750, 2.0315) push every singular value that is not tiny into about [0.7, 1.2] in five steps.
  *   - g: element (i, r, c) at g[i*stride_batch + r*stride_row + c*stride_col] (element strides, >= 0), of
- *     `dtype`; out: [batch][m][n] contiguous, of `dtype`; it may not overlap g;
+ *     `dtype`; out: [batch][m][n] contiguous, of `dtype`; the memory from g's first
+ *     to its last element may not overlap it (CHEBYKAN_EOVERLAP);
  *   - mode CHEBYKAN_MODE_FP32X3: operands held as two fp16 numbers each (22 significant bits), three products
  *     per multiplication, fp32 results; CHEBYKAN_MODE_TF32: operands rounded to fp16 (tf32's 11 significant
  *     bits), one product.  fp32 accumulation in both.  Other modes: CHEBYKAN_EUNSUPPORTED;
@@ -334,7 +336,7 @@ int chebykan_adam_step_graph(float* param, const float* grad, float* exp_avg,
  *     buf <- buf + (1 - momentum) (g - buf);   u = nesterov ? g + momentum (buf - g) : buf
  *     param[:,:,d] <- (1 - lr*weight_decay) param[:,:,d] - lr*update_scale * NS(u[:,:,d])   for every degree d
  * (torch.optim.Muon's update with each degree's in x out slice as a matrix; deg = 0 updates one plain matrix).
- * param, grad and buf are contiguous fp32 and may not overlap.  No host state: safe to capture and replay.
+ * param, grad and buf are contiguous fp32 and may not overlap (CHEBYKAN_EOVERLAP).  No host state: safe to capture and replay.
  */
 #define CHEBYKAN_DTYPE_FP32 0
 #define CHEBYKAN_DTYPE_BF16 1

@@ -98,6 +98,7 @@ const char* chebykan_strerror(int code) {
         case CHEBYKAN_EWORKSPACE: return "workspace or packed buffer too small";
         case CHEBYKAN_EDEVICE: return "current device is not compute capability 10.x (B200)";
         case CHEBYKAN_ESTATIC: return "shape needs more scratch than the library's built-in 16 MiB array; use the workspace variant";
+        case CHEBYKAN_EOVERLAP: return "a tensor that is written overlaps another argument";
         default: return "unknown error code";
     }
 }

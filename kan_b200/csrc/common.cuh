@@ -227,6 +227,13 @@ int check_device();
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// whether two ranges of memory share a byte (a null or an empty one shares none)
+inline bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+    if (!a || !b || a_bytes <= 0 || b_bytes <= 0) return false;
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y ? y - x < (uintptr_t)a_bytes : x - y < (uintptr_t)b_bytes;
+}
+
 // Optional LayerNorm fusion of the tensor-core forward.  stats_* hold two floats per row (sum and
 // sum of squares over the row's features).  With stats_in the kernel normalises its input rows,
 // x' = (x - mean) * rstd * gamma + beta, before tanh; with stats_out it adds the sums of the rows

@@ -433,6 +433,10 @@ int chebykan_orthogonalize(const void* g, int64_t stride_batch, int64_t stride_r
     if (!g || !out || !status) return CHEBYKAN_EINVAL;
     if (!aligned16(out) || !aligned16(workspace)) return CHEBYKAN_EALIGN;
     if (workspace_bytes < need || (need > 0 && !workspace)) return CHEBYKAN_EWORKSPACE;
+    const int64_t size = dtype == CHEBYKAN_DTYPE_FP32 ? 4 : 2;
+    // CTAs write one matrix while others still read the next
+    if (overlap(out, size * batch * m * n, g, size * ((batch - 1) * stride_batch + (m - 1) * stride_row + (n - 1) * stride_col + 1)))
+        return CHEBYKAN_EOVERLAP;
     int rc = check_device();
     if (rc) return rc;
     const Shape sh = shape_of(batch, m, n, mode);
@@ -467,6 +471,8 @@ int chebykan_muon_step(float* param, const float* grad, float* buf, void* worksp
         return CHEBYKAN_EINVAL;
     if (!aligned16(param) || !aligned16(grad) || !aligned16(buf) || !aligned16(workspace)) return CHEBYKAN_EALIGN;
     if (workspace_bytes < need || (need > 0 && !workspace)) return CHEBYKAN_EWORKSPACE;
+    const int64_t bytes = 4 * in * out * (deg + 1);
+    if (overlap(param, bytes, grad, bytes) || overlap(param, bytes, buf, bytes) || overlap(buf, bytes, grad, bytes)) return CHEBYKAN_EOVERLAP;
     int rc = check_device();
     if (rc) return rc;
     const int dp1 = (int)deg + 1;

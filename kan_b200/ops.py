@@ -547,7 +547,7 @@ def orthogonalize(g: torch.Tensor, steps: int = 5, coefficients=NS_COEFFICIENTS,
     X = g / max(|g|_F, eps), then `steps` times X <- (a I + b A + c A A) X with A = X X^T on the shorter side.
     `mode` 'fp32x3' multiplies operands of 22 significant bits in three products, 'tf32' operands of 11 bits in one;
     the default is 'tf32' for bfloat16 tensors, whose 8 bits hide the difference, and 'fp32x3' for the others.
-    A matrix with a NaN or an infinity gives NaN, a zero matrix zeros."""
+    A matrix with a NaN or an infinity gives NaN, a zero matrix zeros.  `out` may not overlap g."""
     _require_any(g, "g", contiguous=False)
     if g.dim() not in (2, 3):
         raise RuntimeError("g must have shape [m, n] or [batch, m, n]")
@@ -582,8 +582,8 @@ def muon_step(param: torch.Tensor, grad: torch.Tensor, momentum_buffer: torch.Te
               momentum: float = 0.95, nesterov: bool = True, coefficients=NS_COEFFICIENTS, eps: float = 1e-7, steps: int = 5,
               adjust: str = "original", grad_scale: float = 1.0, mode="fp32x3") -> None:
     """One Muon update in place of coefficients [in, out, degree+1] (every degree's in x out slice is a matrix of its own)
-    or of a matrix [m, n]; `momentum_buffer` has the parameter's shape and starts at zero.  Safe to capture in a CUDA
-    graph.  `mode`: the operands' precision inside the orthogonalisation, as for ``orthogonalize``."""
+    or of a matrix [m, n]; `momentum_buffer` has the parameter's shape and starts at zero.  The three may not
+    overlap.  Safe to capture in a CUDA graph.  `mode`: the operands' precision inside the orthogonalisation, as for ``orthogonalize``."""
     _require(param, "param")
     if param.dim() not in (2, 3):
         raise RuntimeError("param must have shape [in, out, degree+1] or [m, n]: use SGD or Adam for vectors")

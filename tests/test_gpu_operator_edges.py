@@ -38,3 +38,23 @@ def test_int8_forward_in_a_row_takes_the_scales_of_its_own_rows(B, n_in, n_out, 
         torch.cuda.synchronize()
         assert torch.equal(y, ops.int8_matmul(q, scale, wq, ws, bias))
     ops.check_status()
+
+
+def test_outputs_beside_their_inputs_are_accepted_and_over_them_refused():
+    memory = torch.zeros(6 * 40 * 60, device="cuda")
+    parts = [t.view(2, 40, 60) for t in memory.chunk(3)]                # adjacent, nothing between them
+    parts[0].copy_(randn(2, 40, 60, seed=50))
+    want = ops.orthogonalize(parts[0])
+    assert torch.equal(ops.orthogonalize(parts[0], out=parts[1]), want)
+    turned = memory.view(-1)[:6 * 40 * 40].view(40, 40, 6).permute(2, 0, 1)
+    for g, out in ((parts[0], parts[0]), (turned[:2], parts[0].view(-1)[:3200].view(2, 40, 40)), (turned, memory[4800:].view(-1)[:9600].view(6, 40, 40))):
+        with pytest.raises(RuntimeError, match="overlap"):
+            ops.orthogonalize(g, out=out)
+    p, g, m = parts
+    m.zero_(); g.copy_(randn(2, 40, 60, seed=51))
+    before = p.clone()
+    ops.muon_step(p, g, m, lr=0.1)
+    assert not torch.equal(p, before)
+    for args in ((p, p, m), (p, g, p), (p, g, g)):
+        with pytest.raises(RuntimeError, match="overlap"):
+            ops.muon_step(*args, lr=0.1)
