@@ -352,6 +352,11 @@ int launch_few_rows_to(const void* x, int x_dtype, const int8_t* wq, const float
 }
 
 bool dtype_ok(int dtype) { return dtype >= CHEBYKAN_DTYPE_FP32 && dtype <= CHEBYKAN_DTYPE_FP16; }
+int64_t dtype_size(int dtype) { return dtype == CHEBYKAN_DTYPE_FP32 ? 4 : 2; }
+// whether what is written covers part of the columns' scales or biases
+bool over_vectors(const void* y, int64_t bytes, const float* w_scale, const float* bias, int64_t n) {
+    return overlap(y, bytes, w_scale, 4 * n) || overlap(y, bytes, bias, 4 * n);
+}
 // row numbers are 32-bit inside the kernels, and a tile may reach past the last row
 constexpr int64_t MAX_ROWS = 0x7fffffff - 4096;
 // B rows of in values: the layer limits of the other entry points and an exact integer sum
@@ -385,6 +390,9 @@ int chebykan_int8_pack_coeffs(const float* coeffs, int8_t* wq, float* w_scale, f
                               int64_t deg, void* stream) {
     if (!layer_ok(0, in, out, deg) || !coeffs || !wq || !w_scale || !bias) return CHEBYKAN_EINVAL;
     if (!aligned16(coeffs) || !aligned16(wq) || !aligned16(w_scale) || !aligned16(bias)) return CHEBYKAN_EALIGN;
+    const int64_t read = 4 * in * out * (deg + 1);
+    if (overlap(wq, out * in_pad(in) * deg, coeffs, read) || overlap(w_scale, 4 * out, coeffs, read) || overlap(bias, 4 * out, coeffs, read))
+        return CHEBYKAN_EOVERLAP;
     int rc = check_device();
     if (rc) return rc;
     int8::pack_kernel<<<(unsigned)out, 256, 0, (cudaStream_t)stream>>>(coeffs, wq, w_scale, bias, (int)in, (int)out, (int)deg,
@@ -397,6 +405,8 @@ int chebykan_int8_basis(const void* x, int dtype, int8_t* q, float* scale, int64
     if (B == 0) return CHEBYKAN_OK;
     if (!x || !q || !scale) return CHEBYKAN_EINVAL;
     if (!aligned16(x) || !aligned16(q) || !aligned16(scale)) return CHEBYKAN_EALIGN;
+    const int64_t read = B * in * dtype_size(dtype);
+    if (overlap(q, B * in_pad(in) * deg, x, read) || overlap(scale, 4 * B, x, read)) return CHEBYKAN_EOVERLAP;
     int rc = check_device();
     if (rc) return rc;
     return launch_basis(x, dtype, q, scale, B, in, deg, (cudaStream_t)stream);
@@ -416,6 +426,10 @@ int chebykan_int8_matmul(const int8_t* q, int64_t ldq, const float* q_scale, con
     if (!aligned16(q) || !aligned16(wq) || !aligned16(y) || !aligned16(workspace)) return CHEBYKAN_EALIGN;
     const int64_t need = matmul_workspace_bytes(M, N, K, ldq, ldw);
     if (workspace_bytes < need || (need > 0 && !workspace)) return CHEBYKAN_EWORKSPACE;
+    const int64_t written = M * N * dtype_size(dtype);
+    if (overlap(y, written, q, (M - 1) * ldq + K) || overlap(y, written, wq, (N - 1) * ldw + K) || over_vectors(y, written, w_scale, bias, N) ||
+        overlap(y, written, q_scale, 4 * M))
+        return CHEBYKAN_EOVERLAP;
     int rc = check_device();
     if (rc) return rc;
     return launch_matmul({q, q_scale, wq, w_scale, bias, y, dtype, M, N, K, ldq, ldw}, workspace, status, (cudaStream_t)stream, false);
@@ -438,16 +452,18 @@ int chebykan_int8_fwd(const void* x, int x_dtype, const int8_t* wq, const float*
     if (!x || !wq || !w_scale || !y || !status) return CHEBYKAN_EINVAL;
     if (!aligned16(x) || !aligned16(wq) || !aligned16(y) || !aligned16(workspace)) return CHEBYKAN_EALIGN;
     if (workspace_bytes < need || (need > 0 && !workspace)) return CHEBYKAN_EWORKSPACE;
+    const int64_t K = in_pad(in) * deg, rows = chunk_rows(B, K), x_size = dtype_size(x_dtype), y_size = dtype_size(y_dtype);
+    const int64_t written = B * out * y_size;
+    if (overlap(y, written, x, B * in * x_size) || overlap(y, written, wq, out * K) || over_vectors(y, written, w_scale, bias, out))
+        return CHEBYKAN_EOVERLAP;
     int rc = check_device();
     if (rc) return rc;
-    const int64_t K = in_pad(in) * deg, rows = chunk_rows(B, K);
     if (need == 0) {
         cudaStream_t s = (cudaStream_t)stream;
         if (y_dtype == CHEBYKAN_DTYPE_FP32) return launch_few_rows_to<float>(x, x_dtype, wq, w_scale, bias, y, B, out, in, deg, s);
         if (y_dtype == CHEBYKAN_DTYPE_BF16) return launch_few_rows_to<__nv_bfloat16>(x, x_dtype, wq, w_scale, bias, y, B, out, in, deg, s);
         return launch_few_rows_to<__half>(x, x_dtype, wq, w_scale, bias, y, B, out, in, deg, s);
     }
-    const int64_t x_size = x_dtype == CHEBYKAN_DTYPE_FP32 ? 4 : 2, y_size = y_dtype == CHEBYKAN_DTYPE_FP32 ? 4 : 2;
     char* ws = reinterpret_cast<char*>(workspace);
     int8_t* q = reinterpret_cast<int8_t*>(ws);
     float* scale = reinterpret_cast<float*>(ws + a256(rows * K));

@@ -671,7 +671,8 @@ def _int8_matrix(t: torch.Tensor, name: str, idx: int | None):
 def int8_matmul(q: torch.Tensor, q_scale: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor,
                 bias: torch.Tensor | None = None, out_dtype=torch.float32, out: torch.Tensor | None = None) -> torch.Tensor:
     """y[M, N] = (q[M, K] wq[N, K]^T) * q_scale[M] * w_scale[N] + bias[N] for int8 matrices; the integer sums are exact
-    (K up to 131071).  Row strides that are multiples of 16 bytes are read in place, others through a padded copy."""
+    (K up to 131071).  Row strides that are multiples of 16 bytes are read in place, others through a padded copy.  `out` may
+    not overlap an argument."""
     qp, M, K, ldq = _int8_matrix(q, "q", None)
     idx = q.get_device()
     wp, N, wk, ldw = _int8_matrix(wq, "wq", idx)
@@ -690,7 +691,7 @@ def int8_matmul(q: torch.Tensor, q_scale: torch.Tensor, wq: torch.Tensor, w_scal
 def int8_forward(x: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor, bias: torch.Tensor | None, degree: int,
                  out_dtype=torch.float32, out: torch.Tensor | None = None) -> torch.Tensor:
     """Forward of a Chebyshev layer from coefficients packed by ``int8_pack_coeffs``: y[B, out] of `out_dtype` from x[B, in]
-    (fp32, bf16 or fp16).  ``int8_basis`` followed by ``int8_matmul`` in one call."""
+    (fp32, bf16 or fp16).  ``int8_basis`` followed by ``int8_matmul`` in one call.  `out` may not overlap an argument."""
     if not (type(x) in _TENSORS and x.is_cuda and x.is_contiguous() and not x.data_ptr() & 15):
         _require_any(x, "x")
     if x.dim() != 2:

@@ -58,3 +58,16 @@ def test_outputs_beside_their_inputs_are_accepted_and_over_them_refused():
     for args in ((p, p, m), (p, g, p), (p, g, g)):
         with pytest.raises(RuntimeError, match="overlap"):
             ops.muon_step(*args, lr=0.1)
+
+
+def test_int8_outputs_over_their_inputs_are_refused():
+    x = torch.randn(30, 64, device="cuda")
+    wq, ws, bias = ops.int8_pack_coeffs(torch.randn(64, 64, 4, device="cuda"))
+    q, scale = ops.int8_basis(x, 3)
+    for call in (lambda: ops.int8_forward(x, wq, ws, bias, 3, out=x), lambda: ops.int8_forward(x[:2], wq, ws, bias, 3, out=x[1:3]),
+                 lambda: ops.int8_matmul(q, scale, wq[:1], ws[:1], bias[:1], out=scale.view(30, 1))):
+        with pytest.raises(RuntimeError, match="overlap"):
+            call()
+    memory = torch.empty(60, 64, device="cuda")
+    memory[:30] = x
+    assert torch.equal(ops.int8_forward(memory[:30], wq, ws, bias, 3, out=memory[30:]), ops.int8_forward(x, wq, ws, bias, 3))

@@ -33,3 +33,34 @@ def test_muon_step_refuses_tensors_over_one_another(lib, size):
             assert muon(lib, **tensors, **kw) == EOVERLAP, (a, b, by)
             tensors[a], tensors[b] = tensors[b], tensors[a]
             assert muon(lib, **tensors, **kw) == EOVERLAP, (b, a, by)
+
+
+def test_int8_calls_refuse_outputs_over_their_inputs(lib):
+    n, k, B = 64, 256, 50
+
+    def matmul(y, q=FAR, qs=2 * FAR, wq=3 * FAR, ws_=4 * FAR, bias=5 * FAR, dtype=0, ldq=k):
+        return lib.chebykan_int8_matmul(q, ldq, qs, wq, k, ws_, bias, y, dtype, 7 * FAR, 1 << 30, B, n, k, 4096, None)
+
+    size = {0: 4, 1: 2, 2: 2}
+    for dtype in size:
+        out = B * n * size[dtype]
+        for at, length in ((FAR, B * k), (2 * FAR, 4 * B), (3 * FAR, n * k), (4 * FAR, 4 * n), (5 * FAR, 4 * n)):
+            for y in (at, at + (length - 1) // 16 * 16, at - out + 16):
+                assert matmul(y, dtype=dtype) == EOVERLAP, (dtype, at, y)
+    # rows far apart: the output between them counts as over them
+    assert matmul(FAR + 4096, ldq=1 << 20) == EOVERLAP
+
+    def forward(y, rows, x_dtype=0, y_dtype=0):
+        return lib.chebykan_int8_fwd(FAR, x_dtype, 3 * FAR, 4 * FAR, 5 * FAR, y, y_dtype, 7 * FAR, 1 << 30, rows, 64, n, 4, 4096, None)
+
+    for rows in (1, B):                                  # one launch, and two
+        for xt in size:
+            for yt in size:
+                out = rows * n * size[yt]
+                for at, length in ((FAR, rows * 64 * size[xt]), (3 * FAR, n * k), (4 * FAR, 4 * n), (5 * FAR, 4 * n)):
+                    for y in (at, at + (length - 1) // 16 * 16, at - out + 16):
+                        assert forward(y, rows, xt, yt) == EOVERLAP, (rows, xt, yt, at, y)
+    assert lib.chebykan_int8_basis(FAR, 0, FAR + 4 * B * 64 - 16, 3 * FAR, B, 64, 4, None) == EOVERLAP
+    assert lib.chebykan_int8_basis(FAR, 1, 3 * FAR, FAR + 2 * B * 64 - 16, B, 64, 4, None) == EOVERLAP
+    for wq, ws_, bias in ((FAR, 3 * FAR, 4 * FAR), (3 * FAR, FAR + 16, 4 * FAR), (3 * FAR, 4 * FAR, FAR + 4 * 64 * n * 5 - 16)):
+        assert lib.chebykan_int8_pack_coeffs(FAR, wq, ws_, bias, 64, n, 4, None) == EOVERLAP
