@@ -161,7 +161,11 @@ __device__ __forceinline__ void quantise_row(const T* __restrict__ src, bool liv
     if (!live) return;
     const bool bad = top > 3.f;                    // |T_d| <= 1 up to rounding
     const float s = bad ? __int_as_float(0x7fc00000) : __fdiv_rn(top, 127.f);
-    const float inv = (bad || s == 0.f) ? 0.f : __fdiv_rn(1.f, s);
+    // A degree-1 row may be so small that 1 / s overflows (from degree 2 on top is of the order of 1).  Its values and scale are
+    // lifted by 2^100, which is exact; a subnormal scale has few bits, so that values may lie beyond 127 of it and are clamped
+    const bool tiny = SMALL && top < 1e-30f;
+    const float lift = tiny ? 1.2676506e30f : 1.f;
+    const float inv = (bad || s == 0.f) ? 0.f : __fdiv_rn(1.f, s * lift);
     if (lane == 0) *scale = s;
     const f32x2 plus = pair_of(inv, inv), minus = pair_of(-inv, -inv);
 #pragma unroll
@@ -171,6 +175,15 @@ __device__ __forceinline__ void quantise_row(const T* __restrict__ src, bool liv
         if (i0 >= pad) continue;
         const int n = in - i0;                     // inputs of the chunk; the rest of the padded row is zero
         if (CHUNKS == 0 && chunks > 1 && n > 0) load(i0, tc);
+        if (tiny) {
+            const float most = inv > 0.f ? 127.f * (s * lift) : 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float v0, v1;
+                halves(tc[e], v0, v1);
+                tc[e] = pair_of(fminf(fmaxf(v0 * lift, -most), most), fminf(fmaxf(v1 * lift, -most), most));
+            }
+        }
         uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
         if (bad) keep0 = keep1 = 0;
         else if (n < 8) {

@@ -71,3 +71,27 @@ def test_int8_outputs_over_their_inputs_are_refused():
     memory = torch.empty(60, 64, device="cuda")
     memory[:30] = x
     assert torch.equal(ops.int8_forward(memory[:30], wq, ws, bias, 3, out=memory[30:]), ops.int8_forward(x, wq, ws, bias, 3))
+
+
+@pytest.mark.parametrize("n_in", [7, 100, 300, 3000, 5000])
+def test_int8_basis_of_tiny_rows(n_in):
+    # degree 1: tanh x = x for such values, and the scale is a subnormal number from a largest value of 1.5e-36 down
+    gen = torch.Generator(device="cuda").manual_seed(n_in)
+    tops = [1e-28, 1e-30, 9e-31, 3e-37, 1e-38, 1e-40, 190 * 2.0 ** -149, 64 * 2.0 ** -149, 63 * 2.0 ** -149, 2.0 ** -149]
+    x = torch.rand(len(tops), n_in, generator=gen, device="cuda") * 2 - 1
+    x[:, 0] = 1
+    x[1::2, 0] = -1
+    x[:, 2:4] = 0
+    x *= 2.0 ** 20                                       # keeps products of small factors exact until the last
+    x = (x.double() * torch.tensor(tops, dtype=torch.float64, device="cuda")[:, None] * 2.0 ** -20).float()
+    top = x.abs().amax(dim=1)
+    q, scale = ops.int8_basis(x, 1)
+    assert torch.equal(scale, (top.double() / 127).float())
+    want = torch.where(scale[:, None] > 0, x.double() / scale.double()[:, None], 0.0).clamp(-127, 127)
+    # the reciprocal of the scale and the quotient are rounded to fp32: 127 * 2^-23, and half a step
+    assert float((q[:, :n_in].double() - want).abs().max()) <= 0.5 + 127 * 2.0 ** -23
+    assert bool((q[:, 2:4] == 0).all()) and bool((q[:, n_in:] == 0).all())
+    wq, ws, bias = ops.int8_pack_coeffs(torch.randn(n_in, 20, 2, generator=gen, device="cuda"))
+    for rows in (slice(2, 4), slice(0, len(tops))):
+        y = ops.int8_forward(x[rows].clone(), wq, ws, None, 1)
+        assert torch.equal(y, ops.int8_matmul(q[rows].clone(), scale[rows].clone(), wq, ws)) and bool(torch.isfinite(y).all())
