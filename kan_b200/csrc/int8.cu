@@ -5,6 +5,7 @@
 // Degree 0 is the constant 1 and lives in the bias.  A row with any input near zero has |T_2| close to 1, so from
 // degree 2 on the scale is all but 1/127; it is taken from the row all the same, because a row of small inputs into
 // a layer of degree 1 would lose most of its 8 bits to a fixed one.
+#include <float.h>
 #include "int8.cuh"
 
 namespace chebykan {
@@ -289,7 +290,7 @@ pack_kernel(const float* __restrict__ c, int8_t* __restrict__ wq, float* __restr
         const float* p = c + ((int64_t)i * out + o) * dp1;
         sum += p[0];
         for (int d = 1; d <= deg; ++d) {
-            bad = bad || !(fabsf(p[d]) <= 3.4e38f);
+            bad = bad || !(fabsf(p[d]) <= FLT_MAX);
             top = fmaxf(top, fabsf(p[d]));
         }
     }
@@ -303,7 +304,7 @@ pack_kernel(const float* __restrict__ c, int8_t* __restrict__ wq, float* __restr
     __syncthreads();
     sum = 0.;
     for (int w = 0; w < 8; ++w) { top = fmaxf(top, redm[w]); sum += reds[w]; }
-    bad = top > 3.4e38f;
+    bad = top > FLT_MAX;
     const float s = bad ? __int_as_float(0x7fc00000) : __fdiv_rn(top, 127.f);
     if (threadIdx.x == 0) { w_scale[o] = s; bias[o] = (float)sum; }
     for (int i = threadIdx.x; i < pad; i += 256)

@@ -95,3 +95,19 @@ def test_int8_basis_of_tiny_rows(n_in):
     for rows in (slice(2, 4), slice(0, len(tops))):
         y = ops.int8_forward(x[rows].clone(), wq, ws, None, 1)
         assert torch.equal(y, ops.int8_matmul(q[rows].clone(), scale[rows].clone(), wq, ws)) and bool(torch.isfinite(y).all())
+
+
+def test_int8_pack_of_the_largest_and_of_no_numbers():
+    # finite up to the end of the type; a NaN or an infinity makes its own output NaN
+    top = torch.finfo(torch.float32).max
+    c = torch.randn(20, 7, 4, device="cuda")
+    c[3, 1, 2], c[4, 2, 1], c[5, 3, 3], c[6, 4, 1], c[7, 5, 1:] = top, -3.401e38, float("nan"), -float("inf"), 0
+    wq, ws, _ = ops.int8_pack_coeffs(c)
+    finite = [0, 1, 2, 5, 6]
+    assert torch.equal(ws[finite], (c[:, finite, 1:].abs().amax(dim=(0, 2)).double() / 127).float())
+    assert bool(torch.isnan(ws[3:5]).all()) and bool((wq[3:5] == 0).all())
+    w = wq.view(7, 3, 32)[:, :, :20].float()
+    assert w[1, 1, 3] == 127 and w[2, 0, 4] == -127
+    want = c[:, finite, 1:].double().permute(1, 2, 0) / ws[finite].double()[:, None, None]
+    # the quotient is rounded to fp32 (2^-24 of up to 127) before it is rounded to an integer
+    assert float((w[finite] - want).abs().max()) <= 0.5 + 127 * 2.0 ** -24
