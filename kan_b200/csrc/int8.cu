@@ -384,10 +384,9 @@ bool product_ok(int64_t M, int64_t N, int64_t K, int64_t ldq, int64_t ldw) {
 }
 int64_t a256(int64_t b) { return round_up(b, 256); }
 bool in_one_launch(int64_t B, int64_t K) { return few_rows(B, K) && B * K <= 46 * 1024; }      // the rows fit 48 KB of shared memory
-// rows worked on at a time: 1 GiB of quantised rows at most (4096 rows if they are longer than that)
+// rows worked on at a time: 1 GiB of quantised rows at most (8192 of the longest, MAX_K bytes)
 int64_t chunk_rows(int64_t B, int64_t K) {
-    int64_t rows = ((int64_t)1 << 30) / K / 256 * 256;
-    if (rows < 4096) rows = 4096;
+    const int64_t rows = ((int64_t)1 << 30) / K / 256 * 256;
     return B < rows ? B : rows;
 }
 

@@ -64,3 +64,12 @@ def test_int8_calls_refuse_outputs_over_their_inputs(lib):
     assert lib.chebykan_int8_basis(FAR, 1, 3 * FAR, FAR + 2 * B * 64 - 16, B, 64, 4, None) == EOVERLAP
     for wq, ws_, bias in ((FAR, 3 * FAR, 4 * FAR), (3 * FAR, FAR + 16, 4 * FAR), (3 * FAR, 4 * FAR, FAR + 4 * 64 * n * 5 - 16)):
         assert lib.chebykan_int8_pack_coeffs(FAR, wq, ws_, bias, 64, n, 4, None) == EOVERLAP
+
+
+def test_int8_forward_never_asks_for_more_than_a_gibibyte(lib):
+    for n_in, deg in ((16, 1), (100, 3), (1024, 127), (2000, 65), (16 * 8191, 1)):
+        row = -(-n_in // 16) * 16 * deg
+        rows = (1 << 30) // row // 256 * 256
+        assert rows >= 8192
+        for B in (1 << 27, rows + 1, rows):
+            assert lib.chebykan_int8_fwd_workspace_bytes(B, n_in, 8, deg) == rows * row + -(-rows * 4 // 256) * 256
