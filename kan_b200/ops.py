@@ -489,8 +489,10 @@ def _vector(t: torch.Tensor, name: str, size: int, idx: int) -> int:
         p = t.data_ptr()
         if not p & 15:
             return p
-    _require_any(t, name, torch.float32, torch.device("cuda", idx))       # says what is wrong with it
-    raise RuntimeError(f"{name} must have {size} elements")
+    _require_any(t, name, torch.float32, torch.device("cuda", idx))
+    if t.numel() != size:
+        raise RuntimeError(f"{name} must have {size} elements")
+    return t.data_ptr()
 
 
 _TENSORS = (torch.Tensor, torch.nn.Parameter)
@@ -671,8 +673,8 @@ def _int8_matrix(t: torch.Tensor, name: str, idx: int | None):
 def int8_matmul(q: torch.Tensor, q_scale: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor,
                 bias: torch.Tensor | None = None, out_dtype=torch.float32, out: torch.Tensor | None = None) -> torch.Tensor:
     """y[M, N] = (q[M, K] wq[N, K]^T) * q_scale[M] * w_scale[N] + bias[N] for int8 matrices; the integer sums are exact
-    (K up to 131071).  Row strides that are multiples of 16 bytes are read in place, others through a padded copy.  `out` may
-    not overlap an argument."""
+    (K up to 131071).  Row strides that are multiples of 16 bytes are read in place, others through a padded copy; both
+    matrices start on 16 bytes.  `out` may not overlap an argument."""
     qp, M, K, ldq = _int8_matrix(q, "q", None)
     idx = q.get_device()
     wp, N, wk, ldw = _int8_matrix(wq, "wq", idx)

@@ -111,3 +111,23 @@ def test_int8_pack_of_the_largest_and_of_no_numbers():
     want = c[:, finite, 1:].double().permute(1, 2, 0) / ws[finite].double()[:, None, None]
     # the quotient is rounded to fp32 (2^-24 of up to 127) before it is rounded to an integer
     assert float((w[finite] - want).abs().max()) <= 0.5 + 127 * 2.0 ** -24
+
+
+class Tagged(torch.Tensor):
+    pass
+
+
+def test_int8_calls_take_tensor_subclasses_and_name_what_is_wrong_with_a_vector():
+    x = torch.randn(5, 64, device="cuda")
+    wq, ws, bias = ops.int8_pack_coeffs(torch.randn(64, 12, 4, device="cuda"))
+    q, scale = ops.int8_basis(x, 3)
+    want = ops.int8_matmul(q, scale, wq, ws, bias)
+    as_tagged = [t.as_subclass(Tagged) for t in (q, scale, wq, ws, bias)]
+    assert torch.equal(ops.int8_matmul(*as_tagged).as_subclass(torch.Tensor), want)
+    assert torch.equal(ops.int8_forward(x.as_subclass(Tagged), *as_tagged[2:], 3).as_subclass(torch.Tensor), want)
+    for bad, words in ((ws[:-1], "12 elements"), (ws.double(), "float32"), (ws.cpu(), "CUDA"), (ws.repeat(2)[::2], "contiguous"),
+                       (ws.repeat(2)[1:13], "aligned"), (ws[:-1].as_subclass(Tagged), "12 elements")):
+        with pytest.raises(RuntimeError, match=words):
+            ops.int8_matmul(q, scale, wq, bad, bias)
+        with pytest.raises(RuntimeError, match=words):
+            ops.int8_forward(x, wq, ws, bad, 3)
