@@ -498,6 +498,13 @@ def _vector(t: torch.Tensor, name: str, size: int, idx: int) -> int:
 _TENSORS = (torch.Tensor, torch.nn.Parameter)
 
 
+def _no_gradient(t, name: str) -> None:
+    """Refuses a tensor whose gradient the caller would lose: these operators have no backward pass."""
+    if isinstance(t, torch.Tensor) and t.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{name} requires a gradient, which this operator does not give: call it under torch.no_grad() or "
+                           "on a detached tensor")
+
+
 def _result(out: torch.Tensor | None, shape, dtype, like: torch.Tensor) -> torch.Tensor:
     """`out` checked, or a new tensor of `dtype` on the device of `like`."""
     if out is None:
@@ -549,7 +556,9 @@ def orthogonalize(g: torch.Tensor, steps: int = 5, coefficients=NS_COEFFICIENTS,
     X = g / max(|g|_F, eps), then `steps` times X <- (a I + b A + c A A) X with A = X X^T on the shorter side.
     `mode` 'fp32x3' multiplies operands of 22 significant bits in three products, 'tf32' operands of 11 bits in one;
     the default is 'tf32' for bfloat16 tensors, whose 8 bits hide the difference, and 'fp32x3' for the others.
-    A matrix with a NaN or an infinity gives NaN, a zero matrix zeros.  `out` may not overlap g."""
+    A matrix with a NaN or an infinity gives NaN, a zero matrix zeros.  `out` may not overlap g.
+    There is no backward pass: a g that requires a gradient is refused outside torch.no_grad()."""
+    _no_gradient(g, "g")
     _require_any(g, "g", contiguous=False)
     if g.dim() not in (2, 3):
         raise RuntimeError("g must have shape [m, n] or [batch, m, n]")
@@ -693,7 +702,10 @@ def int8_matmul(q: torch.Tensor, q_scale: torch.Tensor, wq: torch.Tensor, w_scal
 def int8_forward(x: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor, bias: torch.Tensor | None, degree: int,
                  out_dtype=torch.float32, out: torch.Tensor | None = None) -> torch.Tensor:
     """Forward of a Chebyshev layer from coefficients packed by ``int8_pack_coeffs``: y[B, out] of `out_dtype` from x[B, in]
-    (fp32, bf16 or fp16).  ``int8_basis`` followed by ``int8_matmul`` in one call.  `out` may not overlap an argument."""
+    (fp32, bf16 or fp16).  ``int8_basis`` followed by ``int8_matmul`` in one call.  `out` may not overlap an argument.
+    There is no backward pass: an x that requires a gradient is refused outside torch.no_grad()."""
+    if getattr(x, "requires_grad", False):
+        _no_gradient(x, "x")
     if not (type(x) in _TENSORS and x.is_cuda and x.is_contiguous() and not x.data_ptr() & 15):
         _require_any(x, "x")
     if x.dim() != 2:

@@ -1,8 +1,9 @@
 """What the Muon and 8-bit entry points refuse beyond test_operator_refusals.py, without a GPU.  Every call here has to be
 refused before a device is asked for: its pointers are stand-ins."""
 import pytest
+import torch
 
-from kan_b200 import _lib
+from kan_b200 import _lib, ops
 from test_operator_refusals import lib, muon, orth      # noqa: F401  (lib is a fixture)
 
 EOVERLAP = -9
@@ -73,3 +74,13 @@ def test_int8_forward_never_asks_for_more_than_a_gibibyte(lib):
         assert rows >= 8192
         for B in (1 << 27, rows + 1, rows):
             assert lib.chebykan_int8_fwd_workspace_bytes(B, n_in, 8, deg) == rows * row + -(-rows * 4 // 256) * 256
+
+
+def test_operators_without_a_backward_pass_refuse_to_lose_a_gradient():
+    t = torch.zeros(16, 16, requires_grad=True)
+    q, v = torch.zeros(16, 16, dtype=torch.int8), torch.zeros(16)
+    for call in (lambda: ops.orthogonalize(t), lambda: ops.int8_forward(t, q, v, None, 1)):
+        with pytest.raises(RuntimeError, match="gradient"):
+            call()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
+            call()
