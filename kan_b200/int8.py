@@ -39,6 +39,16 @@ class Int8ChebyKANLayer(nn.Module):
         self.register_buffer("w_scale", w_scale)
         self.register_buffer("bias", bias)
 
+    def _apply(self, fn, recurse=True):
+        # model.half(), .to(torch.bfloat16), .double(): the kernels take the 8-bit weights, scales and biases as they were
+        # packed, whatever type the model around them works in; a move to another device is followed
+        packed = dict(self._buffers)
+        super()._apply(fn, recurse)
+        for name, t in packed.items():
+            if self._buffers[name].dtype != t.dtype:
+                self._buffers[name] = t.to(self._buffers[name].device)
+        return self
+
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if torch.is_grad_enabled() and x.requires_grad:
             raise RuntimeError("the 8-bit layer is for inference: it has no gradient (call it under torch.no_grad())")
