@@ -61,13 +61,18 @@ class Int8ChebyKANLayer(nn.Module):
         return f"input_dim={self.input_dim}, output_dim={self.output_dim}, degree={self.degree}"
 
 
+_MODULE_STATE = [name for name, value in nn.Module().__dict__.items() if isinstance(value, (dict, set))]
+
+
 def quantize_int8(model: nn.Module) -> nn.Module:
-    """The model with every ``ChebyKANLayer`` in 8 bits.  Other modules (and their parameters) are shared with `model`,
-    which stays as it is."""
+    """The model with every ``ChebyKANLayer`` in 8 bits.  Other modules, parameters and buffers are shared with `model`,
+    which stays as it is; casting or moving the result reaches what is shared (copy.deepcopy it first)."""
     if _is_cheby(model):
         return Int8ChebyKANLayer(model)
     if not any(_is_cheby(m) for m in model.modules()):
         return model
     clone = copy.copy(model)
+    for name in _MODULE_STATE:          # registering a hook, buffer or parameter with the one leaves the other alone
+        clone.__dict__[name] = copy.copy(model.__dict__[name])
     clone._modules = {name: None if child is None else quantize_int8(child) for name, child in model._modules.items()}
     return clone

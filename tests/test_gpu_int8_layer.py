@@ -36,3 +36,35 @@ def test_a_served_layer_moves_to_the_host_and_back():
         layer(x)
     layer.half().cuda()
     assert torch.equal(layer(x), want)
+
+
+class Scaled(torch.nn.Sequential):
+    def __init__(self, *layers):
+        super().__init__(*layers)
+        self.register_buffer("factor", torch.tensor(2.0))
+
+    def forward(self, x):
+        return super().forward(x) * self.factor
+
+
+def test_what_is_registered_with_the_served_model_stays_off_the_original():
+    model = Scaled(a_layer(), Scaled(torch.nn.LayerNorm(24), a_layer(24, 8))).cuda()
+    served = kan_b200.quantize_int8(model)
+    seen = []
+    for m in (served, served[1]):
+        m.register_forward_hook(lambda *a: seen.append(1))
+        m.register_forward_pre_hook(lambda *a: seen.append(1))
+        m.register_buffer("other", torch.zeros(1))
+        m.register_parameter("more", torch.nn.Parameter(torch.zeros(1)))
+        m.register_full_backward_hook(lambda *a: None)
+        m.register_state_dict_post_hook(lambda *a: None)
+        m.register_buffer("unsaved", torch.zeros(1), persistent=False)
+        m.add_module("extra", torch.nn.Identity())
+    x = torch.randn(5, 40, device="cuda")
+    with torch.no_grad():
+        model(x)
+    assert not seen
+    assert all("extra" not in k and "other" not in k and "more" not in k and "unsaved" not in k
+               for k, _ in [*model.named_modules(), *model.named_buffers(), *model.named_parameters()])
+    assert served.factor is model.factor and served[1][0] is model[1][0]
+    assert "unsaved" not in model._non_persistent_buffers_set
