@@ -21,6 +21,10 @@ def _is_cheby(m) -> bool:
     return hasattr(m, "cheby_coeffs") and hasattr(m, "math_mode") and hasattr(m, "_packed")
 
 
+def _packable(m) -> bool:
+    return _is_cheby(m) and m.degree > 0
+
+
 class Int8ChebyKANLayer(nn.Module):
     """8-bit form of a trained ``ChebyKANLayer`` on the GPU; same flatten rule, output in `out_dtype`."""
 
@@ -65,11 +69,12 @@ _MODULE_STATE = [name for name, value in nn.Module().__dict__.items() if isinsta
 
 
 def quantize_int8(model: nn.Module) -> nn.Module:
-    """The model with every ``ChebyKANLayer`` in 8 bits.  Other modules, parameters and buffers are shared with `model`,
-    which stays as it is; casting or moving the result reaches what is shared (copy.deepcopy it first)."""
-    if _is_cheby(model):
+    """The model with every ``ChebyKANLayer`` in 8 bits; one of degree 0, a constant, stays.  Other modules, parameters and
+    buffers are shared with `model`, which stays as it is; casting or moving the result reaches what is shared (copy.deepcopy
+    it first)."""
+    if _packable(model):
         return Int8ChebyKANLayer(model)
-    if not any(_is_cheby(m) for m in model.modules()):
+    if not any(_packable(m) for m in model.modules()):
         return model
     clone = copy.copy(model)
     for name in _MODULE_STATE:          # registering a hook, buffer or parameter with the one leaves the other alone

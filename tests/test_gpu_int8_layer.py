@@ -68,3 +68,12 @@ def test_what_is_registered_with_the_served_model_stays_off_the_original():
                for k, _ in [*model.named_modules(), *model.named_buffers(), *model.named_parameters()])
     assert served.factor is model.factor and served[1][0] is model[1][0]
     assert "unsaved" not in model._non_persistent_buffers_set
+
+
+def test_a_layer_of_degree_0_stays_among_packed_ones():
+    model = torch.nn.Sequential(a_layer(), a_layer(24, 12, 0, seed=1), a_layer(12, 8, 2, seed=2))
+    served = kan_b200.quantize_int8(model)
+    assert served[1] is model[1] and [type(m).__name__ for m in (served[0], served[2])] == ["Int8ChebyKANLayer"] * 2
+    x = torch.randn(5, 40, device="cuda")
+    with torch.no_grad():
+        assert torch.equal(served(x), served[2](model[1](x.new_zeros(5, 24))))       # the constant is the same for every input

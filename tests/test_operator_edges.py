@@ -3,6 +3,7 @@ refused before a device is asked for: its pointers are stand-ins."""
 import pytest
 import torch
 
+import kan_b200
 from kan_b200 import _lib, ops
 from test_operator_refusals import lib, muon, orth      # noqa: F401  (lib is a fixture)
 
@@ -84,3 +85,9 @@ def test_operators_without_a_backward_pass_refuse_to_lose_a_gradient():
             call()
         with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
             call()
+
+
+def test_quantize_int8_leaves_layers_of_degree_0():
+    constant = kan_b200.ChebyKANLayer(3, 4, 0)
+    model = torch.nn.Sequential(constant, torch.nn.LayerNorm(4))
+    assert kan_b200.quantize_int8(constant) is constant and kan_b200.quantize_int8(model) is model
