@@ -66,14 +66,19 @@ class Int8ChebyKANLayer(nn.Module):
 
 
 _MODULE_STATE = [name for name, value in nn.Module().__dict__.items() if isinstance(value, (dict, set))]
+_FORWARD_HOOKS = [name for name in _MODULE_STATE if name.startswith(("_forward_hooks", "_forward_pre_hooks"))]
 
 
 def quantize_int8(model: nn.Module) -> nn.Module:
-    """The model with every ``ChebyKANLayer`` in 8 bits; one of degree 0, a constant, stays.  Other modules, parameters and
-    buffers are shared with `model`, which stays as it is; casting or moving the result reaches what is shared (copy.deepcopy
-    it first)."""
+    """The model with every ``ChebyKANLayer`` in 8 bits; one of degree 0, a constant, stays.  Forward hooks of a replaced layer
+    go with it.  Other modules, parameters and buffers are shared with `model`, which stays as it is; casting or moving the
+    result reaches what is shared (copy.deepcopy it first)."""
     if _packable(model):
-        return Int8ChebyKANLayer(model)
+        served = Int8ChebyKANLayer(model)
+        served.train(model.training)
+        for name in _FORWARD_HOOKS:
+            served.__dict__[name] = copy.copy(model.__dict__[name])
+        return served
     if not any(_packable(m) for m in model.modules()):
         return model
     clone = copy.copy(model)

@@ -77,3 +77,23 @@ def test_a_layer_of_degree_0_stays_among_packed_ones():
     x = torch.randn(5, 40, device="cuda")
     with torch.no_grad():
         assert torch.equal(served(x), served[2](model[1](x.new_zeros(5, 24))))       # the constant is the same for every input
+
+
+def test_forward_hooks_and_mode_of_a_replaced_layer_go_with_it():
+    model = torch.nn.Sequential(a_layer(), a_layer(24, 8, seed=1).eval()).cuda()
+    seen = []
+    handle = model[0].register_forward_hook(lambda m, args, y: seen.append((type(m).__name__, tuple(y.shape))))
+    model[1].register_forward_pre_hook(lambda m, args, kwargs: ((args[0] * 0,), kwargs), with_kwargs=True)
+    model[1].register_forward_hook(lambda m, args, kwargs, y: y + 1, with_kwargs=True, always_call=True)
+    served = kan_b200.quantize_int8(model)
+    assert [m.training for m in served] == [True, False]
+    x = torch.randn(5, 40, device="cuda")
+    with torch.no_grad():
+        y = served(x)
+        assert seen == [("Int8ChebyKANLayer", (5, 24))]
+        plain = kan_b200.Int8ChebyKANLayer(model[1])
+        assert torch.equal(y, plain(torch.zeros(5, 24, device="cuda")) + 1)
+        handle.remove()                                  # the original's; the served layer has its own copy
+        model(x)
+        served(x)
+    assert len(seen) == 2
