@@ -73,16 +73,26 @@ def quantize_int8(model: nn.Module) -> nn.Module:
     """The model with every ``ChebyKANLayer`` in 8 bits; one of degree 0, a constant, stays.  Forward hooks of a replaced layer
     go with it.  Other modules, parameters and buffers are shared with `model`, which stays as it is; casting or moving the
     result reaches what is shared (copy.deepcopy it first)."""
-    if _packable(model):
-        served = Int8ChebyKANLayer(model)
-        served.train(model.training)
+    return _quantized(model, {})
+
+
+def _quantized(m: nn.Module, done: dict) -> nn.Module:
+    """`done`: what became of the modules met so far, so that a module used twice stays one module."""
+    if m in done:
+        return done[m]
+    if _packable(m):
+        new = Int8ChebyKANLayer(m)
+        new.train(m.training)
         for name in _FORWARD_HOOKS:
-            served.__dict__[name] = copy.copy(model.__dict__[name])
-        return served
-    if not any(_packable(m) for m in model.modules()):
-        return model
-    clone = copy.copy(model)
-    for name in _MODULE_STATE:          # registering a hook, buffer or parameter with the one leaves the other alone
-        clone.__dict__[name] = copy.copy(model.__dict__[name])
-    clone._modules = {name: None if child is None else quantize_int8(child) for name, child in model._modules.items()}
-    return clone
+            new.__dict__[name] = copy.copy(m.__dict__[name])
+    elif any(_packable(c) for c in m.modules()):
+        new = copy.copy(m)
+        for name in _MODULE_STATE:          # registering a hook, buffer or parameter with the one leaves the other alone
+            new.__dict__[name] = copy.copy(m.__dict__[name])
+        done[m] = new
+        for name, child in m._modules.items():
+            new._modules[name] = None if child is None else _quantized(child, done)
+    else:
+        new = m
+    done[m] = new
+    return new

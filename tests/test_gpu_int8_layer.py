@@ -97,3 +97,19 @@ def test_forward_hooks_and_mode_of_a_replaced_layer_go_with_it():
         model(x)
         served(x)
     assert len(seen) == 2
+
+
+def test_a_module_used_twice_stays_one_module():
+    layer = a_layer(24, 24)
+    block = torch.nn.Sequential(torch.nn.LayerNorm(24), layer).cuda()
+    model = torch.nn.Sequential(a_layer(), block, layer, block)
+    served = kan_b200.quantize_int8(model)
+    assert served[1] is served[3] and served[1][1] is served[2] and served[1] is not block
+    packed = [m for m in served.modules() if isinstance(m, kan_b200.Int8ChebyKANLayer)]
+    assert len(packed) == 2 and len(list(served.modules())) == len(list(model.modules()))
+    x = torch.randn(5, 40, device="cuda")
+    with torch.no_grad():
+        y = served[0](x)
+        for m in (block[0], packed[1], packed[1], block[0], packed[1]):
+            y = m(y)
+        assert torch.equal(served(x), y)
