@@ -30,7 +30,8 @@ torch.autograd.graph.set_warn_on_accumulate_grad_stream_mismatch(False)
 class GraphedTrainStep:
     def __init__(self, model: torch.nn.Module, loss_fn: Callable, optimizer, x: torch.Tensor, target: torch.Tensor,
                  warmup: int = 3, status_every: int = 256, all_reduce_grads: bool = True, group=None):
-        """`optimizer` must be graph-capturable (kan_b200.optim.SGD, or Adam(capturable=True)).
+        """`optimizer` must be graph-capturable: kan_b200.optim.SGD, Muon, or Adam(capturable=True), or a list of them that
+        step in turn (Muon for the coefficients, Adam for LayerNorm weights).
 
         With more than one rank in `group` (default: the world) and `all_reduce_grads`, the gradients are summed
         over the ranks between backward and the update, inside the graph; the loss function then has to
@@ -40,7 +41,8 @@ class GraphedTrainStep:
         self.group = group
         self._reduce = bool(all_reduce_grads) and dp.world_info_of(group)[1] > 1
         self._replays = 0
-        if getattr(optimizer, "capturable", True) is False:
+        self.opts = list(optimizer) if isinstance(optimizer, (list, tuple)) else [optimizer]
+        if any(getattr(opt, "capturable", True) is False for opt in self.opts):
             raise ValueError("use kan_b200.optim.Adam(..., capturable=True) for a graphed step")
         self.model, self.loss_fn, self.opt = model, loss_fn, optimizer
         self.x, self.target = x, target
@@ -64,7 +66,8 @@ class GraphedTrainStep:
         self.loss.backward()
         if self._reduce:
             self.grads.all_reduce(self.group)
-        self.opt.step()
+        for opt in self.opts:
+            opt.step()
 
     def close(self) -> None:
         """Destroy the recorded graph (replaying afterwards raises).  A graph that holds a captured collective keeps

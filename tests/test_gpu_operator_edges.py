@@ -3,7 +3,8 @@ tiny and huge values, tensors that are not the plain kind."""
 import pytest
 import torch
 
-from kan_b200 import ops
+import kan_b200
+from kan_b200 import graph, ops, optim
 from test_gpu_muon import muon64, randn, rel
 from _util import FP32_TOL
 
@@ -131,3 +132,29 @@ def test_int8_calls_take_tensor_subclasses_and_name_what_is_wrong_with_a_vector(
             ops.int8_matmul(q, scale, wq, bad, bias)
         with pytest.raises(RuntimeError, match=words):
             ops.int8_forward(x, wq, ws, bad, 3)
+
+
+def test_graphed_step_with_muon_for_the_coefficients_and_adam_for_the_rest():
+    def parts():
+        torch.manual_seed(0)
+        model = torch.nn.Sequential(kan_b200.ChebyKANLayer(12, 24, 4), torch.nn.LayerNorm(24), kan_b200.ChebyKANLayer(24, 8, 4)).cuda()
+        kan = [p for p in model.parameters() if p.dim() == 3]
+        rest = [p for p in model.parameters() if p.dim() != 3]
+        return model, [optim.Muon(kan, lr=0.02), optim.Adam(rest, lr=1e-3, capturable=True)]
+
+    x, t = randn(256, 12, seed=18), randn(256, 8, seed=19)
+    (a, opts_a), (b, opts_b) = parts(), parts()
+    start = [p.detach().clone() for p in a.parameters()]
+    step = graph.GraphedTrainStep(b, kan_b200.mse_loss, opts_b, x, t, warmup=2)
+    for _ in range(4):
+        step()
+    for _ in range(2 + 4):
+        for opt in opts_a:
+            opt.zero_grad(set_to_none=True)
+        kan_b200.mse_loss(a(x), t).backward()
+        for opt in opts_a:
+            opt.step()
+    for p, q, was in zip(a.parameters(), b.parameters(), start):
+        assert torch.equal(p, q) and not torch.equal(p, was)
+    step.close()
+    ops.check_status()

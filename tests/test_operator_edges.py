@@ -91,3 +91,11 @@ def test_quantize_int8_leaves_layers_of_degree_0():
     constant = kan_b200.ChebyKANLayer(3, 4, 0)
     model = torch.nn.Sequential(constant, torch.nn.LayerNorm(4))
     assert kan_b200.quantize_int8(constant) is constant and kan_b200.quantize_int8(model) is model
+
+
+def test_graphed_step_refuses_a_list_with_an_optimizer_that_cannot_be_captured():
+    class Fixed:
+        capturable = False
+
+    with pytest.raises(ValueError, match="capturable"):
+        kan_b200.graph.GraphedTrainStep(torch.nn.Linear(2, 2), kan_b200.mse_loss, [object(), Fixed()], torch.zeros(1, 2), torch.zeros(1, 2))
