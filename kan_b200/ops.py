@@ -577,6 +577,16 @@ def orthogonalize(g: torch.Tensor, steps: int = 5, coefficients=NS_COEFFICIENTS,
     return out
 
 
+def check_newton_schulz(steps: int, coefficients, eps: float) -> None:
+    """Raises ValueError for what ``orthogonalize`` and ``muon_step`` would refuse in a call (needs no GPU)."""
+    a, b, c = coefficients
+    # a batch of no matrices: the library looks at these arguments and returns
+    if _lib.load().chebykan_orthogonalize(None, 0, 0, 0, _lib.DTYPE_FP32, None, None, 0, 0, 1, 1, steps, a, b, c, eps,
+                                          _lib.MODE_FP32X3, None, None):
+        raise ValueError(f"Newton-Schulz iteration with steps={steps}, coefficients={tuple(coefficients)}, eps={eps}: steps must "
+                         "be 1 to 32, eps positive, and no singular value may grow beyond 7")
+
+
 def muon_scale(shape, adjust: str = "original") -> float:
     """Factor on the learning rate for a parameter [in, out, degree+1] (each degree maps `in` inputs to `out` outputs) or
     a plain matrix [rows, columns]: 'original' sqrt(max(1, rows / columns)), 'match_rms_adamw' 0.2 sqrt(max(rows,

@@ -8,8 +8,9 @@ parameter (ChebyKAN coefficients, LayerNorm weights, ...).  ``grad_scale``
 multiplies every gradient first (1/world_size after a sum all-reduce).
 
 ``Muon`` stands in for ``torch.optim.Muon`` in the same way (same arguments and
-defaults) and also takes coefficient tensors [in, out, degree+1], whose degree
-slices are orthogonalised as matrices of their own.
+defaults, with momentum below 1 and 1 to 32 Newton-Schulz steps) and also takes
+coefficient tensors [in, out, degree+1], whose degree slices are orthogonalised
+as matrices of their own.
 """
 from __future__ import annotations
 
@@ -126,10 +127,13 @@ class Muon(_Base):
                                  f"shape {list(p.shape)} to SGD or Adam")
             if p.numel() == 0:
                 raise ValueError("Muon got an empty parameter")
+            if max(p.shape[:2]) > 65536 or p.dim() == 3 and p.shape[2] > 128:
+                raise ValueError(f"Muon takes matrices of up to 65536 x 65536 and degrees up to 127, not shape {list(p.shape)}")
         if math_mode not in ("fp32x3", "tf32"):
             raise ValueError("math_mode must be 'fp32x3' or 'tf32'")
         if not 0.0 <= momentum < 1.0:
             raise ValueError("momentum must be in [0, 1)")
+        ops.check_newton_schulz(ns_steps, ns_coefficients, eps)       # here, not in the first step
         super().__init__(params, lr)
         self.weight_decay = float(weight_decay)
         self.momentum = float(momentum)

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import kan_b200
-from kan_b200 import _lib, ops
+from kan_b200 import _lib, ops, optim
 from test_operator_refusals import lib, muon, orth      # noqa: F401  (lib is a fixture)
 
 EOVERLAP = -9
@@ -99,3 +99,23 @@ def test_graphed_step_refuses_a_list_with_an_optimizer_that_cannot_be_captured()
 
     with pytest.raises(ValueError, match="capturable"):
         kan_b200.graph.GraphedTrainStep(torch.nn.Linear(2, 2), kan_b200.mse_loss, [object(), Fixed()], torch.zeros(1, 2), torch.zeros(1, 2))
+
+
+def test_muon_refuses_its_iteration_when_it_is_made(lib):
+    matrix = [torch.nn.Parameter(torch.zeros(5, 5))]
+    for kw in (dict(ns_steps=0), dict(ns_steps=33), dict(eps=0.0), dict(eps=-1e-7), dict(eps=float("nan")), dict(ns_coefficients=(30.0, -4.775, 2.0315)),
+               dict(ns_coefficients=(float("nan"), 0.0, 0.0))):
+        with pytest.raises(ValueError, match="Newton-Schulz"):
+            optim.Muon(matrix, **kw)
+    for kw in (dict(), dict(ns_steps=32, ns_coefficients=(1.5, -0.5, 0.0)), dict(eps=1e-30)):
+        ops.check_newton_schulz(kw.get("ns_steps", 5), kw.get("ns_coefficients", ops.NS_COEFFICIENTS), kw.get("eps", 1e-7))
+        with pytest.raises(RuntimeError, match="CUDA"):
+            optim.Muon(matrix, **kw)
+
+
+def test_muon_refuses_shapes_when_it_is_made(lib):
+    for shape in ((70000, 1), (1, 70000), (3, 70000, 2), (2, 3, 129)):
+        with pytest.raises(ValueError, match="65536"):
+            optim.Muon([torch.nn.Parameter(torch.zeros(1).expand(shape))])
+        assert lib.chebykan_muon_workspace_bytes(shape[0], shape[1], shape[2] - 1 if len(shape) == 3 else 0, _lib.MODE_FP32X3) == -1
+    assert lib.chebykan_muon_workspace_bytes(65536, 2, 127, _lib.MODE_FP32X3) > 0
