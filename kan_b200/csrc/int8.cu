@@ -222,10 +222,12 @@ basis_kernel(const T* __restrict__ x, int8_t* __restrict__ q, float* __restrict_
 
 // The whole forward of a few rows in one launch: every block quantises the rows for itself, into shared memory, while the first
 // of its weights are on their way, and then takes columns as row_kernel does.  The same arithmetic, so the same bits, as the two
-// kernels, without the launch, the workspace and the wait between them.  In a graph 1 x 2048 -> 2048 of degree 4 takes 4.8 us (7.7
-// as two kernels), 4 x 2048 -> 2048 11.7 (20.7), 4 x 784 -> 64 of degree 8 7.9 (17.9); 2 x 2048 -> 2048 7.3 (5.1) and
-// 8 x 128 -> 4096 9.2 (8.6) lose what every call gains on the host.  Bound by latency: the rows' quantisation, 2 us, then one
-// trip to memory for the weights after the first.
+// kernels, without the launch, the workspace and the wait between them.  Bound by latency: the rows' quantisation, 2 us, then one
+// trip to memory for the weights after the first.  In a graph (us, in brackets as two kernels that overlap) 1 x 2048 -> 2048 of
+// degree 4 takes 4.8 (8.0), 2 x 1024 -> 1000 4.0 (5.1), 4 x 784 -> 64 of degree 8 7.9 (9.3), 8 x 128 -> 4096 9.0 (13.0).  The 256 threads
+// share out the rows, so a row of several has 64 or 128 of them, and beyond 1024 inputs they fall behind: 2 x 1040 -> 1000 5.8
+// (4.7), 2 x 2048 -> 2048 7.4 (5.8), 4 x 1040 -> 1000 8.2 (7.4), 4 x 2048 -> 2048 11.8 (9.6), 4 x 11000 -> 2048 of degree 1 32 (15).
+// There in_one_launch() takes the two kernels, although a call from Python, which is bound by the host, then costs 14.6 instead of 11.
 template <typename OUT, typename T, int ROWS, bool SMALL>
 __global__ void __launch_bounds__(256)
 few_rows_kernel(const T* __restrict__ x, const int8_t* __restrict__ wq, const float* __restrict__ w_scale, const float* __restrict__ bias,
@@ -383,7 +385,12 @@ bool product_ok(int64_t M, int64_t N, int64_t K, int64_t ldq, int64_t ldw) {
            ldq <= ((int64_t)1 << 32) && ldw <= ((int64_t)1 << 32);
 }
 int64_t a256(int64_t b) { return round_up(b, 256); }
-bool in_one_launch(int64_t B, int64_t K) { return few_rows(B, K) && B * K <= 46 * 1024; }      // the rows fit 48 KB of shared memory
+// A few rows go through one launch while they fit 48 KB of shared memory; several only up to 1024 inputs, because the threads of
+// a block then share out the rows and evaluate the basis of longer ones in turn, in every block (see few_rows_kernel)
+bool in_one_launch(int64_t B, int64_t in, int64_t deg) {
+    const int64_t pad = in_pad(in), K = pad * deg;
+    return few_rows(B, K) && B * K <= 46 * 1024 && (B == 1 || pad <= 1024);
+}
 // rows worked on at a time: 1 GiB of quantised rows at most (8192 of the longest, MAX_K bytes)
 int64_t chunk_rows(int64_t B, int64_t K) {
     const int64_t rows = ((int64_t)1 << 30) / K / 256 * 256;
@@ -451,7 +458,7 @@ int chebykan_int8_matmul(const int8_t* q, int64_t ldq, const float* q_scale, con
 int64_t chebykan_int8_fwd_workspace_bytes(int64_t B, int64_t in, int64_t out, int64_t deg) {
     if (!layer_ok(B, in, out, deg)) return CHEBYKAN_EINVAL;
     const int64_t K = in_pad(in) * deg, rows = chunk_rows(B, K);
-    if (in_one_launch(B, K)) return 0;
+    if (in_one_launch(B, in, deg)) return 0;
     return a256(rows * K) + a256(rows * 4);
 }
 

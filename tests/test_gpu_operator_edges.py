@@ -158,3 +158,17 @@ def test_graphed_step_with_muon_for_the_coefficients_and_adam_for_the_rest():
         assert torch.equal(p, q) and not torch.equal(p, was)
     step.close()
     ops.check_status()
+
+
+@pytest.mark.parametrize("B,n_in,n_out,degree", [(2, 1024, 1000, 4), (2, 1025, 70, 4), (3, 1040, 1000, 8), (4, 1024, 300, 8), (4, 2048, 2048, 4),
+                                                 (4, 11000, 40, 1), (1, 11000, 40, 4), (1, 12000, 40, 4), (8, 512, 33, 1), (8, 513, 33, 1)])
+def test_int8_forward_on_both_sides_of_one_launch(B, n_in, n_out, degree):
+    gen = torch.Generator(device="cuda").manual_seed(B * n_in)
+    x = torch.randn(B, n_in, generator=gen, device="cuda")
+    wq, ws, bias = ops.int8_pack_coeffs(torch.randn(n_in, n_out, degree + 1, generator=gen, device="cuda"))
+    for xt in (x, x.half()):
+        q, scale = ops.int8_basis(xt, degree)
+        for dtype in (torch.float32, torch.bfloat16):
+            assert torch.equal(ops.int8_forward(xt, wq, ws, bias, degree, out_dtype=dtype),
+                               ops.int8_matmul(q, scale, wq, ws, bias, out_dtype=dtype))
+    ops.check_status()

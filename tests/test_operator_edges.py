@@ -119,3 +119,15 @@ def test_muon_refuses_shapes_when_it_is_made(lib):
             optim.Muon([torch.nn.Parameter(torch.zeros(1).expand(shape))])
         assert lib.chebykan_muon_workspace_bytes(shape[0], shape[1], shape[2] - 1 if len(shape) == 3 else 0, _lib.MODE_FP32X3) == -1
     assert lib.chebykan_muon_workspace_bytes(65536, 2, 127, _lib.MODE_FP32X3) > 0
+
+
+def test_int8_forward_of_a_few_rows_goes_without_a_workspace_where_one_launch_is_faster(lib):
+    def nbytes(B, n_in, deg):
+        return lib.chebykan_int8_fwd_workspace_bytes(B, n_in, 64, deg)
+
+    assert all(nbytes(1, n, deg) == 0 for n, deg in ((1, 1), (2048, 4), (4096, 8), (11000, 4)))
+    assert all(nbytes(B, n, deg) == 0 for B in (2, 3, 4) for n in (10, 512, 784, 1024) for deg in (1, 4, 8) if B * n * deg <= 46 * 1024)
+    assert all(nbytes(B, n, deg) == 0 for B in (5, 8) for n, deg in ((512, 1), (64, 8), (10, 32)))
+    # longer rows: two kernels, each quantised once
+    assert all(nbytes(B, n, deg) > 0 for B in (2, 3, 4) for n in (1025, 2048, 11000) for deg in (1, 4))
+    assert nbytes(1, 12000, 4) > 0 and nbytes(8, 513, 1) > 0 and nbytes(9, 64, 1) > 0
