@@ -22,7 +22,8 @@
 // Symmetric operands (LSYM, RSYM) are stored only in the 256 x 256 blocks on and above the diagonal: a block below it is
 // loaded from its mirror image and read through the other major-ness, which is a bit of the instruction descriptor.
 // Measured: 65536 x 8192 -> 1024 in int8 340 us alone (3.2 POP/s; the tensor pipe's 512 cycles per K block, plus a tail of one
-// epilogue); 4 x 2048 x 2048 bf16 P X 49 us (1.39 PFLOP/s); 9 x 1024 x 1024 in two planes 127 us for a step's A, P and X' (71 at the
+// epilogue); 4 x 2048 x 2048 bf16 P X 54 to 57 us from its start to the next kernel's (1.2 to
+// 1.28 PFLOP/s); 9 x 1024 x 1024 in two planes 127 us for a step's A, P and X' (71 at the
 // pipe's rate): an epilogue of some 7000 cycles (twice that for P, which also reads A) holds up the 24600 cycles of a tile's MMAs.
 // Every wait is bounded (see tc_common.cuh).
 #pragma once

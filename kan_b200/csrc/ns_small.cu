@@ -13,7 +13,7 @@
 // With at most 64 rows (NARROW) the tail plane lies in the panels' second 64 rows.  Then M = 64, which halves what an MMA reads
 // of its left operand (a product of this size is bound by that: some 80 cycles per MMA of M = 128, whatever N), and one MMA
 // multiplies head x head and head x tail side by side, as N = 128.
-// Products are tcgen05.mma (cta_group::1) issued by one elected lane; between two of them all eight warps turn the
+// Products are tcgen05.mma (cta_group::1) issued by one elected lane; between two of them all sixteen warps turn the
 // accumulator into the next operand.  Heads are summed over at most 128 columns of K in an
 // accumulator: the tensor pipe's sums truncate (see gemm_tc.cuh).
 // Measured: 33 matrices of 64 x 64 24 us, five of 784 x 64 47 us, one of 64 x 10 17 us.  A product takes about 2200 cycles: 650 to

@@ -555,7 +555,8 @@ def orthogonalize(g: torch.Tensor, steps: int = 5, coefficients=NS_COEFFICIENTS,
 
     X = g / max(|g|_F, eps), then `steps` times X <- (a I + b A + c A A) X with A = X X^T on the shorter side.
     `mode` 'fp32x3' multiplies operands of 22 significant bits in three products, 'tf32' operands of 11 bits in one;
-    the default is 'tf32' for bfloat16 tensors, whose 8 bits hide the difference, and 'fp32x3' for the others.
+    the default is 'fp32x3', and 'tf32' for bfloat16 tensors: where rounding the result to bfloat16 leaves an error of 1.7e-3
+    (rms), 'tf32' leaves 1.9e-3 to 2.0e-3, in 0.4 to 0.7 of the time.
     A matrix with a NaN or an infinity gives NaN, a zero matrix zeros.  `out` may not overlap g.
     There is no backward pass: a g that requires a gradient is refused outside torch.no_grad()."""
     _no_gradient(g, "g")
