@@ -46,7 +46,7 @@ class Int8ChebyKANLayer(nn.Module):
     def _apply(self, fn, recurse=True):
         # model.half(), .to(torch.bfloat16), .double(): the kernels take the 8-bit weights, scales and biases as they were
         # packed, whatever type the model around them works in; a move to another device is followed
-        packed = dict(self._buffers)
+        packed = {name: self._buffers[name] for name in ("wq", "w_scale", "bias")}
         super()._apply(fn, recurse)
         for name, t in packed.items():
             if self._buffers[name].dtype != t.dtype:

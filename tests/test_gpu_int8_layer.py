@@ -113,3 +113,12 @@ def test_a_module_used_twice_stays_one_module():
         for m in (block[0], packed[1], packed[1], block[0], packed[1]):
             y = m(y)
         assert torch.equal(served(x), y)
+
+
+def test_buffers_of_the_caller_are_cast():
+    layer = kan_b200.quantize_int8(a_layer())
+    layer.register_buffer("offset", torch.ones(24, device="cuda"))
+    layer.register_buffer("nothing", None)
+    layer.half()
+    assert layer.offset.dtype == torch.float16 and layer.nothing is None and layer.w_scale.dtype == torch.float32
+    assert layer(torch.randn(3, 40, device="cuda")).shape == (3, 24)
