@@ -69,6 +69,10 @@ _MODULE_STATE = [name for name, value in nn.Module().__dict__.items() if isinsta
 _FORWARD_HOOKS = [name for name in _MODULE_STATE if name.startswith(("_forward_hooks", "_forward_pre_hooks"))]
 
 
+def _rebuilds_coefficients(hook) -> bool:
+    return "cheby_coeffs" in (getattr(hook, "_tensor_name", None), getattr(hook, "name", None))
+
+
 def quantize_int8(model: nn.Module) -> nn.Module:
     """The model with every ``ChebyKANLayer`` in 8 bits; one of degree 0, a constant, stays.  Forward hooks of a replaced layer
     go with it.  Other modules, parameters and buffers are shared with `model`, which stays as it is; casting or moving the
@@ -84,7 +88,8 @@ def _quantized(m: nn.Module, done: dict) -> nn.Module:
         new = Int8ChebyKANLayer(m)
         new.train(m.training)
         for name in _FORWARD_HOOKS:
-            new.__dict__[name] = copy.copy(m.__dict__[name])
+            # pruning and weight normalisation hang hooks on a layer that rebuild its coefficients: they are packed already
+            new.__dict__[name].update((key, hook) for key, hook in m.__dict__[name].items() if not _rebuilds_coefficients(hook))
     elif any(_packable(c) for c in m.modules()):
         new = copy.copy(m)
         for name in _MODULE_STATE:          # registering a hook, buffer or parameter with the one leaves the other alone

@@ -1,6 +1,10 @@
 """The 8-bit layer as a module: casts and moves, hooks, shared layers, and the model it was made from."""
+import warnings
+
 import pytest
 import torch
+import torch.nn.utils.parametrize
+import torch.nn.utils.prune
 
 import kan_b200
 
@@ -122,3 +126,33 @@ def test_buffers_of_the_caller_are_cast():
     layer.half()
     assert layer.offset.dtype == torch.float16 and layer.nothing is None and layer.w_scale.dtype == torch.float32
     assert layer(torch.randn(3, 40, device="cuda")).shape == (3, 24)
+
+
+def pruned(layer):
+    torch.nn.utils.prune.random_unstructured(layer, "cheby_coeffs", 0.5)
+
+
+def normalised(layer):
+    with warnings.catch_warnings():
+        warnings.simplefilter("ignore")
+        torch.nn.utils.weight_norm(layer, "cheby_coeffs")
+
+
+def parametrised(layer):
+    torch.nn.utils.parametrize.register_parametrization(layer, "cheby_coeffs", torch.nn.Tanh())
+
+
+@pytest.mark.parametrize("change", [pruned, normalised, parametrised])
+def test_a_layer_whose_coefficients_are_rebuilt_is_packed_as_it_stands(change):
+    layer = a_layer()
+    change(layer)
+    seen = []
+    layer.register_forward_pre_hook(lambda m, args: seen.append(1))
+    x = torch.randn(9, 40, device="cuda")
+    with torch.no_grad():
+        full = layer(x)
+        served = kan_b200.quantize_int8(torch.nn.Sequential(layer))
+        y = served(x)
+        assert len(seen) == 2 and torch.equal(y, kan_b200.Int8ChebyKANLayer(layer)(x))
+        # a basis value is off by half a step of 1/127, a coefficient by half a step of its output's largest: about one percent
+        assert float((y - full).norm() / full.norm()) <= 2e-2
