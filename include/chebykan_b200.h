@@ -372,7 +372,8 @@ int chebykan_muon_step(float* param, const float* grad, float* buf, void* worksp
  * chebykan_int8_fwd: the two in a row; the quantised rows live in the workspace, at most 1 GiB of them at a
  *     time.  One row, or a few of at most 1024 inputs (up to 4, or 8 of at most 512 quantised bytes), 46 KiB of
  *     quantised bytes in all, take one launch: the workspace is 0 bytes and may be NULL.
- * Nothing that a call writes may overlap what it reads (CHEBYKAN_EOVERLAP).
+ * Nothing that a call writes may overlap what it reads, each argument counted from its first byte to its last
+ * (CHEBYKAN_EOVERLAP).
  */
 int chebykan_int8_pack_coeffs(const float* coeffs, int8_t* wq, float* w_scale, float* bias, int64_t in,
                               int64_t out, int64_t deg, void* stream);
