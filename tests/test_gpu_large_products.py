@@ -105,3 +105,33 @@ def test_int8_forward_of_a_full_batch(degree):
     check_product(y[-3000:], q[-3000:], scale[-3000:], wq, ws, bias)
     assert torch.equal(y, ops.int8_forward(x, wq, ws, bias, degree))
     ops.check_status()
+
+
+def test_offsets_beyond_32_bits():
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    # rows of q from byte 2^31 on, on the tensor cores and as a few rows far apart
+    q = torch.zeros(270000, 8192, dtype=torch.int8, device="cuda")
+    q[-3000:] = random_int8(3000, 8192, gen)
+    wq, ws = random_int8(40, 8192, gen), torch.rand(40, generator=gen, device="cuda")
+    qs = torch.rand(270000, generator=gen, device="cuda")
+    y = ops.int8_matmul(q, qs, wq, ws)
+    assert bool((y[:-3000] == 0).all())
+    check_product(y[-3000:], q[-3000:], qs[-3000:], wq, ws, None)
+    far = q[::269999]
+    check_product(ops.int8_matmul(far, qs[:2].clone(), wq, ws), far, qs[:2], wq, ws, None)
+    del q, far
+    # results from element 2^31 on
+    x = torch.randn(2200000, 16, generator=gen, device="cuda")
+    wq, ws, bias = ops.int8_pack_coeffs(torch.randn(16, 1000, 3, generator=gen, device="cuda"))
+    y = ops.int8_forward(x, wq, ws, bias, 2, out_dtype=torch.bfloat16)
+    for first in (0, 1100000, 2147483, 2199000):
+        rows = slice(first, first + 1000)
+        assert torch.equal(y[rows], ops.int8_forward(x[rows].clone(), wq, ws, bias, 2, out_dtype=torch.bfloat16))
+    del x, y
+    # matrices 2^31 elements apart, on chip and through the workspace
+    memory = torch.zeros(2 ** 31 + 300 * 500, dtype=torch.bfloat16, device="cuda")
+    for m, n in ((50, 70), (300, 500)):
+        g = memory.as_strided((2, m, n), (2 ** 31, n, 1))
+        g.copy_(randn(2, m, n, seed=5))
+        assert worst_block(ops.orthogonalize(g, mode="fp32x3"), ns64(g)) <= 1.25 * TOL["fp32x3", torch.bfloat16]
+    ops.check_status()
